@@ -171,6 +171,9 @@ static DevErr* ops_err_ptr() {
   return reinterpret_cast<DevErr*>(addr[dev]);
 }
 
+// the record, for the library's other translation units (not exported)
+extern "C" __attribute__((visibility("hidden"))) void* one_ops_err_record() { return ops_err_ptr(); }
+
 extern "C" int one_ops_error(int32_t* where, int32_t clear) {
   DevErr h{0, 0};
   CK(cudaDeviceSynchronize());

@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_size_t, c_void_p
+from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libone_b200.so")
 
@@ -74,6 +74,20 @@ SIGNATURES = {
     "one_selftest_mean_division": (c_int, [c_void_p, c_int32, c_void_p, c_void_p]),
     "one_sample_tokens": (c_int, [c_void_p, c_int32, c_int32, c_int32, c_int32, c_float, c_int32, c_float,
                                   ctypes.c_uint64, ctypes.c_uint64, c_void_p, c_void_p]),
+    "one_paged_append": (c_int, [c_void_p, c_int64, c_int64, c_int64] * 3 + [c_void_p, c_void_p, c_int32, c_void_p,
+                                 c_void_p, c_void_p, c_int64, c_int64, c_int32, c_int32, c_void_p, c_int64, c_int32,
+                                 c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_void_p, c_int64,
+                                 c_void_p, c_void_p]),
+    "one_paged_attention_workspace_bytes": (c_size_t, [c_int32] * 8),
+    "one_paged_attention": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int32, c_int32,
+                                    c_void_p, c_int64, c_int32, c_void_p, c_int32, c_int32, c_int32, c_int32, c_float,
+                                    c_int32, c_void_p, c_int64, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "one_paged_evict": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int32, c_int32, c_void_p, c_int64, c_int32,
+                                c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_int64, c_int32, c_int32, c_int32,
+                                c_int32, c_int32, c_int32, c_int32, c_void_p, c_int64, c_void_p, c_void_p]),
+    "one_process_logits": (c_int, [c_void_p, c_int64, c_int32, c_int32, c_int32, c_void_p, c_int64, c_int32, c_int32,
+                                   c_void_p, c_void_p, c_float, c_void_p, c_float, c_void_p, c_float, c_void_p, c_int64,
+                                   c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p]),
 }
 
 

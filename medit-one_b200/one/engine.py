@@ -19,6 +19,7 @@ import torch
 
 from . import _capi as C
 from .initialization import param_specs
+from .turbo_ops import _launch
 
 
 def rope_inv_freq(head_dim: int, theta: float) -> torch.Tensor:
@@ -325,3 +326,87 @@ def sample_tokens(logits: torch.Tensor, temperature: float = 1.0, top_k: int = 0
                                     C.ptr(out), ctypes.c_void_p(torch.cuda.current_stream(logits.device).cuda_stream)),
             "one_sample_tokens")
     return out
+
+
+def pack_token_mask(allowed: torch.Tensor) -> torch.Tensor:
+    """The token mask that process_logits takes from truth values allowed [V] or [B, V]: int32 words,
+    bit v % 32 of word v // 32 set = token v allowed."""
+    v = allowed.shape[-1]
+    bits = torch.nn.functional.pad(allowed.to(torch.int64), (0, -v % 32)).unflatten(-1, (-1, 32))
+    words = (bits << torch.arange(32, device=allowed.device)).sum(-1)
+    return torch.where(words >= 2 ** 31, words - 2 ** 32, words).to(torch.int32)
+
+
+def _penalty(x, name, batch):
+    """(fp32 [batch] tensor or None, scalar) of a penalty given as a number or per row."""
+    if isinstance(x, torch.Tensor):
+        if x.shape != (batch,) or x.dtype != torch.float32 or not x.is_contiguous():
+            raise C.OneError(f"{name} must be a number or fp32 [{batch}]")
+        return x, 1.0
+    return None, float(x)
+
+
+def process_logits(logits: torch.Tensor, history: Optional[torch.Tensor] = None,
+                   output_starts: Optional[torch.Tensor] = None, repetition_penalty=1.0, presence_penalty=0.0,
+                   frequency_penalty=0.0, bias: Optional[torch.Tensor] = None, token_mask: Optional[torch.Tensor] = None,
+                   out: Optional[torch.Tensor] = None, return_argmax: bool = False):
+    """A step's logits [B, V] (CUDA, bf16 or fp32) made ready for sample_tokens or greedy choice
+    (one_process_logits), in fp32. With c = how often a token stands in the row's history [B, T]
+    (int32 or int64 ids; ids outside [0, V), such as -1, are padding) from output_starts[b] on (int32
+    [B]; default 0): z = x; z = z / r where z > 0, else z * r, for tokens anywhere in the history
+    (repetition_penalty r); z -= frequency_penalty * c + presence_penalty * (c > 0); z += bias (fp32
+    [V] or [B, V]); z = -inf where token_mask (pack_token_mask's words, [W] or [B, W]) has a 0. Each
+    penalty is a number or fp32 [B]. Returns the scores fp32 [B, V] (`out`, which may be the logits
+    when they are fp32), and with return_argmax also int32 [B]: the token of the largest score, the
+    lowest among equals; NaN is never chosen; 0 when nothing is left."""
+    if logits.dim() != 2:
+        raise C.OneError("process_logits takes logits [batch, vocab]")
+    B, V = logits.shape
+    rep, rep1 = _penalty(repetition_penalty, "repetition_penalty", B)
+    pres, pres1 = _penalty(presence_penalty, "presence_penalty", B)
+    freq, freq1 = _penalty(frequency_penalty, "frequency_penalty", B)
+    if not rep1 > 0.0:
+        raise C.OneError("repetition_penalty must be positive")
+    if history is None and (rep is not None or rep1 != 1.0 or pres is not None or pres1 or freq is not None or freq1):
+        raise C.OneError("penalties need the history")
+    T, hb, hld = 0, 4, 0
+    if history is not None:
+        if history.dim() != 2 or history.shape[0] != B or history.dtype not in (torch.int32, torch.int64):
+            raise C.OneError(f"history must be int32 or int64 [{B}, T]")
+        T, hb = history.shape[1], history.element_size()
+        if T > 1 and history.stride(1) != 1:
+            history = history.contiguous()
+        hld = history.stride(0) if B > 1 else T
+    if output_starts is not None and (output_starts.shape != (B,) or output_starts.dtype != torch.int32
+                                      or not output_starts.is_contiguous()):
+        raise C.OneError(f"output_starts must be int32 [{B}]")
+    words = (V + 31) // 32
+    lds = []
+    for t, width, dt, name in ((bias, V, torch.float32, "bias"), (token_mask, words, torch.int32, "token_mask")):
+        if t is not None and (t.dtype != dt or t.shape not in ((width,), (1, width), (B, width))):
+            raise C.OneError(f"{name} must be {dt} [{width}] or [{B}, {width}], got {tuple(t.shape)}")
+        if t is not None and t.stride(-1) != 1 and width > 1:
+            raise C.OneError(f"{name} rows must be contiguous")
+        lds.append(0 if t is None or t.dim() == 1 or t.shape[0] == 1 else t.stride(0))
+    if out is not None and (out.shape != logits.shape or out.dtype != torch.float32 or (V > 1 and out.stride(1) != 1)):
+        raise C.OneError(f"out must be fp32 [{B}, {V}] with contiguous rows")
+    code = C.dtype_code(logits.dtype)
+    if not logits.is_cuda:
+        raise C.OneError("process_logits takes CUDA logits [batch, vocab]")
+    dev = logits.device
+    for t in (history, output_starts, rep, pres, freq, bias, token_mask, out):
+        if t is not None and t.device != dev:
+            raise C.OneError(f"all tensors must be on one device, got {dev} and {t.device}")
+    if V > 1 and logits.stride(1) != 1:
+        logits = logits.contiguous()
+    if out is None:
+        out = torch.empty((B, V), dtype=torch.float32, device=dev)
+    best = torch.empty((B,), dtype=torch.int32, device=dev) if return_argmax else None
+
+    def at(t):
+        return 0 if t is None else t.data_ptr()
+
+    _launch(C.LIB.one_process_logits, dev, logits.data_ptr(), logits.stride(0) if B > 1 else V, B, V, code,
+            at(history), hld, T, hb, at(output_starts), at(rep), rep1, at(pres), pres1, at(freq), freq1, at(bias), lds[0],
+            at(token_mask), lds[1], out.data_ptr(), out.stride(0) if B > 1 else V, at(best))
+    return (out, best) if return_argmax else out

@@ -230,7 +230,10 @@ class OneForCausalLM(OnePreTrainedModel, GenerationMixin):
     @torch.no_grad()
     def generate(self, input_ids: Optional[torch.LongTensor] = None, generation_config=None, max_length=None,
                  max_new_tokens=None, do_sample=None, temperature=None, top_k=None, top_p=None, eos_token_id=None,
-                 pad_token_id=None, seed: Optional[int] = None, attention_mask=None, **kwargs) -> torch.LongTensor:
+                 pad_token_id=None, seed: Optional[int] = None, attention_mask=None,
+                 repetition_penalty: Optional[float] = None, presence_penalty: Optional[float] = None,
+                 frequency_penalty: Optional[float] = None, logit_bias: Optional[torch.Tensor] = None,
+                 token_mask: Optional[torch.Tensor] = None, **kwargs) -> torch.LongTensor:
         """GenerationMixin.generate for greedy search and multinomial sampling, run on the engine
         (the reference's documented use, README.md:73, model.generate(input_ids, max_length=50,
         temperature=0.7), goes through transformers' generation loop, one/modeling_one.py:845).
@@ -243,6 +246,11 @@ class OneForCausalLM(OnePreTrainedModel, GenerationMixin):
         GPU (one_sample_tokens). Once a sequence emits eos_token_id its later tokens are
         pad_token_id (eos when pad is unset), and generation stops when every sequence has
         finished. `seed` fixes the draws (default: drawn from torch's global generator).
+
+        repetition_penalty (over prompt and new tokens, as transformers'), presence_penalty and
+        frequency_penalty (over the new tokens), logit_bias (fp32 [V] or [B, V]) and token_mask
+        (one.engine.pack_token_mask's words, the same at every step) act on each step's logits before
+        the warpers or the argmax (one.engine.process_logits). They are taken from the call alone.
         Returns [B, S + new tokens]. Beam search, constraints and streaming are not supported."""
         unsupported = {k: v for k, v in kwargs.items()
                        if v is not None and not (k in ("num_beams", "num_return_sequences") and v == 1)
@@ -278,8 +286,32 @@ class OneForCausalLM(OnePreTrainedModel, GenerationMixin):
             return input_ids
         if do_sample and not temperature > 0:
             raise ValueError("do_sample=True needs temperature > 0")
+        rep = 1.0 if repetition_penalty is None else float(repetition_penalty)
+        pres, freq = float(presence_penalty or 0.0), float(frequency_penalty or 0.0)
+        if not rep > 0:
+            raise ValueError("repetition_penalty must be positive")
+        processed = rep != 1.0 or pres != 0.0 or freq != 0.0 or logit_bias is not None or token_mask is not None
         eng = self.engine(max_batch=B, max_tokens=max(B * S, B), max_positions=S + max_new_tokens + 16)
-        if not do_sample:
+        if processed:
+            from .engine import process_logits, sample_tokens
+            if do_sample and seed is None:
+                seed = int(torch.randint(0, 2 ** 62, (1,)).item())
+            lg = eng.prefill(input_ids, logits="last")
+            buf = torch.empty(B, self.config.vocab_size, dtype=lg.dtype, device=lg.device)
+            scores = torch.empty(B, self.config.vocab_size, dtype=torch.float32, device=lg.device)
+            hist = torch.full((B, S + max_new_tokens), -1, dtype=torch.int32, device=lg.device)
+            hist[:, :S] = input_ids
+            starts = torch.full((B,), S, dtype=torch.int32, device=lg.device)
+            for i in range(max_new_tokens):
+                _, tok = process_logits(lg, hist[:, :S + i], starts, rep, pres, freq, logit_bias, token_mask, out=scores,
+                                        return_argmax=True)
+                if do_sample:
+                    sample_tokens(scores, temperature, top_k, top_p, seed, i, out=tok)
+                hist[:, S + i] = tok
+                if i + 1 < max_new_tokens:
+                    lg, _ = eng.step(tok, logits=True, next_ids=False, out=buf)
+            new = hist[:, S:].to(torch.long)
+        elif not do_sample:
             if eng.hist_cap < max_new_tokens:
                 raise ValueError(f"max_new_tokens > engine history capacity ({eng.hist_cap})")
             eng.prefill(input_ids)
