@@ -44,91 +44,6 @@ ONE_DEVINL int paged_page(const PagedCache& c, const int* table, int64_t row, in
   return pg;
 }
 
-struct PagedAttnParams {
-  PagedCache c;
-  const void* q;
-  int64_t q_bs, q_hs;
-  int G;
-  float scale_log2;
-  float* mass;
-  int64_t mass_width;
-  void* out;  // [B][Hq][Dh]
-};
-
-// One CTA per (kv head, sequence): its query heads one after the other, every warp over its share
-// of the slots with the online softmax (running maximum and sum in base 2).
-template <typename T>
-__global__ void __launch_bounds__(256) paged_attn_simple_kernel(const PagedAttnParams p) {
-  pdl_wait();
-  const PagedCache& c = p.c;
-  const int h = blockIdx.x, b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, W = blockDim.x >> 5;
-  const int n = paged_length(c, b, SITE_PAGED_ATTN);
-  __shared__ float sm_m[8], sm_l[8], sm_o[8][128];
-  auto row = [&](int t) -> int64_t {
-    const int pg = paged_page(c, c.table, b * c.table_stride, t / c.page_size, SITE_PAGED_ATTN);
-    return pg < 0 ? -1 : ((int64_t)h * c.page_size + t % c.page_size) * c.Dh + pg * c.k_stride;
-  };
-  auto vrow = [&](int t) -> int64_t {
-    const int pg = c.table[b * c.table_stride + t / c.page_size];
-    return ((int64_t)h * c.page_size + t % c.page_size) * c.Dh + pg * c.v_stride;
-  };
-  for (int g = 0; g < p.G; ++g) {
-    const int hq = h * p.G + g;
-    float q[4], o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int i = 0; i < 4; ++i) {
-      const int d = lane + 32 * i;
-      q[i] = d < c.Dh ? ld<T>((const T*)p.q + b * p.q_bs + hq * p.q_hs + d) * p.scale_log2 : 0.f;
-    }
-    auto score = [&](int64_t at) {
-      float s = 0.f;
-      for (int i = 0; i < 4; ++i) {
-        const int d = lane + 32 * i;
-        if (d < c.Dh) s += q[i] * ld<T>((const T*)c.k + at + d);
-      }
-      return warp_sum(s);
-    };
-    float m = -INFINITY, l = 0.f;
-    for (int t = warp; t < n; t += W) {
-      const int64_t at = row(t);
-      if (at < 0) continue;
-      const float s = score(at), mn = fmaxf(m, s), ms = mn == -INFINITY ? 0.f : mn;
-      const float a = exp2f(m - ms), e = exp2f(s - ms);
-      const int64_t va = vrow(t);
-      l = l * a + e;
-      for (int i = 0; i < 4; ++i) {
-        const int d = lane + 32 * i;
-        if (d < c.Dh) o[i] = o[i] * a + e * ld<T>((const T*)c.v + va + d);
-      }
-      m = mn;
-    }
-    if (lane == 0) {
-      sm_m[warp] = m;
-      sm_l[warp] = l;
-    }
-    for (int i = 0; i < 4; ++i) sm_o[warp][lane + 32 * i] = o[i];
-    __syncthreads();
-    float M = -INFINITY, L = 0.f;
-    for (int w = 0; w < W; ++w) M = fmaxf(M, sm_m[w]);
-    const float Ms = M == -INFINITY ? 0.f : M;
-    for (int w = 0; w < W; ++w) L += sm_l[w] * exp2f(sm_m[w] - Ms);
-    const float inv = L == 0.f ? 0.f : 1.f / L;
-    for (int d = threadIdx.x; d < c.Dh; d += blockDim.x) {
-      float acc = 0.f;
-      for (int w = 0; w < W; ++w) acc += sm_o[w][d] * exp2f(sm_m[w] - Ms);
-      st<T>((T*)p.out + ((int64_t)b * c.Hkv * p.G + hq) * c.Dh + d, acc * inv);
-    }
-    if (p.mass) {
-      for (int t = warp; t < n; t += W) {
-        const int64_t at = row(t);
-        if (at < 0) continue;
-        const float s = score(at);
-        if (lane == 0) p.mass[((int64_t)b * c.Hkv + h) * p.mass_width + t] += exp2f(s - Ms) * inv;
-      }
-    }
-    __syncthreads();
-  }
-}
-
 struct PagedAppendParams {
   PagedCache c;
   const void *k, *v, *q;
@@ -142,15 +57,85 @@ struct PagedAppendParams {
   int N, Hq;
 };
 
-// One warp per row of q, k or v.
+// Where token t of sequence b goes in head h of `pages` (stride: elements per page), or null. A slot
+// beyond the table and a page outside the pool are recorded.
 template <typename T>
-__global__ void __launch_bounds__(256) paged_append_simple_kernel(const PagedAppendParams p) {
+ONE_DEVINL T* append_row(const PagedAppendParams& p, void* pages, int64_t stride, int b, int h, int t, int64_t& slot) {
+  const PagedCache& c = p.c;
+  if (p.counts && t >= p.counts[b]) return nullptr;
+  const int len = c.lengths[b];
+  slot = (int64_t)len + t;
+  if (len < 0 || slot >= (int64_t)c.max_pages * c.page_size) {
+    set_err(c.err, ERR_BAD_ARG, SITE_PAGED_APPEND);
+    return nullptr;
+  }
+  const int index = (int)slot / c.page_size;
+  const int pg = paged_page(c, c.table, b * c.table_stride, index, SITE_PAGED_APPEND);
+  if (pg < 0) return nullptr;
+  return (T*)pages + pg * stride + ((int64_t)h * c.page_size + ((int)slot - index * c.page_size)) * c.Dh;
+}
+
+// New tokens into the pages, rotated: y = x cos + rotate_half(x) sin. A copy with two products per
+// element, bound by HBM (prompts) or by one round trip to it (single tokens).
+//
+// One thread per 8 elements of a row's first half and the matching 8 of its second, so the rotation
+// needs no exchange; the threads of a token's heads are neighbours and share its cos and sin in L1.
+// For rows whose halves are whole 16-byte pieces (Dh a multiple of 16, aligned strides);
+// paged_append_any_kernel takes the rest. Sequence blockIdx.y.
+template <typename T>
+__global__ void __launch_bounds__(256) paged_append_kernel(const __grid_constant__ PagedAppendParams p) {
   pdl_wait();
   const PagedCache& c = p.c;
-  const int lane = threadIdx.x & 31, half = c.Dh / 2, heads = 2 * c.Hkv + (p.q ? p.Hq : 0);
-  const int64_t i = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
-  if (i >= (int64_t)c.B * p.N * heads) return;
-  const int hh = (int)(i % heads), t = (int)(i / heads % p.N), b = (int)(i / heads / p.N);
+  const int units = c.Dh / 16, heads = 2 * c.Hkv + (p.q ? p.Hq : 0), half = c.Dh / 2, b = blockIdx.y;
+  const uint32_t i = blockIdx.x * blockDim.x + threadIdx.x;
+  const uint32_t row = i / units;
+  const int e = (int)(i - row * units) * 8, t = (int)(row / heads), hh = (int)(row - (uint32_t)t * heads);
+  if (t >= p.N) return;
+  const bool is_q = hh >= 2 * c.Hkv, is_v = !is_q && hh >= c.Hkv;
+  const int h = is_q ? hh - 2 * c.Hkv : is_v ? hh - c.Hkv : hh;
+  const T* x;
+  if (is_q) x = (const T*)p.q + b * p.qs[0] + h * p.qs[1] + t * p.qs[2];
+  else if (is_v) x = (const T*)p.v + b * p.vs[0] + h * p.vs[1] + t * p.vs[2];
+  else x = (const T*)p.k + b * p.ks[0] + h * p.ks[1] + t * p.ks[2];
+  float x1[8], x2[8];
+  load8(x + e, x1);
+  load8(x + half + e, x2);
+  T* y;
+  if (is_q) {
+    y = (T*)p.q_out + (((int64_t)b * p.Hq + h) * p.N + t) * c.Dh;
+  } else {
+    int64_t slot;
+    y = append_row<T>(p, is_v ? c.v : c.k, is_v ? c.v_stride : c.k_stride, b, h, t, slot);
+    if (!y) return;
+    if (!is_v && p.mass && e == 0) p.mass[((int64_t)b * c.Hkv + h) * p.mass_width + slot] = 0.f;
+  }
+  if (p.cosv && !is_v) {
+    const int64_t cs = b * p.cos_bs + (int64_t)t * c.Dh + e;
+    float c1[8], c2[8], s1[8], s2[8];
+    load8((const T*)p.cosv + cs, c1);
+    load8((const T*)p.cosv + cs + half, c2);
+    load8((const T*)p.sinv + cs, s1);
+    load8((const T*)p.sinv + cs + half, s2);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float a = x1[k], o = x2[k];
+      x1[k] = a * c1[k] - o * s1[k];
+      x2[k] = o * c2[k] + a * s2[k];
+    }
+  }
+  store8(y + e, x1);
+  store8(y + half + e, x2);
+}
+
+// The same for rows of any alignment: one warp per row of q, k or v.
+template <typename T>
+__global__ void __launch_bounds__(256) paged_append_any_kernel(const __grid_constant__ PagedAppendParams p) {
+  pdl_wait();
+  const PagedCache& c = p.c;
+  const int lane = threadIdx.x & 31, half = c.Dh / 2, heads = 2 * c.Hkv + (p.q ? p.Hq : 0), b = blockIdx.y;
+  const uint32_t row = (blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+  const int t = (int)(row / heads), hh = (int)(row - (uint32_t)t * heads);
+  if (t >= p.N) return;
   const bool is_q = hh >= 2 * c.Hkv, is_v = !is_q && hh >= c.Hkv;
   const int h = is_q ? hh - 2 * c.Hkv : is_v ? hh - c.Hkv : hh;
   const int64_t* s = is_q ? p.qs : is_v ? p.vs : p.ks;
@@ -159,16 +144,9 @@ __global__ void __launch_bounds__(256) paged_append_simple_kernel(const PagedApp
   if (is_q) {
     y = (T*)p.q_out + (((int64_t)b * p.Hq + h) * p.N + t) * c.Dh;
   } else {
-    const int cnt = p.counts ? min(p.counts[b], p.N) : p.N;
-    if (t >= cnt) return;
-    const int64_t slot = (int64_t)c.lengths[b] + t;
-    if (c.lengths[b] < 0 || slot >= (int64_t)c.max_pages * c.page_size) {
-      set_err(c.err, ERR_BAD_ARG, SITE_PAGED_APPEND);
-      return;
-    }
-    const int pg = paged_page(c, c.table, b * c.table_stride, (int)(slot / c.page_size), SITE_PAGED_APPEND);
-    if (pg < 0) return;
-    y = (T*)(is_v ? c.v : c.k) + pg * (is_v ? c.v_stride : c.k_stride) + ((int64_t)h * c.page_size + slot % c.page_size) * c.Dh;
+    int64_t slot;
+    y = append_row<T>(p, is_v ? c.v : c.k, is_v ? c.v_stride : c.k_stride, b, h, t, slot);
+    if (!y) return;
     if (!is_v && p.mass && lane == 0) p.mass[((int64_t)b * c.Hkv + h) * p.mass_width + slot] = 0.f;
   }
   const int64_t cs = b * p.cos_bs + (int64_t)t * c.Dh;
@@ -201,66 +179,151 @@ ONE_DEVINL uint32_t mass_key(float f) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// One CTA per (kv head, sequence): a slot survives when fewer than the free places rank before it.
-__global__ void __launch_bounds__(256) paged_select_simple_kernel(const PagedEvictParams p) {
+// Which slots survive: one CTA per (sequence, kv head) finds the smallest surviving key by radix
+// selection (digits of 11, 11 and 10 bits, counted in shared memory), then writes the surviving slots
+// in order: every warp counts its run of slots, and the counts before it say where its survivors go.
+// Keys are read from HBM once and kept in shared memory up to `cached` of them; longer sequences are
+// read again in each of the five passes. Bound by the passes over shared memory, not by HBM.
+constexpr int kSelThreads = 1024;
+constexpr int kSelCached = 48 * 1024;
+
+__global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const __grid_constant__ PagedEvictParams p, int cached) {
+  extern __shared__ uint32_t keys[];
+  __shared__ uint32_t hist[2048];
+  __shared__ int wsum[2][32];
+  __shared__ uint32_t sh_digit;
+  __shared__ int sh_above;
   pdl_wait();
+  pdl_launch_dependents();
   const PagedCache& c = p.c;
-  const int h = blockIdx.x, b = blockIdx.y;
-  const int n = paged_length(c, b, SITE_PAGED_EVICT);
-  const float* mass = p.mass + ((int64_t)b * c.Hkv + h) * p.mass_width;
-  int* kept = p.kept + ((int64_t)b * c.Hkv + h) * p.budget;
-  __shared__ uint32_t sh_thr;
-  __shared__ int sh_count, sh_at;
-  const int lo = n > p.budget ? p.sink : 0, hi = n > p.budget ? n - p.recent : 0;  // slots that are ranked
-  const int places = p.budget - p.sink - p.recent;
-  // the smallest key that survives, bit by bit
-  uint32_t thr = 0;
-  for (int bit = 31; bit >= 0; --bit) {
-    if (threadIdx.x == 0) sh_count = 0;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t bh = blockIdx.x;
+  const int n = paged_length(c, (int)(bh / c.Hkv), SITE_PAGED_EVICT);
+  int* kept = p.kept + bh * p.budget;
+  if (n <= p.budget) {
+    for (int t = tid; t < p.budget; t += kSelThreads) kept[t] = t < n ? t : -1;
+    return;
+  }
+  const float* mass = p.mass + bh * p.mass_width + p.sink;
+  const int nc = n - p.sink - p.recent, places = p.budget - p.sink - p.recent;  // candidates, and room for them
+  for (int t = tid; t < p.sink; t += kSelThreads) kept[t] = t;
+  for (int t = tid; t < p.recent; t += kSelThreads) kept[p.budget - p.recent + t] = n - p.recent + t;
+  if (places == 0) return;
+  const bool in_smem = nc <= cached;
+  uint32_t prefix = 0, mask = 0;
+  int above = 0;  // candidates above the prefix
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+    for (int i = tid; i < 2048; i += kSelThreads) hist[i] = 0;
     __syncthreads();
-    int mine = 0;
-    for (int t = lo + threadIdx.x; t < hi; t += blockDim.x) mine += mass_key(mass[t]) >= (thr | 1u << bit);
-    atomicAdd(&sh_count, mine);
+    for (int i = tid; i < nc; i += kSelThreads) {
+      const uint32_t k = pass > 0 && in_smem ? keys[i] : mass_key(mass[i]);
+      if (pass == 0 && in_smem) keys[i] = k;
+      if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1)], 1u);
+    }
     __syncthreads();
-    if (sh_count >= places) thr |= 1u << bit;
+    // thread t holds digits 2047 - 2 t and 2046 - 2 t; sums from the top
+    const int d0 = 2047 - 2 * tid, h0 = (int)hist[d0], h1 = (int)hist[d0 - 1];
+    int incl = h0 + h1;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int t = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += t;
+    }
+    if (lane == 31) wsum[0][warp] = incl;
+    __syncthreads();
+    if (warp == 0) {
+      int v = wsum[0][lane];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int t = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += t;
+      }
+      wsum[0][lane] = v;
+    }
+    __syncthreads();
+    const int before = above + (warp ? wsum[0][warp - 1] : 0) + incl - h0 - h1;
+    if (before < places && before + h0 + h1 >= places) {
+      const bool first = before + h0 >= places;
+      sh_digit = (uint32_t)(first ? d0 : d0 - 1);
+      sh_above = first ? before : before + h0;
+    }
+    __syncthreads();
+    prefix |= sh_digit << shift;
+    mask |= ((1u << bits) - 1) << shift;
+    above = sh_above;
     __syncthreads();
   }
-  if (threadIdx.x == 0) {
-    int above = 0, at = 0;
-    for (int t = lo; t < hi; ++t) above += mass_key(mass[t]) > thr;
-    int equal = places - above;
-    for (int t = 0; t < n; ++t) {
-      bool keep = t < lo || t >= hi;
-      if (!keep) {
-        const uint32_t k = mass_key(mass[t]);
-        keep = k > thr || (k == thr && equal-- > 0);
-      }
-      if (keep) kept[at++] = t;
-    }
-    for (; at < p.budget; ++at) kept[at] = -1;
+  // survivors: keys above `prefix`, and the first `ties` that equal it
+  const int ties = places - above;
+  const int run = ((nc + 31) / 32 + 31) / 32 * 32, i0 = warp * run, i1 = min(nc, i0 + run);
+  int gt = 0, eq = 0;
+  for (int i = i0; i < i1; i += 32) {
+    const uint32_t k = i + lane < i1 ? (in_smem ? keys[i + lane] : mass_key(mass[i + lane])) : 0u;
+    gt += __popc(__ballot_sync(0xffffffffu, i + lane < i1 && k > prefix));
+    eq += __popc(__ballot_sync(0xffffffffu, i + lane < i1 && k == prefix));
+  }
+  if (lane == 0) {
+    wsum[0][warp] = gt;
+    wsum[1][warp] = eq;
+  }
+  __syncthreads();
+  gt = eq = 0;
+  for (int w = 0; w < warp; ++w) {
+    gt += wsum[0][w];
+    eq += wsum[1][w];
+  }
+  const uint32_t below = (1u << lane) - 1;
+  for (int i = i0; i < i1; i += 32) {
+    const bool in = i + lane < i1;
+    const uint32_t k = in ? (in_smem ? keys[i + lane] : mass_key(mass[i + lane])) : 0u;
+    const unsigned bg = __ballot_sync(0xffffffffu, in && k > prefix), be = __ballot_sync(0xffffffffu, in && k == prefix);
+    const int myeq = eq + __popc(be & below), at = gt + __popc(bg & below) + min(myeq, ties);
+    if (in && (k > prefix || (k == prefix && myeq < ties))) kept[p.sink + at] = p.sink + i + lane;
+    gt += __popc(bg);
+    eq += __popc(be);
   }
 }
 
-// One warp per survivor's place.
-template <typename T>
-__global__ void __launch_bounds__(256) paged_move_simple_kernel(const PagedEvictParams p) {
+// The survivors' rows and masses to their places, 64 places of one (sequence, kv head) per CTA: the
+// rows' addresses first, then 16 bytes per thread and copy. A gather, bound by HBM.
+constexpr int kMovePlaces = 64;
+
+__global__ void __launch_bounds__(256) paged_move_kernel(const __grid_constant__ PagedEvictParams p, int per_bh, int pieces) {
+  __shared__ int64_t from[2][kMovePlaces], to[2][kMovePlaces];  // 16-byte units; -1: nothing to copy
   pdl_wait();
   const PagedCache& c = p.c;
-  const int lane = threadIdx.x & 31, h = blockIdx.y % c.Hkv, b = blockIdx.y / c.Hkv;
-  const int64_t i = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  if (i >= p.out_width) return;
-  const int64_t bh = (int64_t)b * c.Hkv + h;
-  const int src = i < p.budget ? p.kept[bh * p.budget + i] : -1;
-  if (lane == 0) p.mass_out[bh * p.out_width + i] = src < 0 ? 0.f : p.mass[bh * p.mass_width + src];
-  if (src < 0) return;
-  const int ps = paged_page(c, c.table, b * c.table_stride, src / c.page_size, SITE_PAGED_EVICT);
-  const int pd = paged_page(c, p.dst, b * p.dst_stride, (int)(i / c.page_size), SITE_PAGED_EVICT);
-  if (ps < 0 || pd < 0) return;
-  const int64_t so = ((int64_t)h * c.page_size + src % c.page_size) * c.Dh;
-  const int64_t to = ((int64_t)h * c.page_size + i % c.page_size) * c.Dh;
-  for (int d = lane; d < c.Dh; d += 32) {
-    ((T*)c.k)[pd * c.k_stride + to + d] = ((const T*)c.k)[ps * c.k_stride + so + d];
-    ((T*)c.v)[pd * c.v_stride + to + d] = ((const T*)c.v)[ps * c.v_stride + so + d];
+  const int tid = threadIdx.x;
+  const int64_t bh = blockIdx.x / per_bh;
+  const int i0 = (int)(blockIdx.x % per_bh) * kMovePlaces, b = (int)(bh / c.Hkv), h = (int)(bh % c.Hkv);
+  const int64_t i = (int64_t)i0 + tid;
+  if (tid < kMovePlaces) {
+    const int src = i < p.budget ? p.kept[bh * p.budget + i] : -1;
+    int ps = -1, pd = -1;
+    if (src >= 0) {
+      ps = paged_page(c, c.table, b * c.table_stride, src / c.page_size, SITE_PAGED_EVICT);
+      pd = paged_page(c, p.dst, b * p.dst_stride, (int)i / c.page_size, SITE_PAGED_EVICT);
+    }
+    const bool there = ps >= 0 && pd >= 0;
+    const int64_t row = (int64_t)c.Dh, per16 = row / pieces;  // elements of a row; of 16 bytes
+    const int64_t so = ((int64_t)h * c.page_size + src % c.page_size) * row;
+    const int64_t dt = ((int64_t)h * c.page_size + (int)i % c.page_size) * row;
+    from[0][tid] = there ? (ps * c.k_stride + so) / per16 : -1;
+    from[1][tid] = there ? (ps * c.v_stride + so) / per16 : -1;
+    to[0][tid] = there ? (pd * c.k_stride + dt) / per16 : -1;
+    to[1][tid] = there ? (pd * c.v_stride + dt) / per16 : -1;
+    if (i < p.out_width) p.mass_out[bh * p.out_width + i] = src < 0 ? 0.f : p.mass[bh * p.mass_width + src];
+  }
+  __syncthreads();
+  if (i0 >= p.budget) return;
+  uint4* kp = (uint4*)c.k;
+  uint4* vp = (uint4*)c.v;
+  for (int e = tid; e < kMovePlaces * pieces; e += blockDim.x) {
+    const int place = e / pieces, piece = e - place * pieces;
+    if (from[0][place] < 0) continue;
+    const uint4 a = kp[from[0][place] + piece], v = vp[from[1][place] + piece];
+    kp[to[0][place] + piece] = a;
+    vp[to[1][place] + piece] = v;
   }
 }
 

@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
@@ -13,6 +14,7 @@
 #include "common.cuh"
 #include "logits.cuh"
 #include "paged.cuh"
+#include "paged_attn.cuh"
 
 using namespace one;
 
@@ -32,23 +34,67 @@ int fail(int code, const char* fmt, ...) {
   return one_set_error(code, buf);
 }
 
-template <typename... KArgs, typename... Args>
-cudaError_t launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args&&... args) {
+bool use_pdl() {
   static const bool pdl = [] {
     const char* v = getenv("ONE_B200_NO_PDL");
     return !(v && v[0] == '1');
   }();
+  return pdl;
+}
+
+// Launches with programmatic stream serialization, as clusters of `cluster` CTAs.
+template <typename... KArgs, typename... Args>
+cudaError_t launch_cluster(unsigned cluster, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
+                           cudaStream_t st, Args&&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (use_pdl()) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = cluster;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
   cfg.attrs = attr;
-  cfg.numAttrs = pdl ? 1 : 0;
+  cfg.numAttrs = n;
   return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+}
+
+template <typename... KArgs, typename... Args>
+cudaError_t launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args&&... args) {
+  return launch_cluster(1, kernel, grid, block, smem, st, std::forward<Args>(args)...);
+}
+
+// cudaFuncAttributeMaxDynamicSharedMemorySize of a kernel, once per device.
+constexpr int kMaxDevices = 64;
+template <typename K>
+int allow_smem(K* kernel, int bytes, std::atomic<bool> (&done)[kMaxDevices]) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && dev < kMaxDevices && done[dev].load(std::memory_order_acquire)) return ONE_OK;
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return fail(ONE_ERR_CUDA, "shared memory of a kernel: %s", cudaGetErrorString(e));
+  if (dev < kMaxDevices) done[dev].store(true, std::memory_order_release);
+  return ONE_OK;
+}
+
+// SMs of the current device.
+int num_sms() {
+  static std::atomic<int> sms[kMaxDevices];
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+  if (dev < kMaxDevices && (n = sms[dev].load(std::memory_order_relaxed)) > 0) return n;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1) return 148;
+  if (dev < kMaxDevices) sms[dev].store(n, std::memory_order_relaxed);
+  return n;
 }
 
 int elem_bytes(int dtype) { return dtype == ONE_DTYPE_F32 ? 4 : 2; }
@@ -83,9 +129,66 @@ int launched(cudaError_t e, const char* what) {
 
 }  // namespace
 
+namespace {
+
+constexpr int kMaxSms = 160;  // the workspace's bound on the SMs that share a list
+constexpr int kJoinTiles = 8;  // caches of at most this many tiles are not split
+
+size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
+
+// Query heads that one pass over a kv head's cache serves.
+int paged_rows(int dtype, int G) { return dtype == ONE_DTYPE_F32 ? 4 : G > 8 ? 16 : 8; }
+
+struct PagedWs {
+  size_t part_ml, part_o, row_ml, scores, total;
+  int64_t score_ld;
+  PagedWs(int b, int hq, int rows, int dh_pad, int64_t slots, bool mass) {
+    const size_t parts = 2 * (size_t)kMaxSms * kPaPerSm * rows;
+    part_ml = 0;
+    part_o = align256(parts * 8);
+    row_ml = part_o + align256(parts * dh_pad * 4);
+    scores = row_ml + align256(mass ? (size_t)b * hq * 8 : 0);
+    score_ld = (slots + kPaTile - 1) / kPaTile * kPaTile;
+    total = scores + (mass ? (size_t)b * hq * score_ld * 4 : 0);
+  }
+};
+
+int pad_dh(int dh) { return dh <= 32 ? 32 : dh <= 64 ? 64 : dh <= 96 ? 96 : 128; }
+
+template <typename E>
+int attend_split(PagedAttn& p, cudaStream_t st) {
+  static std::atomic<bool> done[kMaxDevices];
+  int rc = allow_smem(paged_attn_kernel<E, true>, PaSmem<E>::kTotal, done);
+  if (rc) return rc;
+  p.ranges = std::min(num_sms(), kMaxSms) * std::min(kPaPerSm, (int)(kSmPerSm / (PaSmem<E>::kTotal + 1024)));
+  rc = launched(launch(paged_attn_kernel<E, true>, dim3(p.ranges), dim3(kPaWarps * 32), PaSmem<E>::kTotal, st, p),
+                "paged attention");
+  if (rc) return rc;
+  const int64_t joins = (int64_t)p.c.B * p.c.Hkv * p.G + (p.mass ? p.ranges : 0);
+  return launched(launch(paged_join_kernel<E>, dim3((unsigned)joins), dim3(128), 0, st, p), "paged attention join");
+}
+
+template <typename E>
+int attend_whole(PagedAttn& p, cudaStream_t st) {
+  static std::atomic<bool> done[kMaxDevices];
+  int rc = allow_smem(paged_attn_kernel<E, false>, PaSmem<E>::kTotal, done);
+  if (rc) return rc;
+  return launched(launch(paged_attn_kernel<E, false>, dim3(p.c.Hkv * p.hv_per_kv, p.c.B), dim3(kPaWarps * 32),
+                         PaSmem<E>::kTotal, st, p),
+                  "paged attention");
+}
+
+template <typename E>
+int attend(PagedAttn& p, bool split, cudaStream_t st) {
+  return split ? attend_split<E>(p, st) : attend_whole<E>(p, st);
+}
+
+}  // namespace
+
 extern "C" size_t one_paged_attention_workspace_bytes(int32_t b, int32_t hq, int32_t hkv, int32_t dh, int32_t page_size,
                                                       int32_t max_pages, int32_t dtype, int32_t with_mass) {
-  return 1024;
+  if (b < 1 || hq < 1 || hkv < 1 || dh < 1 || page_size < 1 || max_pages < 1) return 0;
+  return PagedWs(b, hq, paged_rows(dtype, hq / hkv), pad_dh(dh), (int64_t)max_pages * page_size, with_mass != 0).total + 256;
 }
 
 extern "C" int one_paged_attention(const void* q, int64_t q_batch_stride, int64_t q_head_stride, const void* k_pages,
@@ -95,23 +198,58 @@ extern "C" int one_paged_attention(const void* q, int64_t q_batch_stride, int64_
                                    int32_t dtype, float* mass, int64_t mass_width, void* out, void* workspace,
                                    size_t workspace_bytes, void* stream) {
   if (!q || !out || !workspace) return fail(ONE_ERR_INVALID, "paged attention: null argument");
-  PagedAttnParams p = {};
+  PagedAttn p = {};
   int rc = check_cache(p.c, const_cast<void*>(k_pages), const_cast<void*>(v_pages), k_page_stride, v_page_stride, num_pages,
                        page_size, block_table, table_stride, max_pages, lengths, b, hkv, dh, dtype);
   if (rc) return rc;
   if (hq < 1 || hq % hkv) return fail(ONE_ERR_INVALID, "paged attention: the query heads must be a multiple of the kv heads");
-  if (mass && mass_width < (int64_t)max_pages * page_size)
+  const int64_t slots = (int64_t)max_pages * page_size;
+  if (mass && mass_width < slots)
     return fail(ONE_ERR_INVALID, "paged attention: mass rows are shorter than the block table's slots");
+  if ((int64_t)b * hq > 0x3fffffff) return fail(ONE_ERR_UNSUPPORTED, "paged attention: too many rows");
   if (workspace_bytes < one_paged_attention_workspace_bytes(b, hq, hkv, dh, page_size, max_pages, dtype, mass != nullptr))
     return fail(ONE_ERR_INVALID, "workspace too small");
   p.q = q; p.q_bs = q_batch_stride; p.q_hs = q_head_stride; p.G = hq / hkv;
+  const int rows = paged_rows(dtype, p.G);
+  p.hv_per_kv = (p.G + rows - 1) / rows;
+  p.q_vec = (reinterpret_cast<uintptr_t>(q) & 15) == 0 && q_batch_stride % 8 == 0 && q_head_stride % 8 == 0;
+  while ((1 << p.div_s) < page_size) ++p.div_s;
+  p.div_m = (uint32_t)((1ull << (31 + p.div_s)) / page_size + 1);
+  p.div_s += 31;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.mass = mass; p.mass_width = mass_width; p.out = out;
-  const dim3 grid(hkv, b);
-  return launched(dtype == ONE_DTYPE_BF16
-                      ? launch(paged_attn_simple_kernel<__nv_bfloat16>, grid, dim3(256), 0, (cudaStream_t)stream, p)
-                      : launch(paged_attn_simple_kernel<float>, grid, dim3(256), 0, (cudaStream_t)stream, p),
-                  "paged attention");
+  const PagedWs w(b, hq, rows, pad_dh(dh), slots, mass != nullptr);
+  uint8_t* ws = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(workspace) + 255) & ~uintptr_t(255));
+  p.part_ml = reinterpret_cast<float*>(ws + w.part_ml);
+  p.part_o = reinterpret_cast<float*>(ws + w.part_o);
+  p.row_ml = reinterpret_cast<float*>(ws + w.row_ml);
+  p.scores = mass ? reinterpret_cast<float*>(ws + w.scores) : nullptr;
+  p.score_ld = w.score_ld;
+  const bool split = slots > kJoinTiles * kPaTile || (mass && p.hv_per_kv > 1);
+  cudaStream_t st = (cudaStream_t)stream;
+  const int d = pad_dh(dh);
+  if (dtype == ONE_DTYPE_F32) {
+    switch (d) {
+      case 32: return attend<PaF32<32>>(p, split, st);
+      case 64: return attend<PaF32<64>>(p, split, st);
+      case 96: return attend<PaF32<96>>(p, split, st);
+      default: return attend<PaF32<128>>(p, split, st);
+    }
+  }
+  if (rows == 16) {
+    switch (d) {
+      case 32: return attend<PaBf16<32, true>>(p, split, st);
+      case 64: return attend<PaBf16<64, true>>(p, split, st);
+      case 96: return attend<PaBf16<96, true>>(p, split, st);
+      default: return attend<PaBf16<128, true>>(p, split, st);
+    }
+  }
+  switch (d) {
+    case 32: return attend<PaBf16<32, false>>(p, split, st);
+    case 64: return attend<PaBf16<64, false>>(p, split, st);
+    case 96: return attend<PaBf16<96, false>>(p, split, st);
+    default: return attend<PaBf16<128, false>>(p, split, st);
+  }
 }
 
 extern "C" int one_paged_append(const void* k, int64_t k_batch_stride, int64_t k_head_stride, int64_t k_token_stride,
@@ -138,12 +276,22 @@ extern "C" int one_paged_append(const void* k, int64_t k_batch_stride, int64_t k
   p.qs[0] = q_batch_stride; p.qs[1] = q_head_stride; p.qs[2] = q_token_stride;
   p.cosv = cosv; p.sinv = sinv; p.cos_bs = cos_batch == 1 ? 0 : (int64_t)n * dh; p.counts = counts;
   p.mass = mass; p.mass_width = mass_width; p.q_out = q_out; p.N = n; p.Hq = hq;
-  const int64_t blocks = ((int64_t)b * n * (2 * hkv + (q ? hq : 0)) + 7) / 8;
-  if (blocks > 0x7fffffff) return fail(ONE_ERR_UNSUPPORTED, "paged append: too many rows");
-  const dim3 grid((unsigned)blocks);
-  return launched(dtype == ONE_DTYPE_BF16
-                      ? launch(paged_append_simple_kernel<__nv_bfloat16>, grid, dim3(256), 0, (cudaStream_t)stream, p)
-                      : launch(paged_append_simple_kernel<float>, grid, dim3(256), 0, (cudaStream_t)stream, p),
+  // 16-byte pieces need aligned rows and halves of whole pieces; anything else goes element by element
+  const int64_t unit = 16 / elem_bytes(dtype);
+  auto aligned = [&](const void* x, const int64_t* s) {
+    return (reinterpret_cast<uintptr_t>(x) & 15) == 0 && s[0] % unit == 0 && s[1] % unit == 0 && s[2] % unit == 0;
+  };
+  const bool vec = dh % 16 == 0 && aligned(k, p.ks) && aligned(v, p.vs) && (!q || aligned(q, p.qs)) &&
+                   ((reinterpret_cast<uintptr_t>(q_out) | reinterpret_cast<uintptr_t>(cosv) | reinterpret_cast<uintptr_t>(sinv)) & 15) == 0;
+  const int64_t threads = (int64_t)n * (2 * (int64_t)hkv + (q ? hq : 0)) * (vec ? dh / 16 : 32);
+  if (threads > 0x7fffffff) return fail(ONE_ERR_UNSUPPORTED, "paged append: too many rows");
+  const dim3 grid((unsigned)((threads + 255) / 256), b);
+  cudaStream_t st = (cudaStream_t)stream;
+  const bool bf = dtype == ONE_DTYPE_BF16;
+  return launched(vec ? bf ? launch(paged_append_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, p)
+                           : launch(paged_append_kernel<float>, grid, dim3(256), 0, st, p)
+                      : bf ? launch(paged_append_any_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, p)
+                           : launch(paged_append_any_kernel<float>, grid, dim3(256), 0, st, p),
                   "paged append");
 }
 
@@ -164,17 +312,32 @@ extern "C" int one_paged_evict(void* k_pages, void* v_pages, int64_t k_page_stri
     return fail(ONE_ERR_INVALID, "paged evict: the destination pages hold fewer slots than the budget");
   if (mass_width < (int64_t)max_pages * page_size || mass_out_width < budget)
     return fail(ONE_ERR_INVALID, "paged evict: mass rows are too short");
-  if ((int64_t)b * hkv > 65535 || mass_out_width > 0x3fffffff) return fail(ONE_ERR_UNSUPPORTED, "paged evict: too many rows");
+  const int64_t per_bh = (mass_out_width + kMovePlaces - 1) / kMovePlaces;
+  if (mass_out_width > 0x3fffffff || per_bh * b * hkv > 0x7fffffff)
+    return fail(ONE_ERR_UNSUPPORTED, "paged evict: too many rows");
   p.dst = dst_table; p.dst_stride = dst_stride; p.mass = mass; p.mass_width = mass_width;
   p.budget = budget; p.recent = recent; p.sink = sink; p.mass_out = mass_out; p.out_width = mass_out_width; p.kept = kept;
   cudaStream_t st = (cudaStream_t)stream;
-  rc = launched(launch(paged_select_simple_kernel, dim3(hkv, b), dim3(256), 0, st, p), "paged select");
+  static std::atomic<bool> done[kMaxDevices];
+  if ((rc = allow_smem(paged_select_kernel, kSelCached * 4, done))) return rc;
+  const int cached = (int)std::min<int64_t>((int64_t)max_pages * page_size, kSelCached);
+  rc = launched(launch(paged_select_kernel, dim3(b * hkv), dim3(kSelThreads), cached * 4, st, p, cached), "paged select");
   if (rc) return rc;
-  const dim3 grid((unsigned)((mass_out_width + 7) / 8), b * hkv);
-  return launched(dtype == ONE_DTYPE_BF16 ? launch(paged_move_simple_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, p)
-                                          : launch(paged_move_simple_kernel<float>, grid, dim3(256), 0, st, p),
+  return launched(launch(paged_move_kernel, dim3((unsigned)(per_bh * b * hkv)), dim3(256), 0, st, p, (int)per_bh,
+                         dh * elem_bytes(dtype) / 16),
                   "paged move");
 }
+
+namespace {
+
+template <typename T, typename I>
+cudaError_t logits_launch(const LogitsParams& p, bool vec, int slice, int ctas, size_t smem, cudaStream_t st) {
+  const dim3 grid((unsigned)p.B * ctas), block(kLogitsThreads);
+  return vec ? launch_cluster(ctas, logits_kernel<T, I, true>, grid, block, smem, st, p, slice, ctas)
+             : launch_cluster(ctas, logits_kernel<T, I, false>, grid, block, smem, st, p, slice, ctas);
+}
+
+}  // namespace
 
 extern "C" int one_process_logits(const void* logits, int64_t ld, int32_t batch, int32_t vocab, int32_t dtype,
                                   const void* history, int64_t hist_ld, int32_t hist_len, int32_t hist_bytes,
@@ -198,11 +361,25 @@ extern "C" int one_process_logits(const void* logits, int64_t ld, int32_t batch,
   p.bias = bias; p.bias_ld = bias_ld; p.mask = reinterpret_cast<const uint32_t*>(token_mask); p.mask_ld = mask_ld;
   p.out = out; p.out_ld = out_ld; p.best = best;
   cudaStream_t st = (cudaStream_t)stream;
-  const dim3 grid(batch), block(512);
+  // enough CTAs per row (at most a portable cluster) to cover the SMs, with a few tokens per thread each
+  int ctas = 1;
+  while (ctas < 8 && (int64_t)batch * ctas < 4 * num_sms() && vocab > ctas * kLogitsThreads * 8) ctas *= 2;
+  const int slice = ((vocab + ctas - 1) / ctas + 31) / 32 * 32;
+  if ((int64_t)batch * ctas > 0x7fffffff) return fail(ONE_ERR_UNSUPPORTED, "process logits: too many rows");
+  const size_t smem = hist_len ? (size_t)std::min(slice, kLogitsCounts) * 4 : 0;
+  auto a16 = [](const void* x, int64_t row_bytes) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0 && row_bytes % 16 == 0; };
+  const bool vec = vocab % 8 == 0 && a16(logits, ld * elem_bytes(dtype)) && a16(out, out_ld * 4) && a16(bias, bias_ld * 4);
   const bool bf = dtype == ONE_DTYPE_BF16, wide = hist_bytes == 8;
-  return launched(bf ? wide ? launch(logits_simple_kernel<__nv_bfloat16, int64_t>, grid, block, 0, st, p)
-                            : launch(logits_simple_kernel<__nv_bfloat16, int32_t>, grid, block, 0, st, p)
-                     : wide ? launch(logits_simple_kernel<float, int64_t>, grid, block, 0, st, p)
-                            : launch(logits_simple_kernel<float, int32_t>, grid, block, 0, st, p),
-                  "process logits");
+  int rc = ONE_OK;
+  static std::atomic<bool> done[8][kMaxDevices];
+  auto run = [&](auto t, auto i, int at) -> int {
+    using T = decltype(t);
+    using I = decltype(i);
+    if ((rc = allow_smem(logits_kernel<T, I, true>, kLogitsCounts * 4, done[at])) ||
+        (rc = allow_smem(logits_kernel<T, I, false>, kLogitsCounts * 4, done[at + 4])))
+      return rc;
+    return launched(logits_launch<T, I>(p, vec, slice, ctas, smem, st), "process logits");
+  };
+  if (bf) return wide ? run(__nv_bfloat16(), int64_t(0), 0) : run(__nv_bfloat16(), int32_t(0), 1);
+  return wide ? run(float(0), int64_t(0), 2) : run(float(0), int32_t(0), 3);
 }
