@@ -6,27 +6,27 @@
 // One pass over K and V with the running maximum and sum; parts of a sequence join by their (m, l, o).
 // HBM bounds it: every K and V row is read once, at 1 flop per byte and query head of a group.
 //
-// Partition. The work is the list of 64-slot tiles of every (sequence, query-head tile) in order; a
+// Partition. The work is the list of tiles (64 slots or more) of every (sequence, query-head tile) in order; a
 // grid that fills the GPU takes equal shares of that list, whatever the lengths, so a ragged batch
 // and a single long sequence keep all SMs busy. A share is a run of pieces of segments (a segment:
 // one sequence's tiles for one query-head tile). A piece that is its whole segment is finished on the
 // spot; the others leave (m, l, o) in the workspace, and paged_join_kernel joins them in a fixed
 // order (no atomics: equal inputs give equal bits).
 //
-// Inside a CTA, each of four warps owns 16 slots of a tile and a ring of stages in shared memory
-// that cp.async fills with the lane's own matrix fragments: no lane reads what another one
-// copied, so the ring needs no barrier, and bytes in flight do not cost registers. The ring runs
-// across segment boundaries.
+// Inside a CTA, each of four warps owns a quarter of a tile (groups of 16 slots) and a ring of stages
+// in shared memory that its own cp.async fill in the order of the matrix fragments: the ring needs no
+// barrier between warps, bytes in flight do not cost registers, and it runs across segment boundaries.
 #pragma once
+
+#include <utility>
 
 #include "paged.cuh"
 
 namespace one {
 
 constexpr int kPaWarps = 4;
-constexpr int kPaTile = 16 * kPaWarps;  // slots per tile
 constexpr size_t kSmPerSm = 228 * 1024;    // shared memory of an SM, 1 KB of it per CTA reserved
-constexpr int kPaPerSm = 4;             // CTAs of these kernels on an SM, at most
+constexpr int kPaPerSm = 3;             // CTAs of these kernels on an SM, at most
 
 struct PagedAttn {
   PagedCache c;
@@ -45,67 +45,89 @@ struct PagedAttn {
   float* row_ml;          // [B * Hq][2], of segments in one piece
   float* scores;          // [B * Hq][score_ld], log2 domain
   int64_t score_ld;
+  long long* before;      // [B + 1]: tiles of one query-head tile before each sequence; the list's length
   int ranges;             // CTAs that share the list
+  int split;
 };
 
-ONE_DEVINL int pa_tiles(const PagedCache& c, int b) { return (paged_length(c, b, SITE_PAGED_ATTN) + kPaTile - 1) / kPaTile; }
+template <int TILE>
+ONE_DEVINL int pa_tiles(const PagedCache& c, int b) {
+  return (paged_length(c, b, SITE_PAGED_ATTN) + TILE - 1) / TILE;
+}
 
 // The list's length and a position in it. Every warp computes them for itself.
+template <int TILE>
 ONE_DEVINL long long pa_total(const PagedAttn& p) {
   long long n = 0;
-  for (int b = threadIdx.x & 31; b < p.c.B; b += 32) n += pa_tiles(p.c, b);
+  for (int b = threadIdx.x & 31; b < p.c.B; b += 32) n += pa_tiles<TILE>(p.c, b);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
   return n * p.c.Hkv * p.hv_per_kv;
 }
-// Tiles (of one query-head tile) of the sequences before `upto`.
-ONE_DEVINL long long pa_before(const PagedAttn& p, int upto) {
-  long long n = 0;
-  for (int b = threadIdx.x & 31; b < upto; b += 32) n += pa_tiles(p.c, b);
+// Tiles (of one query-head tile) of the sequences before each, into p.before, by one warp.
+template <int TILE>
+ONE_DEVINL void pa_write_before(const PagedAttn& p) {
+  const int lane = threadIdx.x & 31;
+  long long run = 0;
+  for (int base = 0; base < p.c.B; base += 32) {
+    const int n = base + lane < p.c.B ? pa_tiles<TILE>(p.c, base + lane) : 0;
+    long long incl = n;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-  return n;
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long t = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += t;
+    }
+    if (base + lane < p.c.B) p.before[base + lane] = run + incl - n;
+    run += __shfl_sync(0xffffffffu, incl, 31);
+  }
 }
 ONE_DEVINL long long pa_chunk(const PagedAttn& p, long long total) { return max(1ll, (total + p.ranges - 1) / p.ranges); }
 
-// A place in the list: tile `tile` of query-head tile hv of sequence b.
+// A place in the list: tile `tile` of query-head tile gi of kv head kv of sequence b; the heads' tiles
+// of a sequence follow one another, ng query-head tiles per kv head.
+template <int TILE>
 struct PaCursor {
-  int b, hv, tile, tiles, len;
+  int b, kv, gi, tile, tiles, len;
   ONE_DEVINL void load(const PagedCache& c) {
     len = b < c.B ? paged_length(c, b, SITE_PAGED_ATTN) : 0;
-    tiles = (len + kPaTile - 1) / kPaTile;
+    tiles = (len + TILE - 1) / TILE;
   }
-  ONE_DEVINL void seek(const PagedCache& c, int HV, long long w) {
+  ONE_DEVINL void seek(const PagedCache& c, int ng, long long w) {
+    const long long HV = (long long)c.Hkv * ng;
     const int lane = threadIdx.x & 31;
     long long run = 0;
     for (int base = 0; base < c.B; base += 32) {
-      const int n = base + lane < c.B ? pa_tiles(c, base + lane) : 0;
+      const int n = base + lane < c.B ? pa_tiles<TILE>(c, base + lane) : 0;
       long long incl = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const long long t = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o) incl += t;
       }
-      const unsigned hit = __ballot_sync(0xffffffffu, w < (long long)HV * (run + incl));
+      const unsigned hit = __ballot_sync(0xffffffffu, w < HV * (run + incl));
       if (hit) {
         const int src = __ffs(hit) - 1;
         b = base + src;
-        const long long first = (long long)HV * (run + __shfl_sync(0xffffffffu, incl - n, src));
+        w -= HV * (run + __shfl_sync(0xffffffffu, incl - n, src));
         load(c);
-        hv = (int)((w - first) / tiles);
-        tile = (int)((w - first) % tiles);
+        const int hv = (int)(w / tiles);
+        tile = (int)(w % tiles);
+        kv = hv / ng;
+        gi = hv % ng;
         return;
       }
       run += __shfl_sync(0xffffffffu, incl, 31);
     }
     b = c.B;
-    hv = tile = tiles = len = 0;
+    kv = gi = tile = tiles = len = 0;
   }
-  ONE_DEVINL void next(const PagedCache& c, int HV) {
+  ONE_DEVINL void next(const PagedCache& c, int ng) {
     if (++tile < tiles) return;
     tile = 0;
-    if (++hv < HV) return;
-    hv = 0;
+    if (++gi < ng) return;
+    gi = 0;
+    if (++kv < c.Hkv) return;
+    kv = 0;
     do {
       ++b;
       load(c);
@@ -117,8 +139,19 @@ struct PaCursor {
 ONE_DEVINL void cp_async16_or_zero(void* smem, const void* gmem, bool there) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(smem)), "l"(gmem), "r"(there ? 16 : 0) : "memory");
 }
-ONE_DEVINL void cp_async8_or_zero(void* smem, const void* gmem, bool there) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(smem_u32(smem)), "l"(gmem), "r"(there ? 8 : 0) : "memory");
+// 16 bytes from g + GO to shared address s + SO; the offsets are part of the instruction
+template <int SO, int GO>
+ONE_DEVINL void cp_async16_at(uint32_t s, const void* g) {
+  asm volatile("cp.async.cg.shared.global [%0 + %2], [%1 + %3], 16;" ::"r"(s), "l"(g), "n"(SO), "n"(GO) : "memory");
+}
+// f(0), f(1), .. as compile-time constants
+template <typename F, int... I>
+ONE_DEVINL void static_for_impl(F&& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+ONE_DEVINL void static_for(F&& f) {
+  static_for_impl(f, std::make_integer_sequence<int, N>{});
 }
 ONE_DEVINL void mma_bf16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -127,15 +160,58 @@ ONE_DEVINL void mma_bf16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// The copies of a group's 16 rows, in pieces of 16 bytes, CH of them per row. Consecutive lanes take
+// consecutive pieces, and D::at(row, piece), where a piece goes, keeps a 128-byte line of a row in one
+// 128-byte line of shared memory with its pieces permuted, which spreads the fragments' reads over
+// the banks. (Pieces that go to lines of their own are asked for one by one, and each 32-byte sector
+// twice: that read 1.5 times the bytes into the SMs and took 96 us where this takes 80, at 64 x 4096
+// ragged tokens.) D::at is linear over exclusive or, so the unrolled loop splits it into a lane's
+// constant and a compile-time one.
+template <typename D, int CH>
+struct PaCopy {
+  static constexpr int N = 16 * CH / 32;
+  // rows that follow one another in memory, the first `live` of them in use, `pieces` of CH there
+  template <bool FULL>
+  ONE_DEVINL static void run(uint8_t* to, const uint8_t* from, int live, int pieces) {
+    const int lane = threadIdx.x & 31;
+    if (FULL && live == 16 && 32 % CH == 0) {
+      const uint32_t s = smem_u32(to), mine = D::at(lane / CH, lane % CH);
+      const uint8_t* g = from + lane * 16;
+      static_for<N>([&](auto n) {
+        constexpr int k = decltype(n)::value, at = D::at(k * 32 / CH, 0);
+        cp_async16_at<(at & ~127), k * 512>(s + (mine ^ (at & 127)), g);
+      });
+      return;
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int e = k * 32 + lane, row = e / CH, ch = e % CH;
+      cp_async16_or_zero(to + D::at(row, ch), from + (FULL ? e : row * pieces + ch) * 16, row < live && (FULL || ch < pieces));
+    }
+  }
+  // rows anywhere: lane first + t holds the byte offset of row t, or -1
+  ONE_DEVINL static void any(uint8_t* to, const uint8_t* base, int64_t off, int first, int pieces) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int e = k * 32 + lane, row = e / CH, ch = e % CH;
+      const int64_t at = __shfl_sync(0xffffffffu, off, first + row);
+      const bool there = at >= 0 && ch < pieces;
+      cp_async16_or_zero(to + D::at(row, ch), base + (there ? at + ch * 16 : 0), there);
+    }
+  }
+};
+
 // ------------------------------------------------------------------ bf16: matrix instructions
 // m16n8k16 with the query heads as the 16 rows. Sums over the head dim and over slots do not depend
-// on the order of their terms, so the fragments are assigned to make every copy a lane's own 16
-// bytes (r = lane / 4, c = lane % 4):
-//   S = Q K^T  the lane's B operand for key column r is chunk c + 4 i of a key row, as it lies in
+// on the order of their terms, so the fragments are assigned to make every shared-memory access a
+// lane's own 16 bytes (r = lane / 4, c = lane % 4):
+//   S = Q K^T  the lane's B operand for key column r is pieces c + 4 i of a key row, as they lie in
 //              memory; Q is read the same way. Column r of key tile j is slot 4 (r / 2) + 2 j + r % 2,
 //   O += P V   so that the lane's four scores are slots 4 c .. 4 c + 3, and its B operand pairs
-//              those four value rows: chunk r (+ 8 i) of each, interleaved in registers. Column r of
-//              value tile j is dim 8 r + j.
+//              those four value rows: piece r (+ 8 i) of each, interleaved in registers. Column r of
+//              value tile j is dim 8 r + j. The last 32 dims of DH = 32 and 96 go by half pieces:
+//              dim 4 r + j.
 // P enters as a bf16 high part plus the bf16 rounding of the remainder (16 significant bits; bf16
 // alone would double the output's rounding error). Up to 8 query heads take rows 0-7 and the low
 // parts ride in rows 8-15 of the same instruction; 9 to 16 heads (WIDE) take a second instruction.
@@ -146,40 +222,41 @@ struct PaBf16 {
   static constexpr int KC = DH / 32;                   // 16-byte chunks of a key row per lane
   static constexpr int VC = DH / 64, VH = DH % 64 / 32;  // 16-byte and 8-byte pieces of a value row per lane
   static constexpr int NT = DH / 8;                    // value tiles
-  static constexpr int kStage = 64 * DH;               // bytes per warp
-  static constexpr int kStages = DH == 32 ? 6 : DH == 64 ? (WIDE ? 3 : 4) : DH == 96 ? (WIDE ? 3 : 4) : (WIDE ? 2 : 3);
+  static constexpr int kGroups = DH <= 64 ? 128 / DH : 1;  // 16-slot groups per warp and step
+  static constexpr int TILE = 16 * kGroups * kPaWarps;
+  static constexpr int kGroup = 64 * DH;               // bytes of a group's keys and values
+  static constexpr int kStages = 2;
   static constexpr int kExtra = 0;                     // further shared bytes per warp
   uint32_t qa[WIDE ? 2 : 1][KC][4];
   float o[NT][4];
   float m[2], l[2];  // rows r and r + 8
 
-  ONE_DEVINL static void issue(const PagedAttn& p, uint8_t* stage, int64_t off, int chunks) {
-    const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-    const T* kb = (const T*)p.c.k;
-    const T* vb = (const T*)p.c.v;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int64_t at = __shfl_sync(0xffffffffu, off, 4 * (r >> 1) + 2 * j + (r & 1));
-#pragma unroll
-      for (int i = 0; i < KC; ++i) {
-        const bool there = at >= 0 && c + 4 * i < chunks;
-        cp_async16_or_zero(stage + ((j * KC + i) * 32 + lane) * 16, kb + (there ? at + (c + 4 * i) * 8 : 0), there);
-      }
+  static constexpr int CH = DH / 8;                    // pieces of a row
+  // piece ch of row `row`: by lines of 64 dims, then the last 32 dims
+  struct KTo {
+    __host__ __device__ static constexpr int at(int row, int ch) {
+      return ch < 8 * VC ? (ch >> 3) * 2048 + row * 128 + ((ch & 7) ^ (row & 1) << 2) * 16 : VC * 2048 + row * 64 + (ch - 8 * VC) * 16;
     }
-    uint8_t* vs = stage + 32 * DH;
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const int64_t at = __shfl_sync(0xffffffffu, off, 16 + 4 * c + t);
-#pragma unroll
-      for (int i = 0; i < VC; ++i) {
-        const bool there = at >= 0 && r + 8 * i < chunks;
-        cp_async16_or_zero(vs + ((t * VC + i) * 32 + lane) * 16, vb + (there ? at + (r + 8 * i) * 8 : 0), there);
-      }
-      if (VH) {
-        const bool there = at >= 0 && 8 * VC + r / 2 < chunks;
-        cp_async8_or_zero(vs + VC * 2048 + (t * 32 + lane) * 8, vb + (there ? at + VC * 64 + r * 4 : 0), there);
-      }
+  };
+  struct VTo {
+    __host__ __device__ static constexpr int at(int row, int ch) {
+      return ch < 8 * VC ? (ch >> 3) * 2048 + row * 128 + ((ch & 7) ^ row >> 2 << 1) * 16
+                         : VC * 2048 + ((row & 3) * 4 + (row >> 2)) * 64 + ((ch - 8 * VC) ^ row >> 3 << 1) * 16;
     }
+  };
+  // 16 slots that lie in one page, the first `live` of them in use; kat, vat: element offsets of the
+  // first. FULL: Dh is DH.
+  template <bool FULL>
+  ONE_DEVINL static void issue_run(const PagedAttn& p, uint8_t* stage, int64_t kat, int64_t vat, int live) {
+    PaCopy<KTo, CH>::template run<FULL>(stage, (const uint8_t*)((const T*)p.c.k + kat), live, p.c.Dh / 8);
+    PaCopy<VTo, CH>::template run<FULL>(stage + 32 * DH, (const uint8_t*)((const T*)p.c.v + vat), live, p.c.Dh / 8);
+  }
+  // 16 slots anywhere: lane t holds the element offset of slot t's key, lane 16 + t that of its value,
+  // or -1.
+  ONE_DEVINL static void issue_any(const PagedAttn& p, uint8_t* stage, int64_t off) {
+    const int64_t at = off < 0 ? -1 : off * (int)sizeof(T);
+    PaCopy<KTo, CH>::any(stage, (const uint8_t*)p.c.k, at, 0, p.c.Dh / 8);
+    PaCopy<VTo, CH>::any(stage + 32 * DH, (const uint8_t*)p.c.v, at, 16, p.c.Dh / 8);
   }
 
   ONE_DEVINL void begin(const PagedAttn& p, uint8_t*, const T* q, int rows) {
@@ -207,35 +284,59 @@ struct PaBf16 {
     for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
   }
 
-  // 16 slots; `live`: a bit per slot. scores: row 0's scores of these slots, or null.
-  ONE_DEVINL void consume(const PagedAttn& p, const uint8_t* stage, uint32_t live, float* scores, int rows) {
+  // kGroups x 16 slots; live: a bit per slot of each group. scores: row 0's scores of these slots, or
+  // null.
+  ONE_DEVINL void consume(const PagedAttn& p, const uint8_t* stage, const uint32_t (&live)[kGroups], float* scores, int rows) {
     const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-    float s[2][4];
+    constexpr int RW = WIDE ? 2 : 1;
+    float pr[kGroups][RW][4];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+    for (int g = 0; g < kGroups; ++g) {
+      float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+      if (live[g]) {
 #pragma unroll
-      for (int i = 0; i < KC; ++i) {
-        const uint4 k = *reinterpret_cast<const uint4*>(stage + ((j * KC + i) * 32 + lane) * 16);
-        mma_bf16_16816(s[j], qa[0][i][0], WIDE ? qa[WIDE][i][0] : 0, qa[0][i][1], WIDE ? qa[WIDE][i][1] : 0, k.x, k.y);
-        mma_bf16_16816(s[j], qa[0][i][2], WIDE ? qa[WIDE][i][2] : 0, qa[0][i][3], WIDE ? qa[WIDE][i][3] : 0, k.z, k.w);
+        for (int i = 0; i < KC; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const uint4 k = *reinterpret_cast<const uint4*>(stage + g * kGroup + KTo::at(4 * (r >> 1) + 2 * j + (r & 1), c + 4 * i));
+            mma_bf16_16816(s[j], qa[0][i][0], WIDE ? qa[WIDE][i][0] : 0, qa[0][i][1], WIDE ? qa[WIDE][i][1] : 0, k.x, k.y);
+            mma_bf16_16816(s[j], qa[0][i][2], WIDE ? qa[WIDE][i][2] : 0, qa[0][i][3], WIDE ? qa[WIDE][i][3] : 0, k.z, k.w);
+          }
+      }
+#pragma unroll
+      for (int w = 0; w < RW; ++w)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) pr[g][w][t] = s[t >> 1][2 * w + (t & 1)] * p.scale_log2;
+      if (live[g] != 0xffffu) {
+        const uint32_t mine = live[g] >> (4 * c);
+#pragma unroll
+        for (int w = 0; w < RW; ++w)
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+            if (!(mine >> t & 1)) pr[g][w][t] = -INFINITY;
+      }
+      if (scores) {
+#pragma unroll
+        for (int w = 0; w < RW; ++w)
+          if (r + 8 * w < rows)
+            *reinterpret_cast<float4*>(scores + (r + 8 * w) * p.score_ld + 16 * g + 4 * c) =
+                make_float4(pr[g][w][0], pr[g][w][1], pr[g][w][2], pr[g][w][3]);
       }
     }
-    constexpr int RW = WIDE ? 2 : 1;
-    float mx[2], pr[RW][4];
-    const uint32_t mine = live >> (4 * c);
+    float mx[RW];
+    bool rises = false;
 #pragma unroll
     for (int w = 0; w < RW; ++w) {
+      mx[w] = pr[0][w][0];
 #pragma unroll
-      for (int t = 0; t < 4; ++t) pr[w][t] = mine >> t & 1 ? s[t >> 1][2 * w + (t & 1)] * p.scale_log2 : -INFINITY;
-      if (scores && r + 8 * w < rows)
-        *reinterpret_cast<float4*>(scores + (r + 8 * w) * p.score_ld + 4 * c) = make_float4(pr[w][0], pr[w][1], pr[w][2], pr[w][3]);
-      mx[w] = fmaxf(fmaxf(pr[w][0], pr[w][1]), fmaxf(pr[w][2], pr[w][3]));
+      for (int g = 0; g < kGroups; ++g) {
+        mx[w] = fmax3(mx[w], pr[g][w][0], pr[g][w][1]);
+        mx[w] = fmax3(mx[w], pr[g][w][2], pr[g][w][3]);
+      }
       mx[w] = fmaxf(mx[w], __shfl_xor_sync(0xffffffffu, mx[w], 1));
       mx[w] = fmaxf(mx[w], __shfl_xor_sync(0xffffffffu, mx[w], 2));
+      rises |= mx[w] > m[w];
     }
-    bool rises = mx[0] > m[0];
-    if (WIDE) rises |= mx[RW - 1] > m[1];
     if (__any_sync(0xffffffffu, rises)) {
       float a[2];
 #pragma unroll
@@ -251,52 +352,57 @@ struct PaBf16 {
         o[i][0] *= a[0]; o[i][1] *= a[0]; o[i][2] *= a[1]; o[i][3] *= a[1];
       }
     }
-    uint32_t hi[RW][2], lo[RW][2];
+    float ms[RW];
 #pragma unroll
-    for (int w = 0; w < RW; ++w) {
-      const float ms = m[w] == -INFINITY ? 0.f : m[w];
+    for (int w = 0; w < RW; ++w) ms[w] = m[w] == -INFINITY ? 0.f : m[w];
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        pr[w][t] = ex2_approx(pr[w][t] - ms);
-        l[w] += pr[w][t];
+    for (int g = 0; g < kGroups; ++g) {
+      if (!live[g]) continue;
+      uint32_t hi[RW][2], lo[RW][2];
+#pragma unroll
+      for (int w = 0; w < RW; ++w) {
+        float (&x)[4] = pr[g][w];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) x[t] = ex2_approx(x[t] - ms[w]);
+        l[w] += (x[0] + x[1]) + (x[2] + x[3]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          hi[w][h] = pack_bf16x2(x[2 * h], x[2 * h + 1]);
+          lo[w][h] = pack_bf16x2(x[2 * h] - bf2_lo(hi[w][h]), x[2 * h + 1] - bf2_hi(hi[w][h]));
+        }
       }
+      const uint8_t* vs = stage + g * kGroup + 32 * DH;
+      auto pv = [&](int tile, uint32_t b0, uint32_t b1) {
+        if (WIDE) {
+          mma_bf16_16816(o[tile], hi[0][0], hi[RW - 1][0], hi[0][1], hi[RW - 1][1], b0, b1);
+          mma_bf16_16816(o[tile], lo[0][0], lo[RW - 1][0], lo[0][1], lo[RW - 1][1], b0, b1);
+        } else {
+          mma_bf16_16816(o[tile], hi[0][0], lo[0][0], hi[0][1], lo[0][1], b0, b1);
+        }
+      };
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        hi[w][h] = pack_bf16x2(pr[w][2 * h], pr[w][2 * h + 1]);
-        lo[w][h] = pack_bf16x2(pr[w][2 * h] - bf2_lo(hi[w][h]), pr[w][2 * h + 1] - bf2_hi(hi[w][h]));
+      for (int i = 0; i < VC; ++i) {
+        uint4 v[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) v[t] = *reinterpret_cast<const uint4*>(vs + VTo::at(4 * c + t, r + 8 * i));
+        const uint32_t x[4][4] = {{v[0].x, v[0].y, v[0].z, v[0].w}, {v[1].x, v[1].y, v[1].z, v[1].w},
+                                  {v[2].x, v[2].y, v[2].z, v[2].w}, {v[3].x, v[3].y, v[3].z, v[3].w}};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          pv(8 * i + 2 * e, __byte_perm(x[0][e], x[1][e], 0x5410), __byte_perm(x[2][e], x[3][e], 0x5410));
+          pv(8 * i + 2 * e + 1, __byte_perm(x[0][e], x[1][e], 0x7632), __byte_perm(x[2][e], x[3][e], 0x7632));
+        }
       }
-    }
-    const uint8_t* vs = stage + 32 * DH;
-    auto pv = [&](int tile, uint32_t b0, uint32_t b1) {
-      if (WIDE) {
-        mma_bf16_16816(o[tile], hi[0][0], hi[RW - 1][0], hi[0][1], hi[RW - 1][1], b0, b1);
-        mma_bf16_16816(o[tile], lo[0][0], lo[RW - 1][0], lo[0][1], lo[RW - 1][1], b0, b1);
-      } else {
-        mma_bf16_16816(o[tile], hi[0][0], lo[0][0], hi[0][1], lo[0][1], b0, b1);
-      }
-    };
+      if (VH) {
+        uint2 v[4];
 #pragma unroll
-    for (int i = 0; i < VC; ++i) {
-      uint4 v[4];
+        for (int t = 0; t < 4; ++t) v[t] = *reinterpret_cast<const uint2*>(vs + VTo::at(4 * c + t, 8 * VC + (r >> 1)) + (r & 1) * 8);
+        const uint32_t x[4][2] = {{v[0].x, v[0].y}, {v[1].x, v[1].y}, {v[2].x, v[2].y}, {v[3].x, v[3].y}};
 #pragma unroll
-      for (int t = 0; t < 4; ++t) v[t] = *reinterpret_cast<const uint4*>(vs + ((t * VC + i) * 32 + lane) * 16);
-      const uint32_t x[4][4] = {{v[0].x, v[0].y, v[0].z, v[0].w}, {v[1].x, v[1].y, v[1].z, v[1].w},
-                                {v[2].x, v[2].y, v[2].z, v[2].w}, {v[3].x, v[3].y, v[3].z, v[3].w}};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        pv(8 * i + 2 * e, __byte_perm(x[0][e], x[1][e], 0x5410), __byte_perm(x[2][e], x[3][e], 0x5410));
-        pv(8 * i + 2 * e + 1, __byte_perm(x[0][e], x[1][e], 0x7632), __byte_perm(x[2][e], x[3][e], 0x7632));
-      }
-    }
-    if (VH) {
-      uint2 v[4];
-#pragma unroll
-      for (int t = 0; t < 4; ++t) v[t] = *reinterpret_cast<const uint2*>(vs + VC * 2048 + (t * 32 + lane) * 8);
-      const uint32_t x[4][2] = {{v[0].x, v[0].y}, {v[1].x, v[1].y}, {v[2].x, v[2].y}, {v[3].x, v[3].y}};
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        pv(8 * VC + 2 * e, __byte_perm(x[0][e], x[1][e], 0x5410), __byte_perm(x[2][e], x[3][e], 0x5410));
-        pv(8 * VC + 2 * e + 1, __byte_perm(x[0][e], x[1][e], 0x7632), __byte_perm(x[2][e], x[3][e], 0x7632));
+        for (int e = 0; e < 2; ++e) {
+          pv(8 * VC + 2 * e, __byte_perm(x[0][e], x[1][e], 0x5410), __byte_perm(x[2][e], x[3][e], 0x5410));
+          pv(8 * VC + 2 * e + 1, __byte_perm(x[0][e], x[1][e], 0x7632), __byte_perm(x[2][e], x[3][e], 0x7632));
+        }
       }
     }
   }
@@ -335,33 +441,32 @@ struct PaF32 {
   using T = float;
   static constexpr int DH = DH_, ROWS = 4;
   static constexpr int KC = DH / 16, VC = DH / 32;
-  static constexpr int kStage = 128 * DH;
+  static constexpr int kGroups = 1, TILE = 16 * kPaWarps;
+  static constexpr int kGroup = 128 * DH;
   static constexpr int kStages = DH == 32 ? 4 : DH == 96 ? 2 : 3;
   static constexpr int kExtra = 4 * DH * 4 + 16 * 16;  // q [4][DH], weights [16][4]
   float o[4][VC];
   float m, l;  // of head c
   float *qs, *ps;
 
-  ONE_DEVINL static void issue(const PagedAttn& p, uint8_t* stage, int64_t off, int chunks) {
-    const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-    const T* kb = (const T*)p.c.k;
-    const T* vb = (const T*)p.c.v;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int64_t at = __shfl_sync(0xffffffffu, off, r + 8 * j);
-#pragma unroll
-      for (int i = 0; i < KC; ++i) {
-        const bool there = at >= 0 && c + 4 * i < 2 * chunks;
-        cp_async16_or_zero(stage + ((j * KC + i) * 32 + lane) * 16, kb + (there ? at + (c + 4 * i) * 4 : 0), there);
-      }
+  static constexpr int CH = DH / 4;
+  struct KTo {
+    __host__ __device__ static constexpr int at(int row, int ch) {
+      return (ch >> 3) * 2048 + row * 128 + ((ch & 7) ^ (row & 1) << 2) * 16;
     }
-#pragma unroll
-    for (int i = 0; i < DH / 8; ++i) {
-      const int e = lane + 32 * i, t = e / (DH / 4), ch = e % (DH / 4);
-      const int64_t at = __shfl_sync(0xffffffffu, off, 16 + t);
-      const bool there = at >= 0 && ch < 2 * chunks;
-      cp_async16_or_zero(stage + 64 * DH + e * 16, vb + (there ? at + ch * 4 : 0), there);
-    }
+  };
+  struct VTo {
+    __host__ __device__ static constexpr int at(int row, int ch) { return (row * CH + ch) * 16; }
+  };
+  template <bool FULL>
+  ONE_DEVINL static void issue_run(const PagedAttn& p, uint8_t* stage, int64_t kat, int64_t vat, int live) {
+    PaCopy<KTo, CH>::template run<FULL>(stage, (const uint8_t*)((const T*)p.c.k + kat), live, p.c.Dh / 4);
+    PaCopy<VTo, CH>::template run<FULL>(stage + 64 * DH, (const uint8_t*)((const T*)p.c.v + vat), live, p.c.Dh / 4);
+  }
+  ONE_DEVINL static void issue_any(const PagedAttn& p, uint8_t* stage, int64_t off) {
+    const int64_t at = off < 0 ? -1 : off * (int)sizeof(T);
+    PaCopy<KTo, CH>::any(stage, (const uint8_t*)p.c.k, at, 0, p.c.Dh / 4);
+    PaCopy<VTo, CH>::any(stage + 64 * DH, (const uint8_t*)p.c.v, at, 16, p.c.Dh / 4);
   }
 
   ONE_DEVINL void begin(const PagedAttn& p, uint8_t* extra, const T* q, int rows) {
@@ -382,13 +487,18 @@ struct PaF32 {
       for (int i = 0; i < VC; ++i) o[g][i] = 0.f;
   }
 
-  ONE_DEVINL void consume(const PagedAttn& p, const uint8_t* stage, uint32_t live, float* scores, int rows) {
+  ONE_DEVINL void consume(const PagedAttn& p, const uint8_t* stage, const uint32_t (&lives)[1], float* scores, int rows) {
     const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+    const uint32_t live = lives[0];
+    if (!live) {  // nothing was copied; here for the scores alone
+      if (c < rows) scores[c * p.score_ld + r] = scores[c * p.score_ld + r + 8] = -INFINITY;
+      return;
+    }
     float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
     for (int i = 0; i < KC; ++i) {
-      const float4 a = *reinterpret_cast<const float4*>(stage + (i * 32 + lane) * 16);
-      const float4 b = *reinterpret_cast<const float4*>(stage + ((KC + i) * 32 + lane) * 16);
+      const float4 a = *reinterpret_cast<const float4*>(stage + KTo::at(r, c + 4 * i));
+      const float4 b = *reinterpret_cast<const float4*>(stage + KTo::at(r + 8, c + 4 * i));
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const float4 q = *reinterpret_cast<const float4*>(qs + g * DH + (c + 4 * i) * 4);
@@ -463,111 +573,140 @@ struct PaF32 {
 
 template <typename E>
 struct PaSmem {
-  static constexpr int kRing = kPaWarps * E::kStage * E::kStages;
-  static constexpr int kO = kRing;                                       // [warps][ROWS][DH] floats
-  static constexpr int kML = kO + kPaWarps * E::ROWS * E::DH * 4;        // [warps][ROWS][2]
+  static constexpr int kStage = E::kGroup * E::kGroups;                  // bytes per warp
+  static constexpr int kWarp = kStage * E::kStages;
+  static constexpr int kML = kPaWarps * kWarp;                           // [warps][ROWS][2]
   static constexpr int kFin = kML + kPaWarps * E::ROWS * 8;              // [ROWS][2]: m, 1 / l
-  static constexpr int kLive = kFin + E::ROWS * 8;                       // [warps][stages] live masks
-  static constexpr int kExtra = kLive + kPaWarps * E::kStages * 4 + 16 - (kPaWarps * E::kStages * 4) % 16;
+  static constexpr int kExtra = kFin + (E::ROWS * 8 + 15) / 16 * 16;
   static constexpr int kTotal = kExtra + kPaWarps * E::kExtra;
+  static constexpr int kPerSm = kSmPerSm / (kTotal + 1024) < 3 ? kSmPerSm / (kTotal + 1024) : 3;
+  // a warp's sums fit the stage that it consumed last
+  static_assert(kStage >= E::ROWS * E::DH * 4, "stage");
 };
 
-// SPLIT: CTA i takes the i-th share of the list. Otherwise CTA (hv, b) takes that segment whole and
-// nothing is left to join (short caches: one launch).
-template <typename E, bool SPLIT>
-__global__ void __launch_bounds__(kPaWarps * 32) paged_attn_kernel(const __grid_constant__ PagedAttn p) {
+// p.split: CTA i takes the i-th share of the list. Otherwise CTA (hv, b) takes that segment whole and
+// nothing is left to join (short caches: one launch). RUN: pages hold a multiple of 16 slots and Dh is
+// E::DH, so that a group lies in one page and its copies need two addresses.
+template <typename E, bool RUN>
+__global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E>::kPerSm) paged_attn_kernel(const __grid_constant__ PagedAttn p) {
   extern __shared__ __align__(16) uint8_t smem[];
   using S = PaSmem<E>;
   using T = typename E::T;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  uint8_t* ring = smem + warp * (E::kStage * E::kStages);
-  float* so = reinterpret_cast<float*>(smem + S::kO);
+  constexpr int TILE = E::TILE, GR = E::kGroups;
+  uint8_t* ring = smem + warp * S::kWarp;
   float* ml = reinterpret_cast<float*>(smem + S::kML);
   float* fin = reinterpret_cast<float*>(smem + S::kFin);
-  volatile uint32_t* lives = reinterpret_cast<uint32_t*>(smem + S::kLive) + warp * E::kStages;
   uint8_t* extra = smem + S::kExtra + warp * E::kExtra;
   const PagedCache& c = p.c;
-  const int chunks = c.Dh / 8, HV = c.Hkv * p.hv_per_kv;
+  const int ng = p.hv_per_kv;
   pdl_wait();
   pdl_launch_dependents();
-  PaCursor cur;
-  long long w0, w1;
-  if (SPLIT) {
-    const long long total = pa_total(p), chunk = pa_chunk(p, total);
-    w0 = chunk * blockIdx.x;
-    w1 = min(w0 + chunk, total);
-    if (w0 >= w1) return;
-    cur.seek(c, HV, w0);
+  PaCursor<TILE> cur;
+  int left;  // tiles to do
+  if (p.split) {
+    const long long total = pa_total<TILE>(p), chunk = pa_chunk(p, total), w0 = chunk * blockIdx.x;
+    if (blockIdx.x == 0) {  // for the join
+      if (threadIdx.x < 32) pa_write_before<TILE>(p);
+      if (threadIdx.x == 0) p.before[c.B] = total;
+    }
+    if (w0 >= total) return;
+    left = (int)min(chunk, total - w0);
+    cur.seek(c, ng, w0);
   } else {
     cur.b = blockIdx.y;
-    cur.hv = blockIdx.x;
+    cur.kv = blockIdx.x / ng;
+    cur.gi = blockIdx.x % ng;
     cur.tile = 0;
     cur.load(c);
-    w0 = 0;
-    w1 = cur.tiles;
+    left = cur.tiles;
   }
-  // ---- the copying side: page numbers are asked for one tile ahead of the copies
-  PaCursor src = cur;
-  long long asked = w0;
-  int pg = -1;
+  // ---- the copying side: page numbers are asked for one tile ahead of the copies. RUN: one per group;
+  //      otherwise lane t and lane 16 + t look slot t up.
+  PaCursor<TILE> src = cur;
+  int to_copy = left, pg[GR], in_page[GR];
+  uint32_t live[E::kStages][GR];  // slots in use of the tiles in the ring, the oldest first
+#pragma unroll
+  for (int k = 0; k < E::kStages; ++k)
+#pragma unroll
+    for (int g = 0; g < GR; ++g) live[k][g] = 0;
+  const int mine = warp * (16 * GR) + (RUN ? 0 : lane & 15);
   auto ask = [&] {
-    pg = -1;
-    const int t = src.tile * kPaTile + warp * 16 + (lane & 15);
-    if (asked < w1 && t < src.len) {
-      pg = c.table[src.b * c.table_stride + (int)(((uint64_t)(uint32_t)t * p.div_m) >> p.div_s)];
-      if (pg < 0 || pg >= c.num_pages) {
-        set_err(c.err, ERR_BAD_ARG, SITE_PAGED_ATTN);
-        pg = -1;
+#pragma unroll
+    for (int g = 0; g < GR; ++g) {
+      const int t = src.tile * TILE + mine + 16 * g;
+      pg[g] = -1;
+      if (to_copy > 0 && t < src.len) {
+        const int index = (int)(((uint64_t)(uint32_t)t * p.div_m) >> p.div_s);
+        in_page[g] = t - index * c.page_size;
+        pg[g] = c.table[src.b * c.table_stride + index];
       }
     }
   };
-  int put = 0, get = 0;
+  uint32_t put = 0, get = 0;  // byte offsets of stages
   auto copy = [&] {
-    if (asked < w1) {
-      const int t = src.tile * kPaTile + warp * 16 + (lane & 15);
-      const int slot = t - (int)(((uint64_t)(uint32_t)t * p.div_m) >> p.div_s) * c.page_size;
-      const int64_t off =
-          pg < 0 ? -1 : pg * (lane < 16 ? c.k_stride : c.v_stride) + ((int64_t)(src.hv / p.hv_per_kv) * c.page_size + slot) * c.Dh;
-      const uint32_t live = __ballot_sync(0xffffffffu, off >= 0) & 0xffffu;
-      if (lane == 0) lives[put] = live;
-      if (live) E::issue(p, ring + put * E::kStage, off, chunks);
-      ++asked;
-      if (asked < w1) src.next(c, HV);
+#pragma unroll
+    for (int k = 0; k + 1 < E::kStages; ++k)
+#pragma unroll
+      for (int g = 0; g < GR; ++g) live[k][g] = live[k + 1][g];
+    if (to_copy > 0) {
+#pragma unroll
+      for (int g = 0; g < GR; ++g) {
+        const int t = src.tile * TILE + mine + 16 * g;
+        if ((uint32_t)pg[g] >= (uint32_t)c.num_pages && t < src.len) {
+          set_err(c.err, ERR_BAD_ARG, SITE_PAGED_ATTN);
+          pg[g] = -1;
+        }
+        const int row = (src.kv * c.page_size + in_page[g]) * c.Dh;
+        if (RUN) {
+          const int n = pg[g] < 0 ? 0 : min(16, src.len - t);
+          live[E::kStages - 1][g] = (1u << n) - 1;
+          if (n > 0)
+            E::template issue_run<true>(p, ring + put + g * E::kGroup, (int64_t)pg[g] * (int)c.k_stride + row,
+                                        (int64_t)pg[g] * (int)c.v_stride + row, n);
+        } else {
+          const int64_t off = pg[g] < 0 ? -1 : (int64_t)pg[g] * (int)(lane < 16 ? c.k_stride : c.v_stride) + row;
+          const uint32_t some = __ballot_sync(0xffffffffu, off >= 0) & 0xffffu;
+          live[E::kStages - 1][g] = some;
+          if (some) E::issue_any(p, ring + put + g * E::kGroup, off);
+        }
+      }
+      if (--to_copy > 0) src.next(c, ng);
       ask();
     }
     cp_async_commit();
-    put = put + 1 == E::kStages ? 0 : put + 1;
+    put = put + S::kStage == S::kWarp ? 0 : put + S::kStage;
   };
   ask();
 #pragma unroll 1
   for (int i = 0; i < E::kStages - 1; ++i) copy();
   // ---- the computing side, piece by piece
   E eng;
-  long long w = w0;
+  bool begun_inside = false;  // the piece does not start this CTA's share
   do {
-    const int kv = cur.hv / p.hv_per_kv, g0 = (cur.hv % p.hv_per_kv) * E::ROWS, rows = min(E::ROWS, p.G - g0);
+    const int kv = cur.kv, g0 = cur.gi * E::ROWS, rows = min(E::ROWS, p.G - g0);
     const int64_t hq0 = ((int64_t)cur.b * c.Hkv + kv) * p.G + g0;  // output row of this query-head tile
-    const int first = cur.tile, last = (int)min((long long)cur.tiles, cur.tile + (w1 - w));
+    const int first = cur.tile, last = min(cur.tiles, cur.tile + left);
     if (cur.b >= c.B || (last <= first && cur.tiles > 0)) break;  // lengths that changed during the call
     eng.begin(p, extra, (const T*)p.q + cur.b * p.q_bs + ((int64_t)kv * p.G + g0) * p.q_hs, rows);
     for (int tile = first; tile < last; ++tile) {
       copy();
       cp_async_wait<E::kStages - 1>();
+      uint32_t any = 0;
+#pragma unroll
+      for (int g = 0; g < GR; ++g) any |= live[0][g];
       __syncwarp();
-      const uint32_t live = lives[get];
-      if (live)
-        eng.consume(p, ring + get * E::kStage, live,
-                    p.scores ? p.scores + hq0 * p.score_ld + tile * kPaTile + warp * 16 : nullptr, rows);
-      else if (p.scores)
-        for (int i = lane; i < rows * 16; i += 32)
-          p.scores[(hq0 + i / 16) * p.score_ld + tile * kPaTile + warp * 16 + i % 16] = -INFINITY;
+      if (any || p.scores)
+        eng.consume(p, ring + get, live[0], p.scores ? p.scores + hq0 * p.score_ld + tile * TILE + warp * (16 * GR) : nullptr, rows);
       __syncwarp();
-      get = get + 1 == E::kStages ? 0 : get + 1;
+      get = get + S::kStage == S::kWarp ? 0 : get + S::kStage;
     }
-    eng.leave(ml + warp * E::ROWS * 2, so + warp * E::ROWS * E::DH);
+    // the warps' sums go where each of them consumed last: the stage that is filled next
+    eng.leave(ml + warp * E::ROWS * 2, reinterpret_cast<float*>(ring + put));
     __syncthreads();
+    const float* so = reinterpret_cast<const float*>(smem + put);
     const bool whole = first == 0 && last == cur.tiles;
-    const int64_t part = 2ll * blockIdx.x + (w > w0 ? 1 : 0);
+    const int64_t part = 2ll * blockIdx.x + begun_inside;
     for (int i = threadIdx.x; i < rows * (E::DH / 4); i += blockDim.x) {
       const int g = i / (E::DH / 4), d = i % (E::DH / 4) * 4;
       float M = -INFINITY, L = 0.f;
@@ -579,7 +718,7 @@ __global__ void __launch_bounds__(kPaWarps * 32) paged_attn_kernel(const __grid_
       for (int k = 0; k < kPaWarps; ++k) {
         const float f = exp2f(ml[(k * E::ROWS + g) * 2] - Ms);
         L += f * ml[(k * E::ROWS + g) * 2 + 1];
-        const float4 x = *reinterpret_cast<const float4*>(so + (k * E::ROWS + g) * E::DH + d);
+        const float4 x = *reinterpret_cast<const float4*>(so + k * (S::kWarp / 4) + g * E::DH + d);
         a.x += f * x.x; a.y += f * x.y; a.z += f * x.z; a.w += f * x.w;
       }
       if (whole) {
@@ -591,7 +730,7 @@ __global__ void __launch_bounds__(kPaWarps * 32) paged_attn_kernel(const __grid_
         if (d == 0) {
           fin[2 * g] = Ms;
           fin[2 * g + 1] = inv;
-          if (SPLIT && p.mass) {
+          if (p.split && p.mass) {
             p.row_ml[2 * (hq0 + g)] = Ms;
             p.row_ml[2 * (hq0 + g) + 1] = inv;
           }
@@ -605,7 +744,7 @@ __global__ void __launch_bounds__(kPaWarps * 32) paged_attn_kernel(const __grid_
       }
     }
     __syncthreads();
-    if (!SPLIT && p.mass) {  // one query-head tile per kv head: this CTA wrote all of its scores
+    if (!p.split && p.mass) {  // one query-head tile per kv head: this CTA wrote all of its scores
       float* mass = p.mass + ((int64_t)cur.b * c.Hkv + kv) * p.mass_width;
       for (int t = threadIdx.x; t < cur.len; t += blockDim.x) {
         float a = 0.f;
@@ -613,10 +752,11 @@ __global__ void __launch_bounds__(kPaWarps * 32) paged_attn_kernel(const __grid_
         mass[t] += a;
       }
     }
-    w += last - first;
+    begun_inside = true;
+    left -= last - first;
     cur.tile = last - 1;
-    if (w < w1) cur.next(c, HV);
-  } while (w < w1);
+    if (left > 0) cur.next(c, ng);
+  } while (left > 0);
 }
 
 // The parts of a segment [s0, s1) of the list, cut every `chunk` tiles.
@@ -628,20 +768,20 @@ struct PaParts {
   ONE_DEVINL int64_t at(long long i) const { return 2 * i + (i == first && inner ? 1 : 0); }
 };
 
-// Joins what paged_attn_kernel<SPLIT> left. Blocks below B * Hq: one output row each. With mass,
+// Joins what paged_attn_kernel left of a split list. Blocks below B * Hq: one output row each. With mass,
 // further blocks add the weights: block i takes the i-th share of the tiles of every (sequence, kv
 // head), recomputing the joint (m, l) of its rows from the parts.
 template <typename E>
 __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ PagedAttn p) {
   using T = typename E::T;
-  constexpr int ROWS = E::ROWS, DH = E::DH;
+  constexpr int ROWS = E::ROWS, DH = E::DH, TILE = E::TILE;
   __shared__ float4 red[128];
   __shared__ float fin[2][128];  // m and 1 / l of a kv head's query heads
   const PagedCache& c = p.c;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int hq = c.Hkv * p.G;
   pdl_wait();
-  const long long total = pa_total(p), chunk = pa_chunk(p, total);
+  const long long total = p.before[c.B], chunk = pa_chunk(p, total);
   const int HV = c.Hkv * p.hv_per_kv;
   // joint m and 1 / l of row g of the parts, by one warp
   auto joint = [&](const PaParts& parts, int g, float& M, float& inv) {
@@ -659,14 +799,14 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
   };
   if ((long long)blockIdx.x < (long long)c.B * hq) {
     const int b = blockIdx.x / hq, j = blockIdx.x % hq, kv = j / p.G, g = j % p.G;
-    const int tiles = pa_tiles(c, b);
+    const int tiles = pa_tiles<TILE>(c, b);
     T* out = (T*)p.out + (int64_t)blockIdx.x * c.Dh;
     if (tiles == 0) {
       for (int d = tid; d < c.Dh; d += blockDim.x) st<T>(out + d, 0.f);
       return;
     }
     const int hv = kv * p.hv_per_kv + g / ROWS;
-    const long long s0 = HV * pa_before(p, b) + (long long)hv * tiles;
+    const long long s0 = HV * p.before[b] + (long long)hv * tiles;
     const PaParts parts(s0, s0 + tiles, chunk);
     if (parts.first == parts.last) return;
     const int row = g % ROWS;
@@ -699,20 +839,20 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
   long long w = share * (blockIdx.x - (long long)c.B * hq);
   const long long w1 = min(w + share, mtotal);
   if (w >= w1) return;
-  PaCursor cur;
-  cur.seek(c, c.Hkv, w);
+  PaCursor<TILE> cur;
+  cur.seek(c, 1, w);
   while (w < w1) {
     const int first = cur.tile, last = (int)min((long long)cur.tiles, cur.tile + (w1 - w));
     if (cur.b >= c.B || last <= first) break;
-    const long long before = HV * pa_before(p, cur.b);
-    const int t0 = first * kPaTile, t1 = min(last * kPaTile, cur.len);
-    float* mass = p.mass + ((int64_t)cur.b * c.Hkv + cur.hv) * p.mass_width;
-    const int64_t row0 = ((int64_t)cur.b * c.Hkv + cur.hv) * p.G;
+    const long long before = HV * p.before[cur.b];
+    const int t0 = first * TILE, t1 = min(last * TILE, cur.len);
+    float* mass = p.mass + ((int64_t)cur.b * c.Hkv + cur.kv) * p.mass_width;
+    const int64_t row0 = ((int64_t)cur.b * c.Hkv + cur.kv) * p.G;
     for (int gb = 0; gb < p.G; gb += 128) {
       const int gn = min(128, p.G - gb);
       __syncthreads();
       for (int g = gb + warp; g < gb + gn; g += 4) {
-        const long long s0 = before + (long long)(cur.hv * p.hv_per_kv + g / ROWS) * cur.tiles;
+        const long long s0 = before + (long long)(cur.kv * p.hv_per_kv + g / ROWS) * cur.tiles;
         const PaParts parts(s0, s0 + cur.tiles, chunk);
         float M, inv;
         if (parts.first == parts.last) {
@@ -735,7 +875,7 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
     }
     w += last - first;
     cur.tile = last - 1;
-    if (w < w1) cur.next(c, c.Hkv);
+    if (w < w1) cur.next(c, 1);
   }
 }
 

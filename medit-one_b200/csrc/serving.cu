@@ -113,6 +113,7 @@ int check_cache(PagedCache& c, void* k_pages, void* v_pages, int64_t ks, int64_t
     return fail(ONE_ERR_UNSUPPORTED, "paged cache: at most 2^30 - 1 slots per sequence");
   if (table_stride < max_pages) return fail(ONE_ERR_INVALID, "paged cache: block table rows overlap");
   const int64_t page = (int64_t)hkv * page_size * dh, es = elem_bytes(dtype);
+  if (ks > 0x7fffffff || vs > 0x7fffffff) return fail(ONE_ERR_UNSUPPORTED, "paged cache: pages of at most 2^31 - 1 elements");
   if (ks < page || vs < page) return fail(ONE_ERR_INVALID, "paged cache: pages overlap");
   if (((reinterpret_cast<uintptr_t>(k_pages) | reinterpret_cast<uintptr_t>(v_pages)) & 15) || ks * es % 16 || vs * es % 16)
     return fail(ONE_ERR_INVALID, "paged cache: pages must start on 16-byte boundaries");
@@ -132,7 +133,8 @@ int launched(cudaError_t e, const char* what) {
 namespace {
 
 constexpr int kMaxSms = 160;  // the workspace's bound on the SMs that share a list
-constexpr int kJoinTiles = 8;  // caches of at most this many tiles are not split
+constexpr int kMaxTile = 256;  // slots of the largest tile
+constexpr int kWhole = 512;    // caches of at most this many slots are not split
 
 size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
@@ -140,47 +142,38 @@ size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 int paged_rows(int dtype, int G) { return dtype == ONE_DTYPE_F32 ? 4 : G > 8 ? 16 : 8; }
 
 struct PagedWs {
-  size_t part_ml, part_o, row_ml, scores, total;
+  size_t part_ml, part_o, row_ml, before, scores, total;
   int64_t score_ld;
   PagedWs(int b, int hq, int rows, int dh_pad, int64_t slots, bool mass) {
     const size_t parts = 2 * (size_t)kMaxSms * kPaPerSm * rows;
     part_ml = 0;
     part_o = align256(parts * 8);
     row_ml = part_o + align256(parts * dh_pad * 4);
-    scores = row_ml + align256(mass ? (size_t)b * hq * 8 : 0);
-    score_ld = (slots + kPaTile - 1) / kPaTile * kPaTile;
+    before = row_ml + align256(mass ? (size_t)b * hq * 8 : 0);
+    scores = before + align256(((size_t)b + 1) * 8);
+    score_ld = (slots + kMaxTile - 1) / kMaxTile * kMaxTile;
     total = scores + (mass ? (size_t)b * hq * score_ld * 4 : 0);
   }
 };
 
 int pad_dh(int dh) { return dh <= 32 ? 32 : dh <= 64 ? 64 : dh <= 96 ? 96 : 128; }
 
-template <typename E>
-int attend_split(PagedAttn& p, cudaStream_t st) {
+template <typename E, bool RUN>
+int attend(PagedAttn& p, cudaStream_t st) {
   static std::atomic<bool> done[kMaxDevices];
-  int rc = allow_smem(paged_attn_kernel<E, true>, PaSmem<E>::kTotal, done);
+  int rc = allow_smem(paged_attn_kernel<E, RUN>, PaSmem<E>::kTotal, done);
   if (rc) return rc;
-  p.ranges = std::min(num_sms(), kMaxSms) * std::min(kPaPerSm, (int)(kSmPerSm / (PaSmem<E>::kTotal + 1024)));
-  rc = launched(launch(paged_attn_kernel<E, true>, dim3(p.ranges), dim3(kPaWarps * 32), PaSmem<E>::kTotal, st, p),
-                "paged attention");
-  if (rc) return rc;
+  p.ranges = std::min(num_sms(), kMaxSms) * PaSmem<E>::kPerSm;
+  const dim3 grid = p.split ? dim3(p.ranges) : dim3(p.c.Hkv * p.hv_per_kv, p.c.B);
+  rc = launched(launch(paged_attn_kernel<E, RUN>, grid, dim3(kPaWarps * 32), PaSmem<E>::kTotal, st, p), "paged attention");
+  if (rc || !p.split) return rc;
   const int64_t joins = (int64_t)p.c.B * p.c.Hkv * p.G + (p.mass ? p.ranges : 0);
   return launched(launch(paged_join_kernel<E>, dim3((unsigned)joins), dim3(128), 0, st, p), "paged attention join");
 }
 
 template <typename E>
-int attend_whole(PagedAttn& p, cudaStream_t st) {
-  static std::atomic<bool> done[kMaxDevices];
-  int rc = allow_smem(paged_attn_kernel<E, false>, PaSmem<E>::kTotal, done);
-  if (rc) return rc;
-  return launched(launch(paged_attn_kernel<E, false>, dim3(p.c.Hkv * p.hv_per_kv, p.c.B), dim3(kPaWarps * 32),
-                         PaSmem<E>::kTotal, st, p),
-                  "paged attention");
-}
-
-template <typename E>
-int attend(PagedAttn& p, bool split, cudaStream_t st) {
-  return split ? attend_split<E>(p, st) : attend_whole<E>(p, st);
+int attend(PagedAttn& p, cudaStream_t st) {
+  return p.c.page_size % 16 == 0 && p.c.Dh == E::DH ? attend<E, true>(p, st) : attend<E, false>(p, st);
 }
 
 }  // namespace
@@ -206,7 +199,7 @@ extern "C" int one_paged_attention(const void* q, int64_t q_batch_stride, int64_
   const int64_t slots = (int64_t)max_pages * page_size;
   if (mass && mass_width < slots)
     return fail(ONE_ERR_INVALID, "paged attention: mass rows are shorter than the block table's slots");
-  if ((int64_t)b * hq > 0x3fffffff) return fail(ONE_ERR_UNSUPPORTED, "paged attention: too many rows");
+  if ((int64_t)b * hq > 0x3fffffff || (int64_t)b * hq * (slots / 64 + 1) / 128 > 0x7fffffff) return fail(ONE_ERR_UNSUPPORTED, "paged attention: too many rows");
   if (workspace_bytes < one_paged_attention_workspace_bytes(b, hq, hkv, dh, page_size, max_pages, dtype, mass != nullptr))
     return fail(ONE_ERR_INVALID, "workspace too small");
   p.q = q; p.q_bs = q_batch_stride; p.q_hs = q_head_stride; p.G = hq / hkv;
@@ -223,32 +216,33 @@ extern "C" int one_paged_attention(const void* q, int64_t q_batch_stride, int64_
   p.part_ml = reinterpret_cast<float*>(ws + w.part_ml);
   p.part_o = reinterpret_cast<float*>(ws + w.part_o);
   p.row_ml = reinterpret_cast<float*>(ws + w.row_ml);
+  p.before = reinterpret_cast<long long*>(ws + w.before);
   p.scores = mass ? reinterpret_cast<float*>(ws + w.scores) : nullptr;
   p.score_ld = w.score_ld;
-  const bool split = slots > kJoinTiles * kPaTile || (mass && p.hv_per_kv > 1);
+  p.split = slots > kWhole || (mass && p.hv_per_kv > 1);
   cudaStream_t st = (cudaStream_t)stream;
   const int d = pad_dh(dh);
   if (dtype == ONE_DTYPE_F32) {
     switch (d) {
-      case 32: return attend<PaF32<32>>(p, split, st);
-      case 64: return attend<PaF32<64>>(p, split, st);
-      case 96: return attend<PaF32<96>>(p, split, st);
-      default: return attend<PaF32<128>>(p, split, st);
+      case 32: return attend<PaF32<32>>(p, st);
+      case 64: return attend<PaF32<64>>(p, st);
+      case 96: return attend<PaF32<96>>(p, st);
+      default: return attend<PaF32<128>>(p, st);
     }
   }
   if (rows == 16) {
     switch (d) {
-      case 32: return attend<PaBf16<32, true>>(p, split, st);
-      case 64: return attend<PaBf16<64, true>>(p, split, st);
-      case 96: return attend<PaBf16<96, true>>(p, split, st);
-      default: return attend<PaBf16<128, true>>(p, split, st);
+      case 32: return attend<PaBf16<32, true>>(p, st);
+      case 64: return attend<PaBf16<64, true>>(p, st);
+      case 96: return attend<PaBf16<96, true>>(p, st);
+      default: return attend<PaBf16<128, true>>(p, st);
     }
   }
   switch (d) {
-    case 32: return attend<PaBf16<32, false>>(p, split, st);
-    case 64: return attend<PaBf16<64, false>>(p, split, st);
-    case 96: return attend<PaBf16<96, false>>(p, split, st);
-    default: return attend<PaBf16<128, false>>(p, split, st);
+    case 32: return attend<PaBf16<32, false>>(p, st);
+    case 64: return attend<PaBf16<64, false>>(p, st);
+    case 96: return attend<PaBf16<96, false>>(p, st);
+    default: return attend<PaBf16<128, false>>(p, st);
   }
 }
 
