@@ -241,47 +241,58 @@ int one_sample_tokens(const void* logits, int32_t batch, int32_t vocab, int32_t 
 /* The operators of one serving step over a paged key-value cache. They have no counterpart in the
  * reference, whose attention reads whole dense prompts (one/flash_attention.py:224-324).
  *
- * The cache: k_pages, v_pages hold num_pages pages [hkv][page_size][dh] in dtype, one page
- * k_page_stride (v_page_stride) elements after the other (at least hkv * page_size * dh; both
- * pools start, and their pages lie, on 16-byte boundaries). Any page_size; dh a multiple of 8, at
- * most 128. block_table int32 [b][max_pages], rows table_stride apart, names the pages of each
- * sequence in order: slot t of sequence i is row t % page_size of page
- * block_table[i][t / page_size]. Entries past a sequence's last used page are not read. Sequences
- * may share pages that are only read. lengths int32 [b]: slots in use (0 allowed); no call writes
- * it, so the layers of a model share it and a call can be repeated. A page number outside
- * [0, num_pages) where one is used, a length below 0 or beyond the table's slots: the rows are
- * neither read nor written, and the error record (one_ops_error) holds code 2.
- * mass (optional) fp32 [b][hkv][mass_width], mass_width >= max_pages * page_size: the attention
- * weight that each slot has received. */
+ * k_pages, v_pages hold num_pages pages [hkv][page_size][dh] in dtype, one page k_page_stride
+ * (v_page_stride) elements after the other (at least hkv * page_size * dh, at most 2^31 - 1; the
+ * pools and every page start on 16-byte boundaries). Any page_size; dh a multiple of 8, at most 128.
+ * block_table int32 [b][max_pages], rows table_stride apart, names the pages of each sequence in
+ * order: slot t of sequence i is row t % page_size of page block_table[i][t / page_size]. Entries
+ * past a sequence's last used page are not read. Sequences may share pages that are only read.
+ * lengths int32 [b]: slots in use (0 allowed); no call writes it, so the layers of a model share it
+ * and a call can be repeated. A page number outside [0, num_pages) where one is used, a length below
+ * 0 or beyond the table's slots: the rows are neither read nor written, and the error record
+ * (one_ops_error) holds code 2. mass fp32 [b][hkv][mass_width], mass_width >= max_pages * page_size:
+ * the attention weight that each slot has received; NULL where it is not kept. */
+typedef struct one_paged_cache {
+  void* k_pages;
+  void* v_pages;
+  int64_t k_page_stride, v_page_stride;
+  const int32_t* block_table;
+  int64_t table_stride;
+  const int32_t* lengths;
+  float* mass;
+  int64_t mass_width;
+  int32_t num_pages, page_size, max_pages, b, hkv, dh, dtype, reserved;
+} one_paged_cache;
 
-/* New tokens into the cache: keys k and values v [b, hkv, n, dh] and, optionally, queries q
- * [b, hq, n, dh] (element strides given; rows contiguous). With cos, sin [cos_batch, n, dh]
- * (cos_batch = b, or 1 when shared; NULL: no rotation) q and k are rotated as
- * apply_rotary_pos_emb_flash does (one/flash_attention.py:20-33: x cos + rotate_half(x) sin), in
- * fp32 with one rounding. Token t < counts[i] of sequence i (counts NULL: n) goes to slot
- * lengths[i] + t, whose mass becomes 0; tokens from counts[i] on are not stored. q_out
- * [b, hq, n, dh] receives every rotated query. The caller advances lengths. */
-int one_paged_append(const void* k, int64_t k_batch_stride, int64_t k_head_stride, int64_t k_token_stride, const void* v,
-                     int64_t v_batch_stride, int64_t v_head_stride, int64_t v_token_stride, const void* q,
-                     int64_t q_batch_stride, int64_t q_head_stride, int64_t q_token_stride, const void* cos,
-                     const void* sin, int32_t cos_batch, const int32_t* counts, void* k_pages, void* v_pages,
-                     int64_t k_page_stride, int64_t v_page_stride, int32_t num_pages, int32_t page_size,
-                     const int32_t* block_table, int64_t table_stride, int32_t max_pages, const int32_t* lengths, int32_t b,
-                     int32_t n, int32_t hq, int32_t hkv, int32_t dh, int32_t dtype, float* mass, int64_t mass_width,
-                     void* q_out, void* stream);
+/* New tokens of a batch: keys k, values v [b, hkv, n, dh] and, optionally, queries q [b, hq, n, dh]
+ * (element strides of batch, head and token; rows contiguous). cos, sin [cos_batch, n, dh]
+ * (cos_batch = b, or 1 when shared), or NULL: no rotation. counts int32 [b], or NULL: n. */
+typedef struct one_paged_tokens {
+  const void *k, *v, *q;
+  int64_t k_strides[3], v_strides[3], q_strides[3];
+  const void *cos, *sin;
+  const int32_t* counts;
+  void* q_out;
+  int32_t n, hq, cos_batch, reserved;
+} one_paged_tokens;
+
+/* New tokens into the cache. q and k are rotated as apply_rotary_pos_emb_flash does
+ * (one/flash_attention.py:20-33: x cos + rotate_half(x) sin), in fp32 with one rounding. Token
+ * t < counts[i] of sequence i goes to slot lengths[i] + t, whose mass (if kept) becomes 0; tokens
+ * from counts[i] on are not stored. q_out [b, hq, n, dh] (with q) receives every rotated query. The
+ * caller advances lengths. */
+int one_paged_append(const one_paged_cache* cache, const one_paged_tokens* tokens, void* stream);
 
 /* Attention of one new token per sequence over its cached slots: softmax(q k^T * scale) v with an
  * fp32 softmax over the slots below lengths[i]. q [b, hq] rows of dh (element strides given), hq a
  * multiple of hkv: query head j reads kv head j / (hq / hkv). out [b, hq, dh]. A sequence without
- * slots, or whose scores are all -inf, gives zeros. mass, if not NULL, grows by the softmax weights
- * summed over the query heads of each kv head. */
+ * slots, or whose scores are all -inf, gives zeros. The cache's mass, if kept, grows by the softmax
+ * weights summed over the query heads of each kv head. The workspace may be NULL where its size
+ * is 0. */
 size_t one_paged_attention_workspace_bytes(int32_t b, int32_t hq, int32_t hkv, int32_t dh, int32_t page_size,
                                            int32_t max_pages, int32_t dtype, int32_t with_mass);
-int one_paged_attention(const void* q, int64_t q_batch_stride, int64_t q_head_stride, const void* k_pages,
-                        const void* v_pages, int64_t k_page_stride, int64_t v_page_stride, int32_t num_pages,
-                        int32_t page_size, const int32_t* block_table, int64_t table_stride, int32_t max_pages,
-                        const int32_t* lengths, int32_t b, int32_t hq, int32_t hkv, int32_t dh, float scale, int32_t dtype,
-                        float* mass, int64_t mass_width, void* out, void* workspace, size_t workspace_bytes, void* stream);
+int one_paged_attention(const one_paged_cache* cache, const void* q, int64_t q_batch_stride, int64_t q_head_stride,
+                        int32_t hq, float scale, void* out, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Eviction by accumulated attention weight: of each (sequence, kv head), at most `budget` slots
  * survive: the first `sink`, the last `recent`, and of the rest those with the largest mass (equal
@@ -292,32 +303,41 @@ int one_paged_attention(const void* q, int64_t q_batch_stride, int64_t q_head_st
  * slots, then -1. mass_out fp32 [b][hkv][mass_out_width] (mass_out_width >= budget, no overlap with
  * mass): their masses, then 0. The caller swaps the tables and sets lengths to
  * min(lengths, budget). */
-int one_paged_evict(void* k_pages, void* v_pages, int64_t k_page_stride, int64_t v_page_stride, int32_t num_pages,
-                    int32_t page_size, const int32_t* block_table, int64_t table_stride, int32_t max_pages,
-                    const int32_t* dst_table, int64_t dst_stride, int32_t dst_max_pages, const int32_t* lengths,
-                    const float* mass, int64_t mass_width, int32_t b, int32_t hkv, int32_t dh, int32_t dtype,
+int one_paged_evict(const one_paged_cache* cache, const int32_t* dst_table, int64_t dst_stride, int32_t dst_max_pages,
                     int32_t budget, int32_t recent, int32_t sink, float* mass_out, int64_t mass_out_width, int32_t* kept,
                     void* stream);
 
+/* What one_process_logits does to a row. history [batch][history_ld]: history_len ids of
+ * history_bytes = 4 or 8 bytes; ids outside [0, vocab) are padding; NULL: none. output_starts int32
+ * [batch], or NULL: 0. repetition, presence, frequency: fp32 [batch], or NULL for the scalar of the
+ * same name (1, 0, 0: off). bias fp32 [vocab] (bias_ld 0) or [batch][bias_ld], or NULL. token_mask
+ * int32 words, bit v % 32 of word v / 32 set = allowed, [ceil(vocab / 32)] (mask_ld 0) or
+ * [batch][mask_ld], or NULL. */
+typedef struct one_logits_rules {
+  const void* history;
+  int64_t history_ld;
+  const int32_t* output_starts;
+  const float *repetition, *presence, *frequency;
+  const float* bias;
+  int64_t bias_ld;
+  const int32_t* token_mask;
+  int64_t mask_ld;
+  int32_t history_len, history_bytes;
+  float repetition_all, presence_all, frequency_all;
+  int32_t reserved;
+} one_logits_rules;
+
 /* A step's logits [batch][ld] (first `vocab` entries) made ready for one_sample_tokens or greedy
- * choice, in fp32: with c = how often the token stands in the row's history from
- * output_starts[i] on (NULL: from the start) and the row's penalties r, p, f,
+ * choice, in fp32: with c = how often the token stands in the row's history from its output_start
+ * on and the row's penalties r, p, f,
  *   z = x; z = z > 0 ? z / r : z * r if the token stands anywhere in the history;
  *   z -= f * c + (c > 0 ? p : 0); z += bias; z = -inf where the token's mask bit is 0.
- * history [batch][hist_ld], hist_len ids of hist_bytes = 4 or 8 bytes; ids outside [0, vocab) are
- * padding. repetition, presence, frequency: fp32 [batch], or NULL for the scalar beside each
- * (1, 0, 0: off). bias fp32 [vocab] (bias_ld 0) or [batch][bias_ld], or NULL; token_mask int32
- * words, bit v % 32 of word v / 32 set = allowed, [ceil(vocab / 32)] (mask_ld 0) or
- * [batch][mask_ld], or NULL. out fp32 [batch][out_ld] (may be the logits themselves when they are
- * fp32). best int32 [batch] or NULL: the token of the largest score, the lowest among equals; NaN
- * is never chosen; 0 when nothing is left. Replaces transformers' RepetitionPenaltyLogitsProcessor
- * and its like in GenerationMixin.generate (one/modeling_one.py:845). */
-int one_process_logits(const void* logits, int64_t ld, int32_t batch, int32_t vocab, int32_t dtype, const void* history,
-                       int64_t hist_ld, int32_t hist_len, int32_t hist_bytes, const int32_t* output_starts,
-                       const float* repetition, float repetition_all, const float* presence, float presence_all,
-                       const float* frequency, float frequency_all, const float* bias, int64_t bias_ld,
-                       const int32_t* token_mask, int64_t mask_ld, float* out, int64_t out_ld, int32_t* best,
-                       void* stream);
+ * out fp32 [batch][out_ld] (may be the logits themselves when they are fp32). best int32 [batch] or
+ * NULL: the token of the largest score, the lowest among equals; NaN is never chosen; 0 when nothing
+ * is left. Replaces transformers' RepetitionPenaltyLogitsProcessor and its like in
+ * GenerationMixin.generate (one/modeling_one.py:845). */
+int one_process_logits(const one_logits_rules* rules, const void* logits, int64_t ld, int32_t batch, int32_t vocab,
+                       int32_t dtype, float* out, int64_t out_ld, int32_t* best, void* stream);
 
 #ifdef __cplusplus
 }

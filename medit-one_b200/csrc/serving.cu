@@ -100,26 +100,29 @@ int num_sms() {
 int elem_bytes(int dtype) { return dtype == ONE_DTYPE_F32 ? 4 : 2; }
 
 // What every operator over a cache asks of it.
-int check_cache(PagedCache& c, void* k_pages, void* v_pages, int64_t ks, int64_t vs, int num_pages, int page_size,
-                const int32_t* table, int64_t table_stride, int max_pages, const int32_t* lengths, int b, int hkv,
-                int dh, int dtype) {
-  if (!k_pages || !v_pages || !table || !lengths) return fail(ONE_ERR_INVALID, "paged cache: null argument");
-  if (dtype != ONE_DTYPE_BF16 && dtype != ONE_DTYPE_F32) return fail(ONE_ERR_INVALID, "paged cache: dtype");
-  if (num_pages < 1 || page_size < 1 || max_pages < 1 || b < 1 || hkv < 1 || dh < 1)
+int check_cache(PagedCache& c, const one_paged_cache* x) {
+  if (!x || !x->k_pages || !x->v_pages || !x->block_table || !x->lengths)
+    return fail(ONE_ERR_INVALID, "paged cache: null argument");
+  if (x->dtype != ONE_DTYPE_BF16 && x->dtype != ONE_DTYPE_F32) return fail(ONE_ERR_INVALID, "paged cache: dtype");
+  if (x->num_pages < 1 || x->page_size < 1 || x->max_pages < 1 || x->b < 1 || x->hkv < 1 || x->dh < 1)
     return fail(ONE_ERR_INVALID, "paged cache: sizes must be positive");
-  if (dh > 128 || dh % 8) return fail(ONE_ERR_UNSUPPORTED, "paged cache: head_dim a multiple of 8, at most 128");
-  if (b > 65535 || hkv > 65535) return fail(ONE_ERR_UNSUPPORTED, "paged cache: at most 65535 sequences and heads");
-  if ((int64_t)max_pages * page_size > 0x3fffffff)
+  if (x->dh > 128 || x->dh % 8) return fail(ONE_ERR_UNSUPPORTED, "paged cache: head_dim a multiple of 8, at most 128");
+  if (x->b > 65535 || x->hkv > 65535) return fail(ONE_ERR_UNSUPPORTED, "paged cache: at most 65535 sequences and heads");
+  if ((int64_t)x->max_pages * x->page_size > 0x3fffffff)
     return fail(ONE_ERR_UNSUPPORTED, "paged cache: at most 2^30 - 1 slots per sequence");
-  if (table_stride < max_pages) return fail(ONE_ERR_INVALID, "paged cache: block table rows overlap");
-  const int64_t page = (int64_t)hkv * page_size * dh, es = elem_bytes(dtype);
-  if (ks > 0x7fffffff || vs > 0x7fffffff) return fail(ONE_ERR_UNSUPPORTED, "paged cache: pages of at most 2^31 - 1 elements");
+  if (x->table_stride < x->max_pages) return fail(ONE_ERR_INVALID, "paged cache: block table rows overlap");
+  const int64_t page = (int64_t)x->hkv * x->page_size * x->dh, es = elem_bytes(x->dtype);
+  const int64_t ks = x->k_page_stride, vs = x->v_page_stride;
+  if (ks > 0x7fffffff || vs > 0x7fffffff || page > 0x7fffffff)
+    return fail(ONE_ERR_UNSUPPORTED, "paged cache: pages of at most 2^31 - 1 elements");
   if (ks < page || vs < page) return fail(ONE_ERR_INVALID, "paged cache: pages overlap");
-  if (((reinterpret_cast<uintptr_t>(k_pages) | reinterpret_cast<uintptr_t>(v_pages)) & 15) || ks * es % 16 || vs * es % 16)
+  if (((reinterpret_cast<uintptr_t>(x->k_pages) | reinterpret_cast<uintptr_t>(x->v_pages)) & 15) || ks * es % 16 || vs * es % 16)
     return fail(ONE_ERR_INVALID, "paged cache: pages must start on 16-byte boundaries");
-  c.k = k_pages; c.v = v_pages; c.k_stride = ks; c.v_stride = vs;
-  c.table = table; c.table_stride = table_stride; c.lengths = lengths;
-  c.num_pages = num_pages; c.page_size = page_size; c.max_pages = max_pages; c.B = b; c.Hkv = hkv; c.Dh = dh;
+  if (x->mass && x->mass_width < (int64_t)x->max_pages * x->page_size)
+    return fail(ONE_ERR_INVALID, "paged cache: mass rows are shorter than the block table's slots");
+  c.k = x->k_pages; c.v = x->v_pages; c.k_stride = ks; c.v_stride = vs;
+  c.table = x->block_table; c.table_stride = x->table_stride; c.lengths = x->lengths;
+  c.num_pages = x->num_pages; c.page_size = x->page_size; c.max_pages = x->max_pages; c.B = x->b; c.Hkv = x->hkv; c.Dh = x->dh;
   c.err = reinterpret_cast<DevErr*>(one_ops_err_record());
   return ONE_OK;
 }
@@ -181,27 +184,26 @@ int attend(PagedAttn& p, cudaStream_t st) {
 extern "C" size_t one_paged_attention_workspace_bytes(int32_t b, int32_t hq, int32_t hkv, int32_t dh, int32_t page_size,
                                                       int32_t max_pages, int32_t dtype, int32_t with_mass) {
   if (b < 1 || hq < 1 || hkv < 1 || dh < 1 || page_size < 1 || max_pages < 1) return 0;
-  return PagedWs(b, hq, paged_rows(dtype, hq / hkv), pad_dh(dh), (int64_t)max_pages * page_size, with_mass != 0).total + 256;
+  const int64_t slots = (int64_t)max_pages * page_size;
+  if (!with_mass && slots <= kWhole) return 0;
+  return PagedWs(b, hq, paged_rows(dtype, hq / hkv), pad_dh(dh), slots, with_mass != 0).total + 256;
 }
 
-extern "C" int one_paged_attention(const void* q, int64_t q_batch_stride, int64_t q_head_stride, const void* k_pages,
-                                   const void* v_pages, int64_t k_page_stride, int64_t v_page_stride, int32_t num_pages,
-                                   int32_t page_size, const int32_t* block_table, int64_t table_stride, int32_t max_pages,
-                                   const int32_t* lengths, int32_t b, int32_t hq, int32_t hkv, int32_t dh, float scale,
-                                   int32_t dtype, float* mass, int64_t mass_width, void* out, void* workspace,
+extern "C" int one_paged_attention(const one_paged_cache* cache, const void* q, int64_t q_batch_stride,
+                                   int64_t q_head_stride, int32_t hq, float scale, void* out, void* workspace,
                                    size_t workspace_bytes, void* stream) {
-  if (!q || !out || !workspace) return fail(ONE_ERR_INVALID, "paged attention: null argument");
+  if (!q || !out) return fail(ONE_ERR_INVALID, "paged attention: null argument");
   PagedAttn p = {};
-  int rc = check_cache(p.c, const_cast<void*>(k_pages), const_cast<void*>(v_pages), k_page_stride, v_page_stride, num_pages,
-                       page_size, block_table, table_stride, max_pages, lengths, b, hkv, dh, dtype);
+  int rc = check_cache(p.c, cache);
   if (rc) return rc;
+  const int b = cache->b, hkv = cache->hkv, dh = cache->dh, dtype = cache->dtype, page_size = cache->page_size;
+  float* mass = cache->mass;
   if (hq < 1 || hq % hkv) return fail(ONE_ERR_INVALID, "paged attention: the query heads must be a multiple of the kv heads");
-  const int64_t slots = (int64_t)max_pages * page_size;
-  if (mass && mass_width < slots)
-    return fail(ONE_ERR_INVALID, "paged attention: mass rows are shorter than the block table's slots");
-  if ((int64_t)b * hq > 0x3fffffff || (int64_t)b * hq * (slots / 64 + 1) / 128 > 0x7fffffff) return fail(ONE_ERR_UNSUPPORTED, "paged attention: too many rows");
-  if (workspace_bytes < one_paged_attention_workspace_bytes(b, hq, hkv, dh, page_size, max_pages, dtype, mass != nullptr))
-    return fail(ONE_ERR_INVALID, "workspace too small");
+  const int64_t slots = (int64_t)cache->max_pages * page_size;
+  if ((int64_t)b * hq > 0x3fffffff || (int64_t)b * hq * (slots / 64 + 1) / 128 > 0x7fffffff)
+    return fail(ONE_ERR_UNSUPPORTED, "paged attention: too many rows");
+  const size_t need = one_paged_attention_workspace_bytes(b, hq, hkv, dh, page_size, cache->max_pages, dtype, mass != nullptr);
+  if (need && (!workspace || workspace_bytes < need)) return fail(ONE_ERR_INVALID, "workspace too small");
   p.q = q; p.q_bs = q_batch_stride; p.q_hs = q_head_stride; p.G = hq / hkv;
   const int rows = paged_rows(dtype, p.G);
   p.hv_per_kv = (p.G + rows - 1) / rows;
@@ -210,7 +212,7 @@ extern "C" int one_paged_attention(const void* q, int64_t q_batch_stride, int64_
   p.div_m = (uint32_t)((1ull << (31 + p.div_s)) / page_size + 1);
   p.div_s += 31;
   p.scale_log2 = scale * 1.4426950408889634f;
-  p.mass = mass; p.mass_width = mass_width; p.out = out;
+  p.mass = mass; p.mass_width = cache->mass_width; p.out = out;
   const PagedWs w(b, hq, rows, pad_dh(dh), slots, mass != nullptr);
   uint8_t* ws = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(workspace) + 255) & ~uintptr_t(255));
   p.part_ml = reinterpret_cast<float*>(ws + w.part_ml);
@@ -246,37 +248,32 @@ extern "C" int one_paged_attention(const void* q, int64_t q_batch_stride, int64_
   }
 }
 
-extern "C" int one_paged_append(const void* k, int64_t k_batch_stride, int64_t k_head_stride, int64_t k_token_stride,
-                                const void* v, int64_t v_batch_stride, int64_t v_head_stride, int64_t v_token_stride,
-                                const void* q, int64_t q_batch_stride, int64_t q_head_stride, int64_t q_token_stride,
-                                const void* cosv, const void* sinv, int32_t cos_batch, const int32_t* counts, void* k_pages, void* v_pages,
-                                int64_t k_page_stride, int64_t v_page_stride, int32_t num_pages, int32_t page_size,
-                                const int32_t* block_table, int64_t table_stride, int32_t max_pages,
-                                const int32_t* lengths, int32_t b, int32_t n, int32_t hq, int32_t hkv, int32_t dh,
-                                int32_t dtype, float* mass, int64_t mass_width, void* q_out, void* stream) {
-  if (!k || !v || !q != !q_out || !cosv != !sinv)
+extern "C" int one_paged_append(const one_paged_cache* cache, const one_paged_tokens* tokens, void* stream) {
+  if (!tokens || !tokens->k || !tokens->v || !tokens->q != !tokens->q_out || !tokens->cos != !tokens->sin)
     return fail(ONE_ERR_INVALID, "paged append: null argument");
   PagedAppendParams p = {};
-  int rc = check_cache(p.c, k_pages, v_pages, k_page_stride, v_page_stride, num_pages, page_size, block_table, table_stride,
-                       max_pages, lengths, b, hkv, dh, dtype);
+  int rc = check_cache(p.c, cache);
   if (rc) return rc;
-  if (n < 1 || (q && hq < 1)) return fail(ONE_ERR_INVALID, "paged append: sizes must be positive");
-  if (cosv && cos_batch != 1 && cos_batch != b) return fail(ONE_ERR_INVALID, "cos_batch must be 1 or b");
-  if (mass && mass_width < (int64_t)max_pages * page_size)
-    return fail(ONE_ERR_INVALID, "paged append: mass rows are shorter than the block table's slots");
+  const one_paged_tokens& x = *tokens;
+  const int b = cache->b, hkv = cache->hkv, dh = cache->dh, dtype = cache->dtype, n = x.n, hq = x.hq;
+  if (n < 1 || (x.q && hq < 1)) return fail(ONE_ERR_INVALID, "paged append: sizes must be positive");
+  if (x.cos && x.cos_batch != 1 && x.cos_batch != b) return fail(ONE_ERR_INVALID, "cos_batch must be 1 or b");
+  const void *k = x.k, *v = x.v, *q = x.q, *cosv = x.cos, *sinv = x.sin;
   p.k = k; p.v = v; p.q = q;
-  p.ks[0] = k_batch_stride; p.ks[1] = k_head_stride; p.ks[2] = k_token_stride;
-  p.vs[0] = v_batch_stride; p.vs[1] = v_head_stride; p.vs[2] = v_token_stride;
-  p.qs[0] = q_batch_stride; p.qs[1] = q_head_stride; p.qs[2] = q_token_stride;
-  p.cosv = cosv; p.sinv = sinv; p.cos_bs = cos_batch == 1 ? 0 : (int64_t)n * dh; p.counts = counts;
-  p.mass = mass; p.mass_width = mass_width; p.q_out = q_out; p.N = n; p.Hq = hq;
+  for (int i = 0; i < 3; ++i) {
+    p.ks[i] = x.k_strides[i];
+    p.vs[i] = x.v_strides[i];
+    p.qs[i] = x.q_strides[i];
+  }
+  p.cosv = cosv; p.sinv = sinv; p.cos_bs = x.cos_batch == 1 ? 0 : (int64_t)n * dh; p.counts = x.counts;
+  p.mass = cache->mass; p.mass_width = cache->mass_width; p.q_out = x.q_out; p.N = n; p.Hq = hq;
   // 16-byte pieces need aligned rows and halves of whole pieces; anything else goes element by element
   const int64_t unit = 16 / elem_bytes(dtype);
-  auto aligned = [&](const void* x, const int64_t* s) {
-    return (reinterpret_cast<uintptr_t>(x) & 15) == 0 && s[0] % unit == 0 && s[1] % unit == 0 && s[2] % unit == 0;
+  auto aligned = [&](const void* at, const int64_t* s) {
+    return (reinterpret_cast<uintptr_t>(at) & 15) == 0 && s[0] % unit == 0 && s[1] % unit == 0 && s[2] % unit == 0;
   };
   const bool vec = dh % 16 == 0 && aligned(k, p.ks) && aligned(v, p.vs) && (!q || aligned(q, p.qs)) &&
-                   ((reinterpret_cast<uintptr_t>(q_out) | reinterpret_cast<uintptr_t>(cosv) | reinterpret_cast<uintptr_t>(sinv)) & 15) == 0;
+                   ((reinterpret_cast<uintptr_t>(x.q_out) | reinterpret_cast<uintptr_t>(cosv) | reinterpret_cast<uintptr_t>(sinv)) & 15) == 0;
   const int64_t threads = (int64_t)n * (2 * (int64_t)hkv + (q ? hq : 0)) * (vec ? dh / 16 : 32);
   if (threads > 0x7fffffff) return fail(ONE_ERR_UNSUPPORTED, "paged append: too many rows");
   const dim3 grid((unsigned)((threads + 255) / 256), b);
@@ -289,32 +286,28 @@ extern "C" int one_paged_append(const void* k, int64_t k_batch_stride, int64_t k
                   "paged append");
 }
 
-extern "C" int one_paged_evict(void* k_pages, void* v_pages, int64_t k_page_stride, int64_t v_page_stride,
-                               int32_t num_pages, int32_t page_size, const int32_t* block_table, int64_t table_stride,
-                               int32_t max_pages, const int32_t* dst_table, int64_t dst_stride, int32_t dst_max_pages,
-                               const int32_t* lengths, const float* mass, int64_t mass_width, int32_t b, int32_t hkv,
-                               int32_t dh, int32_t dtype, int32_t budget, int32_t recent, int32_t sink, float* mass_out,
+extern "C" int one_paged_evict(const one_paged_cache* cache, const int32_t* dst_table, int64_t dst_stride,
+                               int32_t dst_max_pages, int32_t budget, int32_t recent, int32_t sink, float* mass_out,
                                int64_t mass_out_width, int32_t* kept, void* stream) {
   PagedEvictParams p = {};
-  if (!dst_table || !mass || !mass_out || !kept) return fail(ONE_ERR_INVALID, "paged evict: null argument");
-  int rc = check_cache(p.c, k_pages, v_pages, k_page_stride, v_page_stride, num_pages, page_size, block_table, table_stride,
-                       max_pages, lengths, b, hkv, dh, dtype);
+  if (!dst_table || !mass_out || !kept || !cache || !cache->mass) return fail(ONE_ERR_INVALID, "paged evict: null argument");
+  int rc = check_cache(p.c, cache);
   if (rc) return rc;
+  const int b = cache->b, hkv = cache->hkv, dh = cache->dh, dtype = cache->dtype, page_size = cache->page_size;
   if (budget < 1 || recent < 0 || sink < 0 || (int64_t)recent + sink > budget)
     return fail(ONE_ERR_INVALID, "paged evict: 1 <= budget, 0 <= recent, sink and recent + sink <= budget");
   if (dst_max_pages < 1 || dst_stride < dst_max_pages || (int64_t)dst_max_pages * page_size < budget)
     return fail(ONE_ERR_INVALID, "paged evict: the destination pages hold fewer slots than the budget");
-  if (mass_width < (int64_t)max_pages * page_size || mass_out_width < budget)
-    return fail(ONE_ERR_INVALID, "paged evict: mass rows are too short");
+  if (mass_out_width < budget) return fail(ONE_ERR_INVALID, "paged evict: mass rows are too short");
   const int64_t per_bh = (mass_out_width + kMovePlaces - 1) / kMovePlaces;
   if (mass_out_width > 0x3fffffff || per_bh * b * hkv > 0x7fffffff)
     return fail(ONE_ERR_UNSUPPORTED, "paged evict: too many rows");
-  p.dst = dst_table; p.dst_stride = dst_stride; p.mass = mass; p.mass_width = mass_width;
+  p.dst = dst_table; p.dst_stride = dst_stride; p.mass = cache->mass; p.mass_width = cache->mass_width;
   p.budget = budget; p.recent = recent; p.sink = sink; p.mass_out = mass_out; p.out_width = mass_out_width; p.kept = kept;
   cudaStream_t st = (cudaStream_t)stream;
   static std::atomic<bool> done[kMaxDevices];
   if ((rc = allow_smem(paged_select_kernel, kSelCached * 4, done))) return rc;
-  const int cached = (int)std::min<int64_t>((int64_t)max_pages * page_size, kSelCached);
+  const int cached = (int)std::min<int64_t>((int64_t)cache->max_pages * page_size, kSelCached);
   rc = launched(launch(paged_select_kernel, dim3(b * hkv), dim3(kSelThreads), cached * 4, st, p, cached), "paged select");
   if (rc) return rc;
   return launched(launch(paged_move_kernel, dim3((unsigned)(per_bh * b * hkv)), dim3(256), 0, st, p, (int)per_bh,
@@ -333,26 +326,29 @@ cudaError_t logits_launch(const LogitsParams& p, bool vec, int slice, int ctas, 
 
 }  // namespace
 
-extern "C" int one_process_logits(const void* logits, int64_t ld, int32_t batch, int32_t vocab, int32_t dtype,
-                                  const void* history, int64_t hist_ld, int32_t hist_len, int32_t hist_bytes,
-                                  const int32_t* output_starts, const float* repetition, float repetition_all,
-                                  const float* presence, float presence_all, const float* frequency, float frequency_all,
-                                  const float* bias, int64_t bias_ld, const int32_t* token_mask, int64_t mask_ld,
-                                  float* out, int64_t out_ld, int32_t* best, void* stream) {
-  if (!logits || !out || (!history && hist_len)) return fail(ONE_ERR_INVALID, "process logits: null argument");
-  if (batch < 1 || vocab < 1 || ld < vocab || out_ld < vocab || hist_len < 0 || (hist_len && hist_ld < hist_len))
+extern "C" int one_process_logits(const one_logits_rules* rules, const void* logits, int64_t ld, int32_t batch,
+                                  int32_t vocab, int32_t dtype, float* out, int64_t out_ld, int32_t* best, void* stream) {
+  if (!rules || !logits || !out || (!rules->history && rules->history_len))
+    return fail(ONE_ERR_INVALID, "process logits: null argument");
+  const one_logits_rules& x = *rules;
+  const int hist_len = x.history_len;
+  if (batch < 1 || vocab < 1 || ld < vocab || out_ld < vocab || hist_len < 0 || (hist_len && x.history_ld < hist_len))
     return fail(ONE_ERR_INVALID, "process logits: bad sizes");
   if (vocab > 0x3fffffff) return fail(ONE_ERR_UNSUPPORTED, "process logits: at most 2^30 - 1 tokens");
   if (dtype != ONE_DTYPE_BF16 && dtype != ONE_DTYPE_F32) return fail(ONE_ERR_INVALID, "dtype");
-  if (hist_len && hist_bytes != 4 && hist_bytes != 8) return fail(ONE_ERR_INVALID, "process logits: int32 or int64 history");
-  if (!(repetition_all > 0.0f)) return fail(ONE_ERR_INVALID, "process logits: the repetition penalty must be positive");
-  if ((bias && bias_ld && bias_ld < vocab) || (token_mask && mask_ld && mask_ld < (vocab + 31) / 32))
+  if (hist_len && x.history_bytes != 4 && x.history_bytes != 8)
+    return fail(ONE_ERR_INVALID, "process logits: int32 or int64 history");
+  if (!(x.repetition_all > 0.0f)) return fail(ONE_ERR_INVALID, "process logits: the repetition penalty must be positive");
+  if ((x.bias && x.bias_ld && x.bias_ld < vocab) || (x.token_mask && x.mask_ld && x.mask_ld < (vocab + 31) / 32))
     return fail(ONE_ERR_INVALID, "process logits: bias or mask rows overlap");
+  const float* bias = x.bias;
+  const int64_t bias_ld = x.bias_ld;
+  const int hist_bytes = x.history_bytes;
   LogitsParams p = {};
-  p.logits = logits; p.ld = ld; p.B = batch; p.V = vocab; p.history = history; p.hist_ld = hist_ld; p.T = hist_len;
-  p.starts = output_starts; p.rep = repetition; p.pres = presence; p.freq = frequency;
-  p.rep1 = repetition_all; p.pres1 = presence_all; p.freq1 = frequency_all;
-  p.bias = bias; p.bias_ld = bias_ld; p.mask = reinterpret_cast<const uint32_t*>(token_mask); p.mask_ld = mask_ld;
+  p.logits = logits; p.ld = ld; p.B = batch; p.V = vocab; p.history = x.history; p.hist_ld = x.history_ld; p.T = hist_len;
+  p.starts = x.output_starts; p.rep = x.repetition; p.pres = x.presence; p.freq = x.frequency;
+  p.rep1 = x.repetition_all; p.pres1 = x.presence_all; p.freq1 = x.frequency_all;
+  p.bias = bias; p.bias_ld = bias_ld; p.mask = reinterpret_cast<const uint32_t*>(x.token_mask); p.mask_ld = x.mask_ld;
   p.out = out; p.out_ld = out_ld; p.best = best;
   cudaStream_t st = (cudaStream_t)stream;
   // enough CTAs per row (at most a portable cluster) to cover the SMs, with a few tokens per thread each

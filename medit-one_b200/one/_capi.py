@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libone_b200.so")
@@ -31,6 +32,13 @@ class OneConfigC(ctypes.Structure):
                                        "top_k", "r", "mlp_bias", "dtype")] + [("rms_norm_eps", c_float),
                                                                               ("rope_theta", c_float),
                                                                               ("use_flash_attention", c_int32)]
+
+
+# The serving operators' structures, packed per call (struct modules pack faster than ctypes fields):
+# one_paged_cache, one_paged_tokens and one_logits_rules of include/one_b200.h.
+PAGED_CACHE = struct.Struct("=QQqqQqQQq7i4x").pack
+PAGED_TOKENS = struct.Struct("=QQQ9qQQQQiii4x").pack
+LOGITS_RULES = struct.Struct("=QqQQQQQqQqiifff4x").pack
 
 
 # name -> (restype, argtypes); exactly the functions declared in include/one_b200.h
@@ -74,20 +82,14 @@ SIGNATURES = {
     "one_selftest_mean_division": (c_int, [c_void_p, c_int32, c_void_p, c_void_p]),
     "one_sample_tokens": (c_int, [c_void_p, c_int32, c_int32, c_int32, c_int32, c_float, c_int32, c_float,
                                   ctypes.c_uint64, ctypes.c_uint64, c_void_p, c_void_p]),
-    "one_paged_append": (c_int, [c_void_p, c_int64, c_int64, c_int64] * 3 + [c_void_p, c_void_p, c_int32, c_void_p,
-                                 c_void_p, c_void_p, c_int64, c_int64, c_int32, c_int32, c_void_p, c_int64, c_int32,
-                                 c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_void_p, c_int64,
-                                 c_void_p, c_void_p]),
+    "one_paged_append": (c_int, [c_void_p, c_void_p, c_void_p]),
     "one_paged_attention_workspace_bytes": (c_size_t, [c_int32] * 8),
-    "one_paged_attention": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int32, c_int32,
-                                    c_void_p, c_int64, c_int32, c_void_p, c_int32, c_int32, c_int32, c_int32, c_float,
-                                    c_int32, c_void_p, c_int64, c_void_p, c_void_p, c_size_t, c_void_p]),
-    "one_paged_evict": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int32, c_int32, c_void_p, c_int64, c_int32,
-                                c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_int64, c_int32, c_int32, c_int32,
-                                c_int32, c_int32, c_int32, c_int32, c_void_p, c_int64, c_void_p, c_void_p]),
-    "one_process_logits": (c_int, [c_void_p, c_int64, c_int32, c_int32, c_int32, c_void_p, c_int64, c_int32, c_int32,
-                                   c_void_p, c_void_p, c_float, c_void_p, c_float, c_void_p, c_float, c_void_p, c_int64,
-                                   c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p]),
+    "one_paged_attention": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int32, c_float, c_void_p, c_void_p, c_size_t,
+                                    c_void_p]),
+    "one_paged_evict": (c_int, [c_void_p, c_void_p, c_int64, c_int32, c_int32, c_int32, c_int32, c_void_p, c_int64,
+                                c_void_p, c_void_p]),
+    "one_process_logits": (c_int, [c_void_p, c_void_p, c_int64, c_int32, c_int32, c_int32, c_void_p, c_int64, c_void_p,
+                                   c_void_p]),
 }
 
 

@@ -337,13 +337,28 @@ def pack_token_mask(allowed: torch.Tensor) -> torch.Tensor:
     return torch.where(words >= 2 ** 31, words - 2 ** 32, words).to(torch.int32)
 
 
-def _penalty(x, name, batch):
-    """(fp32 [batch] tensor or None, scalar) of a penalty given as a number or per row."""
-    if isinstance(x, torch.Tensor):
-        if x.shape != (batch,) or x.dtype != torch.float32 or not x.is_contiguous():
-            raise C.OneError(f"{name} must be a number or fp32 [{batch}]")
-        return x, 1.0
-    return None, float(x)
+def _penalty(x, name, batch, used):
+    """(address of fp32 [batch] or 0, scalar) of a penalty given as a number or per row."""
+    if not isinstance(x, torch.Tensor):
+        return 0, float(x)
+    if x.shape != (batch,) or x.dtype is not torch.float32 or not x.is_contiguous():
+        raise C.OneError(f"{name} must be a number or fp32 [{batch}]")
+    used.append(x)
+    return x.data_ptr(), 1.0
+
+
+def _rows(t, width, batch, dtype, name, used):
+    """(address, row stride) of an optional [width], [1, width] or [batch, width] argument; stride 0:
+    one row for all."""
+    if t is None:
+        return 0, 0
+    shape = t.shape
+    if t.dtype is not dtype or (shape != (width,) and shape != (batch, width) and shape != (1, width)):
+        raise C.OneError(f"{name} must be {dtype} [{width}] or [{batch}, {width}], got {tuple(shape)}")
+    if width > 1 and t.stride(-1) != 1:
+        raise C.OneError(f"{name} rows must be contiguous")
+    used.append(t)
+    return t.data_ptr(), 0 if len(shape) == 1 or shape[0] == 1 else t.stride(0)
 
 
 def process_logits(logits: torch.Tensor, history: Optional[torch.Tensor] = None,
@@ -359,54 +374,57 @@ def process_logits(logits: torch.Tensor, history: Optional[torch.Tensor] = None,
     penalty is a number or fp32 [B]. Returns the scores fp32 [B, V] (`out`, which may be the logits
     when they are fp32), and with return_argmax also int32 [B]: the token of the largest score, the
     lowest among equals; NaN is never chosen; 0 when nothing is left."""
-    if logits.dim() != 2:
+    shape = logits.shape
+    if len(shape) != 2:
         raise C.OneError("process_logits takes logits [batch, vocab]")
-    B, V = logits.shape
-    rep, rep1 = _penalty(repetition_penalty, "repetition_penalty", B)
-    pres, pres1 = _penalty(presence_penalty, "presence_penalty", B)
-    freq, freq1 = _penalty(frequency_penalty, "frequency_penalty", B)
+    B, V = shape
+    dev = logits.get_device()
+    used = []
+    rep, rep1 = _penalty(repetition_penalty, "repetition_penalty", B, used)
+    pres, pres1 = _penalty(presence_penalty, "presence_penalty", B, used)
+    freq, freq1 = _penalty(frequency_penalty, "frequency_penalty", B, used)
     if not rep1 > 0.0:
         raise C.OneError("repetition_penalty must be positive")
-    if history is None and (rep is not None or rep1 != 1.0 or pres is not None or pres1 or freq is not None or freq1):
-        raise C.OneError("penalties need the history")
-    T, hb, hld = 0, 4, 0
+    T, hb, hld, hptr = 0, 4, 0, 0
     if history is not None:
-        if history.dim() != 2 or history.shape[0] != B or history.dtype not in (torch.int32, torch.int64):
+        hshape = history.shape
+        if len(hshape) != 2 or hshape[0] != B or history.dtype not in (torch.int32, torch.int64):
             raise C.OneError(f"history must be int32 or int64 [{B}, T]")
-        T, hb = history.shape[1], history.element_size()
+        T, hb = hshape[1], history.element_size()
         if T > 1 and history.stride(1) != 1:
             history = history.contiguous()
         hld = history.stride(0) if B > 1 else T
-    if output_starts is not None and (output_starts.shape != (B,) or output_starts.dtype != torch.int32
-                                      or not output_starts.is_contiguous()):
-        raise C.OneError(f"output_starts must be int32 [{B}]")
-    words = (V + 31) // 32
-    lds = []
-    for t, width, dt, name in ((bias, V, torch.float32, "bias"), (token_mask, words, torch.int32, "token_mask")):
-        if t is not None and (t.dtype != dt or t.shape not in ((width,), (1, width), (B, width))):
-            raise C.OneError(f"{name} must be {dt} [{width}] or [{B}, {width}], got {tuple(t.shape)}")
-        if t is not None and t.stride(-1) != 1 and width > 1:
-            raise C.OneError(f"{name} rows must be contiguous")
-        lds.append(0 if t is None or t.dim() == 1 or t.shape[0] == 1 else t.stride(0))
-    if out is not None and (out.shape != logits.shape or out.dtype != torch.float32 or (V > 1 and out.stride(1) != 1)):
-        raise C.OneError(f"out must be fp32 [{B}, {V}] with contiguous rows")
+        hptr = history.data_ptr()
+        used.append(history)
+    elif used or rep1 != 1.0 or pres1 or freq1:
+        raise C.OneError("penalties need the history")
+    sptr = 0
+    if output_starts is not None:
+        if output_starts.shape != (B,) or output_starts.dtype is not torch.int32 or not output_starts.is_contiguous():
+            raise C.OneError(f"output_starts must be int32 [{B}]")
+        sptr = output_starts.data_ptr()
+        used.append(output_starts)
+    bptr, bld = _rows(bias, V, B, torch.float32, "bias", used)
+    mptr, mld = _rows(token_mask, (V + 31) // 32, B, torch.int32, "token_mask", used)
+    if out is not None:
+        if out.shape != shape or out.dtype is not torch.float32 or (V > 1 and out.stride(1) != 1):
+            raise C.OneError(f"out must be fp32 [{B}, {V}] with contiguous rows")
+        used.append(out)
     code = C.dtype_code(logits.dtype)
-    if not logits.is_cuda:
+    if dev < 0:
         raise C.OneError("process_logits takes CUDA logits [batch, vocab]")
-    dev = logits.device
-    for t in (history, output_starts, rep, pres, freq, bias, token_mask, out):
-        if t is not None and t.device != dev:
-            raise C.OneError(f"all tensors must be on one device, got {dev} and {t.device}")
+    for t in used:
+        if t.get_device() != dev:
+            raise C.OneError(f"all tensors must be on one device, got {logits.device} and {t.device}")
     if V > 1 and logits.stride(1) != 1:
         logits = logits.contiguous()
     if out is None:
-        out = torch.empty((B, V), dtype=torch.float32, device=dev)
-    best = torch.empty((B,), dtype=torch.int32, device=dev) if return_argmax else None
-
-    def at(t):
-        return 0 if t is None else t.data_ptr()
-
-    _launch(C.LIB.one_process_logits, dev, logits.data_ptr(), logits.stride(0) if B > 1 else V, B, V, code,
-            at(history), hld, T, hb, at(output_starts), at(rep), rep1, at(pres), pres1, at(freq), freq1, at(bias), lds[0],
-            at(token_mask), lds[1], out.data_ptr(), out.stride(0) if B > 1 else V, at(best))
+        out = logits.new_empty(shape, dtype=torch.float32)
+    best, best_ptr = None, 0
+    if return_argmax:
+        best = logits.new_empty((B,), dtype=torch.int32)
+        best_ptr = best.data_ptr()
+    rules = C.LOGITS_RULES(hptr, hld, sptr, rep, pres, freq, bptr, bld, mptr, mld, T, hb, rep1, pres1, freq1)
+    _launch(C.LIB.one_process_logits, dev, rules, logits.data_ptr(), logits.stride(0) if B > 1 else V, B, V, code,
+            out.data_ptr(), out.stride(0) if B > 1 else V, best_ptr)
     return (out, best) if return_argmax else out

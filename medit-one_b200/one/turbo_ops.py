@@ -6,6 +6,7 @@ There is no CPU fallback: the turbo functions require CUDA tensors and raise oth
 from __future__ import annotations
 
 import ctypes
+import functools
 import warnings
 from typing import Optional, Tuple
 
@@ -153,58 +154,74 @@ def turbo_combined_rope_attention(single_x, key, value, cos, sin, lin_q, lin_k, 
 # most 128, any page size. Page numbers or lengths out of range are recorded (ops_error) and the
 # rows that they name left alone.
 
-def _paged(k_pages, v_pages, block_table, lengths, heads_of):
-    """Checks a cache; returns its part of the C argument lists and its sizes."""
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
+_I32, _F32 = torch.int32, torch.float32
+_current_device = torch.cuda.current_device
+# current_stream(dev).cuda_stream without the Stream object around it
+_stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+
+
+def _page_stride(p, n, inner):
+    """Elements from one page to the next; inner: strides of a contiguous page. Dimensions of size 1
+    may have any stride."""
+    s = p.stride()
+    if s[1:] != inner and any(d > 1 and x != y for d, x, y in zip(p.shape[1:], s[1:], inner)):
+        raise ValueError("each page must be contiguous [Hkv, page_size, Dh]")
+    return s[0] if n > 1 else p.shape[1] * inner[0]
+
+
+def _paged(k_pages, v_pages, block_table, lengths, mass, dtype):
+    """Checks a cache and packs it for the C entry points: (device, packed, (B, Hkv, page_size, Dh, max_pages))."""
+    shape = k_pages.shape
+    if len(shape) != 4 or v_pages.shape != shape:
         raise ValueError("k_pages and v_pages must have the same shape [num_pages, Hkv, page_size, Dh]")
-    if block_table.dim() != 2 or lengths.dim() != 1 or block_table.shape[0] != lengths.shape[0]:
+    tshape = block_table.shape
+    if len(tshape) != 2 or lengths.shape != tshape[:1]:
         raise ValueError("block_table must be [B, max_pages] and lengths [B]")
-    if block_table.dtype != torch.int32 or lengths.dtype != torch.int32:
+    if block_table.dtype is not _I32 or lengths.dtype is not _I32:
         raise ValueError("block_table and lengths must be int32")
-    n, hkv, ps, dh = k_pages.shape
-    if heads_of.dtype != k_pages.dtype or v_pages.dtype != k_pages.dtype:
+    if k_pages.dtype is not dtype or v_pages.dtype is not dtype:
         raise ValueError("the cache and the new tokens must have one dtype")
-    strides = []
-    for p in (k_pages, v_pages):
-        s = p.stride()
-        if (dh > 1 and s[3] != 1) or (ps > 1 and s[2] != dh) or (hkv > 1 and s[1] != ps * dh):
-            raise ValueError("each page must be contiguous [Hkv, page_size, Dh]")
-        strides.append(s[0] if n > 1 else hkv * ps * dh)
-    b, mp = block_table.shape
-    if (mp > 1 and block_table.stride(1) != 1) or (b > 1 and lengths.stride(0) != 1):
+    n, hkv, ps, dh = shape
+    b, mp = tshape
+    inner = (ps * dh, dh, 1)
+    ks, vs = _page_stride(k_pages, n, inner), _page_stride(v_pages, n, inner)
+    ts, tc = block_table.stride()
+    if (mp > 1 and tc != 1) or not lengths.is_contiguous():
         raise ValueError("block_table rows and lengths must be contiguous")
-    pools = (k_pages.data_ptr(), v_pages.data_ptr(), strides[0], strides[1], n, ps)
-    table = (block_table.data_ptr(), block_table.stride(0) if b > 1 else mp, mp)
-    return pools, table, (b, hkv, ps, dh, mp)
+    dev = k_pages.get_device()
+    mptr = mw = 0
+    if mass is not None:
+        mshape = mass.shape
+        if len(mshape) != 3 or mass.dtype is not _F32 or mshape[0] != b or mshape[1] != hkv or mshape[2] < mp * ps:
+            raise ValueError(f"mass must be fp32 [{b}, {hkv}, at least {mp * ps}]")
+        if not mass.is_contiguous():
+            raise ValueError("mass must be contiguous")
+        mptr, mw = mass.data_ptr(), mshape[2]
+        if mass.get_device() != dev:
+            raise ValueError("all tensors must be on one device")
+    if v_pages.get_device() != dev or block_table.get_device() != dev or lengths.get_device() != dev:
+        raise ValueError("all tensors must be on one device")
+    code = C.dtype_code(dtype) if C is not None else 0
+    packed = C.PAGED_CACHE(k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, block_table.data_ptr(), ts if b > 1 else mp,
+                           lengths.data_ptr(), mptr, mw, n, ps, mp, b, hkv, dh, code) if C is not None else b""
+    return dev, packed, (b, hkv, ps, dh, mp)
 
 
-def _paged_mass(mass, b, hkv, slots, what="mass"):
-    if mass is None:
-        return 0, 0
-    if mass.dim() != 3 or mass.dtype != torch.float32 or mass.shape[:2] != (b, hkv) or mass.shape[2] < slots:
-        raise ValueError(f"{what} must be fp32 [{b}, {hkv}, at least {slots}]")
-    if not mass.is_contiguous():
-        raise ValueError(f"{what} must be contiguous")
-    return mass.data_ptr(), mass.shape[2]
+def _cuda(dev, first):
+    """Refuses tensors that are not on a GPU."""
+    if dev < 0 or not TURBO_MODE:
+        _need(first)
 
 
-def _launch(fn, device, *args):
-    """Calls a C entry point on `device`'s current stream; every tensor must live on that device."""
-    if torch.cuda.current_device() == device.index:
-        rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+def _launch(fn, dev, *args):
+    """Calls a C entry point on the current stream of device `dev`, where every tensor lives."""
+    if _current_device() == dev:
+        rc = fn(*args, _stream_of(dev))
     else:
-        with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+        with torch.cuda.device(dev):
+            rc = fn(*args, _stream_of(dev))
     if rc:
         C.check(rc, fn.__name__)
-
-
-def _one_device(first, *ts):
-    _need(first)
-    for t in ts:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"all tensors must be on one device, got {first.device} and {t.device}")
-    return first.device
 
 
 def _rows_last(t):
@@ -220,42 +237,59 @@ def turbo_paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, 
     .. lengths[b] + counts[b] - 1 (counts int32 [B], default N), k rotated by cos, sin [B or 1, N, Dh]
     (apply_rotary_pos_emb_flash in fp32, rounded once) when they are given; the slots' mass becomes 0.
     Returns q [B, Hq, N, Dh] rotated the same way, or None without q. The caller advances lengths."""
-    pools, table, (b, hkv, ps, dh, mp) = _paged(k_pages, v_pages, block_table, lengths, k)
-    if k.dim() != 4 or k.shape != v.shape or k.shape[0] != b or k.shape[1] != hkv or k.shape[3] != dh:
+    dt = k.dtype
+    dev, cache, (b, hkv, ps, dh, mp) = _paged(k_pages, v_pages, block_table, lengths, mass, dt)
+    shape = k.shape
+    if len(shape) != 4 or v.shape != shape or shape[0] != b or shape[1] != hkv or shape[3] != dh:
         raise ValueError(f"k and v must be [{b}, {hkv}, N, {dh}], got {tuple(k.shape)} and {tuple(v.shape)}")
-    n = k.shape[2]
-    if v.dtype != k.dtype or (q is not None and q.dtype != k.dtype):
+    n = shape[2]
+    if v.dtype is not dt or (q is not None and q.dtype is not dt):
         raise ValueError("the cache and the new tokens must have one dtype")
-    if q is not None and (q.dim() != 4 or (q.shape[0], q.shape[2], q.shape[3]) != (b, n, dh)):
-        raise ValueError(f"q must be [{b}, Hq, {n}, {dh}], got {tuple(q.shape)}")
-    if counts is not None and (counts.dtype != torch.int32 or counts.shape != (b,) or not counts.is_contiguous()):
-        raise ValueError(f"counts must be int32 [{b}]")
+    hq = cptr = 0
+    if q is not None:
+        qshape = q.shape
+        if len(qshape) != 4 or qshape[0] != b or qshape[2] != n or qshape[3] != dh:
+            raise ValueError(f"q must be [{b}, Hq, {n}, {dh}], got {tuple(qshape)}")
+        hq = qshape[1]
+        if q.get_device() != dev:
+            raise ValueError("all tensors must be on one device")
+    if counts is not None:
+        if counts.dtype is not _I32 or counts.shape != (b,) or not counts.is_contiguous():
+            raise ValueError(f"counts must be int32 [{b}]")
+        cptr = counts.data_ptr()
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin come together")
     cb = 1
     if cos is not None:
-        cb = cos.shape[0] if cos.dim() == 3 else 1
-        if cos.shape[-2:] != (n, dh) or sin.shape != cos.shape or cos.dim() not in (2, 3) or cb not in (1, b):
-            raise ValueError(f"cos / sin must be [B or 1, {n}, {dh}], got {tuple(cos.shape)}")
-    ms = _paged_mass(mass, b, hkv, mp * ps)
-    dt = C.dtype_code(k.dtype) if C else 0
-    dev = _one_device(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, counts, mass)
-    k, v = _rows_last(k), _rows_last(v)
-    out, qa, hq = None, (0, 0, 0, 0), 0
+        cshape = cos.shape
+        cb = cshape[0] if len(cshape) == 3 else 1
+        if cshape[-2:] != (n, dh) or sin.shape != cshape or len(cshape) not in (2, 3) or cb not in (1, b):
+            raise ValueError(f"cos / sin must be [B or 1, {n}, {dh}], got {tuple(cshape)}")
+    for t in (k, v, counts, cos, sin):
+        if t is not None and t.get_device() != dev:
+            raise ValueError("all tensors must be on one device")
+    _cuda(dev, k)
+    out, optr, qptr, qs = None, 0, 0, (0, 0, 0, 0)
     if q is not None:
         q = _rows_last(q)
-        hq = q.shape[1]
-        out = torch.empty((b, hq, n, dh), dtype=q.dtype, device=dev)
-        qs = q.stride()
-        qa = (q.data_ptr(), qs[0], qs[1], qs[2])
+        out = q.new_empty((b, hq, n, dh))
+        optr, qptr, qs = out.data_ptr(), q.data_ptr(), q.stride()
+    cosp = sinp = 0
     if cos is not None:
-        cos, sin = cos.to(k.dtype).contiguous(), sin.to(k.dtype).contiguous()
-    kst, vst = k.stride(), v.stride()
-    _launch(C.LIB.one_paged_append, dev, k.data_ptr(), kst[0], kst[1], kst[2], v.data_ptr(), vst[0], vst[1], vst[2], *qa,
-            0 if cos is None else cos.data_ptr(), 0 if sin is None else sin.data_ptr(), cb,
-            0 if counts is None else counts.data_ptr(), *pools, *table, lengths.data_ptr(), b, n, hq, hkv, dh, dt, *ms,
-            0 if out is None else out.data_ptr())
+        if cos.dtype is not dt or sin.dtype is not dt or not cos.is_contiguous() or not sin.is_contiguous():
+            cos, sin = cos.to(dt).contiguous(), sin.to(dt).contiguous()
+        cosp, sinp = cos.data_ptr(), sin.data_ptr()
+    k, v = _rows_last(k), _rows_last(v)
+    ks, vs = k.stride(), v.stride()
+    _launch(C.LIB.one_paged_append, dev, cache,
+            C.PAGED_TOKENS(k.data_ptr(), v.data_ptr(), qptr, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], qs[0], qs[1], qs[2],
+                           cosp, sinp, cptr, optr, n, hq, cb))
     return out
+
+
+@functools.lru_cache(maxsize=1024)
+def _attention_workspace(*sizes):
+    return C.LIB.one_paged_attention_workspace_bytes(*sizes)
 
 
 def turbo_paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
@@ -265,23 +299,25 @@ def turbo_paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch
     lengths[b]: softmax(q k^T * scale) v with an fp32 softmax, scale 1/sqrt(Dh) by default. Hq is a
     multiple of Hkv: query head j reads kv head j // (Hq // Hkv). A sequence without slots gives
     zeros. mass grows by the softmax weights, summed over each kv head's query heads."""
-    pools, table, (b, hkv, ps, dh, mp) = _paged(k_pages, v_pages, block_table, lengths, q)
-    if q.dim() != 4 or q.shape[0] != b or q.shape[2] != 1 or q.shape[3] != dh or q.shape[1] % hkv:
-        raise ValueError(f"q must be [{b}, a multiple of {hkv}, 1, {dh}], got {tuple(q.shape)}")
-    hq = q.shape[1]
-    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous()):
-        raise ValueError(f"out must be contiguous {tuple(q.shape)} in {q.dtype}")
-    ms = _paged_mass(mass, b, hkv, mp * ps)
-    dt = C.dtype_code(q.dtype) if C else 0
-    dev = _one_device(q, k_pages, v_pages, block_table, lengths, mass, out)
+    dt = q.dtype
+    dev, cache, (b, hkv, ps, dh, mp) = _paged(k_pages, v_pages, block_table, lengths, mass, dt)
+    shape = q.shape
+    if len(shape) != 4 or shape[0] != b or shape[2] != 1 or shape[3] != dh or shape[1] % hkv:
+        raise ValueError(f"q must be [{b}, a multiple of {hkv}, 1, {dh}], got {tuple(shape)}")
+    if q.get_device() != dev or (out is not None and out.get_device() != dev):
+        raise ValueError("all tensors must be on one device")
+    if out is not None and (out.shape != shape or out.dtype is not dt or not out.is_contiguous()):
+        raise ValueError(f"out must be contiguous {tuple(shape)} in {dt}")
+    _cuda(dev, q)
+    hq = shape[1]
     q = _rows_last(q)
     if out is None:
-        out = torch.empty((b, hq, 1, dh), dtype=q.dtype, device=dev)
-    nws = C.LIB.one_paged_attention_workspace_bytes(b, hq, hkv, dh, ps, mp, dt, mass is not None)
-    ws = torch.empty(nws, dtype=torch.uint8, device=dev)
+        out = q.new_empty(shape)
+    nws = _attention_workspace(b, hq, hkv, dh, ps, mp, C.dtype_code(dt), mass is not None)
+    ws = q.new_empty(nws, dtype=torch.uint8) if nws else None
     qs = q.stride()
-    _launch(C.LIB.one_paged_attention, dev, q.data_ptr(), qs[0], qs[1], *pools, *table, lengths.data_ptr(), b, hq, hkv, dh,
-            1.0 / (dh ** 0.5) if scale_factor is None else float(scale_factor), dt, *ms, out.data_ptr(), ws.data_ptr(), nws)
+    _launch(C.LIB.one_paged_attention, dev, cache, q.data_ptr(), qs[0], qs[1], hq,
+            dh ** -0.5 if scale_factor is None else float(scale_factor), out.data_ptr(), ws.data_ptr() if nws else 0, nws)
     return out
 
 
@@ -294,27 +330,29 @@ def turbo_paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table:
     that dst_block_table [B, dst pages] names, none of which block_table may use. Returns (mass_out
     [B, Hkv, dst pages * page_size]: the survivors' masses, then 0; kept int32 [B, Hkv, budget]: their
     slots, then -1). The caller goes on with dst_block_table and lengths.clamp(max=budget)."""
-    pools, table, (b, hkv, ps, dh, mp) = _paged(k_pages, v_pages, block_table, lengths, k_pages)
+    if mass is None:
+        raise ValueError("eviction goes by mass")
+    dev, cache, (b, hkv, ps, dh, mp) = _paged(k_pages, v_pages, block_table, lengths, mass, k_pages.dtype)
     budget, recent, sink = int(budget), int(recent), int(sink)
     if budget < 1 or recent < 0 or sink < 0 or recent + sink > budget:
         raise ValueError("1 <= budget, 0 <= recent, 0 <= sink and recent + sink <= budget")
     d = dst_block_table
-    if d.dim() != 2 or d.dtype != torch.int32 or d.shape[0] != b or (d.shape[1] > 1 and d.stride(1) != 1):
+    dshape = d.shape
+    if len(dshape) != 2 or d.dtype is not _I32 or dshape[0] != b or (dshape[1] > 1 and d.stride(1) != 1):
         raise ValueError(f"dst_block_table must be int32 [{b}, dst pages] with contiguous rows")
-    if d.shape[1] * ps < budget:
-        raise ValueError(f"dst_block_table holds {d.shape[1] * ps} slots, fewer than the budget {budget}")
+    dp = dshape[1]
+    width = dp * ps
+    if width < budget:
+        raise ValueError(f"dst_block_table holds {width} slots, fewer than the budget {budget}")
     if d.data_ptr() == block_table.data_ptr():
         raise ValueError("survivors go to other pages: dst_block_table is block_table")
-    if mass is None:
-        raise ValueError("eviction goes by mass")
-    ms = _paged_mass(mass, b, hkv, mp * ps)
-    dt = C.dtype_code(k_pages.dtype) if C else 0
-    dev = _one_device(k_pages, v_pages, block_table, d, lengths, mass)
-    width = d.shape[1] * ps
-    mass_out = torch.empty((b, hkv, width), dtype=torch.float32, device=dev)
-    kept = torch.empty((b, hkv, budget), dtype=torch.int32, device=dev)
-    _launch(C.LIB.one_paged_evict, dev, *pools, *table, d.data_ptr(), d.stride(0) if b > 1 else d.shape[1], d.shape[1],
-            lengths.data_ptr(), *ms, b, hkv, dh, dt, budget, recent, sink, mass_out.data_ptr(), width, kept.data_ptr())
+    if d.get_device() != dev:
+        raise ValueError("all tensors must be on one device")
+    _cuda(dev, k_pages)
+    mass_out = mass.new_empty((b, hkv, width))
+    kept = d.new_empty((b, hkv, budget))
+    _launch(C.LIB.one_paged_evict, dev, cache, d.data_ptr(), d.stride(0) if b > 1 else dp, dp, budget, recent, sink,
+            mass_out.data_ptr(), width, kept.data_ptr())
     return mass_out, kept
 
 

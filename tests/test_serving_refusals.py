@@ -1,5 +1,7 @@
 """What the serving operators refuse, on the CPU: in Python before any CUDA call, and at the C entry
 points before any launch."""
+import ctypes
+
 import pytest
 import torch
 
@@ -121,50 +123,107 @@ def test_token_mask_words():
     assert torch.equal(pack_token_mask(allowed[0]), w[0])
 
 
-def test_c_entry_points_refuse_before_launching():
-    """Valid-looking addresses that no launch may reach: every call here is refused by its sizes."""
-    a, b = 4096, 2048
+class Cache(ctypes.Structure):
+    """one_paged_cache of include/one_b200.h, field by field."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("kp", "vp")] + [(n, ctypes.c_int64) for n in ("ks", "vs")]
+                + [("table", ctypes.c_void_p), ("ts", ctypes.c_int64), ("ln", ctypes.c_void_p), ("mass", ctypes.c_void_p),
+                   ("mw", ctypes.c_int64)] + [(n, ctypes.c_int32) for n in ("pages", "ps", "mp", "B", "hkv", "dh", "dt", "reserved")])
 
-    def attention(**kw):
-        d = dict(q=a, qb=256, qh=64, k=a, v=a, ks=2048, vs=2048, pages=4, ps=16, table=b, ts=3, mp=3, ln=b, B=2, hq=4, hkv=2, dh=64,
-                 scale=0.1, dt=0, mass=0, mw=0, out=a, ws=a, wb=1 << 30, st=0)
-        d.update(kw)
-        return C.LIB.one_paged_attention(*d.values())
 
-    for kw in (dict(q=0), dict(k=0), dict(table=0), dict(ln=0), dict(out=0), dict(ws=0), dict(wb=0), dict(dt=2), dict(hq=3),
-               dict(hq=0), dict(B=0), dict(ps=0), dict(pages=0), dict(mp=0), dict(ts=2), dict(ks=2047), dict(vs=100), dict(k=a + 2),
-               dict(ks=2052), dict(mass=a, mw=47)):
-        assert attention(**kw) == C.ONE_ERR_INVALID, kw
-    for kw in (dict(dh=60), dict(dh=136, ks=1 << 20, vs=1 << 20), dict(B=70000), dict(hkv=70000, hq=70000, ks=1 << 30, vs=1 << 30),
-               dict(ps=1 << 20, mp=1 << 12, ts=1 << 12, ks=1 << 30, vs=1 << 30)):
-        assert attention(**kw) == C.ONE_ERR_UNSUPPORTED, kw
+class Tokens(ctypes.Structure):
+    """one_paged_tokens."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in "kvq"] + [(n, ctypes.c_int64 * 3) for n in ("k_s", "v_s", "q_s")]
+                + [(n, ctypes.c_void_p) for n in ("cos", "sin", "counts", "out")]
+                + [(n, ctypes.c_int32) for n in ("n", "hq", "cb", "reserved")])
 
-    def append(**kw):
-        d = dict(k=a, k1=1, k2=1, k3=1, v=a, v1=1, v2=1, v3=1, q=a, q1=1, q2=1, q3=1, cos=a, sin=a, cb=1, cnt=0, kp=a, vp=a, ks=2048,
-                 vs=2048, pages=4, ps=16, table=b, ts=3, mp=3, ln=b, B=2, n=1, hq=2, hkv=2, dh=64, dt=0, mass=0, mw=0, out=a, st=0)
-        d.update(kw)
-        return C.LIB.one_paged_append(*d.values())
 
-    for kw in (dict(k=0), dict(v=0), dict(out=0), dict(q=0), dict(sin=0), dict(cb=3), dict(n=0), dict(hq=0), dict(kp=0),
-               dict(mass=a, mw=1)):
-        assert append(**kw) == C.ONE_ERR_INVALID, kw
+class Rules(ctypes.Structure):
+    """one_logits_rules."""
+    _fields_ = ([("h", ctypes.c_void_p), ("hl", ctypes.c_int64)] + [(n, ctypes.c_void_p) for n in ("starts", "r", "p", "f", "bias")]
+                + [("bl", ctypes.c_int64), ("mask", ctypes.c_void_p), ("ml", ctypes.c_int64)]
+                + [(n, ctypes.c_int32) for n in ("T", "hb")] + [(n, ctypes.c_float) for n in ("r1", "p1", "f1")]
+                + [("reserved", ctypes.c_int32)])
 
-    def evict(**kw):
-        d = dict(kp=a, vp=a, ks=2048, vs=2048, pages=4, ps=16, table=b, ts=3, mp=3, dst=a, ds=2, dm=2, ln=b, mass=a, mw=48, B=2, hkv=2,
-                 dh=64, dt=0, budget=32, recent=8, sink=4, mo=b, mow=32, kept=b, st=0)
-        d.update(kw)
-        return C.LIB.one_paged_evict(*d.values())
 
-    for kw in (dict(budget=0), dict(recent=30), dict(sink=-1), dict(budget=33, mow=33), dict(mow=31), dict(mw=47), dict(ds=1),
-               dict(kept=0), dict(mass=0), dict(mo=0), dict(dst=0)):
-        assert evict(**kw) == C.ONE_ERR_INVALID, kw
+A, B_ = 4096, 2048  # valid-looking addresses that no launch may reach: every call below is refused
+CACHE = dict(kp=A, vp=A, ks=2048, vs=2048, table=B_, ts=3, ln=B_, mass=0, mw=0, pages=4, ps=16, mp=3, B=2, hkv=2, dh=64, dt=0)
 
-    def logits(**kw):
-        d = dict(x=a, ld=100, B=2, V=100, dt=0, h=a, hl=5, T=5, hb=8, st0=0, r=0, r1=1.0, p=0, p1=0.0, f=0, f1=0.0, bias=0, bl=0,
-                 mask=0, ml=0, out=b, ol=100, best=0, st=0)
-        d.update(kw)
-        return C.LIB.one_process_logits(*d.values())
 
-    for kw in (dict(x=0), dict(out=0), dict(h=0), dict(ld=99), dict(ol=99), dict(hl=4), dict(hb=2), dict(dt=5), dict(r1=0.0),
-               dict(r1=float("nan")), dict(bias=a, bl=99), dict(mask=a, ml=3), dict(B=0), dict(V=0), dict(T=-1)):
-        assert logits(**kw) == C.ONE_ERR_INVALID, kw
+def packs(struct, packed, values):
+    """The packed form that the package hands to the library equals the structure's."""
+    x = struct(**values)
+    assert bytes(x) == packed and ctypes.sizeof(struct) == len(packed)
+
+
+def test_packed_structures_match_the_header():
+    v = dict(zip([n for n, _ in Cache._fields_ if n != "reserved"], range(1, 17)))
+    packs(Cache, C.PAGED_CACHE(*v.values()), v)
+    n = [x for x, _ in Tokens._fields_ if x != "reserved"]
+    flat = list(range(1, 4)) + list(range(10, 19)) + list(range(20, 27))
+    v = dict(zip(n[:3], flat[:3]), k_s=(ctypes.c_int64 * 3)(10, 11, 12), v_s=(ctypes.c_int64 * 3)(13, 14, 15),
+             q_s=(ctypes.c_int64 * 3)(16, 17, 18), **dict(zip(n[6:], flat[12:])))
+    packs(Tokens, C.PAGED_TOKENS(*flat), v)
+    v = dict(zip([x for x, _ in Rules._fields_ if x != "reserved"], range(1, 16)))
+    packs(Rules, C.LOGITS_RULES(*v.values()), v)
+
+
+def refused(call, base, invalid, unsupported=()):
+    for kw in invalid:
+        assert call(**{**base, **kw}) == C.ONE_ERR_INVALID, kw
+    for kw in unsupported:
+        assert call(**{**base, **kw}) == C.ONE_ERR_UNSUPPORTED, kw
+
+
+def cache_of(d):
+    return ctypes.byref(Cache(**{k: d[k] for k in CACHE}))
+
+
+BAD_CACHE = [dict(kp=0), dict(vp=0), dict(table=0), dict(ln=0), dict(dt=2), dict(B=0), dict(ps=0), dict(pages=0), dict(mp=0),
+             dict(ts=2), dict(ks=2047), dict(vs=100), dict(kp=A + 2), dict(ks=2052), dict(mass=A, mw=47)]
+BIG_CACHE = [dict(dh=60), dict(dh=136, ks=1 << 20, vs=1 << 20), dict(B=70000), dict(hkv=70000, hq=70000, ks=1 << 30, vs=1 << 30),
+             dict(ps=1 << 20, mp=1 << 12, ts=1 << 12, ks=1 << 30, vs=1 << 30), dict(ks=1 << 31), dict(vs=1 << 33)]
+
+
+def test_c_attention_refuses_before_launching():
+    def call(q, qb, qh, hq, out, ws, wb, **cache):
+        return C.LIB.one_paged_attention(cache_of(cache), q, qb, qh, hq, 0.1, out, ws, wb, 0)
+    base = dict(CACHE, mp=64, ts=64, q=A, qb=256, qh=64, hq=4, out=A, ws=A, wb=1 << 30)
+    refused(call, base, [k for k in BAD_CACHE if k != dict(ts=2)] + [dict(ts=63), dict(q=0), dict(out=0), dict(ws=0), dict(wb=64),
+                                                                    dict(hq=3), dict(hq=0)], BIG_CACHE)
+    assert C.LIB.one_paged_attention(None, A, 1, 1, 4, 0.1, A, A, 1 << 30, 0) == C.ONE_ERR_INVALID
+    # short caches need no workspace, others do
+    assert C.LIB.one_paged_attention_workspace_bytes(2, 4, 2, 64, 16, 3, 0, 0) == 0
+    assert C.LIB.one_paged_attention_workspace_bytes(2, 4, 2, 64, 16, 3, 0, 1) > 0
+    assert C.LIB.one_paged_attention_workspace_bytes(2, 4, 2, 64, 16, 100, 0, 0) > 0
+
+
+def test_c_append_refuses_before_launching():
+    three = (ctypes.c_int64 * 3)(64, 64, 64)
+
+    def call(k, v, q, cos, sin, out, n, hq, cb, **cache):
+        t = Tokens(k=k, v=v, q=q, k_s=three, v_s=three, q_s=three, cos=cos, sin=sin, counts=0, out=out, n=n, hq=hq, cb=cb)
+        return C.LIB.one_paged_append(cache_of(cache), ctypes.byref(t), 0)
+    base = dict(CACHE, k=A, v=A, q=A, cos=A, sin=A, out=A, n=1, hq=2, cb=1)
+    refused(call, base, BAD_CACHE + [dict(k=0), dict(v=0), dict(out=0), dict(q=0), dict(sin=0), dict(cos=0), dict(cb=3), dict(n=0),
+                                     dict(hq=0)], [x for x in BIG_CACHE if "hq" not in x] + [dict(n=1 << 30)])
+    assert C.LIB.one_paged_append(cache_of(CACHE), None, 0) == C.ONE_ERR_INVALID
+
+
+def test_c_evict_refuses_before_launching():
+    def call(dst, ds, dm, budget, recent, sink, mo, mow, kept, **cache):
+        return C.LIB.one_paged_evict(cache_of(cache), dst, ds, dm, budget, recent, sink, mo, mow, kept, 0)
+    base = dict(CACHE, mass=A, mw=48, dst=A, ds=2, dm=2, budget=32, recent=8, sink=4, mo=B_, mow=32, kept=B_)
+    refused(call, base, [k for k in BAD_CACHE if "mass" not in k] + [
+        dict(budget=0), dict(recent=30), dict(sink=-1), dict(recent=-1), dict(budget=33, mow=33), dict(mow=31), dict(mw=47), dict(ds=1),
+        dict(dm=0), dict(kept=0), dict(mass=0), dict(mo=0), dict(dst=0)], [dict(dh=60), dict(B=70000), dict(mow=1 << 31)])
+
+
+def test_c_logits_refuse_before_launching():
+    def call(x, ld, B, V, dt, out, ol, **rules):
+        return C.LIB.one_process_logits(ctypes.byref(Rules(**rules)), x, ld, B, V, dt, out, ol, 0, 0)
+    base = dict(x=A, ld=100, B=2, V=100, dt=0, out=B_, ol=100, h=A, hl=5, T=5, hb=8, starts=0, r=0, r1=1.0, p=0, p1=0.0, f=0, f1=0.0,
+                bias=0, bl=0, mask=0, ml=0)
+    refused(call, base, [dict(x=0), dict(out=0), dict(h=0), dict(ld=99), dict(ol=99), dict(hl=4), dict(hb=2), dict(dt=5), dict(r1=0.0),
+                         dict(r1=float("nan")), dict(bias=A, bl=99), dict(mask=A, ml=3), dict(B=0), dict(V=0), dict(T=-1)],
+            [dict(V=1 << 30, ld=1 << 30, ol=1 << 30)])
+    assert C.LIB.one_process_logits(None, A, 100, 2, 100, 0, B_, 100, 0, 0) == C.ONE_ERR_INVALID
