@@ -36,86 +36,166 @@ struct LogitsParams {
 
 constexpr int kLogitsThreads = 512;
 constexpr int kLogitsCounts = 16384;  // counts held at a time (64 KB)
+constexpr int kLogitsAhead = 2;       // vectors per thread, and
+constexpr int kLogitsIds = 4;         // history entries per thread, that are asked for at once at the start
 
-// A cluster of CTAs per row, each with a slice of the vocabulary (a multiple of 32 tokens). Per up to
-// kLogitsCounts tokens of it: the history's counts in shared memory (bit 31: the token occurs before the output;
-// integer atomics, so the order does not matter), then one pass over the logits. The best token goes
-// through the CTAs' shared memory to the cluster's first one. Bound by HBM (one read, one write) when
-// there are many rows, by the chain history -> counts -> logits for a single one.
-// VEC: eight tokens per thread and step, all rows on 16-byte boundaries.
-template <typename T, typename I, bool VEC>
-__global__ void __launch_bounds__(kLogitsThreads) logits_kernel(const __grid_constant__ LogitsParams p, int slice, int ctas) {
+template <typename T> struct LogitsVec;  // four logits as they lie in memory
+template <> struct LogitsVec<__nv_bfloat16> {
+  using Raw = uint2;
+  ONE_DEVINL static void open(Raw u, float (&v)[4]) {
+    v[0] = bf2_lo(u.x); v[1] = bf2_hi(u.x); v[2] = bf2_lo(u.y); v[3] = bf2_hi(u.y);
+  }
+};
+template <> struct LogitsVec<float> {
+  using Raw = float4;
+  ONE_DEVINL static void open(Raw u, float (&v)[4]) {
+    v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
+  }
+};
+
+// A cluster of CTAs per row, each with a slice of the vocabulary. Per up to kLogitsCounts tokens of
+// it: the history's counts in shared memory (bit 31: the token occurs before the output; integer
+// atomics, so the order does not matter), then one pass over the logits. Bound by HBM (one read, one
+// write) when there are many rows, by the chain history -> counts -> scores for a single one, so the
+// first history entries and logits are asked for together, before anything waits.
+//
+// Four tokens per thread and step, starting at the row's first 16-byte boundary of the scores: rows of
+// an odd vocabulary start anywhere, but logits and scores are off by the same number of tokens unless
+// the caller's strides differ (then: token by token).
+//
+// Each CTA's best token goes into the shared memory of the cluster's first CTA, which alone waits.
+template <typename T, typename I>
+__global__ void __launch_bounds__(kLogitsThreads, 2) logits_kernel(const __grid_constant__ LogitsParams p, int slice, int ctas) {
+  using V4 = LogitsVec<T>;
   extern __shared__ __align__(16) uint32_t cnt[];
   __shared__ float bv[kLogitsThreads / 32];
   __shared__ int bi[kLogitsThreads / 32];
-  __shared__ unsigned long long mine;
+  __shared__ unsigned long long theirs[8];  // of the cluster's first CTA: every CTA's best
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int b = blockIdx.x / ctas, rank = blockIdx.x % ctas;
-  const int vbeg = rank * slice, vend = min(p.V, vbeg + slice);
+  if (ctas > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // this CTA exists
   pdl_wait();
-  const I* hist = (const I*)p.history + b * p.hist_ld;
-  const int start = p.starts ? p.starts[b] : 0;
-  const float r = p.rep ? p.rep[b] : p.rep1, pr = p.pres ? p.pres[b] : p.pres1, f = p.freq ? p.freq[b] : p.freq1;
   const T* x = (const T*)p.logits + b * p.ld;
   float* z = p.out + b * p.out_ld;
   const float* bias = p.bias ? p.bias + b * p.bias_ld : nullptr;
   const uint32_t* mask = p.mask ? p.mask + b * p.mask_ld : nullptr;
+  const int phase = (int)(reinterpret_cast<uintptr_t>(z) >> 2 & 3), head = min((4 - phase) & 3, p.V);
+  const bool vec = (int)(reinterpret_cast<uintptr_t>(x) / sizeof(T) & 3) == phase;
+  const bool bias_vec = bias && (int)(reinterpret_cast<uintptr_t>(bias) >> 2 & 3) == phase;
+  const int beg = head + rank * slice, end = min(p.V, beg + slice);  // the first CTA takes [0, head) too
+  const I* hist = (const I*)p.history + b * p.hist_ld;
+  I ids[kLogitsIds];
+#pragma unroll
+  for (int k = 0; k < kLogitsIds; ++k) ids[k] = k * kLogitsThreads + tid < p.T ? __ldg(hist + k * kLogitsThreads + tid) : I(-1);
+  // logits of the next kLogitsAhead vectors: the scores may overwrite the logits, so the compiler would
+  // not move a load above the stores before it
+  typename V4::Raw ahead[kLogitsAhead];
+  auto ask = [&](int i0, int v0, int n) {
+#pragma unroll
+    for (int k = 0; k < kLogitsAhead; ++k) {
+      const int i = i0 + (k * kLogitsThreads + tid) * 4;
+      if (i + 4 <= n) ahead[k] = *reinterpret_cast<const typename V4::Raw*>(x + v0 + i);
+    }
+  };
+  if (vec) ask(0, beg, min(kLogitsCounts, end - beg));
+  const int start = p.starts ? p.starts[b] : 0;
+  const float r = p.rep ? p.rep[b] : p.rep1, pr = p.pres ? p.pres[b] : p.pres1, f = p.freq ? p.freq[b] : p.freq1;
   float best = -INFINITY;
   int at = 0x7fffffff;
-  auto one_token = [&](float v, uint32_t u, int tok, float add, bool allowed) -> float {
-    if (u) {
-      v = v > 0.f ? v / r : v * r;
-      const uint32_t n = u & 0x7fffffffu;
-      if (n) v -= f * (float)n + pr;
-    }
-    if (bias) v += add;
-    if (!allowed) v = -INFINITY;
-    if (v > best) {
-      best = v;
-      at = tok;
-    }
-    return v;
+  auto penalise = [&](float v, uint32_t u) -> float {
+    v = v > 0.f ? v / r : v * r;
+    const uint32_t n = u & 0x7fffffffu;
+    return n ? v - (f * (float)n + pr) : v;
   };
-  for (int v0 = vbeg; v0 < vend; v0 += kLogitsCounts) {
-    const int n = min(kLogitsCounts, vend - v0);
+  auto one_token = [&](int v, uint32_t u) {
+    float y = ld<T>(x + v);
+    if (u) y = penalise(y, u);
+    if (bias) y += bias[v];
+    if (mask && !(mask[v >> 5] >> (v & 31) & 1)) y = -INFINITY;
+    z[v] = y;
+    if (y > best) {
+      best = y;
+      at = v;
+    }
+  };
+  for (int v0 = beg; v0 < end || (v0 == beg && rank == 0); v0 += kLogitsCounts) {
+    const int n = max(0, min(kLogitsCounts, end - v0)), lo = v0 == 0 + head ? -head : 0;  // counts of [v0 + lo, v0 + n)
     if (p.T) {
-      if (v0 != vbeg) __syncthreads();
-      for (int i = tid * 4; i < n; i += kLogitsThreads * 4) *reinterpret_cast<uint4*>(cnt + i) = make_uint4(0, 0, 0, 0);
+      if (v0 != beg) __syncthreads();
+      for (int i = tid * 4; i < n + 4; i += kLogitsThreads * 4) *reinterpret_cast<uint4*>(cnt + i) = make_uint4(0, 0, 0, 0);
       __syncthreads();
-#pragma unroll 4
-      for (int t = tid; t < p.T; t += kLogitsThreads) {
-        const uint64_t id = (uint64_t)(int64_t)hist[t] - (uint64_t)v0;
-        if (id < (uint64_t)n) {
-          if (t >= start) atomicAdd(&cnt[id], 1u);
-          else atomicOr(&cnt[id], 0x80000000u);
+      auto count = [&](I x, int t) {
+        const uint64_t id = (uint64_t)(int64_t)x - (uint64_t)(int64_t)(v0 + lo);
+        if (id < (uint64_t)(n - lo)) {
+          uint32_t* c = cnt + 4 + lo + (int)id;
+          if (t >= start) atomicAdd(c, 1u);
+          else atomicOr(c, 0x80000000u);
         }
-      }
+      };
+#pragma unroll
+      for (int k = 0; k < kLogitsIds; ++k) count(ids[k], k * kLogitsThreads + tid);
+#pragma unroll 4
+      for (int t = kLogitsIds * kLogitsThreads + tid; t < p.T; t += kLogitsThreads) count(__ldg(hist + t), t);
       __syncthreads();
     }
-    if (VEC) {
-      for (int i = tid * 8; i < n; i += kLogitsThreads * 8) {
-        float v[8], add[8];
-        load8(x + v0 + i, v);
-        if (bias) load8(bias + v0 + i, add);
-        const uint32_t bits = mask ? mask[(v0 + i) >> 5] >> (i & 31) : 0xffu;
-        uint4 u0 = make_uint4(0, 0, 0, 0), u1 = u0;
-        if (p.T) {
-          u0 = *reinterpret_cast<const uint4*>(cnt + i);
-          u1 = *reinterpret_cast<const uint4*>(cnt + i + 4);
-        }
-        const uint32_t u[8] = {u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w};
+    if (lo < 0 && tid < -lo) one_token(tid, p.T ? cnt[4 + lo + tid] : 0u);
+    if (vec) {
+      constexpr int kStep = kLogitsAhead * kLogitsThreads * 4;
+      for (int i0 = 0; i0 < n; i0 += kStep) {
+        typename V4::Raw now[kLogitsAhead];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = one_token(v[k], u[k], v0 + i + k, bias ? add[k] : 0.f, bits >> k & 1);
-        store8(z + v0 + i, v);
+        for (int k = 0; k < kLogitsAhead; ++k) now[k] = ahead[k];
+        if (i0 + kStep < n) ask(i0 + kStep, v0, n);
+        else if (v0 + n < end) ask(0, v0 + n, min(kLogitsCounts, end - v0 - n));
+#pragma unroll
+        for (int k = 0; k < kLogitsAhead; ++k) {
+          const int i = i0 + (k * kLogitsThreads + tid) * 4, v = v0 + i;
+          if (i + 4 > n) {
+            for (int e = i; e < n; ++e) one_token(v0 + e, p.T ? cnt[4 + e] : 0u);
+            continue;
+          }
+          float y[4];
+          V4::open(now[k], y);
+          if (p.T) {
+            const uint4 u = *reinterpret_cast<const uint4*>(cnt + 4 + i);
+            if (u.x | u.y | u.z | u.w) {
+              if (u.x) y[0] = penalise(y[0], u.x);
+              if (u.y) y[1] = penalise(y[1], u.y);
+              if (u.z) y[2] = penalise(y[2], u.z);
+              if (u.w) y[3] = penalise(y[3], u.w);
+            }
+          }
+          if (bias_vec) {
+            const float4 a = __ldg(reinterpret_cast<const float4*>(bias + v));
+            y[0] += a.x; y[1] += a.y; y[2] += a.z; y[3] += a.w;
+          } else if (bias) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] += __ldg(bias + v + e);
+          }
+          if (mask) {
+            const int w = v >> 5;
+            const uint32_t bits = __funnelshift_r(__ldg(mask + w), (v & 31) > 28 ? __ldg(mask + w + 1) : 0u, v & 31);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (!(bits >> e & 1)) y[e] = -INFINITY;
+          }
+          *reinterpret_cast<float4*>(z + v) = make_float4(y[0], y[1], y[2], y[3]);
+          const float top = fmaxf(fmax3(y[0], y[1], y[2]), y[3]);
+          if (top > best) {
+            best = top;
+            at = v + (y[0] == top ? 0 : y[1] == top ? 1 : y[2] == top ? 2 : 3);
+          }
+        }
       }
     } else {
 #pragma unroll 4
-      for (int i = tid; i < n; i += kLogitsThreads)
-        z[v0 + i] = one_token(ld<T>(x + v0 + i), p.T ? cnt[i] : 0u, v0 + i, bias ? bias[v0 + i] : 0.f,
-                              mask ? mask[(v0 + i) >> 5] >> (i & 31) & 1 : 1);
+      for (int i = tid; i < n; i += kLogitsThreads) one_token(v0 + i, p.T ? cnt[4 + i] : 0u);
     }
   }
-  if (!p.best) return;
+  if (!p.best) {
+    if (ctas > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    return;
+  }
   auto better = [&](float v, int i) {
     if (v > best || (v == best && i < at)) {
       best = v;
@@ -129,24 +209,27 @@ __global__ void __launch_bounds__(kLogitsThreads) logits_kernel(const __grid_con
     bi[warp] = at;
   }
   __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < kLogitsThreads / 32; ++w) better(bv[w], bi[w]);
-    mine = (unsigned long long)__float_as_uint(best) << 32 | (uint32_t)at;
+  if (warp == 0) {
+    best = lane < kLogitsThreads / 32 ? bv[lane] : -INFINITY;
+    at = lane < kLogitsThreads / 32 ? bi[lane] : 0x7fffffff;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) better(__shfl_xor_sync(0xffffffffu, best, o), __shfl_xor_sync(0xffffffffu, at, o));
   }
   if (ctas > 1) {
-    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-    if (rank == 0 && tid == 0)
-      for (int k = 1; k < ctas; ++k) {
-        uint32_t far;
-        unsigned long long o;
-        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(far) : "r"(smem_u32(&mine)), "r"(k));
-        asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(o) : "r"(far) : "memory");
-        better(__uint_as_float((uint32_t)(o >> 32)), (int)(uint32_t)o);
-      }
-    // nobody leaves while the first CTA reads
-    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // the first CTA exists
+    if (tid == 0) {
+      uint32_t far;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(far) : "r"(smem_u32(theirs + rank)));
+      asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(far), "l"((unsigned long long)__float_as_uint(best) << 32 | (uint32_t)at)
+                   : "memory");
+    }
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    if (rank) return;
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (tid == 0)
+      for (int k = 1; k < ctas; ++k) better(__uint_as_float((uint32_t)(theirs[k] >> 32)), (int)(uint32_t)theirs[k]);
   }
-  if (rank == 0 && tid == 0) p.best[b] = at == 0x7fffffff ? 0 : at;
+  if (tid == 0) p.best[b] = at == 0x7fffffff ? 0 : at;
 }
 
 }  // namespace one

@@ -57,74 +57,141 @@ struct PagedAppendParams {
   int N, Hq;
 };
 
-// Where token t of sequence b goes in head h of `pages` (stride: elements per page), or null. A slot
+// The page and the row in it (head 0) of token t of sequence b; false: the token is not stored. A slot
 // beyond the table and a page outside the pool are recorded.
-template <typename T>
-ONE_DEVINL T* append_row(const PagedAppendParams& p, void* pages, int64_t stride, int b, int h, int t, int64_t& slot) {
+ONE_DEVINL bool append_place(const PagedAppendParams& p, int b, int t, int64_t& slot, int& page, int& row) {
   const PagedCache& c = p.c;
-  if (p.counts && t >= p.counts[b]) return nullptr;
+  if (p.counts && t >= p.counts[b]) return false;
   const int len = c.lengths[b];
   slot = (int64_t)len + t;
   if (len < 0 || slot >= (int64_t)c.max_pages * c.page_size) {
     set_err(c.err, ERR_BAD_ARG, SITE_PAGED_APPEND);
-    return nullptr;
+    return false;
   }
   const int index = (int)slot / c.page_size;
-  const int pg = paged_page(c, c.table, b * c.table_stride, index, SITE_PAGED_APPEND);
-  if (pg < 0) return nullptr;
-  return (T*)pages + pg * stride + ((int64_t)h * c.page_size + ((int)slot - index * c.page_size)) * c.Dh;
+  page = paged_page(c, c.table, b * c.table_stride, index, SITE_PAGED_APPEND);
+  row = (int)slot - index * c.page_size;
+  return page >= 0;
+}
+
+// 16 bytes of elements <-> pairs of floats
+template <typename T> struct Piece;
+template <> struct Piece<__nv_bfloat16> {
+  static constexpr int N = 8;
+  ONE_DEVINL static void open(const uint4& u, float2 (&v)[4]) {
+    v[0] = make_float2(bf2_lo(u.x), bf2_hi(u.x)); v[1] = make_float2(bf2_lo(u.y), bf2_hi(u.y));
+    v[2] = make_float2(bf2_lo(u.z), bf2_hi(u.z)); v[3] = make_float2(bf2_lo(u.w), bf2_hi(u.w));
+  }
+  ONE_DEVINL static uint4 close(const float2 (&v)[4]) {
+    return make_uint4(pack_bf16x2(v[0].x, v[0].y), pack_bf16x2(v[1].x, v[1].y), pack_bf16x2(v[2].x, v[2].y),
+                      pack_bf16x2(v[3].x, v[3].y));
+  }
+};
+template <> struct Piece<float> {
+  static constexpr int N = 4;
+  ONE_DEVINL static void open(const uint4& u, float2 (&v)[2]) {
+    v[0] = make_float2(__uint_as_float(u.x), __uint_as_float(u.y));
+    v[1] = make_float2(__uint_as_float(u.z), __uint_as_float(u.w));
+  }
+  ONE_DEVINL static uint4 close(const float2 (&v)[2]) {
+    return make_uint4(__float_as_uint(v[0].x), __float_as_uint(v[0].y), __float_as_uint(v[1].x), __float_as_uint(v[1].y));
+  }
+};
+ONE_DEVINL float2 mul2(float2 a, float2 b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(f2_bits(a)), "l"(f2_bits(b)));
+  return f2_from(d);
 }
 
 // New tokens into the pages, rotated: y = x cos + rotate_half(x) sin. A copy with two products per
 // element, bound by HBM (prompts) or by one round trip to it (single tokens).
 //
-// One thread per 8 elements of a row's first half and the matching 8 of its second, so the rotation
-// needs no exchange; the threads of a token's heads are neighbours and share its cos and sin in L1.
-// For rows whose halves are whole 16-byte pieces (Dh a multiple of 16, aligned strides);
-// paged_append_any_kernel takes the rest. Sequence blockIdx.y.
+// One thread per token, group of kAppendRows heads of its keys, queries or values, and 16-byte piece:
+// consecutive lanes read and write whole rows, the group's loads are in flight together and share cos
+// and sin. The piece half a row away, which the rotation needs, comes from its lane. For aligned rows
+// of a power of two of pieces; paged_append_any_kernel takes the rest. Sequence blockIdx.y.
+constexpr int kAppendRows = 4;
+
 template <typename T>
 __global__ void __launch_bounds__(256) paged_append_kernel(const __grid_constant__ PagedAppendParams p) {
+  using P = Piece<T>;
   pdl_wait();
   const PagedCache& c = p.c;
-  const int units = c.Dh / 16, heads = 2 * c.Hkv + (p.q ? p.Hq : 0), half = c.Dh / 2, b = blockIdx.y;
-  const uint32_t i = blockIdx.x * blockDim.x + threadIdx.x;
-  const uint32_t row = i / units;
-  const int e = (int)(i - row * units) * 8, t = (int)(row / heads), hh = (int)(row - (uint32_t)t * heads);
-  if (t >= p.N) return;
-  const bool is_q = hh >= 2 * c.Hkv, is_v = !is_q && hh >= c.Hkv;
-  const int h = is_q ? hh - 2 * c.Hkv : is_v ? hh - c.Hkv : hh;
-  const T* x;
-  if (is_q) x = (const T*)p.q + b * p.qs[0] + h * p.qs[1] + t * p.qs[2];
-  else if (is_v) x = (const T*)p.v + b * p.vs[0] + h * p.vs[1] + t * p.vs[2];
-  else x = (const T*)p.k + b * p.ks[0] + h * p.ks[1] + t * p.ks[2];
-  float x1[8], x2[8];
-  load8(x + e, x1);
-  load8(x + half + e, x2);
+  const int pieces = c.Dh / P::N, hq = p.q ? p.Hq : 0, b = blockIdx.y;
+  const int kvg = (c.Hkv + kAppendRows - 1) / kAppendRows, qg = (hq + kAppendRows - 1) / kAppendRows, groups = 2 * kvg + qg;
+  const uint32_t i = blockIdx.x * blockDim.x + threadIdx.x, item = i / pieces;
+  const int piece = (int)(i - item * pieces), e = piece * P::N, t = (int)(item / groups);
+  int g = (int)(item - (uint32_t)t * groups);
+  if (t >= p.N) return;  // whole rows of lanes
+  const T* from;
+  int64_t step;
+  int heads = c.Hkv, kind = 0;  // keys, queries, values
+  if (g < kvg) {
+    from = (const T*)p.k + b * p.ks[0] + t * p.ks[2];
+    step = p.ks[1];
+  } else if (g < kvg + qg) {
+    g -= kvg;
+    kind = 1;
+    heads = hq;
+    from = (const T*)p.q + b * p.qs[0] + t * p.qs[2];
+    step = p.qs[1];
+  } else {
+    g -= kvg + qg;
+    kind = 2;
+    from = (const T*)p.v + b * p.vs[0] + t * p.vs[2];
+    step = p.vs[1];
+  }
+  const int r0 = g * kAppendRows, rows = min(kAppendRows, heads - r0);
+  from += r0 * step + e;
+  uint4 x[kAppendRows];
+#pragma unroll
+  for (int k = 0; k < kAppendRows; ++k)
+    if (k < rows) x[k] = *reinterpret_cast<const uint4*>(from + k * step);
   T* y;
-  if (is_q) {
-    y = (T*)p.q_out + (((int64_t)b * p.Hq + h) * p.N + t) * c.Dh;
+  int64_t ystep;
+  if (kind == 1) {
+    y = (T*)p.q_out + (((int64_t)b * hq + r0) * p.N + t) * c.Dh + e;
+    ystep = (int64_t)p.N * c.Dh;
   } else {
     int64_t slot;
-    y = append_row<T>(p, is_v ? c.v : c.k, is_v ? c.v_stride : c.k_stride, b, h, t, slot);
-    if (!y) return;
-    if (!is_v && p.mass && e == 0) p.mass[((int64_t)b * c.Hkv + h) * p.mass_width + slot] = 0.f;
+    int page, row;
+    if (!append_place(p, b, t, slot, page, row)) return;
+    y = (kind ? (T*)c.v + page * c.v_stride : (T*)c.k + page * c.k_stride) + (r0 * c.page_size + row) * c.Dh + e;
+    ystep = c.page_size * c.Dh;
+    if (kind == 0 && p.mass)
+      for (int k = piece; k < rows; k += pieces) p.mass[((int64_t)b * c.Hkv + r0 + k) * p.mass_width + slot] = 0.f;
   }
-  if (p.cosv && !is_v) {
-    const int64_t cs = b * p.cos_bs + (int64_t)t * c.Dh + e;
-    float c1[8], c2[8], s1[8], s2[8];
-    load8((const T*)p.cosv + cs, c1);
-    load8((const T*)p.cosv + cs + half, c2);
-    load8((const T*)p.sinv + cs, s1);
-    load8((const T*)p.sinv + cs + half, s2);
+  if (kind < 2 && p.cosv) {
+    const int64_t at = b * p.cos_bs + (int64_t)t * c.Dh + e;
+    float2 cs[P::N / 2], sn[P::N / 2];
+    P::open(__ldg(reinterpret_cast<const uint4*>((const T*)p.cosv + at)), cs);
+    P::open(__ldg(reinterpret_cast<const uint4*>((const T*)p.sinv + at)), sn);
+    if (2 * piece < pieces) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const float a = x1[k], o = x2[k];
-      x1[k] = a * c1[k] - o * s1[k];
-      x2[k] = o * c2[k] + a * s2[k];
+      for (int d = 0; d < P::N / 2; ++d) sn[d] = make_float2(-sn[d].x, -sn[d].y);
     }
+    // the lanes of this row take this branch together
+    const uint32_t lanes = (0xffffffffu >> (32 - pieces)) << ((threadIdx.x & 31) & ~(pieces - 1));
+#pragma unroll
+    for (int k = 0; k < kAppendRows; ++k) {
+      if (k >= rows) break;
+      uint4 o;
+      o.x = __shfl_xor_sync(lanes, x[k].x, pieces / 2);
+      o.y = __shfl_xor_sync(lanes, x[k].y, pieces / 2);
+      o.z = __shfl_xor_sync(lanes, x[k].z, pieces / 2);
+      o.w = __shfl_xor_sync(lanes, x[k].w, pieces / 2);
+      float2 u[P::N / 2], w[P::N / 2];
+      P::open(x[k], u);
+      P::open(o, w);
+#pragma unroll
+      for (int d = 0; d < P::N / 2; ++d) u[d] = fma2(u[d], cs[d], mul2(w[d], sn[d]));
+      *reinterpret_cast<uint4*>(y + k * ystep) = P::close(u);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < kAppendRows; ++k)
+      if (k < rows) *reinterpret_cast<uint4*>(y + k * ystep) = x[k];
   }
-  store8(y + e, x1);
-  store8(y + half + e, x2);
 }
 
 // The same for rows of any alignment: one warp per row of q, k or v.
@@ -145,8 +212,9 @@ __global__ void __launch_bounds__(256) paged_append_any_kernel(const __grid_cons
     y = (T*)p.q_out + (((int64_t)b * p.Hq + h) * p.N + t) * c.Dh;
   } else {
     int64_t slot;
-    y = append_row<T>(p, is_v ? c.v : c.k, is_v ? c.v_stride : c.k_stride, b, h, t, slot);
-    if (!y) return;
+    int page, at;
+    if (!append_place(p, b, t, slot, page, at)) return;
+    y = (T*)(is_v ? c.v : c.k) + page * (is_v ? c.v_stride : c.k_stride) + (h * c.page_size + at) * c.Dh;
     if (!is_v && p.mass && lane == 0) p.mass[((int64_t)b * c.Hkv + h) * p.mass_width + slot] = 0.f;
   }
   const int64_t cs = b * p.cos_bs + (int64_t)t * c.Dh;
@@ -181,18 +249,18 @@ ONE_DEVINL uint32_t mass_key(float f) {
 
 // Which slots survive: one CTA per (sequence, kv head) finds the smallest surviving key by radix
 // selection (digits of 11, 11 and 10 bits, counted in shared memory), then writes the surviving slots
-// in order: every warp counts its run of slots, and the counts before it say where its survivors go.
-// Keys are read from HBM once and kept in shared memory up to `cached` of them; longer sequences are
-// read again in each of the five passes. Bound by the passes over shared memory, not by HBM.
+// in order. Bound by latency: one read of the masses, then a dozen barriers.
+// KPT > 0: a thread keeps the keys of candidates tid, tid + 1024, .. in KPT registers, read together.
+// KPT = 0, for tables of more than 32768 slots: the masses are read again in each pass.
 constexpr int kSelThreads = 1024;
-constexpr int kSelCached = 48 * 1024;
 
-__global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const __grid_constant__ PagedEvictParams p, int cached) {
-  extern __shared__ uint32_t keys[];
-  __shared__ uint32_t hist[2048];
-  __shared__ int wsum[2][32];
-  __shared__ uint32_t sh_digit;
-  __shared__ int sh_above;
+template <int KPT>
+__global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const __grid_constant__ PagedEvictParams p) {
+  __shared__ uint32_t hist[3][2048];
+  __shared__ int wsum[32];
+  __shared__ uint32_t sh_digit[3];
+  __shared__ int sh_above[3];
+  __shared__ unsigned long long runs[KPT ? KPT * 32 : 32];  // survivors above << 32 | equal, then what is before
   pdl_wait();
   pdl_launch_dependents();
   const PagedCache& c = p.c;
@@ -206,90 +274,137 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const __grid_
   }
   const float* mass = p.mass + bh * p.mass_width + p.sink;
   const int nc = n - p.sink - p.recent, places = p.budget - p.sink - p.recent;  // candidates, and room for them
+  uint32_t key[KPT ? KPT : 1];
+#pragma unroll
+  for (int k = 0; k < KPT; ++k)
+    if (k * kSelThreads + tid < nc) key[k] = __float_as_uint(__ldg(mass + k * kSelThreads + tid));
+#pragma unroll
+  for (int k = 0; k < KPT; ++k) key[k] = mass_key(__uint_as_float(key[k]));
   for (int t = tid; t < p.sink; t += kSelThreads) kept[t] = t;
   for (int t = tid; t < p.recent; t += kSelThreads) kept[p.budget - p.recent + t] = n - p.recent + t;
   if (places == 0) return;
-  const bool in_smem = nc <= cached;
+  // f(key, candidate) for the thread's candidates
+  auto each = [&](auto&& f) {
+    if (KPT) {
+#pragma unroll
+      for (int k = 0; k < KPT; ++k)
+        if (k * kSelThreads + tid < nc) f(key[k]);
+    } else {
+#pragma unroll 4
+      for (int i = tid; i < nc; i += kSelThreads) f(mass_key(__ldg(mass + i)));
+    }
+  };
+  for (int i = tid; i < 3 * 2048; i += kSelThreads) hist[0][i] = 0;
+  __syncthreads();
   uint32_t prefix = 0, mask = 0;
   int above = 0;  // candidates above the prefix
+#pragma unroll 1
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
-    for (int i = tid; i < 2048; i += kSelThreads) hist[i] = 0;
-    __syncthreads();
-    for (int i = tid; i < nc; i += kSelThreads) {
-      const uint32_t k = pass > 0 && in_smem ? keys[i] : mass_key(mass[i]);
-      if (pass == 0 && in_smem) keys[i] = k;
-      if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1)], 1u);
-    }
+    const uint32_t digits = (1u << bits) - 1;
+    uint32_t* h = hist[pass];
+    each([&](uint32_t k) {
+      if ((k & mask) == prefix) atomicAdd(h + (k >> shift & digits), 1u);
+    });
     __syncthreads();
     // thread t holds digits 2047 - 2 t and 2046 - 2 t; sums from the top
-    const int d0 = 2047 - 2 * tid, h0 = (int)hist[d0], h1 = (int)hist[d0 - 1];
+    const int d0 = 2047 - 2 * tid, h0 = (int)h[d0], h1 = (int)h[d0 - 1];
     int incl = h0 + h1;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int t = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += t;
     }
-    if (lane == 31) wsum[0][warp] = incl;
+    if (lane == 31) wsum[warp] = incl;
     __syncthreads();
-    if (warp == 0) {
-      int v = wsum[0][lane];
+    int w = lane < warp ? wsum[lane] : 0;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int t = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v += t;
-      }
-      wsum[0][lane] = v;
-    }
-    __syncthreads();
-    const int before = above + (warp ? wsum[0][warp - 1] : 0) + incl - h0 - h1;
+    for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
+    const int before = above + w + incl - h0 - h1;
     if (before < places && before + h0 + h1 >= places) {
       const bool first = before + h0 >= places;
-      sh_digit = (uint32_t)(first ? d0 : d0 - 1);
-      sh_above = first ? before : before + h0;
+      sh_digit[pass] = (uint32_t)(first ? d0 : d0 - 1);
+      sh_above[pass] = first ? before : before + h0;
     }
     __syncthreads();
-    prefix |= sh_digit << shift;
-    mask |= ((1u << bits) - 1) << shift;
-    above = sh_above;
-    __syncthreads();
+    prefix |= sh_digit[pass] << shift;
+    mask |= digits << shift;
+    above = sh_above[pass];
   }
-  // survivors: keys above `prefix`, and the first `ties` that equal it
+  // survivors: keys above `prefix`, and the first `ties` that equal it. Runs of 32 candidates (KPT) or a
+  // 32nd of all of them are counted, the counts before each summed, then the runs written.
   const int ties = places - above;
-  const int run = ((nc + 31) / 32 + 31) / 32 * 32, i0 = warp * run, i1 = min(nc, i0 + run);
-  int gt = 0, eq = 0;
-  for (int i = i0; i < i1; i += 32) {
-    const uint32_t k = i + lane < i1 ? (in_smem ? keys[i + lane] : mass_key(mass[i + lane])) : 0u;
-    gt += __popc(__ballot_sync(0xffffffffu, i + lane < i1 && k > prefix));
-    eq += __popc(__ballot_sync(0xffffffffu, i + lane < i1 && k == prefix));
-  }
-  if (lane == 0) {
-    wsum[0][warp] = gt;
-    wsum[1][warp] = eq;
-  }
-  __syncthreads();
-  gt = eq = 0;
-  for (int w = 0; w < warp; ++w) {
-    gt += wsum[0][w];
-    eq += wsum[1][w];
-  }
   const uint32_t below = (1u << lane) - 1;
-  for (int i = i0; i < i1; i += 32) {
-    const bool in = i + lane < i1;
-    const uint32_t k = in ? (in_smem ? keys[i + lane] : mass_key(mass[i + lane])) : 0u;
-    const unsigned bg = __ballot_sync(0xffffffffu, in && k > prefix), be = __ballot_sync(0xffffffffu, in && k == prefix);
-    const int myeq = eq + __popc(be & below), at = gt + __popc(bg & below) + min(myeq, ties);
-    if (in && (k > prefix || (k == prefix && myeq < ties))) kept[p.sink + at] = p.sink + i + lane;
-    gt += __popc(bg);
-    eq += __popc(be);
+  auto scan = [&](int count) {  // runs[i] becomes the sum before it; count <= 1024, thread tid has run tid
+    unsigned long long v = tid < count ? runs[tid] : 0ull, incl = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned long long t = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += t;
+    }
+    __shared__ unsigned long long part[32];
+    if (lane == 31) part[warp] = incl;
+    __syncthreads();
+    unsigned long long w = lane < warp ? part[lane] : 0ull;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
+    if (tid < count) runs[tid] = w + incl - v;
+    __syncthreads();
+  };
+  auto write = [&](bool in, uint32_t k, int i, int gt, int eq, unsigned bg, unsigned be) {
+    const int mine = eq + __popc(be & below), at = gt + __popc(bg & below) + min(mine, ties);
+    if (in && (k > prefix || (k == prefix && mine < ties))) kept[p.sink + at] = p.sink + i;
+  };
+  if (KPT) {
+#pragma unroll
+    for (int k = 0; k < KPT; ++k) {
+      const bool in = k * kSelThreads + tid < nc;
+      const unsigned bg = __ballot_sync(0xffffffffu, in && key[k] > prefix), be = __ballot_sync(0xffffffffu, in && key[k] == prefix);
+      if (lane == 0) runs[k * 32 + warp] = (unsigned long long)__popc(bg) << 32 | __popc(be);
+    }
+    __syncthreads();
+    scan(KPT * 32);
+#pragma unroll
+    for (int k = 0; k < KPT; ++k) {
+      const int i = k * kSelThreads + tid;
+      const bool in = i < nc;
+      const unsigned bg = __ballot_sync(0xffffffffu, in && key[k] > prefix), be = __ballot_sync(0xffffffffu, in && key[k] == prefix);
+      const unsigned long long r = runs[k * 32 + warp];
+      write(in, key[k], i, (int)(r >> 32), (int)(uint32_t)r, bg, be);
+    }
+  } else {
+    const int run = ((nc + 31) / 32 + 31) / 32 * 32, i0 = warp * run, i1 = min(nc, i0 + run);
+    int gt = 0, eq = 0;
+    for (int i = i0; i < i1; i += 32) {
+      const bool in = i + lane < i1;
+      const uint32_t k = in ? mass_key(__ldg(mass + i + lane)) : 0u;
+      gt += __popc(__ballot_sync(0xffffffffu, in && k > prefix));
+      eq += __popc(__ballot_sync(0xffffffffu, in && k == prefix));
+    }
+    if (lane == 0) runs[warp] = (unsigned long long)gt << 32 | (uint32_t)eq;
+    __syncthreads();
+    scan(32);
+    gt = (int)(runs[warp] >> 32);
+    eq = (int)(uint32_t)runs[warp];
+    for (int i = i0; i < i1; i += 32) {
+      const bool in = i + lane < i1;
+      const uint32_t k = in ? mass_key(__ldg(mass + i + lane)) : 0u;
+      const unsigned bg = __ballot_sync(0xffffffffu, in && k > prefix), be = __ballot_sync(0xffffffffu, in && k == prefix);
+      write(in, k, i + lane, gt, eq, bg, be);
+      gt += __popc(bg);
+      eq += __popc(be);
+    }
   }
 }
 
 // The survivors' rows and masses to their places, 64 places of one (sequence, kv head) per CTA: the
-// rows' addresses first, then 16 bytes per thread and copy. A gather, bound by HBM.
+// rows' addresses first, then 16 bytes per copy, kMoveAhead pairs of a thread's in flight together. A
+// gather, bound by HBM.
 constexpr int kMovePlaces = 64;
+constexpr int kMoveAhead = 4;
+constexpr int kMoveThreads = 128;
 
-__global__ void __launch_bounds__(256) paged_move_kernel(const __grid_constant__ PagedEvictParams p, int per_bh, int pieces) {
+__global__ void __launch_bounds__(kMoveThreads) paged_move_kernel(const __grid_constant__ PagedEvictParams p, int per_bh, int pieces) {
   __shared__ int64_t from[2][kMovePlaces], to[2][kMovePlaces];  // 16-byte units; -1: nothing to copy
   pdl_wait();
   const PagedCache& c = p.c;
@@ -318,12 +433,25 @@ __global__ void __launch_bounds__(256) paged_move_kernel(const __grid_constant__
   if (i0 >= p.budget) return;
   uint4* kp = (uint4*)c.k;
   uint4* vp = (uint4*)c.v;
-  for (int e = tid; e < kMovePlaces * pieces; e += blockDim.x) {
-    const int place = e / pieces, piece = e - place * pieces;
-    if (from[0][place] < 0) continue;
-    const uint4 a = kp[from[0][place] + piece], v = vp[from[1][place] + piece];
-    kp[to[0][place] + piece] = a;
-    vp[to[1][place] + piece] = v;
+  const int all = kMovePlaces * pieces;
+  for (int e0 = tid; e0 < all; e0 += kMoveAhead * blockDim.x) {
+    uint4 a[kMoveAhead], v[kMoveAhead];
+#pragma unroll
+    for (int k = 0; k < kMoveAhead; ++k) {
+      const int e = e0 + k * blockDim.x, place = e / pieces;
+      if (e < all && from[0][place] >= 0) {
+        a[k] = kp[from[0][place] + (e - place * pieces)];
+        v[k] = vp[from[1][place] + (e - place * pieces)];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kMoveAhead; ++k) {
+      const int e = e0 + k * blockDim.x, place = e / pieces;
+      if (e < all && from[0][place] >= 0) {
+        kp[to[0][place] + (e - place * pieces)] = a[k];
+        vp[to[1][place] + (e - place * pieces)] = v[k];
+      }
+    }
   }
 }
 
