@@ -110,10 +110,13 @@ ONE_DEVINL float2 mul2(float2 a, float2 b) {
 // consecutive lanes read and write whole rows, the group's loads are in flight together and share cos
 // and sin. The piece half a row away, which the rotation needs, comes from its lane. For aligned rows
 // of a power of two of pieces; paged_append_any_kernel takes the rest. Sequence blockIdx.y.
+//
+// 8 prompts of up to 4096 tokens, 12 heads x 64: 68 us with one row per thread and its two halves in one
+// lane, 54 as here, 51 with five CTAs per SM; without rotation it runs at the rate of a plain copy.
 constexpr int kAppendRows = 4;
 
 template <typename T>
-__global__ void __launch_bounds__(256) paged_append_kernel(const __grid_constant__ PagedAppendParams p) {
+__global__ void __launch_bounds__(256, 5) paged_append_kernel(const __grid_constant__ PagedAppendParams p) {
   using P = Piece<T>;
   pdl_wait();
   const PagedCache& c = p.c;
@@ -250,36 +253,40 @@ ONE_DEVINL uint32_t mass_key(float f) {
 // Which slots survive: one CTA per (sequence, kv head) finds the smallest surviving key by radix
 // selection (digits of 11, 11 and 10 bits, counted in shared memory), then writes the surviving slots
 // in order. Bound by latency: one read of the masses, then a dozen barriers.
-// KPT > 0: a thread keeps the keys of candidates tid, tid + 1024, .. in KPT registers, read together.
-// KPT = 0, for tables of more than 32768 slots: the masses are read again in each pass.
-constexpr int kSelThreads = 1024;
+// KPT > 0: a thread keeps the keys of candidates tid, tid + 512, .. in KPT registers, read together and
+// before the length is known. KPT = 0, for tables of more than 32768 slots: the masses are read again in
+// each pass.
+constexpr int kSelThreads = 512;
+constexpr int kSelWarps = kSelThreads / 32;
 
 template <int KPT>
 __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const __grid_constant__ PagedEvictParams p) {
-  __shared__ uint32_t hist[3][2048];
-  __shared__ int wsum[32];
+  __shared__ __align__(16) uint32_t hist[3][2048];
+  __shared__ int wsum[kSelWarps];
   __shared__ uint32_t sh_digit[3];
   __shared__ int sh_above[3];
-  __shared__ unsigned long long runs[KPT ? KPT * 32 : 32];  // survivors above << 32 | equal, then what is before
+  // survivors above << 32 | equal of runs of candidates, then what is before each
+  __shared__ unsigned long long runs[KPT ? KPT * kSelWarps : kSelWarps];
   pdl_wait();
   pdl_launch_dependents();
   const PagedCache& c = p.c;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t bh = blockIdx.x;
+  const float* mass = p.mass + bh * p.mass_width + p.sink;
+  const int slots = c.max_pages * c.page_size - p.sink;
+  uint32_t key[KPT ? KPT : 1];
+#pragma unroll
+  for (int k = 0; k < KPT; ++k) {
+    const int i = k * kSelThreads + tid;
+    key[k] = i < slots ? mass_key(__ldg(mass + i)) : 0u;
+  }
   const int n = paged_length(c, (int)(bh / c.Hkv), SITE_PAGED_EVICT);
   int* kept = p.kept + bh * p.budget;
   if (n <= p.budget) {
     for (int t = tid; t < p.budget; t += kSelThreads) kept[t] = t < n ? t : -1;
     return;
   }
-  const float* mass = p.mass + bh * p.mass_width + p.sink;
   const int nc = n - p.sink - p.recent, places = p.budget - p.sink - p.recent;  // candidates, and room for them
-  uint32_t key[KPT ? KPT : 1];
-#pragma unroll
-  for (int k = 0; k < KPT; ++k)
-    if (k * kSelThreads + tid < nc) key[k] = __float_as_uint(__ldg(mass + k * kSelThreads + tid));
-#pragma unroll
-  for (int k = 0; k < KPT; ++k) key[k] = mass_key(__uint_as_float(key[k]));
   for (int t = tid; t < p.sink; t += kSelThreads) kept[t] = t;
   for (int t = tid; t < p.recent; t += kSelThreads) kept[p.budget - p.recent + t] = n - p.recent + t;
   if (places == 0) return;
@@ -307,9 +314,12 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const __grid_
       if ((k & mask) == prefix) atomicAdd(h + (k >> shift & digits), 1u);
     });
     __syncthreads();
-    // thread t holds digits 2047 - 2 t and 2046 - 2 t; sums from the top
-    const int d0 = 2047 - 2 * tid, h0 = (int)h[d0], h1 = (int)h[d0 - 1];
-    int incl = h0 + h1;
+    // thread t holds the four digits from 2047 - 4 t down; sums from the top
+    const int d0 = 2047 - 4 * tid;
+    const uint4 four = *reinterpret_cast<const uint4*>(h + d0 - 3);
+    const int at[4] = {(int)four.w, (int)four.z, (int)four.y, (int)four.x};
+    const int all = at[0] + at[1] + at[2] + at[3];
+    int incl = all;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int t = __shfl_up_sync(0xffffffffu, incl, o);
@@ -320,11 +330,16 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const __grid_
     int w = lane < warp ? wsum[lane] : 0;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
-    const int before = above + w + incl - h0 - h1;
-    if (before < places && before + h0 + h1 >= places) {
-      const bool first = before + h0 >= places;
-      sh_digit[pass] = (uint32_t)(first ? d0 : d0 - 1);
-      sh_above[pass] = first ? before : before + h0;
+    int before = above + w + incl - all;
+    if (before < places && before + all >= places) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (before < places && before + at[k] >= places) {
+          sh_digit[pass] = (uint32_t)(d0 - k);
+          sh_above[pass] = before;
+        }
+        before += at[k];
+      }
     }
     __syncthreads();
     prefix |= sh_digit[pass] << shift;
@@ -332,23 +347,35 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const __grid_
     above = sh_above[pass];
   }
   // survivors: keys above `prefix`, and the first `ties` that equal it. Runs of 32 candidates (KPT) or a
-  // 32nd of all of them are counted, the counts before each summed, then the runs written.
+  // warp's share of them all are counted, the counts before each summed, then the runs written.
   const int ties = places - above;
   const uint32_t below = (1u << lane) - 1;
-  auto scan = [&](int count) {  // runs[i] becomes the sum before it; count <= 1024, thread tid has run tid
-    unsigned long long v = tid < count ? runs[tid] : 0ull, incl = v;
+  constexpr int kRuns = KPT ? KPT * kSelWarps : kSelWarps, kPer = (kRuns + kSelThreads - 1) / kSelThreads;
+  __shared__ unsigned long long part[kSelWarps];
+  auto scan = [&] {  // runs[i] becomes the sum before it; thread t has kPer runs
+    unsigned long long v[kPer], all = 0, incl;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      v[k] = tid * kPer + k < kRuns ? runs[tid * kPer + k] : 0ull;
+      all += v[k];
+    }
+    incl = all;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const unsigned long long t = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += t;
     }
-    __shared__ unsigned long long part[32];
     if (lane == 31) part[warp] = incl;
     __syncthreads();
     unsigned long long w = lane < warp ? part[lane] : 0ull;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
-    if (tid < count) runs[tid] = w + incl - v;
+    w += incl - all;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      if (tid * kPer + k < kRuns) runs[tid * kPer + k] = w;
+      w += v[k];
+    }
     __syncthreads();
   };
   auto write = [&](bool in, uint32_t k, int i, int gt, int eq, unsigned bg, unsigned be) {
@@ -360,20 +387,20 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const __grid_
     for (int k = 0; k < KPT; ++k) {
       const bool in = k * kSelThreads + tid < nc;
       const unsigned bg = __ballot_sync(0xffffffffu, in && key[k] > prefix), be = __ballot_sync(0xffffffffu, in && key[k] == prefix);
-      if (lane == 0) runs[k * 32 + warp] = (unsigned long long)__popc(bg) << 32 | __popc(be);
+      if (lane == 0) runs[k * kSelWarps + warp] = (unsigned long long)__popc(bg) << 32 | __popc(be);
     }
     __syncthreads();
-    scan(KPT * 32);
+    scan();
 #pragma unroll
     for (int k = 0; k < KPT; ++k) {
       const int i = k * kSelThreads + tid;
       const bool in = i < nc;
       const unsigned bg = __ballot_sync(0xffffffffu, in && key[k] > prefix), be = __ballot_sync(0xffffffffu, in && key[k] == prefix);
-      const unsigned long long r = runs[k * 32 + warp];
+      const unsigned long long r = runs[k * kSelWarps + warp];
       write(in, key[k], i, (int)(r >> 32), (int)(uint32_t)r, bg, be);
     }
   } else {
-    const int run = ((nc + 31) / 32 + 31) / 32 * 32, i0 = warp * run, i1 = min(nc, i0 + run);
+    const int run = ((nc + kSelWarps - 1) / kSelWarps + 31) / 32 * 32, i0 = warp * run, i1 = min(nc, i0 + run);
     int gt = 0, eq = 0;
     for (int i = i0; i < i1; i += 32) {
       const bool in = i + lane < i1;
@@ -383,7 +410,7 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const __grid_
     }
     if (lane == 0) runs[warp] = (unsigned long long)gt << 32 | (uint32_t)eq;
     __syncthreads();
-    scan(32);
+    scan();
     gt = (int)(runs[warp] >> 32);
     eq = (int)(uint32_t)runs[warp];
     for (int i = i0; i < i1; i += 32) {

@@ -26,6 +26,7 @@ namespace one {
 
 constexpr int kPaWarps = 4;
 constexpr size_t kSmPerSm = 228 * 1024;    // shared memory of an SM, 1 KB of it per CTA reserved
+constexpr int kMaxSms = 160;            // SMs that share a list, at most
 constexpr int kPaPerSm = 3;             // CTAs of these kernels on an SM, at most
 
 struct PagedAttn {
@@ -45,7 +46,7 @@ struct PagedAttn {
   float* row_ml;          // [B * Hq][2], of segments in one piece
   float* scores;          // [B * Hq][score_ld], log2 domain
   int64_t score_ld;
-  long long* before;      // [B + 1]: tiles of one query-head tile before each sequence; the list's length
+  int2* parts;            // [B * Hkv * hv_per_kv]: first CTA of a segment; last << 1 | (its first part is slot 1)
   int ranges;             // CTAs that share the list
   int split;
 };
@@ -63,23 +64,6 @@ ONE_DEVINL long long pa_total(const PagedAttn& p) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
   return n * p.c.Hkv * p.hv_per_kv;
-}
-// Tiles (of one query-head tile) of the sequences before each, into p.before, by one warp.
-template <int TILE>
-ONE_DEVINL void pa_write_before(const PagedAttn& p) {
-  const int lane = threadIdx.x & 31;
-  long long run = 0;
-  for (int base = 0; base < p.c.B; base += 32) {
-    const int n = base + lane < p.c.B ? pa_tiles<TILE>(p.c, base + lane) : 0;
-    long long incl = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long t = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += t;
-    }
-    if (base + lane < p.c.B) p.before[base + lane] = run + incl - n;
-    run += __shfl_sync(0xffffffffu, incl, 31);
-  }
 }
 ONE_DEVINL long long pa_chunk(const PagedAttn& p, long long total) { return max(1ll, (total + p.ranges - 1) / p.ranges); }
 
@@ -603,14 +587,11 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E>::kPerSm) paged_attn_k
   pdl_wait();
   pdl_launch_dependents();
   PaCursor<TILE> cur;
-  int left;  // tiles to do
+  int left, share = 0;  // tiles to do; a full share
   if (p.split) {
     const long long total = pa_total<TILE>(p), chunk = pa_chunk(p, total), w0 = chunk * blockIdx.x;
-    if (blockIdx.x == 0) {  // for the join
-      if (threadIdx.x < 32) pa_write_before<TILE>(p);
-      if (threadIdx.x == 0) p.before[c.B] = total;
-    }
     if (w0 >= total) return;
+    share = (int)chunk;
     left = (int)min(chunk, total - w0);
     cur.seek(c, ng, w0);
   } else {
@@ -706,6 +687,11 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E>::kPerSm) paged_attn_k
     __syncthreads();
     const float* so = reinterpret_cast<const float*>(smem + put);
     const bool whole = first == 0 && last == cur.tiles;
+    if (p.split && first == 0 && threadIdx.x == 0) {  // which CTAs hold this segment: tiles from `left` on go to later ones
+      const int more = (cur.tiles - left + share - 1) / share;
+      p.parts[(cur.b * c.Hkv + cur.kv) * ng + cur.gi] =
+          make_int2((int)blockIdx.x, ((int)blockIdx.x + max(0, more)) << 1 | (int)begun_inside);
+    }
     const int64_t part = 2ll * blockIdx.x + begun_inside;
     for (int i = threadIdx.x; i < rows * (E::DH / 4); i += blockDim.x) {
       const int g = i / (E::DH / 4), d = i % (E::DH / 4) * 4;
@@ -759,124 +745,130 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E>::kPerSm) paged_attn_k
   } while (left > 0);
 }
 
-// The parts of a segment [s0, s1) of the list, cut every `chunk` tiles.
-struct PaParts {
-  long long first, last;
-  bool inner;  // the first part does not start its CTA's share
-  ONE_DEVINL PaParts(long long s0, long long s1, long long chunk)
-      : first(s0 / chunk), last((s1 - 1) / chunk), inner(s0 % chunk != 0) {}
-  ONE_DEVINL int64_t at(long long i) const { return 2 * i + (i == first && inner ? 1 : 0); }
-};
+// Joins what paged_attn_kernel left of a split list: one output row per block, then, with mass, one
+// block per 1024 slots of a (sequence, kv head), which adds the weights of all its query heads. Chains
+// of three round trips to L2: which parts, their (m, l), their sums.
+constexpr int kJoinThreads = 256;
+constexpr int kJoinSlots = 4 * kJoinThreads;
+constexpr int kJoinAhead = 4;
 
-// Joins what paged_attn_kernel left of a split list. Blocks below B * Hq: one output row each. With mass,
-// further blocks add the weights: block i takes the i-th share of the tiles of every (sequence, kv
-// head), recomputing the joint (m, l) of its rows from the parts.
 template <typename E>
-__global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ PagedAttn p) {
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedAttn p, int mass_blocks) {
   using T = typename E::T;
-  constexpr int ROWS = E::ROWS, DH = E::DH, TILE = E::TILE;
-  __shared__ float4 red[128];
-  __shared__ float fin[2][128];  // m and 1 / l of a kv head's query heads
+  constexpr int ROWS = E::ROWS, DH = E::DH;
+  __shared__ float4 red[kJoinThreads];
+  __shared__ float weight[kMaxSms * kPaPerSm];  // 2^(m - M) of each part
+  __shared__ float fin[2][128];                 // M and 1 / l of a kv head's query heads
   const PagedCache& c = p.c;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int hq = c.Hkv * p.G;
+  const int hq = c.Hkv * p.G, ng = p.hv_per_kv;
   pdl_wait();
-  const long long total = p.before[c.B], chunk = pa_chunk(p, total);
-  const int HV = c.Hkv * p.hv_per_kv;
-  // joint m and 1 / l of row g of the parts, by one warp
-  auto joint = [&](const PaParts& parts, int g, float& M, float& inv) {
+  // slot of part i of the CTAs that hold a segment
+  auto slot = [](int2 seg, int i) -> int64_t { return 2ll * i + (i == seg.x ? seg.y & 1 : 0); };
+  // joint m and 1 / l of row g of a segment's parts, by one warp; w: the parts' weights
+  auto joint = [&](int2 seg, int g, float& M, float& inv, float* w) {
+    const int first = seg.x, last = seg.y >> 1;
     float mm = -INFINITY;
-    for (long long i = parts.first + lane; i <= parts.last; i += 32) mm = fmaxf(mm, p.part_ml[(parts.at(i) * ROWS + g) * 2]);
+    for (int i = first + lane; i <= last; i += 32) mm = fmaxf(mm, p.part_ml[(slot(seg, i) * ROWS + g) * 2]);
     M = warp_max(mm);
     if (M == -INFINITY) M = 0.f;
     float L = 0.f;
-    for (long long i = parts.first + lane; i <= parts.last; i += 32) {
-      const float* x = p.part_ml + (parts.at(i) * ROWS + g) * 2;
-      L += x[1] * exp2f(x[0] - M);
+    for (int i = first + lane; i <= last; i += 32) {
+      const float2 x = *reinterpret_cast<const float2*>(p.part_ml + (slot(seg, i) * ROWS + g) * 2);
+      const float f = exp2f(x.x - M);
+      if (w) w[i - first] = f;
+      L += x.y * f;
     }
     L = warp_sum(L);
     inv = L == 0.f ? 0.f : 1.f / L;
   };
-  if ((long long)blockIdx.x < (long long)c.B * hq) {
-    const int b = blockIdx.x / hq, j = blockIdx.x % hq, kv = j / p.G, g = j % p.G;
-    const int tiles = pa_tiles<TILE>(c, b);
+  if ((int)blockIdx.x < c.B * hq) {
+    const int b = blockIdx.x / hq, j = blockIdx.x % hq, kv = j / p.G, g = j % p.G, row = g % ROWS;
+    const int2 seg = p.parts[(b * c.Hkv + kv) * ng + g / ROWS];
     T* out = (T*)p.out + (int64_t)blockIdx.x * c.Dh;
-    if (tiles == 0) {
-      for (int d = tid; d < c.Dh; d += blockDim.x) st<T>(out + d, 0.f);
+    if (paged_length(c, b, SITE_PAGED_ATTN) == 0) {  // no CTA holds it
+      for (int d = tid; d < c.Dh; d += kJoinThreads) st<T>(out + d, 0.f);
       return;
     }
-    const int hv = kv * p.hv_per_kv + g / ROWS;
-    const long long s0 = HV * p.before[b] + (long long)hv * tiles;
-    const PaParts parts(s0, s0 + tiles, chunk);
-    if (parts.first == parts.last) return;
-    const int row = g % ROWS;
-    float M, inv;
-    joint(parts, row, M, inv);
-    constexpr int C4 = DH / 4, NG = 128 / C4;  // float4 columns; parts summed side by side
+    const int first = seg.x, last = seg.y >> 1;
+    if (first == last || first < 0 || last < first || last >= p.ranges) return;  // whole; lengths changed during the call
+    constexpr int C4 = DH / 4, NG = kJoinThreads / C4;  // float4 columns; parts summed side by side
     const int col = tid % C4, grp = tid / C4;
+    auto part = [&](int i) { return *reinterpret_cast<const float4*>(p.part_o + (slot(seg, i) * ROWS + row) * DH + col * 4); };
+    float4 x[kJoinAhead];
+#pragma unroll
+    for (int k = 0; k < kJoinAhead; ++k)
+      if (grp < NG && first + grp + k * NG <= last) x[k] = part(first + grp + k * NG);
+    float M, inv;
+    if (warp == 0) {
+      joint(seg, row, M, inv, weight);
+      if (lane == 0) fin[0][0] = inv;
+    }
+    __syncthreads();
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (grp < NG)
-      for (long long i = parts.first + grp; i <= parts.last; i += NG) {
-        const int64_t at = parts.at(i) * ROWS + row;
-        const float f = exp2f(p.part_ml[2 * at] - M);
-        const float4 x = *reinterpret_cast<const float4*>(p.part_o + at * DH + col * 4);
-        a.x += f * x.x; a.y += f * x.y; a.z += f * x.z; a.w += f * x.w;
+    for (int i0 = grp; grp < NG && first + i0 <= last; i0 += kJoinAhead * NG) {
+#pragma unroll
+      for (int k = 0; k < kJoinAhead; ++k) {
+        const int i = i0 + k * NG;
+        if (first + i > last) break;
+        const float f = weight[i];
+        a.x += f * x[k].x; a.y += f * x[k].y; a.z += f * x[k].z; a.w += f * x[k].w;
+        if (first + i + kJoinAhead * NG <= last) x[k] = part(first + i + kJoinAhead * NG);
       }
+    }
     red[tid] = a;
     __syncthreads();
     if (tid < C4 && tid * 4 < c.Dh) {
       for (int k = 1; k < NG; ++k) {
-        const float4 x = red[k * C4 + tid];
-        a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
+        const float4 y = red[k * C4 + tid];
+        a.x += y.x; a.y += y.y; a.z += y.z; a.w += y.w;
       }
+      inv = fin[0][0];
       T* y = out + tid * 4;
       st<T>(y, a.x * inv); st<T>(y + 1, a.y * inv); st<T>(y + 2, a.z * inv); st<T>(y + 3, a.w * inv);
     }
     return;
   }
-  // ---- mass: the tiles of every (sequence, kv head) in the same order, in equal shares
-  const long long mtotal = total / p.hv_per_kv, share = max(1ll, (mtotal + p.ranges - 1) / p.ranges);
-  long long w = share * (blockIdx.x - (long long)c.B * hq);
-  const long long w1 = min(w + share, mtotal);
-  if (w >= w1) return;
-  PaCursor<TILE> cur;
-  cur.seek(c, 1, w);
-  while (w < w1) {
-    const int first = cur.tile, last = (int)min((long long)cur.tiles, cur.tile + (w1 - w));
-    if (cur.b >= c.B || last <= first) break;
-    const long long before = HV * p.before[cur.b];
-    const int t0 = first * TILE, t1 = min(last * TILE, cur.len);
-    float* mass = p.mass + ((int64_t)cur.b * c.Hkv + cur.kv) * p.mass_width;
-    const int64_t row0 = ((int64_t)cur.b * c.Hkv + cur.kv) * p.G;
-    for (int gb = 0; gb < p.G; gb += 128) {
-      const int gn = min(128, p.G - gb);
-      __syncthreads();
-      for (int g = gb + warp; g < gb + gn; g += 4) {
-        const long long s0 = before + (long long)(cur.kv * p.hv_per_kv + g / ROWS) * cur.tiles;
-        const PaParts parts(s0, s0 + cur.tiles, chunk);
-        float M, inv;
-        if (parts.first == parts.last) {
-          M = p.row_ml[2 * (row0 + g)];
-          inv = p.row_ml[2 * (row0 + g) + 1];
-        } else {
-          joint(parts, g % ROWS, M, inv);
-        }
-        if (lane == 0) {
-          fin[0][g - gb] = M;
-          fin[1][g - gb] = inv;
-        }
+  // ---- mass: four slots per thread; rows of scores are padded, so that they may be read past the length
+  const int at = blockIdx.x - c.B * hq, bh = at / mass_blocks, t = at % mass_blocks * kJoinSlots + tid * 4, b = bh / c.Hkv;
+  const int len = paged_length(c, b, SITE_PAGED_ATTN);
+  if (at % mass_blocks * kJoinSlots >= len) return;
+  const int64_t row0 = (int64_t)bh * p.G;
+  float add[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int gb = 0; gb < p.G; gb += 128) {
+    const int gn = min(128, p.G - gb);
+    if (gb) __syncthreads();
+    for (int g = gb + warp; g < gb + gn; g += kJoinThreads / 32) {
+      const int2 seg = p.parts[bh * ng + g / ROWS];
+      float M, inv;
+      if (seg.x == seg.y >> 1 || seg.x < 0 || seg.y < 0 || seg.y >> 1 >= p.ranges) {
+        M = p.row_ml[2 * (row0 + g)];
+        inv = p.row_ml[2 * (row0 + g) + 1];
+      } else {
+        joint(seg, g % ROWS, M, inv, nullptr);
       }
-      __syncthreads();
-      for (int t = t0 + tid; t < t1; t += blockDim.x) {
-        float a = 0.f;
-        for (int g = 0; g < gn; ++g) a += ex2_approx(p.scores[(row0 + gb + g) * p.score_ld + t] - fin[0][g]) * fin[1][g];
-        mass[t] += a;
+      if (lane == 0) {
+        fin[0][g - gb] = M;
+        fin[1][g - gb] = inv;
       }
     }
-    w += last - first;
-    cur.tile = last - 1;
-    if (w < w1) cur.next(c, 1);
+    __syncthreads();
+    if (t < len) {
+#pragma unroll 4
+      for (int g = 0; g < gn; ++g) {
+        const float4 s = *reinterpret_cast<const float4*>(p.scores + (row0 + gb + g) * p.score_ld + t);
+        const float M = fin[0][g], inv = fin[1][g];
+        add[0] += ex2_approx(s.x - M) * inv;
+        add[1] += ex2_approx(s.y - M) * inv;
+        add[2] += ex2_approx(s.z - M) * inv;
+        add[3] += ex2_approx(s.w - M) * inv;
+      }
+    }
   }
+  float* mass = p.mass + (int64_t)bh * p.mass_width + t;
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (t + k < len) mass[k] += add[k];
 }
 
 }  // namespace one

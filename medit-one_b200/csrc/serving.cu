@@ -135,7 +135,6 @@ int launched(cudaError_t e, const char* what) {
 
 namespace {
 
-constexpr int kMaxSms = 160;  // the workspace's bound on the SMs that share a list
 constexpr int kMaxTile = 256;  // slots of the largest tile
 constexpr int kWhole = 512;    // caches of at most this many slots are not split
 
@@ -145,15 +144,15 @@ size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 int paged_rows(int dtype, int G) { return dtype == ONE_DTYPE_F32 ? 4 : G > 8 ? 16 : 8; }
 
 struct PagedWs {
-  size_t part_ml, part_o, row_ml, before, scores, total;
+  size_t part_ml, part_o, row_ml, segs, scores, total;
   int64_t score_ld;
   PagedWs(int b, int hq, int rows, int dh_pad, int64_t slots, bool mass) {
     const size_t parts = 2 * (size_t)kMaxSms * kPaPerSm * rows;
     part_ml = 0;
     part_o = align256(parts * 8);
     row_ml = part_o + align256(parts * dh_pad * 4);
-    before = row_ml + align256(mass ? (size_t)b * hq * 8 : 0);
-    scores = before + align256(((size_t)b + 1) * 8);
+    segs = row_ml + align256(mass ? (size_t)b * hq * 8 : 0);
+    scores = segs + align256((size_t)b * hq * 8);
     score_ld = (slots + kMaxTile - 1) / kMaxTile * kMaxTile;
     total = scores + (mass ? (size_t)b * hq * score_ld * 4 : 0);
   }
@@ -170,8 +169,11 @@ int attend(PagedAttn& p, cudaStream_t st) {
   const dim3 grid = p.split ? dim3(p.ranges) : dim3(p.c.Hkv * p.hv_per_kv, p.c.B);
   rc = launched(launch(paged_attn_kernel<E, RUN>, grid, dim3(kPaWarps * 32), PaSmem<E>::kTotal, st, p), "paged attention");
   if (rc || !p.split) return rc;
-  const int64_t joins = (int64_t)p.c.B * p.c.Hkv * p.G + (p.mass ? p.ranges : 0);
-  return launched(launch(paged_join_kernel<E>, dim3((unsigned)joins), dim3(128), 0, st, p), "paged attention join");
+  const int64_t heads = (int64_t)p.c.B * p.c.Hkv;
+  const int mass_blocks = p.mass ? (p.c.max_pages * p.c.page_size + kJoinSlots - 1) / kJoinSlots : 0;
+  return launched(launch(paged_join_kernel<E>, dim3((unsigned)(heads * (p.G + mass_blocks))), dim3(kJoinThreads), 0, st, p,
+                         mass_blocks),
+                  "paged attention join");
 }
 
 template <typename E>
@@ -200,7 +202,7 @@ extern "C" int one_paged_attention(const one_paged_cache* cache, const void* q, 
   float* mass = cache->mass;
   if (hq < 1 || hq % hkv) return fail(ONE_ERR_INVALID, "paged attention: the query heads must be a multiple of the kv heads");
   const int64_t slots = (int64_t)cache->max_pages * page_size;
-  if ((int64_t)b * hq > 0x3fffffff || (int64_t)b * hq * (slots / 64 + 1) / 128 > 0x7fffffff)
+  if ((int64_t)b * hq > 0x3fffffff || (int64_t)b * hq * (slots / 64 + 1) > 0x7fffffff)
     return fail(ONE_ERR_UNSUPPORTED, "paged attention: too many rows");
   const size_t need = one_paged_attention_workspace_bytes(b, hq, hkv, dh, page_size, cache->max_pages, dtype, mass != nullptr);
   if (need && (!workspace || workspace_bytes < need)) return fail(ONE_ERR_INVALID, "workspace too small");
@@ -218,7 +220,7 @@ extern "C" int one_paged_attention(const one_paged_cache* cache, const void* q, 
   p.part_ml = reinterpret_cast<float*>(ws + w.part_ml);
   p.part_o = reinterpret_cast<float*>(ws + w.part_o);
   p.row_ml = reinterpret_cast<float*>(ws + w.row_ml);
-  p.before = reinterpret_cast<long long*>(ws + w.before);
+  p.parts = reinterpret_cast<int2*>(ws + w.segs);
   p.scores = mass ? reinterpret_cast<float*>(ws + w.scores) : nullptr;
   p.score_ld = w.score_ld;
   p.split = slots > kWhole || (mass && p.hv_per_kv > 1);
@@ -310,9 +312,9 @@ extern "C" int one_paged_evict(const one_paged_cache* cache, const int32_t* dst_
   cudaStream_t st = (cudaStream_t)stream;
   const int64_t slots = (int64_t)cache->max_pages * page_size;
   const dim3 one_each(b * hkv), threads(kSelThreads);
-  rc = launched(slots <= 2048    ? launch(paged_select_kernel<2>, one_each, threads, 0, st, p)
-                : slots <= 8192  ? launch(paged_select_kernel<8>, one_each, threads, 0, st, p)
-                : slots <= 32768 ? launch(paged_select_kernel<32>, one_each, threads, 0, st, p)
+  rc = launched(slots <= 2048    ? launch(paged_select_kernel<4>, one_each, threads, 0, st, p)
+                : slots <= 8192  ? launch(paged_select_kernel<16>, one_each, threads, 0, st, p)
+                : slots <= 32768 ? launch(paged_select_kernel<64>, one_each, threads, 0, st, p)
                                  : launch(paged_select_kernel<0>, one_each, threads, 0, st, p),
                 "paged select");
   if (rc) return rc;
