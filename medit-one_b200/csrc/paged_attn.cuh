@@ -56,16 +56,15 @@ ONE_DEVINL int pa_tiles(const PagedCache& c, int b) {
   return (paged_length(c, b, SITE_PAGED_ATTN) + TILE - 1) / TILE;
 }
 
-// The list's length and a position in it. Every warp computes them for itself.
+// Tiles in the list (the host bounds them to 2^31). Every warp computes them for itself.
 template <int TILE>
-ONE_DEVINL long long pa_total(const PagedAttn& p) {
-  long long n = 0;
+ONE_DEVINL int pa_total(const PagedAttn& p) {
+  int n = 0;
   for (int b = threadIdx.x & 31; b < p.c.B; b += 32) n += pa_tiles<TILE>(p.c, b);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
   return n * p.c.Hkv * p.hv_per_kv;
 }
-ONE_DEVINL long long pa_chunk(const PagedAttn& p, long long total) { return max(1ll, (total + p.ranges - 1) / p.ranges); }
 
 // A place in the list: tile `tile` of query-head tile gi of kv head kv of sequence b; the heads' tiles
 // of a sequence follow one another, ng query-head tiles per kv head.
@@ -76,31 +75,29 @@ struct PaCursor {
     len = b < c.B ? paged_length(c, b, SITE_PAGED_ATTN) : 0;
     tiles = (len + TILE - 1) / TILE;
   }
-  ONE_DEVINL void seek(const PagedCache& c, int ng, long long w) {
-    const long long HV = (long long)c.Hkv * ng;
-    const int lane = threadIdx.x & 31;
-    long long run = 0;
+  ONE_DEVINL void seek(const PagedCache& c, int ng, int w) {
+    const int HV = c.Hkv * ng, lane = threadIdx.x & 31;
     for (int base = 0; base < c.B; base += 32) {
       const int n = base + lane < c.B ? pa_tiles<TILE>(c, base + lane) : 0;
-      long long incl = n;
+      int incl = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const long long t = __shfl_up_sync(0xffffffffu, incl, o);
+        const int t = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o) incl += t;
       }
-      const unsigned hit = __ballot_sync(0xffffffffu, w < HV * (run + incl));
+      const unsigned hit = __ballot_sync(0xffffffffu, w < HV * incl);
       if (hit) {
         const int src = __ffs(hit) - 1;
         b = base + src;
-        w -= HV * (run + __shfl_sync(0xffffffffu, incl - n, src));
+        w -= HV * __shfl_sync(0xffffffffu, incl - n, src);
         load(c);
-        const int hv = (int)(w / tiles);
-        tile = (int)(w % tiles);
+        const int hv = w / tiles;
+        tile = w - hv * tiles;
         kv = hv / ng;
-        gi = hv % ng;
+        gi = hv - kv * ng;
         return;
       }
-      run += __shfl_sync(0xffffffffu, incl, 31);
+      w -= HV * __shfl_sync(0xffffffffu, incl, 31);
     }
     b = c.B;
     kv = gi = tile = tiles = len = 0;
@@ -589,11 +586,12 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E>::kPerSm) paged_attn_k
   PaCursor<TILE> cur;
   int left, share = 0;  // tiles to do; a full share
   if (p.split) {
-    const long long total = pa_total<TILE>(p), chunk = pa_chunk(p, total), w0 = chunk * blockIdx.x;
+    const int total = pa_total<TILE>(p);
+    share = max(1, (total + p.ranges - 1) / p.ranges);
+    const long long w0 = (long long)share * blockIdx.x;
     if (w0 >= total) return;
-    share = (int)chunk;
-    left = (int)min(chunk, total - w0);
-    cur.seek(c, ng, w0);
+    left = min(share, total - (int)w0);
+    cur.seek(c, ng, (int)w0);
   } else {
     cur.b = blockIdx.y;
     cur.kv = blockIdx.x / ng;

@@ -129,10 +129,14 @@ def ptr(t) -> c_void_p:
     return c_void_p(0) if t is None else c_void_p(t.data_ptr())
 
 
+_dtype_codes = {}
+
+
 def dtype_code(dt) -> int:
-    import torch
-    if dt == torch.bfloat16:
-        return ONE_DTYPE_BF16
-    if dt == torch.float32:
-        return ONE_DTYPE_F32
-    raise OneError(f"unsupported dtype {dt}: the engine computes in bf16 or fp32")
+    if not _dtype_codes:
+        import torch
+        _dtype_codes.update({torch.bfloat16: ONE_DTYPE_BF16, torch.float32: ONE_DTYPE_F32})
+    code = _dtype_codes.get(dt)
+    if code is None:
+        raise OneError(f"unsupported dtype {dt}: the engine computes in bf16 or fp32")
+    return code

@@ -312,7 +312,7 @@ def turbo_paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch
     hq = shape[1]
     q = _rows_last(q)
     if out is None:
-        out = q.new_empty(shape)
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(shape)
     nws = _attention_workspace(b, hq, hkv, dh, ps, mp, C.dtype_code(dt), mass is not None)
     ws = q.new_empty(nws, dtype=torch.uint8) if nws else None
     qs = q.stride()
