@@ -250,176 +250,270 @@ ONE_DEVINL uint32_t mass_key(float f) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// Which slots survive: one CTA per (sequence, kv head) finds the smallest surviving key by radix
-// selection (digits of 11, 11 and 10 bits, counted in shared memory), then writes the surviving slots
-// in order. Bound by latency: one read of the masses, then a dozen barriers.
+// Eviction. A CTA finds which slots of a (sequence, kv head) survive:
+//  - the smallest surviving key by radix selection (digits of 9, 12 and 11 bits, counted in shared
+//    memory; the first, sign and exponent, in eight copies, since masses crowd in few exponents); then
+//    the survivors' ranks, from counts of runs of 32 candidates.
+// Bound by latency: one read of the masses and a dozen barriers.
+// MOVE: each of `parts` CTAs selects for itself and copies a part of the survivors: the slots whose rank
+// lies in it go into a list in shared memory, and their rows and masses to their places, kEvictAhead
+// pairs of a thread's 16-byte pieces in flight together. One launch, for as many CTAs as the SMs hold at
+// once (4 x 1040 slots to 1024, 12 heads x 64: 12.3 us in two launches, 10.3 in one; 16 x 8192 to 2048:
+// 51 in two, 70 in one). Otherwise one CTA writes the survivors' list and paged_move_kernel copies.
 // KPT > 0: a thread keeps the keys of candidates tid, tid + 512, .. in KPT registers, read together and
 // before the length is known. KPT = 0, for tables of more than 32768 slots: the masses are read again in
 // each pass.
-constexpr int kSelThreads = 512;
-constexpr int kSelWarps = kSelThreads / 32;
+constexpr int kEvictThreads = 512;
+constexpr int kEvictWarps = kEvictThreads / 32;
+constexpr int kEvictList = 512;  // places listed at a time, one per thread
+constexpr int kEvictAhead = 4;
 
-template <int KPT>
-__global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const __grid_constant__ PagedEvictParams p) {
-  __shared__ __align__(16) uint32_t hist[3][2048];
-  __shared__ int wsum[kSelWarps];
+template <int N>
+struct Int {
+  static constexpr int value = N;
+};
+
+template <int KPT, bool MOVE>
+__global__ void __launch_bounds__(kEvictThreads, KPT > 16 ? 1 : 2)
+    paged_evict_kernel(const __grid_constant__ PagedEvictParams p, int parts, int pieces) {
+  // digit counts [512][8], [4096], [2048]; the first part's room then holds the listed rows' addresses in
+  // 16 bytes: [from, to][keys, values][places], from -1: nothing to copy
+  __shared__ __align__(16) uint32_t hist[10240];
+  static_assert(sizeof(int64_t) * 4 * kEvictList <= 4 * 4096, "addresses");
+  int64_t* from = reinterpret_cast<int64_t*>(hist);
+  int64_t* to = from + 2 * kEvictList;
+  __shared__ int wsum[kEvictWarps];
   __shared__ uint32_t sh_digit[3];
   __shared__ int sh_above[3];
-  // survivors above << 32 | equal of runs of candidates, then what is before each
-  __shared__ unsigned long long runs[KPT ? KPT * kSelWarps : kSelWarps];
+  // the second part's: survivors above << 32 | equal of runs of candidates, then what is before each
+  unsigned long long* runs = reinterpret_cast<unsigned long long*>(hist + 4096);
+  static_assert(sizeof(unsigned long long) * (KPT + 1) * kEvictWarps <= 4 * 4096, "runs");
+  __shared__ unsigned long long part_sum[kEvictWarps];
+  __shared__ int list[kEvictList];
   pdl_wait();
-  pdl_launch_dependents();
+  if (!MOVE) pdl_launch_dependents();
   const PagedCache& c = p.c;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int64_t bh = blockIdx.x;
-  const float* mass = p.mass + bh * p.mass_width + p.sink;
-  const int slots = c.max_pages * c.page_size - p.sink;
+  const int64_t bh = blockIdx.x / parts;
+  const int part = blockIdx.x % parts, b = (int)(bh / c.Hkv), h = (int)(bh % c.Hkv);
+  const float* row_mass = p.mass + bh * p.mass_width;
+  const int cap = c.max_pages * c.page_size, slots = max(1, cap - p.sink);
+  const float* mass = row_mass + min(p.sink, cap - 1);  // a budget may exceed the table; then nothing is selected
   uint32_t key[KPT ? KPT : 1];
 #pragma unroll
-  for (int k = 0; k < KPT; ++k) {
-    const int i = k * kSelThreads + tid;
-    key[k] = i < slots ? mass_key(__ldg(mass + i)) : 0u;
-  }
-  const int n = paged_length(c, (int)(bh / c.Hkv), SITE_PAGED_EVICT);
+  for (int k = 0; k < KPT; ++k) key[k] = __float_as_uint(__ldg(mass + min(k * kEvictThreads + tid, slots - 1)));
+  const int n = paged_length(c, b, SITE_PAGED_EVICT), all = min(n, p.budget);
+  // this part's places; the last part also clears the masses behind the survivors
+  const int per = (p.budget + parts - 1) / parts, beg = min(part * per, p.budget), end = min(beg + per, p.budget);
   int* kept = p.kept + bh * p.budget;
-  if (n <= p.budget) {
-    for (int t = tid; t < p.budget; t += kSelThreads) kept[t] = t < n ? t : -1;
-    return;
+  float* mass_out = p.mass_out + bh * p.out_width;
+  for (int i = max(beg, all) + tid; i < end; i += kEvictThreads) {
+    kept[i] = -1;
+    if (MOVE) mass_out[i] = 0.f;
   }
+  if (MOVE && part == parts - 1)
+    for (int64_t i = p.budget + tid; i < p.out_width; i += kEvictThreads) mass_out[i] = 0.f;
+  if (beg >= all) return;
   const int nc = n - p.sink - p.recent, places = p.budget - p.sink - p.recent;  // candidates, and room for them
-  for (int t = tid; t < p.sink; t += kSelThreads) kept[t] = t;
-  for (int t = tid; t < p.recent; t += kSelThreads) kept[p.budget - p.recent + t] = n - p.recent + t;
-  if (places == 0) return;
-  // f(key, candidate) for the thread's candidates
-  auto each = [&](auto&& f) {
-    if (KPT) {
-#pragma unroll
-      for (int k = 0; k < KPT; ++k)
-        if (k * kSelThreads + tid < nc) f(key[k]);
-    } else {
-#pragma unroll 4
-      for (int i = tid; i < nc; i += kSelThreads) f(mass_key(__ldg(mass + i)));
-    }
-  };
-  for (int i = tid; i < 3 * 2048; i += kSelThreads) hist[0][i] = 0;
-  __syncthreads();
-  uint32_t prefix = 0, mask = 0;
+  const bool select = n > p.budget && places > 0;
+  uint32_t prefix = 0;
   int above = 0;  // candidates above the prefix
-#pragma unroll 1
-  for (int pass = 0; pass < 3; ++pass) {
-    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
-    const uint32_t digits = (1u << bits) - 1;
-    uint32_t* h = hist[pass];
-    each([&](uint32_t k) {
-      if ((k & mask) == prefix) atomicAdd(h + (k >> shift & digits), 1u);
-    });
-    __syncthreads();
-    // thread t holds the four digits from 2047 - 4 t down; sums from the top
-    const int d0 = 2047 - 4 * tid;
-    const uint4 four = *reinterpret_cast<const uint4*>(h + d0 - 3);
-    const int at[4] = {(int)four.w, (int)four.z, (int)four.y, (int)four.x};
-    const int all = at[0] + at[1] + at[2] + at[3];
-    int incl = all;
+  if (select) {
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int t = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += t;
-    }
-    if (lane == 31) wsum[warp] = incl;
-    __syncthreads();
-    int w = lane < warp ? wsum[lane] : 0;
+    for (int k = 0; k < KPT; ++k) key[k] = mass_key(__uint_as_float(key[k]));
+    // f(key) for the thread's candidates
+    auto each = [&](auto&& f) {
+      if (KPT) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
-    int before = above + w + incl - all;
-    if (before < places && before + all >= places) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if (before < places && before + at[k] >= places) {
-          sh_digit[pass] = (uint32_t)(d0 - k);
-          sh_above[pass] = before;
-        }
-        before += at[k];
+        for (int k = 0; k < KPT; ++k)
+          if (k * kEvictThreads + tid < nc) f(key[k]);
+      } else {
+#pragma unroll 4
+        for (int i = tid; i < nc; i += kEvictThreads) f(mass_key(__ldg(mass + i)));
       }
-    }
+    };
+    for (int i = tid * 4; i < 10240; i += kEvictThreads * 4) *reinterpret_cast<uint4*>(hist + i) = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    prefix |= sh_digit[pass] << shift;
-    mask |= digits << shift;
-    above = sh_above[pass];
+    uint32_t mask = 0;
+    // one digit: PER of its values per thread, thread t from the top; COPIES counts of each, side by side
+    auto pass = [&](auto which, uint32_t* hs, int shift, int bits, auto per, auto copies) {
+      constexpr int P = decltype(which)::value, PER = decltype(per)::value, COPIES = decltype(copies)::value;
+      const uint32_t digits = (1u << bits) - 1;
+      each([&](uint32_t k) {
+        if ((k & mask) == prefix) atomicAdd(hs + (k >> shift & digits) * COPIES + (COPIES > 1 ? lane % COPIES : 0), 1u);
+      });
+      __syncthreads();
+      const int d0 = (int)digits - PER * tid;
+      int at[PER], sum = 0;
+#pragma unroll
+      for (int k = 0; k < PER; ++k) {
+        at[k] = 0;
+#pragma unroll
+        for (int j = 0; j < COPIES; ++j) at[k] += (int)hs[(d0 - k) * COPIES + j];
+        sum += at[k];
+      }
+      int incl = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int t = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += t;
+      }
+      if (lane == 31) wsum[warp] = incl;
+      __syncthreads();
+      int w = lane < warp ? wsum[lane] : 0;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
+      int before = above + w + incl - sum;
+      if (before < places && before + sum >= places) {
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+          if (before < places && before + at[k] >= places) {
+            sh_digit[P] = (uint32_t)(d0 - k);
+            sh_above[P] = before;
+          }
+          before += at[k];
+        }
+      }
+      __syncthreads();
+      prefix |= sh_digit[P] << shift;
+      mask |= digits << shift;
+      above = sh_above[P];
+    };
+    pass(Int<0>{}, hist, 23, 9, Int<1>{}, Int<8>{});
+    pass(Int<1>{}, hist + 4096, 11, 12, Int<8>{}, Int<1>{});
+    pass(Int<2>{}, hist + 8192, 0, 11, Int<4>{}, Int<1>{});
   }
   // survivors: keys above `prefix`, and the first `ties` that equal it. Runs of 32 candidates (KPT) or a
-  // warp's share of them all are counted, the counts before each summed, then the runs written.
+  // warp's share of them all are counted, and the counts before each summed.
   const int ties = places - above;
   const uint32_t below = (1u << lane) - 1;
-  constexpr int kRuns = KPT ? KPT * kSelWarps : kSelWarps, kPer = (kRuns + kSelThreads - 1) / kSelThreads;
-  __shared__ unsigned long long part[kSelWarps];
-  auto scan = [&] {  // runs[i] becomes the sum before it; thread t has kPer runs
-    unsigned long long v[kPer], all = 0, incl;
+  const int run = ((nc + kEvictWarps - 1) / kEvictWarps + 31) / 32 * 32, i0 = warp * run, i1 = min(nc, i0 + run);  // KPT = 0
+  if (select) {
+    if (KPT) {
+#pragma unroll
+      for (int k = 0; k < KPT; ++k) {
+        const bool in = k * kEvictThreads + tid < nc;
+        const unsigned bg = __ballot_sync(0xffffffffu, in && key[k] > prefix), be = __ballot_sync(0xffffffffu, in && key[k] == prefix);
+        if (lane == 0) runs[k * kEvictWarps + warp] = (unsigned long long)__popc(bg) << 32 | __popc(be);
+      }
+    } else {
+      int gt = 0, eq = 0;
+      for (int i = i0; i < i1; i += 32) {
+        const bool in = i + lane < i1;
+        const uint32_t k = in ? mass_key(__ldg(mass + i + lane)) : 0u;
+        gt += __popc(__ballot_sync(0xffffffffu, in && k > prefix));
+        eq += __popc(__ballot_sync(0xffffffffu, in && k == prefix));
+      }
+      if (lane == 0) runs[warp] = (unsigned long long)gt << 32 | (uint32_t)eq;
+    }
+    __syncthreads();
+    constexpr int kRuns = KPT ? KPT * kEvictWarps : kEvictWarps, kPer = (kRuns + kEvictThreads - 1) / kEvictThreads;
+    unsigned long long v[kPer], sum = 0, incl;
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
       v[k] = tid * kPer + k < kRuns ? runs[tid * kPer + k] : 0ull;
-      all += v[k];
+      sum += v[k];
     }
-    incl = all;
+    incl = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const unsigned long long t = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += t;
     }
-    if (lane == 31) part[warp] = incl;
+    if (lane == 31) part_sum[warp] = incl;
     __syncthreads();
-    unsigned long long w = lane < warp ? part[lane] : 0ull;
+    unsigned long long w = lane < warp ? part_sum[lane] : 0ull;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
-    w += incl - all;
+    w += incl - sum;
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
       if (tid * kPer + k < kRuns) runs[tid * kPer + k] = w;
       w += v[k];
     }
+  }
+  uint4* kp = (uint4*)c.k;
+  uint4* vp = (uint4*)c.v;
+  const int per16 = c.Dh / pieces, head = h * c.page_size;  // elements of 16 bytes; the head's first row in a page
+  const int64_t ks = c.k_stride / per16, vs = c.v_stride / per16;
+  const int step = MOVE ? kEvictList : p.budget;
+  for (int lo = beg; lo < min(end, all); lo += step) {
+    const int hi = MOVE ? min(lo + step, min(end, all)) : all;
+    int* to_list = MOVE ? list : kept;
     __syncthreads();
-  };
-  auto write = [&](bool in, uint32_t k, int i, int gt, int eq, unsigned bg, unsigned be) {
-    const int mine = eq + __popc(be & below), at = gt + __popc(bg & below) + min(mine, ties);
-    if (in && (k > prefix || (k == prefix && mine < ties))) kept[p.sink + at] = p.sink + i;
-  };
-  if (KPT) {
+    // list the survivors of places [lo, hi)
+    auto put = [&](int place, int slot) {
+      if (place >= lo && place < hi) to_list[place - lo] = slot;
+    };
+    if (!select) {  // all of them, or the first and the last ones alone
+      for (int i = lo + tid; i < hi; i += kEvictThreads) to_list[i - lo] = n <= p.budget || i < p.sink ? i : n - p.budget + i;
+    } else {
+      for (int i = tid; i < p.sink; i += kEvictThreads) put(i, i);
+      for (int i = tid; i < p.recent; i += kEvictThreads) put(p.budget - p.recent + i, n - p.recent + i);
+      auto candidate = [&](bool in, uint32_t k, int i, int gt, int eq, unsigned bg, unsigned be) {
+        const int mine = eq + __popc(be & below);
+        if (in && (k > prefix || (k == prefix && mine < ties))) put(p.sink + gt + __popc(bg & below) + min(mine, ties), p.sink + i);
+      };
+      if (KPT) {
 #pragma unroll
-    for (int k = 0; k < KPT; ++k) {
-      const bool in = k * kSelThreads + tid < nc;
-      const unsigned bg = __ballot_sync(0xffffffffu, in && key[k] > prefix), be = __ballot_sync(0xffffffffu, in && key[k] == prefix);
-      if (lane == 0) runs[k * kSelWarps + warp] = (unsigned long long)__popc(bg) << 32 | __popc(be);
+        for (int k = 0; k < KPT; ++k) {
+          const int i = k * kEvictThreads + tid;
+          const bool in = i < nc;
+          const unsigned bg = __ballot_sync(0xffffffffu, in && key[k] > prefix), be = __ballot_sync(0xffffffffu, in && key[k] == prefix);
+          const unsigned long long r = runs[k * kEvictWarps + warp];
+          candidate(in, key[k], i, (int)(r >> 32), (int)(uint32_t)r, bg, be);
+        }
+      } else {
+        int gt = (int)(runs[warp] >> 32), eq = (int)(uint32_t)runs[warp];
+        for (int i = i0; i < i1; i += 32) {
+          const bool in = i + lane < i1;
+          const uint32_t k = in ? mass_key(__ldg(mass + i + lane)) : 0u;
+          const unsigned bg = __ballot_sync(0xffffffffu, in && k > prefix), be = __ballot_sync(0xffffffffu, in && k == prefix);
+          candidate(in, k, i + lane, gt, eq, bg, be);
+          gt += __popc(bg);
+          eq += __popc(be);
+        }
+      }
+    }
+    if (!MOVE) return;
+    __syncthreads();
+    static_assert(kEvictList == kEvictThreads, "one place per thread");
+    if (tid < hi - lo) {
+      const int i = lo + tid, src = list[tid], si = src / c.page_size, di = i / c.page_size;
+      kept[i] = src;
+      mass_out[i] = row_mass[src];
+      const int ps = paged_page(c, c.table, b * c.table_stride, si, SITE_PAGED_EVICT);
+      const int pd = paged_page(c, p.dst, b * p.dst_stride, di, SITE_PAGED_EVICT);
+      const bool there = ps >= 0 && pd >= 0;
+      const int64_t sr = (int64_t)(head + src - si * c.page_size) * pieces, dr = (int64_t)(head + i - di * c.page_size) * pieces;
+      from[tid] = there ? ps * ks + sr : -1;
+      from[kEvictList + tid] = there ? ps * vs + sr : -1;
+      to[tid] = pd * ks + dr;
+      to[kEvictList + tid] = pd * vs + dr;
     }
     __syncthreads();
-    scan();
+    const int count = (hi - lo) * pieces;
+    for (int e0 = tid; e0 < count; e0 += kEvictAhead * kEvictThreads) {
+      uint4 a[kEvictAhead], v[kEvictAhead];
+      int place[kEvictAhead];
 #pragma unroll
-    for (int k = 0; k < KPT; ++k) {
-      const int i = k * kSelThreads + tid;
-      const bool in = i < nc;
-      const unsigned bg = __ballot_sync(0xffffffffu, in && key[k] > prefix), be = __ballot_sync(0xffffffffu, in && key[k] == prefix);
-      const unsigned long long r = runs[k * kSelWarps + warp];
-      write(in, key[k], i, (int)(r >> 32), (int)(uint32_t)r, bg, be);
-    }
-  } else {
-    const int run = ((nc + kSelWarps - 1) / kSelWarps + 31) / 32 * 32, i0 = warp * run, i1 = min(nc, i0 + run);
-    int gt = 0, eq = 0;
-    for (int i = i0; i < i1; i += 32) {
-      const bool in = i + lane < i1;
-      const uint32_t k = in ? mass_key(__ldg(mass + i + lane)) : 0u;
-      gt += __popc(__ballot_sync(0xffffffffu, in && k > prefix));
-      eq += __popc(__ballot_sync(0xffffffffu, in && k == prefix));
-    }
-    if (lane == 0) runs[warp] = (unsigned long long)gt << 32 | (uint32_t)eq;
-    __syncthreads();
-    scan();
-    gt = (int)(runs[warp] >> 32);
-    eq = (int)(uint32_t)runs[warp];
-    for (int i = i0; i < i1; i += 32) {
-      const bool in = i + lane < i1;
-      const uint32_t k = in ? mass_key(__ldg(mass + i + lane)) : 0u;
-      const unsigned bg = __ballot_sync(0xffffffffu, in && k > prefix), be = __ballot_sync(0xffffffffu, in && k == prefix);
-      write(in, k, i + lane, gt, eq, bg, be);
-      gt += __popc(bg);
-      eq += __popc(be);
+      for (int k = 0; k < kEvictAhead; ++k) {
+        const int e = e0 + k * kEvictThreads;
+        place[k] = e < count ? e / pieces : -1;
+        if (place[k] < 0 || from[place[k]] < 0) {
+          place[k] = -1;
+          continue;
+        }
+        a[k] = kp[from[place[k]] + (e - place[k] * pieces)];
+        v[k] = vp[from[kEvictList + place[k]] + (e - place[k] * pieces)];
+      }
+#pragma unroll
+      for (int k = 0; k < kEvictAhead; ++k) {
+        if (place[k] < 0) continue;
+        const int piece = e0 + k * kEvictThreads - place[k] * pieces;
+        kp[to[place[k]] + piece] = a[k];
+        vp[to[kEvictList + place[k]] + piece] = v[k];
+      }
     }
   }
 }

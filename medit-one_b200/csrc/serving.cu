@@ -304,22 +304,25 @@ extern "C" int one_paged_evict(const one_paged_cache* cache, const int32_t* dst_
   if (dst_max_pages < 1 || dst_stride < dst_max_pages || (int64_t)dst_max_pages * page_size < budget)
     return fail(ONE_ERR_INVALID, "paged evict: the destination pages hold fewer slots than the budget");
   if (mass_out_width < budget) return fail(ONE_ERR_INVALID, "paged evict: mass rows are too short");
-  const int64_t per_bh = (mass_out_width + kMovePlaces - 1) / kMovePlaces;
-  if (mass_out_width > 0x3fffffff || per_bh * b * hkv > 0x7fffffff)
-    return fail(ONE_ERR_UNSUPPORTED, "paged evict: too many rows");
+  if (mass_out_width > 0x3fffffff) return fail(ONE_ERR_UNSUPPORTED, "paged evict: too many rows");
   p.dst = dst_table; p.dst_stride = dst_stride; p.mass = cache->mass; p.mass_width = cache->mass_width;
   p.budget = budget; p.recent = recent; p.sink = sink; p.mass_out = mass_out; p.out_width = mass_out_width; p.kept = kept;
   cudaStream_t st = (cudaStream_t)stream;
-  const int64_t slots = (int64_t)cache->max_pages * page_size;
-  const dim3 one_each(b * hkv), threads(kSelThreads);
-  rc = launched(slots <= 2048    ? launch(paged_select_kernel<4>, one_each, threads, 0, st, p)
-                : slots <= 8192  ? launch(paged_select_kernel<16>, one_each, threads, 0, st, p)
-                : slots <= 32768 ? launch(paged_select_kernel<64>, one_each, threads, 0, st, p)
-                                 : launch(paged_select_kernel<0>, one_each, threads, 0, st, p),
-                "paged select");
-  if (rc) return rc;
-  return launched(launch(paged_move_kernel, dim3((unsigned)(per_bh * b * hkv)), dim3(kMoveThreads), 0, st, p, (int)per_bh,
-                         dh * elem_bytes(dtype) / 16),
+  const int64_t slots = (int64_t)cache->max_pages * page_size, heads = (int64_t)b * hkv;
+  const int64_t parts = (budget + 255) / 256, per_bh = (mass_out_width + kMovePlaces - 1) / kMovePlaces;
+  const bool one_launch = heads * parts <= 2 * num_sms();  // two CTAs per SM
+  if (heads * std::max(parts, per_bh) > 0x7fffffff) return fail(ONE_ERR_UNSUPPORTED, "paged evict: too many rows");
+  const int pieces = dh * elem_bytes(dtype) / 16;
+  auto evict = [&](auto keys) {
+    constexpr int KPT = decltype(keys)::value;
+    return one_launch ? launch(paged_evict_kernel<KPT, true>, dim3((unsigned)(heads * parts)), dim3(kEvictThreads), 0, st, p,
+                               (int)parts, pieces)
+                      : launch(paged_evict_kernel<KPT, false>, dim3((unsigned)heads), dim3(kEvictThreads), 0, st, p, 1, pieces);
+  };
+  rc = launched(slots <= 2048 ? evict(Int<4>()) : slots <= 8192 ? evict(Int<16>()) : slots <= 32768 ? evict(Int<64>()) : evict(Int<0>()),
+                "paged evict");
+  if (rc || one_launch) return rc;
+  return launched(launch(paged_move_kernel, dim3((unsigned)(per_bh * heads)), dim3(kMoveThreads), 0, st, p, (int)per_bh, pieces),
                   "paged move");
 }
 

@@ -283,7 +283,7 @@ def test_append_row_strides_that_are_not_aligned():
 EVICT = [  # hkv, dh, page, lengths, budget, recent, sink
     (2, 64, 16, [40, 33, 32, 31, 0, 1], 32, 8, 4), (1, 64, 16, [1000], 999, 0, 0), (3, 32, 7, [200, 64, 70], 64, 64, 0),
     (1, 128, 48, [5000, 2], 100, 30, 70), (2, 8, 1, [9, 3], 1, 0, 0), (1, 40, 5, [300, 299], 128, 5, 1),
-    (12, 64, 16, [2049, 2048, 500], 2048, 100, 4), (1, 16, 128, [70000], 1000, 100, 0), (1, 64, 16, [50], 60, 10, 0),
+    (12, 64, 16, [2049, 2048, 500], 2048, 100, 4), (1, 16, 128, [70000], 1000, 100, 0), (1, 64, 16, [50], 60, 10, 0), (2, 32, 16, [48, 3], 70, 5, 64),
     (2, 64, 16, [20000, 16384], 16000, 0, 0),
 ]
 
