@@ -102,17 +102,19 @@ struct PaCursor {
     b = c.B;
     kv = gi = tile = tiles = len = 0;
   }
-  ONE_DEVINL void next(const PagedCache& c, int ng) {
-    if (++tile < tiles) return;
+  // Returns whether this is another segment.
+  ONE_DEVINL bool next(const PagedCache& c, int ng) {
+    if (++tile < tiles) return false;
     tile = 0;
-    if (++gi < ng) return;
+    if (++gi < ng) return true;
     gi = 0;
-    if (++kv < c.Hkv) return;
+    if (++kv < c.Hkv) return true;
     kv = 0;
     do {
       ++b;
       load(c);
     } while (tiles == 0 && b < c.B);
+    return true;
   }
 };
 
@@ -151,23 +153,30 @@ ONE_DEVINL void mma_bf16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t
 template <typename D, int CH>
 struct PaCopy {
   static constexpr int N = 16 * CH / 32;
-  // rows that follow one another in memory, the first `live` of them in use, `pieces` of CH there
-  template <bool FULL>
-  ONE_DEVINL static void run(uint8_t* to, const uint8_t* from, int live, int pieces) {
+  // 16 whole rows that follow one another in memory, from this lane's first piece on
+  ONE_DEVINL static void full(uint32_t to, const uint8_t* from) {
     const int lane = threadIdx.x & 31;
-    if (FULL && live == 16 && 32 % CH == 0) {
-      const uint32_t s = smem_u32(to), mine = D::at(lane / CH, lane % CH);
-      const uint8_t* g = from + lane * 16;
+    if constexpr (32 % CH == 0) {
+      const uint32_t mine = D::at(lane / CH, lane % CH);
       static_for<N>([&](auto n) {
         constexpr int k = decltype(n)::value, at = D::at(k * 32 / CH, 0);
-        cp_async16_at<(at & ~127), k * 512>(s + (mine ^ (at & 127)), g);
+        cp_async16_at<(at & ~127), k * 512>(to + (mine ^ (at & 127)), from);
       });
-      return;
+    } else {
+      static_for<N>([&](auto n) {
+        constexpr int k = decltype(n)::value;
+        const int e = k * 32 + lane;
+        cp_async16_at<0, k * 512>(to + D::at(e / CH, e % CH), from);
+      });
     }
+  }
+  // the first `live` of such rows, the rest as zeros
+  ONE_DEVINL static void some(uint8_t* to, const uint8_t* from, int live) {
+    const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       const int e = k * 32 + lane, row = e / CH, ch = e % CH;
-      cp_async16_or_zero(to + D::at(row, ch), from + (FULL ? e : row * pieces + ch) * 16, row < live && (FULL || ch < pieces));
+      cp_async16_or_zero(to + D::at(row, ch), from + k * 512, row < live);
     }
   }
   // rows anywhere: lane first + t holds the byte offset of row t, or -1
@@ -225,19 +234,15 @@ struct PaBf16 {
                          : VC * 2048 + ((row & 3) * 4 + (row >> 2)) * 64 + ((ch - 8 * VC) ^ row >> 3 << 1) * 16;
     }
   };
-  // 16 slots that lie in one page, the first `live` of them in use; kat, vat: element offsets of the
-  // first. FULL: Dh is DH.
-  template <bool FULL>
-  ONE_DEVINL static void issue_run(const PagedAttn& p, uint8_t* stage, int64_t kat, int64_t vat, int live) {
-    PaCopy<KTo, CH>::template run<FULL>(stage, (const uint8_t*)((const T*)p.c.k + kat), live, p.c.Dh / 8);
-    PaCopy<VTo, CH>::template run<FULL>(stage + 32 * DH, (const uint8_t*)((const T*)p.c.v + vat), live, p.c.Dh / 8);
-  }
+  static constexpr int kValues = 32 * DH;  // where a group's values start
   // 16 slots anywhere: lane t holds the element offset of slot t's key, lane 16 + t that of its value,
   // or -1.
-  ONE_DEVINL static void issue_any(const PagedAttn& p, uint8_t* stage, int64_t off) {
+  using Keys = PaCopy<KTo, CH>;
+  using Values = PaCopy<VTo, CH>;
+  ONE_DEVINL static void issue_any(uint8_t* stage, const T* keys, const T* values, int64_t off, int Dh) {
     const int64_t at = off < 0 ? -1 : off * (int)sizeof(T);
-    PaCopy<KTo, CH>::any(stage, (const uint8_t*)p.c.k, at, 0, p.c.Dh / 8);
-    PaCopy<VTo, CH>::any(stage + 32 * DH, (const uint8_t*)p.c.v, at, 16, p.c.Dh / 8);
+    Keys::any(stage, (const uint8_t*)keys, at, 0, Dh / 8);
+    Values::any(stage + kValues, (const uint8_t*)values, at, 16, Dh / 8);
   }
 
   ONE_DEVINL void begin(const PagedAttn& p, uint8_t*, const T* q, int rows) {
@@ -439,15 +444,13 @@ struct PaF32 {
   struct VTo {
     __host__ __device__ static constexpr int at(int row, int ch) { return (row * CH + ch) * 16; }
   };
-  template <bool FULL>
-  ONE_DEVINL static void issue_run(const PagedAttn& p, uint8_t* stage, int64_t kat, int64_t vat, int live) {
-    PaCopy<KTo, CH>::template run<FULL>(stage, (const uint8_t*)((const T*)p.c.k + kat), live, p.c.Dh / 4);
-    PaCopy<VTo, CH>::template run<FULL>(stage + 64 * DH, (const uint8_t*)((const T*)p.c.v + vat), live, p.c.Dh / 4);
-  }
-  ONE_DEVINL static void issue_any(const PagedAttn& p, uint8_t* stage, int64_t off) {
+  static constexpr int kValues = 64 * DH;
+  using Keys = PaCopy<KTo, CH>;
+  using Values = PaCopy<VTo, CH>;
+  ONE_DEVINL static void issue_any(uint8_t* stage, const T* keys, const T* values, int64_t off, int Dh) {
     const int64_t at = off < 0 ? -1 : off * (int)sizeof(T);
-    PaCopy<KTo, CH>::any(stage, (const uint8_t*)p.c.k, at, 0, p.c.Dh / 4);
-    PaCopy<VTo, CH>::any(stage + 64 * DH, (const uint8_t*)p.c.v, at, 16, p.c.Dh / 4);
+    Keys::any(stage, (const uint8_t*)keys, at, 0, Dh / 4);
+    Values::any(stage + kValues, (const uint8_t*)values, at, 16, Dh / 4);
   }
 
   ONE_DEVINL void begin(const PagedAttn& p, uint8_t* extra, const T* q, int rows) {
@@ -603,25 +606,35 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E>::kPerSm) paged_attn_k
   // ---- the copying side: page numbers are asked for one tile ahead of the copies. RUN: one per group;
   //      otherwise lane t and lane 16 + t look slot t up.
   PaCursor<TILE> src = cur;
-  int to_copy = left, pg[GR], in_page[GR];
-  uint32_t live[E::kStages][GR];  // slots in use of the tiles in the ring, the oldest first
+  int to_copy = left, pg[GR], row[GR];  // page and first element in its head of each group
+  uint32_t live[E::kStages][GR];        // slots in use of the tiles in the ring, the oldest first
 #pragma unroll
   for (int k = 0; k < E::kStages; ++k)
 #pragma unroll
     for (int g = 0; g < GR; ++g) live[k][g] = 0;
   const int mine = warp * (16 * GR) + (RUN ? 0 : lane & 15);
+  const int* table;          // of the segment being copied:
+  const T *keys, *values;    // its block table, and its head in page 0 (RUN: this lane's first piece)
+  auto segment = [&] {
+    const int64_t head = (int64_t)src.kv * c.page_size * c.Dh + (RUN ? lane * (int)(16 / sizeof(T)) : 0);
+    table = c.table + src.b * c.table_stride;
+    keys = (const T*)c.k + head;
+    values = (const T*)c.v + head;
+  };
+  int ahead = src.len - src.tile * TILE - mine;  // slots from this warp's first one to the end
   auto ask = [&] {
+    const int t0 = src.len - ahead;
 #pragma unroll
     for (int g = 0; g < GR; ++g) {
-      const int t = src.tile * TILE + mine + 16 * g;
       pg[g] = -1;
-      if (to_copy > 0 && t < src.len) {
-        const int index = (int)(((uint64_t)(uint32_t)t * p.div_m) >> p.div_s);
-        in_page[g] = t - index * c.page_size;
-        pg[g] = c.table[src.b * c.table_stride + index];
+      if (ahead > 16 * g) {
+        const int t = t0 + 16 * g, index = (int)(((uint64_t)(uint32_t)t * p.div_m) >> p.div_s);
+        row[g] = (t - index * c.page_size) * c.Dh;
+        pg[g] = table[index];
       }
     }
   };
+  const int ks = (int)c.k_stride, vs = (int)c.v_stride;
   uint32_t put = 0, get = 0;  // byte offsets of stages
   auto copy = [&] {
 #pragma unroll
@@ -631,31 +644,46 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E>::kPerSm) paged_attn_k
     if (to_copy > 0) {
 #pragma unroll
       for (int g = 0; g < GR; ++g) {
-        const int t = src.tile * TILE + mine + 16 * g;
-        if ((uint32_t)pg[g] >= (uint32_t)c.num_pages && t < src.len) {
-          set_err(c.err, ERR_BAD_ARG, SITE_PAGED_ATTN);
-          pg[g] = -1;
-        }
-        const int row = (src.kv * c.page_size + in_page[g]) * c.Dh;
+        uint8_t* to = ring + put + g * E::kGroup;
+        uint32_t& alive = live[E::kStages - 1][g];
+        const bool good = (uint32_t)pg[g] < (uint32_t)c.num_pages;
+        if (!good && ahead > 16 * g) set_err(c.err, ERR_BAD_ARG, SITE_PAGED_ATTN);
         if (RUN) {
-          const int n = pg[g] < 0 ? 0 : min(16, src.len - t);
-          live[E::kStages - 1][g] = (1u << n) - 1;
-          if (n > 0)
-            E::template issue_run<true>(p, ring + put + g * E::kGroup, (int64_t)pg[g] * (int)c.k_stride + row,
-                                        (int64_t)pg[g] * (int)c.v_stride + row, n);
+          alive = 0;
+          if (good) {
+            const uint8_t* kp = (const uint8_t*)(keys + ((int64_t)pg[g] * ks + row[g]));
+            const uint8_t* vp = (const uint8_t*)(values + ((int64_t)pg[g] * vs + row[g]));
+            if (ahead >= 16 * g + 16) {
+              alive = 0xffffu;
+              E::Keys::full(smem_u32(to), kp);
+              E::Values::full(smem_u32(to) + E::kValues, vp);
+            } else {
+              const int n = ahead - 16 * g;
+              alive = (1u << n) - 1;
+              E::Keys::some(to, kp, n);
+              E::Values::some(to + E::kValues, vp, n);
+            }
+          }
         } else {
-          const int64_t off = pg[g] < 0 ? -1 : (int64_t)pg[g] * (int)(lane < 16 ? c.k_stride : c.v_stride) + row;
-          const uint32_t some = __ballot_sync(0xffffffffu, off >= 0) & 0xffffu;
-          live[E::kStages - 1][g] = some;
-          if (some) E::issue_any(p, ring + put + g * E::kGroup, off);
+          const int64_t off = !good ? -1 : lane < 16 ? (int64_t)pg[g] * ks + row[g] : (int64_t)pg[g] * vs + row[g];
+          alive = __ballot_sync(0xffffffffu, good) & 0xffffu;
+          if (alive) E::issue_any(to, keys, values, off, c.Dh);
         }
       }
-      if (--to_copy > 0) src.next(c, ng);
-      ask();
+      if (--to_copy > 0) {
+        ahead -= TILE;
+        if (src.next(c, ng)) {
+          segment();
+          ahead = src.len - src.tile * TILE - mine;
+        }
+        ask();
+      }
     }
     cp_async_commit();
     put = put + S::kStage == S::kWarp ? 0 : put + S::kStage;
   };
+  segment();
+  if (to_copy == 0) ahead = 0;
   ask();
 #pragma unroll 1
   for (int i = 0; i < E::kStages - 1; ++i) copy();
