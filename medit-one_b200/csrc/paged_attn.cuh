@@ -48,7 +48,7 @@ struct PagedAttn {
   int64_t score_ld;
   int2* parts;            // [B * Hkv * hv_per_kv]: first CTA of a segment; last << 1 | (its first part is slot 1)
   int ranges;             // CTAs that share the list
-  int split;
+  int cluster;            // CTAs per segment, where there is no list
 };
 
 template <int TILE>
@@ -215,7 +215,7 @@ struct PaBf16 {
   static constexpr int kGroups = DH <= 64 ? 128 / DH : 1;  // 16-slot groups per warp and step
   static constexpr int TILE = 16 * kGroups * kPaWarps;
   static constexpr int kGroup = 64 * DH;               // bytes of a group's keys and values
-  static constexpr int kStages = 2;
+  static constexpr int kStages = 2, kStagesFew = 3;    // of a list, that fills the SMs; of clusters
   static constexpr int kExtra = 0;                     // further shared bytes per warp
   uint32_t qa[WIDE ? 2 : 1][KC][4];
   float o[NT][4];
@@ -419,23 +419,24 @@ struct PaBf16 {
 };
 
 // ------------------------------------------------------------------ fp32: FMA units
-// Four query heads. Scores: lane (r, c) takes slots r and r + 8 and every fourth 16-byte chunk of
-// their keys, for all four heads; the sums over c are exchanged so that lane c ends with head c.
-// Weighted sum: the weights pass through shared memory, a lane owns the dims lane + 32 i.
-template <int DH_>
+// ROWS query heads, 1 or 4. Scores: lane (r, c) takes slots r and r + 8 and every fourth 16-byte piece
+// of their keys, for all heads; the sums over c are exchanged so that lane c ends with head c (one
+// head: every lane with its score). Weighted sum: the weights pass through shared memory, a lane owns
+// the dims lane + 32 i.
+template <int DH_, int ROWS_>
 struct PaF32 {
   using T = float;
-  static constexpr int DH = DH_, ROWS = 4;
-  static constexpr int KC = DH / 16, VC = DH / 32;
+  static constexpr int DH = DH_, ROWS = ROWS_;
+  static constexpr int KC = DH / 16, VC = DH / 32, CH = DH / 4;
   static constexpr int kGroups = 1, TILE = 16 * kPaWarps;
   static constexpr int kGroup = 128 * DH;
-  static constexpr int kStages = DH == 32 ? 4 : DH == 96 ? 2 : 3;
-  static constexpr int kExtra = 4 * DH * 4 + 16 * 16;  // q [4][DH], weights [16][4]
-  float o[4][VC];
+  static constexpr int kValues = 64 * DH;
+  static constexpr int kStages = DH == 32 ? 4 : DH == 96 ? 2 : 3, kStagesFew = kStages;
+  static constexpr int kExtra = ROWS * DH * 4 + 16 * ROWS * 4;  // q [ROWS][DH], weights [16][ROWS]
+  float o[ROWS][VC];
   float m, l;  // of head c
   float *qs, *ps;
 
-  static constexpr int CH = DH / 4;
   struct KTo {
     __host__ __device__ static constexpr int at(int row, int ch) {
       return (ch >> 3) * 2048 + row * 128 + ((ch & 7) ^ (row & 1) << 2) * 16;
@@ -444,7 +445,6 @@ struct PaF32 {
   struct VTo {
     __host__ __device__ static constexpr int at(int row, int ch) { return (row * CH + ch) * 16; }
   };
-  static constexpr int kValues = 64 * DH;
   using Keys = PaCopy<KTo, CH>;
   using Values = PaCopy<VTo, CH>;
   ONE_DEVINL static void issue_any(uint8_t* stage, const T* keys, const T* values, int64_t off, int Dh) {
@@ -456,9 +456,9 @@ struct PaF32 {
   ONE_DEVINL void begin(const PagedAttn& p, uint8_t* extra, const T* q, int rows) {
     const int lane = threadIdx.x & 31;
     qs = reinterpret_cast<float*>(extra);
-    ps = qs + 4 * DH;
+    ps = qs + ROWS * DH;
     __syncwarp();
-    for (int i = lane; i < 4 * DH; i += 32) {
+    for (int i = lane; i < ROWS * DH; i += 32) {
       const int g = i / DH, d = i % DH;
       qs[i] = g < rows && d < p.c.Dh ? q[g * p.q_hs + d] : 0.f;
     }
@@ -466,7 +466,7 @@ struct PaF32 {
     m = -INFINITY;
     l = 0.f;
 #pragma unroll
-    for (int g = 0; g < 4; ++g)
+    for (int g = 0; g < ROWS; ++g)
 #pragma unroll
       for (int i = 0; i < VC; ++i) o[g][i] = 0.f;
   }
@@ -478,13 +478,15 @@ struct PaF32 {
       if (c < rows) scores[c * p.score_ld + r] = scores[c * p.score_ld + r + 8] = -INFINITY;
       return;
     }
-    float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    float s[2][ROWS];
+#pragma unroll
+    for (int g = 0; g < ROWS; ++g) s[0][g] = s[1][g] = 0.f;
 #pragma unroll
     for (int i = 0; i < KC; ++i) {
       const float4 a = *reinterpret_cast<const float4*>(stage + KTo::at(r, c + 4 * i));
       const float4 b = *reinterpret_cast<const float4*>(stage + KTo::at(r + 8, c + 4 * i));
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
+      for (int g = 0; g < ROWS; ++g) {
         const float4 q = *reinterpret_cast<const float4*>(qs + g * DH + (c + 4 * i) * 4);
         s[0][g] += q.x * a.x + q.y * a.y + q.z * a.z + q.w * a.w;
         s[1][g] += q.x * b.x + q.y * b.y + q.z * b.z + q.w * b.w;
@@ -492,11 +494,16 @@ struct PaF32 {
     }
     float x[2];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {  // lane c keeps head c
-      const float k0 = c & 2 ? s[j][2] : s[j][0], k1 = c & 2 ? s[j][3] : s[j][1];
-      const float g0 = c & 2 ? s[j][0] : s[j][2], g1 = c & 2 ? s[j][1] : s[j][3];
-      const float y0 = k0 + __shfl_xor_sync(0xffffffffu, g0, 2), y1 = k1 + __shfl_xor_sync(0xffffffffu, g1, 2);
-      x[j] = (c & 1 ? y1 : y0) + __shfl_xor_sync(0xffffffffu, c & 1 ? y0 : y1, 1);
+    for (int j = 0; j < 2; ++j) {
+      if constexpr (ROWS == 4) {  // lane c keeps head c
+        const float k0 = c & 2 ? s[j][2] : s[j][0], k1 = c & 2 ? s[j][3] : s[j][1];
+        const float g0 = c & 2 ? s[j][0] : s[j][2], g1 = c & 2 ? s[j][1] : s[j][3];
+        const float y0 = k0 + __shfl_xor_sync(0xffffffffu, g0, 2), y1 = k1 + __shfl_xor_sync(0xffffffffu, g1, 2);
+        x[j] = (c & 1 ? y1 : y0) + __shfl_xor_sync(0xffffffffu, c & 1 ? y0 : y1, 1);
+      } else {
+        x[j] = s[j][0] + __shfl_xor_sync(0xffffffffu, s[j][0], 2);
+        x[j] += __shfl_xor_sync(0xffffffffu, x[j], 1);
+      }
       x[j] = live >> (r + 8 * j) & 1 ? x[j] * p.scale_log2 : -INFINITY;
       if (scores && c < rows) scores[c * p.score_ld + r + 8 * j] = x[j];
     }
@@ -509,8 +516,8 @@ struct PaF32 {
       m = mn;
       l *= a;
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const float ag = __shfl_sync(0xffffffffu, a, g);
+      for (int g = 0; g < ROWS; ++g) {
+        const float ag = ROWS == 1 ? a : __shfl_sync(0xffffffffu, a, g);
 #pragma unroll
         for (int i = 0; i < VC; ++i) o[g][i] *= ag;
       }
@@ -520,21 +527,23 @@ struct PaF32 {
     for (int j = 0; j < 2; ++j) {
       x[j] = exp2f(x[j] - ms);
       l += x[j];
-      ps[(r + 8 * j) * 4 + c] = x[j];
+      if (c < ROWS) ps[(r + 8 * j) * ROWS + c] = x[j];
     }
     __syncwarp();
-    const float* vs = reinterpret_cast<const float*>(stage + 64 * DH);
+    const float* vs = reinterpret_cast<const float*>(stage + kValues);
 #pragma unroll
-    for (int t = 0; t < 16; ++t) {
-      const float4 w = *reinterpret_cast<const float4*>(ps + 4 * t);
+    for (int t0 = 0; t0 < 16; t0 += 4) {
+      float w[4][ROWS];
 #pragma unroll
-      for (int i = 0; i < VC; ++i) {
-        const float v = vs[t * DH + lane + 32 * i];
-        o[0][i] += w.x * v;
-        o[1][i] += w.y * v;
-        o[2][i] += w.z * v;
-        o[3][i] += w.w * v;
-      }
+      for (int t = 0; t < 4 * ROWS; t += 4) *reinterpret_cast<float4*>(&w[0][0] + t) = *reinterpret_cast<const float4*>(ps + t0 * ROWS + t);
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < VC; ++i) {
+          const float v = vs[(t0 + t) * DH + lane + 32 * i];
+#pragma unroll
+          for (int g = 0; g < ROWS; ++g) o[g][i] += w[t][g] * v;
+        }
     }
     __syncwarp();
   }
@@ -544,37 +553,62 @@ struct PaF32 {
     float t = l;
 #pragma unroll
     for (int d = 4; d < 32; d <<= 1) t += __shfl_xor_sync(0xffffffffu, t, d);
-    if (r == 0) {
+    if (r == 0 && c < ROWS) {
       ml[2 * c] = m;
       ml[2 * c + 1] = t;
     }
 #pragma unroll
-    for (int g = 0; g < 4; ++g)
+    for (int g = 0; g < ROWS; ++g)
 #pragma unroll
       for (int i = 0; i < VC; ++i) so[g * DH + lane + 32 * i] = o[g][i];
   }
 };
 
-template <typename E>
+ONE_DEVINL void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+ONE_DEVINL uint32_t cluster_at(const void* mine, int rank) {
+  uint32_t far;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(far) : "r"(smem_u32(mine)), "r"(rank));
+  return far;
+}
+// what CTA `rank` of the cluster has where this one has `mine`
+ONE_DEVINL float2 cluster_ld2(const float* mine, int rank) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(cluster_at(mine, rank)) : "memory");
+  return v;
+}
+ONE_DEVINL float4 cluster_ld4(const float* mine, int rank) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(cluster_at(mine, rank))
+               : "memory");
+  return v;
+}
+
+template <typename E, bool SPLIT>
 struct PaSmem {
   static constexpr int kStage = E::kGroup * E::kGroups;                  // bytes per warp
-  static constexpr int kWarp = kStage * E::kStages;
+  static constexpr int kStages = SPLIT ? E::kStages : E::kStagesFew;
+  static constexpr int kWarp = kStage * kStages;
   static constexpr int kML = kPaWarps * kWarp;                           // [warps][ROWS][2]
   static constexpr int kFin = kML + kPaWarps * E::ROWS * 8;              // [ROWS][2]: m, 1 / l
   static constexpr int kExtra = kFin + (E::ROWS * 8 + 15) / 16 * 16;
-  static constexpr int kTotal = kExtra + kPaWarps * E::kExtra;
+  static constexpr int kSum = kExtra + kPaWarps * E::kExtra;             // [ROWS][DH]: this CTA's sums, for its cluster
+  static constexpr int kTotal = kSum + E::ROWS * E::DH * 4;
   static constexpr int kPerSm = kSmPerSm / (kTotal + 1024) < 3 ? kSmPerSm / (kTotal + 1024) : 3;
   // a warp's sums fit the stage that it consumed last
   static_assert(kStage >= E::ROWS * E::DH * 4, "stage");
 };
 
-// p.split: CTA i takes the i-th share of the list. Otherwise CTA (hv, b) takes that segment whole and
-// nothing is left to join (short caches: one launch). RUN: pages hold a multiple of 16 slots and Dh is
+// SPLIT: CTA i takes the i-th share of the list. Otherwise a cluster of p.cluster CTAs (1 to 8) takes
+// each segment, in equal shares, and joins them through its shared memory: one launch, for small batches. RUN: pages hold a multiple of 16 slots and Dh is
 // E::DH, so that a group lies in one page and its copies need two addresses.
-template <typename E, bool RUN>
-__global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E>::kPerSm) paged_attn_kernel(const __grid_constant__ PagedAttn p) {
+template <typename E, bool RUN, bool SPLIT>
+__global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, SPLIT>::kPerSm) paged_attn_kernel(const __grid_constant__ PagedAttn p) {
   extern __shared__ __align__(16) uint8_t smem[];
-  using S = PaSmem<E>;
+  using S = PaSmem<E, SPLIT>;
   using T = typename E::T;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int TILE = E::TILE, GR = E::kGroups;
@@ -588,7 +622,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E>::kPerSm) paged_attn_k
   pdl_launch_dependents();
   PaCursor<TILE> cur;
   int left, share = 0;  // tiles to do; a full share
-  if (p.split) {
+  if (SPLIT) {
     const int total = pa_total<TILE>(p);
     share = max(1, (total + p.ranges - 1) / p.ranges);
     const long long w0 = (long long)share * blockIdx.x;
@@ -596,20 +630,21 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E>::kPerSm) paged_attn_k
     left = min(share, total - (int)w0);
     cur.seek(c, ng, (int)w0);
   } else {
-    cur.b = blockIdx.y;
-    cur.kv = blockIdx.x / ng;
-    cur.gi = blockIdx.x % ng;
-    cur.tile = 0;
+    const int seg = blockIdx.x / p.cluster, rank = blockIdx.x % p.cluster, HV = c.Hkv * ng;
+    cur.b = seg / HV;
+    cur.kv = (seg - cur.b * HV) / ng;
+    cur.gi = seg % ng;
     cur.load(c);
-    left = cur.tiles;
+    cur.tile = (int)((int64_t)cur.tiles * rank / p.cluster);
+    left = (int)((int64_t)cur.tiles * (rank + 1) / p.cluster) - cur.tile;
   }
   // ---- the copying side: page numbers are asked for one tile ahead of the copies. RUN: one per group;
   //      otherwise lane t and lane 16 + t look slot t up.
   PaCursor<TILE> src = cur;
   int to_copy = left, pg[GR], row[GR];  // page and first element in its head of each group
-  uint32_t live[E::kStages][GR];        // slots in use of the tiles in the ring, the oldest first
+  uint32_t live[S::kStages][GR];        // slots in use of the tiles in the ring, the oldest first
 #pragma unroll
-  for (int k = 0; k < E::kStages; ++k)
+  for (int k = 0; k < S::kStages; ++k)
 #pragma unroll
     for (int g = 0; g < GR; ++g) live[k][g] = 0;
   const int mine = warp * (16 * GR) + (RUN ? 0 : lane & 15);
@@ -638,14 +673,14 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E>::kPerSm) paged_attn_k
   uint32_t put = 0, get = 0;  // byte offsets of stages
   auto copy = [&] {
 #pragma unroll
-    for (int k = 0; k + 1 < E::kStages; ++k)
+    for (int k = 0; k + 1 < S::kStages; ++k)
 #pragma unroll
       for (int g = 0; g < GR; ++g) live[k][g] = live[k + 1][g];
     if (to_copy > 0) {
 #pragma unroll
       for (int g = 0; g < GR; ++g) {
         uint8_t* to = ring + put + g * E::kGroup;
-        uint32_t& alive = live[E::kStages - 1][g];
+        uint32_t& alive = live[S::kStages - 1][g];
         const bool good = (uint32_t)pg[g] < (uint32_t)c.num_pages;
         if (!good && ahead > 16 * g) set_err(c.err, ERR_BAD_ARG, SITE_PAGED_ATTN);
         if (RUN) {
@@ -686,7 +721,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E>::kPerSm) paged_attn_k
   if (to_copy == 0) ahead = 0;
   ask();
 #pragma unroll 1
-  for (int i = 0; i < E::kStages - 1; ++i) copy();
+  for (int i = 0; i < S::kStages - 1; ++i) copy();
   // ---- the computing side, piece by piece
   E eng;
   bool begun_inside = false;  // the piece does not start this CTA's share
@@ -694,11 +729,11 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E>::kPerSm) paged_attn_k
     const int kv = cur.kv, g0 = cur.gi * E::ROWS, rows = min(E::ROWS, p.G - g0);
     const int64_t hq0 = ((int64_t)cur.b * c.Hkv + kv) * p.G + g0;  // output row of this query-head tile
     const int first = cur.tile, last = min(cur.tiles, cur.tile + left);
-    if (cur.b >= c.B || (last <= first && cur.tiles > 0)) break;  // lengths that changed during the call
+    if (SPLIT && (cur.b >= c.B || last <= first)) break;  // lengths that changed during the call
     eng.begin(p, extra, (const T*)p.q + cur.b * p.q_bs + ((int64_t)kv * p.G + g0) * p.q_hs, rows);
     for (int tile = first; tile < last; ++tile) {
       copy();
-      cp_async_wait<E::kStages - 1>();
+      cp_async_wait<S::kStages - 1>();
       uint32_t any = 0;
 #pragma unroll
       for (int g = 0; g < GR; ++g) any |= live[0][g];
@@ -713,12 +748,13 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E>::kPerSm) paged_attn_k
     __syncthreads();
     const float* so = reinterpret_cast<const float*>(smem + put);
     const bool whole = first == 0 && last == cur.tiles;
-    if (p.split && first == 0 && threadIdx.x == 0) {  // which CTAs hold this segment: tiles from `left` on go to later ones
+    if (SPLIT && first == 0 && threadIdx.x == 0) {  // which CTAs hold this segment: tiles from `left` on go to later ones
       const int more = (cur.tiles - left + share - 1) / share;
       p.parts[(cur.b * c.Hkv + cur.kv) * ng + cur.gi] =
           make_int2((int)blockIdx.x, ((int)blockIdx.x + max(0, more)) << 1 | (int)begun_inside);
     }
     const int64_t part = 2ll * blockIdx.x + begun_inside;
+    float* sum = reinterpret_cast<float*>(smem + S::kSum);
     for (int i = threadIdx.x; i < rows * (E::DH / 4); i += blockDim.x) {
       const int g = i / (E::DH / 4), d = i % (E::DH / 4) * 4;
       float M = -INFINITY, L = 0.f;
@@ -733,7 +769,13 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E>::kPerSm) paged_attn_k
         const float4 x = *reinterpret_cast<const float4*>(so + k * (S::kWarp / 4) + g * E::DH + d);
         a.x += f * x.x; a.y += f * x.y; a.z += f * x.z; a.w += f * x.w;
       }
-      if (whole) {
+      if (!SPLIT && p.cluster > 1) {
+        *reinterpret_cast<float4*>(sum + g * E::DH + d) = a;
+        if (d == 0) {
+          fin[2 * g] = M;
+          fin[2 * g + 1] = L;
+        }
+      } else if (whole) {
         const float inv = L == 0.f ? 0.f : 1.f / L;
         if (d < c.Dh) {
           T* y = (T*)p.out + (hq0 + g) * c.Dh + d;
@@ -742,7 +784,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E>::kPerSm) paged_attn_k
         if (d == 0) {
           fin[2 * g] = Ms;
           fin[2 * g + 1] = inv;
-          if (p.split && p.mass) {
+          if (SPLIT && p.mass) {
             p.row_ml[2 * (hq0 + g)] = Ms;
             p.row_ml[2 * (hq0 + g) + 1] = inv;
           }
@@ -756,14 +798,68 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E>::kPerSm) paged_attn_k
       }
     }
     __syncthreads();
-    if (!p.split && p.mass) {  // one query-head tile per kv head: this CTA wrote all of its scores
+    const float* joint = fin;  // m, 1 / l of the whole segment
+    if (!SPLIT && p.cluster > 1) {
+      cluster_sync();
+      // thread t joins pieces of the rows; with mass, thread g the row g as well
+      const int cs = p.cluster, rank = blockIdx.x % cs;
+      auto row = [&](int g, float (&f)[8], float& inv) -> float {  // each CTA's weight over the joint l; returns m
+        float2 x[8];
+        float M = -INFINITY, L = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          if (k >= cs) break;
+          x[k] = cluster_ld2(fin + 2 * g, k);
+          M = fmaxf(M, x[k].x);
+        }
+        if (M == -INFINITY) M = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          if (k >= cs) break;
+          f[k] = exp2f(x[k].x - M);
+          L += f[k] * x[k].y;
+        }
+        inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) f[k] *= inv;
+        return M;
+      };
+      for (int i = rank * kPaWarps * 32 + threadIdx.x; i < rows * (E::DH / 4); i += cs * kPaWarps * 32) {
+        const int g = i / (E::DH / 4), d = i % (E::DH / 4) * 4;
+        float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        float inv;
+        row(g, f, inv);
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          if (k >= cs) break;
+          const float4 x = cluster_ld4(sum + g * E::DH + d, k);
+          a.x += f[k] * x.x; a.y += f[k] * x.y; a.z += f[k] * x.z; a.w += f[k] * x.w;
+        }
+        if (d < c.Dh) {
+          T* y = (T*)p.out + (hq0 + g) * c.Dh + d;
+          st<T>(y, a.x); st<T>(y + 1, a.y); st<T>(y + 2, a.z); st<T>(y + 3, a.w);
+        }
+      }
+      if (p.mass) {
+        if (threadIdx.x < rows) {
+          float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, inv;
+          ml[2 * threadIdx.x] = row(threadIdx.x, f, inv);
+          ml[2 * threadIdx.x + 1] = inv;
+        }
+        __syncthreads();
+        joint = ml;
+      }
+    }
+    if (!SPLIT && p.mass) {  // one query-head tile per kv head: this CTA wrote all the scores of its slots
       float* mass = p.mass + ((int64_t)cur.b * c.Hkv + kv) * p.mass_width;
-      for (int t = threadIdx.x; t < cur.len; t += blockDim.x) {
+      for (int t = first * TILE + threadIdx.x; t < min(last * TILE, cur.len); t += blockDim.x) {
         float a = 0.f;
-        for (int g = 0; g < rows; ++g) a += ex2_approx(p.scores[(hq0 + g) * p.score_ld + t] - fin[2 * g]) * fin[2 * g + 1];
+        for (int g = 0; g < rows; ++g) a += ex2_approx(p.scores[(hq0 + g) * p.score_ld + t] - joint[2 * g]) * joint[2 * g + 1];
         mass[t] += a;
       }
     }
+    if (!SPLIT && p.cluster > 1) cluster_sync();  // nobody leaves while its sums are read
     begun_inside = true;
     left -= last - first;
     cur.tile = last - 1;

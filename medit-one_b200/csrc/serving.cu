@@ -136,12 +136,29 @@ int launched(cudaError_t e, const char* what) {
 namespace {
 
 constexpr int kMaxTile = 256;  // slots of the largest tile
-constexpr int kWhole = 512;    // caches of at most this many slots are not split
+constexpr int kWhole = 512;    // slots that one CTA takes rather than split them
+
+// CTAs per segment, when segments are not cut from a list: up to 296 in all (two per SM), and no more than
+// one per 256 slots of the table.
+int paged_cluster(int64_t segments, int64_t slots) {
+  int n = 1;
+  while (n < 8 && segments * n * 2 <= 296 && slots > 256 * n) n *= 2;
+  return n;
+}
+
+// Whether the segments are cut from a list. A cluster per segment has one launch and no second pass, but
+// at most 8 CTAs for a long sequence, and fewer than the SMs hold for a few. Both sides, per call: 8 x 3001
+// slots, 4 heads x 64 in fp32 (8 CTAs of 384 slots) 13.4 us by clusters, 15.3 from a list; 16 x 2500, 4 kv
+// heads (4 CTAs of 640 slots) 16.6 by clusters, 15.2 from a list.
+bool paged_split(int64_t segments, int64_t slots) {
+  const int64_t n = paged_cluster(segments, slots);
+  return slots > kWhole * n;
+}
 
 size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
 // Query heads that one pass over a kv head's cache serves.
-int paged_rows(int dtype, int G) { return dtype == ONE_DTYPE_F32 ? 4 : G > 8 ? 16 : 8; }
+int paged_rows(int dtype, int G) { return dtype == ONE_DTYPE_F32 ? (G > 1 ? 4 : 1) : G > 8 ? 16 : 8; }
 
 struct PagedWs {
   size_t part_ml, part_o, row_ml, segs, scores, total;
@@ -160,25 +177,30 @@ struct PagedWs {
 
 int pad_dh(int dh) { return dh <= 32 ? 32 : dh <= 64 ? 64 : dh <= 96 ? 96 : 128; }
 
-template <typename E, bool RUN>
+template <typename E, bool RUN, bool SPLIT>
 int attend(PagedAttn& p, cudaStream_t st) {
   static std::atomic<bool> done[kMaxDevices];
-  int rc = allow_smem(paged_attn_kernel<E, RUN>, PaSmem<E>::kTotal, done);
+  int rc = allow_smem(paged_attn_kernel<E, RUN, SPLIT>, PaSmem<E, SPLIT>::kTotal, done);
   if (rc) return rc;
-  p.ranges = std::min(num_sms(), kMaxSms) * PaSmem<E>::kPerSm;
-  const dim3 grid = p.split ? dim3(p.ranges) : dim3(p.c.Hkv * p.hv_per_kv, p.c.B);
-  rc = launched(launch(paged_attn_kernel<E, RUN>, grid, dim3(kPaWarps * 32), PaSmem<E>::kTotal, st, p), "paged attention");
-  if (rc || !p.split) return rc;
+  const int64_t segments = (int64_t)p.c.B * p.c.Hkv * p.hv_per_kv, slots = (int64_t)p.c.max_pages * p.c.page_size;
+  p.ranges = std::min(num_sms(), kMaxSms) * PaSmem<E, SPLIT>::kPerSm;
+  p.cluster = SPLIT ? 1 : paged_cluster(segments, slots);
+  rc = launched(launch_cluster(p.cluster, paged_attn_kernel<E, RUN, SPLIT>, dim3((unsigned)(SPLIT ? p.ranges : segments * p.cluster)),
+                               dim3(kPaWarps * 32), PaSmem<E, SPLIT>::kTotal, st, p),
+                "paged attention");
+  if (rc || !SPLIT) return rc;
   const int64_t heads = (int64_t)p.c.B * p.c.Hkv;
-  const int mass_blocks = p.mass ? (p.c.max_pages * p.c.page_size + kJoinSlots - 1) / kJoinSlots : 0;
+  const int mass_blocks = p.mass ? (int)((slots + kJoinSlots - 1) / kJoinSlots) : 0;
   return launched(launch(paged_join_kernel<E>, dim3((unsigned)(heads * (p.G + mass_blocks))), dim3(kJoinThreads), 0, st, p,
                          mass_blocks),
                   "paged attention join");
 }
 
 template <typename E>
-int attend(PagedAttn& p, cudaStream_t st) {
-  return p.c.page_size % 16 == 0 && p.c.Dh == E::DH ? attend<E, true>(p, st) : attend<E, false>(p, st);
+int attend(PagedAttn& p, bool split, cudaStream_t st) {
+  const bool run = p.c.page_size % 16 == 0 && p.c.Dh == E::DH;
+  return split ? run ? attend<E, true, true>(p, st) : attend<E, false, true>(p, st)
+               : run ? attend<E, true, false>(p, st) : attend<E, false, false>(p, st);
 }
 
 }  // namespace
@@ -187,8 +209,9 @@ extern "C" size_t one_paged_attention_workspace_bytes(int32_t b, int32_t hq, int
                                                       int32_t max_pages, int32_t dtype, int32_t with_mass) {
   if (b < 1 || hq < 1 || hkv < 1 || dh < 1 || page_size < 1 || max_pages < 1) return 0;
   const int64_t slots = (int64_t)max_pages * page_size;
-  if (!with_mass && slots <= kWhole) return 0;
-  return PagedWs(b, hq, paged_rows(dtype, hq / hkv), pad_dh(dh), slots, with_mass != 0).total + 256;
+  const int rows = paged_rows(dtype, hq / hkv), tiles = (hq / hkv + rows - 1) / rows;
+  if (!with_mass && !paged_split((int64_t)b * hkv * tiles, slots)) return 0;
+  return PagedWs(b, hq, rows, pad_dh(dh), slots, with_mass != 0).total + 256;
 }
 
 extern "C" int one_paged_attention(const one_paged_cache* cache, const void* q, int64_t q_batch_stride,
@@ -223,30 +246,38 @@ extern "C" int one_paged_attention(const one_paged_cache* cache, const void* q, 
   p.parts = reinterpret_cast<int2*>(ws + w.segs);
   p.scores = mass ? reinterpret_cast<float*>(ws + w.scores) : nullptr;
   p.score_ld = w.score_ld;
-  p.split = slots > kWhole || (mass && p.hv_per_kv > 1);
+  const bool split = paged_split((int64_t)b * hkv * p.hv_per_kv, slots) || (mass && p.hv_per_kv > 1);
   cudaStream_t st = (cudaStream_t)stream;
   const int d = pad_dh(dh);
   if (dtype == ONE_DTYPE_F32) {
+    if (rows == 1) {
+      switch (d) {
+        case 32: return attend<PaF32<32, 1>>(p, split, st);
+        case 64: return attend<PaF32<64, 1>>(p, split, st);
+        case 96: return attend<PaF32<96, 1>>(p, split, st);
+        default: return attend<PaF32<128, 1>>(p, split, st);
+      }
+    }
     switch (d) {
-      case 32: return attend<PaF32<32>>(p, st);
-      case 64: return attend<PaF32<64>>(p, st);
-      case 96: return attend<PaF32<96>>(p, st);
-      default: return attend<PaF32<128>>(p, st);
+      case 32: return attend<PaF32<32, 4>>(p, split, st);
+      case 64: return attend<PaF32<64, 4>>(p, split, st);
+      case 96: return attend<PaF32<96, 4>>(p, split, st);
+      default: return attend<PaF32<128, 4>>(p, split, st);
     }
   }
   if (rows == 16) {
     switch (d) {
-      case 32: return attend<PaBf16<32, true>>(p, st);
-      case 64: return attend<PaBf16<64, true>>(p, st);
-      case 96: return attend<PaBf16<96, true>>(p, st);
-      default: return attend<PaBf16<128, true>>(p, st);
+      case 32: return attend<PaBf16<32, true>>(p, split, st);
+      case 64: return attend<PaBf16<64, true>>(p, split, st);
+      case 96: return attend<PaBf16<96, true>>(p, split, st);
+      default: return attend<PaBf16<128, true>>(p, split, st);
     }
   }
   switch (d) {
-    case 32: return attend<PaBf16<32, false>>(p, st);
-    case 64: return attend<PaBf16<64, false>>(p, st);
-    case 96: return attend<PaBf16<96, false>>(p, st);
-    default: return attend<PaBf16<128, false>>(p, st);
+    case 32: return attend<PaBf16<32, false>>(p, split, st);
+    case 64: return attend<PaBf16<64, false>>(p, split, st);
+    case 96: return attend<PaBf16<96, false>>(p, split, st);
+    default: return attend<PaBf16<128, false>>(p, split, st);
   }
 }
 

@@ -50,6 +50,8 @@ SHAPES = [  # hkv, group, dh, page, lengths
     (2, 1, 64, 16, LENS), (1, 3, 64, 1, [0, 1, 5, 33]), (2, 8, 32, 7, LENS), (1, 12, 128, 48, LENS), (3, 2, 40, 16, [77, 3, 0]),
     (1, 20, 96, 64, [500, 64]), (4, 16, 64, 32, [129, 2]), (1, 1, 8, 5, [40, 0, 1]), (2, 7, 128, 128, [4097, 127]),
     (12, 1, 64, 16, [2049]), (1, 8, 64, 16, [20000, 3]), (1, 1, 16, 3, [0, 0]), (5, 4, 112, 24, [1500, 31, 600]),
+    (16, 1, 64, 16, [(i * 97) % 701 for i in range(30)]), (10, 2, 32, 32, [(i * 331) % 1300 for i in range(50)]),
+    (1, 4, 64, 16, [300]), (2, 9, 128, 16, [4096, 1]), (1, 2, 96, 16, [8192 * 3, 5, 0]),
 ]
 
 
@@ -81,11 +83,12 @@ def test_attention_repeats_bit_for_bit_and_takes_scales(dt):
 
 
 @pytest.mark.parametrize("dt", [BF, F32], ids=["bf16", "fp32"])
-def test_attention_large_scores(dt):
+@pytest.mark.parametrize("n", [2500, 9000])
+def test_attention_large_scores(dt, n):
     """Scores of thousands, of both signs: one slot takes the whole weight; the running maximum rises
     within and across the parts of a split sequence."""
     gen = torch.Generator().manual_seed(4)
-    k, v, table, ln = P.make_cache([2500], 1, 64, 16, dt, gen)
+    k, v, table, ln = P.make_cache([n], 1, 64, 16, dt, gen)
     q = (300 * torch.randn(1, 4, 1, 64, generator=gen)).to(dt)
     d = cuda(q, k, v, table, ln)
     got = ops().turbo_paged_attention(*d)
