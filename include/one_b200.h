@@ -287,8 +287,9 @@ int one_paged_append(const one_paged_cache* cache, const one_paged_tokens* token
  * fp32 softmax over the slots below lengths[i]. q [b, hq] rows of dh (element strides given), hq a
  * multiple of hkv: query head j reads kv head j / (hq / hkv). out [b, hq, dh]. A sequence without
  * slots, or whose scores are all -inf, gives zeros. The cache's mass, if kept, grows by the softmax
- * weights summed over the query heads of each kv head. The workspace may be NULL where its size
- * is 0. */
+ * weights summed over the query heads of each kv head. out must not overlap q. Infinities or NaN in
+ * an attended slot give non-finite results; those in other slots are never seen. The workspace may be
+ * NULL where its size is 0. */
 size_t one_paged_attention_workspace_bytes(int32_t b, int32_t hq, int32_t hkv, int32_t dh, int32_t page_size,
                                            int32_t max_pages, int32_t dtype, int32_t with_mass);
 int one_paged_attention(const one_paged_cache* cache, const void* q, int64_t q_batch_stride, int64_t q_head_stride,

@@ -359,10 +359,13 @@ extern "C" int one_paged_evict(const one_paged_cache* cache, const int32_t* dst_
 
 extern "C" int one_process_logits(const one_logits_rules* rules, const void* logits, int64_t ld, int32_t batch,
                                   int32_t vocab, int32_t dtype, float* out, int64_t out_ld, int32_t* best, void* stream) {
-  if (!rules || !logits || !out || (!rules->history && rules->history_len))
+  if (!rules || !logits || !out || (!rules->history && rules->history_len) || rules->history_len < 0)
     return fail(ONE_ERR_INVALID, "process logits: null argument");
   const one_logits_rules& x = *rules;
-  const int hist_len = x.history_len;
+  // a history that no penalty uses is not read
+  const bool counted = x.repetition || x.presence || x.frequency || x.repetition_all != 1.0f || x.presence_all != 0.0f ||
+                       x.frequency_all != 0.0f;
+  const int hist_len = counted ? x.history_len : 0;
   if (batch < 1 || vocab < 1 || ld < vocab || out_ld < vocab || hist_len < 0 || (hist_len && x.history_ld < hist_len))
     return fail(ONE_ERR_INVALID, "process logits: bad sizes");
   if (vocab > 0x3fffffff) return fail(ONE_ERR_UNSUPPORTED, "process logits: at most 2^30 - 1 tokens");

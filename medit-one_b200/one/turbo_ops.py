@@ -298,7 +298,8 @@ def turbo_paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch
     """Attention of one new token per sequence, q [B, Hq, 1, Dh], over the cached slots below
     lengths[b]: softmax(q k^T * scale) v with an fp32 softmax, scale 1/sqrt(Dh) by default. Hq is a
     multiple of Hkv: query head j reads kv head j // (Hq // Hkv). A sequence without slots gives
-    zeros. mass grows by the softmax weights, summed over each kv head's query heads."""
+    zeros. mass grows by the softmax weights, summed over each kv head's query heads; that takes a
+    workspace of 4 bytes per query head and slot of the table. `out` must not overlap q."""
     dt = q.dtype
     dev, cache, (b, hkv, ps, dh, mp) = _paged(k_pages, v_pages, block_table, lengths, mass, dt)
     shape = q.shape
@@ -308,6 +309,8 @@ def turbo_paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch
         raise ValueError("all tensors must be on one device")
     if out is not None and (out.shape != shape or out.dtype is not dt or not out.is_contiguous()):
         raise ValueError(f"out must be contiguous {tuple(shape)} in {dt}")
+    if out is q:
+        raise ValueError("out must not be q")
     _cuda(dev, q)
     hq = shape[1]
     q = _rows_last(q)

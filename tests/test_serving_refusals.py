@@ -57,6 +57,7 @@ def test_attention_refusals():
     bad(f, q, k, v, t, n, mass=torch.zeros(2, 2, 48, dtype=torch.float64))
     bad(f, q, k, v, t, n, mass=torch.zeros(2, 2, 96)[..., ::2])
     bad(f, q, k, v, t, n, out=torch.zeros(2, 4, 1, 64))
+    bad(f, q, k, v, t, n, out=q)
 
 
 def test_append_refusals():
@@ -187,14 +188,14 @@ BIG_CACHE = [dict(dh=60), dict(dh=136, ks=1 << 20, vs=1 << 20), dict(B=70000), d
 def test_c_attention_refuses_before_launching():
     def call(q, qb, qh, hq, out, ws, wb, **cache):
         return C.LIB.one_paged_attention(cache_of(cache), q, qb, qh, hq, 0.1, out, ws, wb, 0)
-    base = dict(CACHE, mp=64, ts=64, q=A, qb=256, qh=64, hq=4, out=A, ws=A, wb=1 << 30)
-    refused(call, base, [k for k in BAD_CACHE if k != dict(ts=2)] + [dict(ts=63), dict(q=0), dict(out=0), dict(ws=0), dict(wb=64),
+    base = dict(CACHE, mp=4096, ts=4096, q=A, qb=256, qh=64, hq=4, out=A, ws=A, wb=1 << 30)
+    refused(call, base, [k for k in BAD_CACHE if k != dict(ts=2)] + [dict(ts=4095), dict(q=0), dict(out=0), dict(ws=0), dict(wb=64),
                                                                     dict(hq=3), dict(hq=0)], BIG_CACHE)
     assert C.LIB.one_paged_attention(None, A, 1, 1, 4, 0.1, A, A, 1 << 30, 0) == C.ONE_ERR_INVALID
-    # short caches need no workspace, others do
+    # small caches need no workspace, others do
     assert C.LIB.one_paged_attention_workspace_bytes(2, 4, 2, 64, 16, 3, 0, 0) == 0
     assert C.LIB.one_paged_attention_workspace_bytes(2, 4, 2, 64, 16, 3, 0, 1) > 0
-    assert C.LIB.one_paged_attention_workspace_bytes(2, 4, 2, 64, 16, 100, 0, 0) > 0
+    assert C.LIB.one_paged_attention_workspace_bytes(2, 4, 2, 64, 16, 4096, 0, 0) > 0
 
 
 def test_c_append_refuses_before_launching():
