@@ -359,13 +359,10 @@ extern "C" int one_paged_evict(const one_paged_cache* cache, const int32_t* dst_
 
 extern "C" int one_process_logits(const one_logits_rules* rules, const void* logits, int64_t ld, int32_t batch,
                                   int32_t vocab, int32_t dtype, float* out, int64_t out_ld, int32_t* best, void* stream) {
-  if (!rules || !logits || !out || (!rules->history && rules->history_len) || rules->history_len < 0)
+  if (!rules || !logits || !out || (!rules->history && rules->history_len))
     return fail(ONE_ERR_INVALID, "process logits: null argument");
   const one_logits_rules& x = *rules;
-  // a history that no penalty uses is not read
-  const bool counted = x.repetition || x.presence || x.frequency || x.repetition_all != 1.0f || x.presence_all != 0.0f ||
-                       x.frequency_all != 0.0f;
-  const int hist_len = counted ? x.history_len : 0;
+  int hist_len = x.history_len;
   if (batch < 1 || vocab < 1 || ld < vocab || out_ld < vocab || hist_len < 0 || (hist_len && x.history_ld < hist_len))
     return fail(ONE_ERR_INVALID, "process logits: bad sizes");
   if (vocab > 0x3fffffff) return fail(ONE_ERR_UNSUPPORTED, "process logits: at most 2^30 - 1 tokens");
@@ -375,6 +372,9 @@ extern "C" int one_process_logits(const one_logits_rules* rules, const void* log
   if (!(x.repetition_all > 0.0f)) return fail(ONE_ERR_INVALID, "process logits: the repetition penalty must be positive");
   if ((x.bias && x.bias_ld && x.bias_ld < vocab) || (x.token_mask && x.mask_ld && x.mask_ld < (vocab + 31) / 32))
     return fail(ONE_ERR_INVALID, "process logits: bias or mask rows overlap");
+  // a history that no penalty uses is not read
+  if (!x.repetition && !x.presence && !x.frequency && x.repetition_all == 1.0f && x.presence_all == 0.0f && x.frequency_all == 0.0f)
+    hist_len = 0;
   LogitsParams p = {};
   p.logits = logits; p.ld = ld; p.B = batch; p.V = vocab; p.history = x.history; p.hist_ld = x.history_ld; p.T = hist_len;
   p.starts = x.output_starts; p.rep = x.repetition; p.pres = x.presence; p.freq = x.frequency;
