@@ -35,7 +35,7 @@ struct LogitsParams {
 };
 
 constexpr int kLogitsThreads = 512;
-constexpr int kLogitsCounts = 16384;  // counts held at a time (64 KB)
+constexpr int kLogitsBytes = 65536;   // counts held at a time
 constexpr int kLogitsAhead = 2;       // vectors per thread, and
 constexpr int kLogitsIds = 4;         // history entries per thread, that are asked for at once at the start
 
@@ -53,9 +53,36 @@ template <> struct LogitsVec<float> {
   }
 };
 
-// A cluster of CTAs per row, each with a slice of the vocabulary. Per up to kLogitsCounts tokens of
-// it: the history's counts in shared memory (bit 31: the token occurs before the output; integer
-// atomics, so the order does not matter), then one pass over the logits. Bound by HBM (one read, one
+// How often the tokens of a slice stand in the history, as words of shared memory: 16 bits per token, or
+// 32 for histories whose counts might not fit; the top bit says that the token occurs before the output.
+template <bool WIDE> struct LogitsCounts;
+template <> struct LogitsCounts<false> {
+  static constexpr int N = kLogitsBytes / 2, kTop = 0x8000;
+  ONE_DEVINL static void add(uint32_t* w, int i, bool output) {
+    const int s = 16 * (i & 1);
+    if (output) atomicAdd(w + (i >> 1), 1u << s);
+    else atomicOr(w + (i >> 1), 0x8000u << s);
+  }
+  ONE_DEVINL static uint32_t get(const uint32_t* w, int i) { return w[i >> 1] >> 16 * (i & 1) & 0xffffu; }
+  ONE_DEVINL static uint4 get4(const uint32_t* w, int i) {  // i a multiple of 4
+    const uint2 u = *reinterpret_cast<const uint2*>(w + (i >> 1));
+    return make_uint4(u.x & 0xffffu, u.x >> 16, u.y & 0xffffu, u.y >> 16);
+  }
+};
+template <> struct LogitsCounts<true> {
+  static constexpr int N = kLogitsBytes / 4;
+  static constexpr uint32_t kTop = 0x80000000u;
+  ONE_DEVINL static void add(uint32_t* w, int i, bool output) {
+    if (output) atomicAdd(w + i, 1u);
+    else atomicOr(w + i, 0x80000000u);
+  }
+  ONE_DEVINL static uint32_t get(const uint32_t* w, int i) { return w[i]; }
+  ONE_DEVINL static uint4 get4(const uint32_t* w, int i) { return *reinterpret_cast<const uint4*>(w + i); }
+};
+
+// A cluster of CTAs per row, each with a slice of the vocabulary. Per up to Counts::N tokens of it: the
+// history's counts in shared memory (integer atomics, so the order does not matter), then one pass over
+// the logits. Bound by HBM (one read, one
 // write) when there are many rows, by the chain history -> counts -> scores for a single one, so the
 // first history entries and logits are asked for together, before anything waits.
 //
@@ -64,9 +91,11 @@ template <> struct LogitsVec<float> {
 // the caller's strides differ (then: token by token).
 //
 // Each CTA's best token goes into the shared memory of the cluster's first CTA, which alone waits.
-template <typename T, typename I>
+template <typename T, typename I, bool WIDE>
 __global__ void __launch_bounds__(kLogitsThreads, 2) logits_kernel(const __grid_constant__ LogitsParams p, int slice, int ctas) {
   using V4 = LogitsVec<T>;
+  using Counts = LogitsCounts<WIDE>;
+  constexpr int kLogitsCounts = Counts::N, kPer16 = WIDE ? 4 : 8;  // tokens; in 16 bytes
   extern __shared__ __align__(16) uint32_t cnt[];
   __shared__ float bv[kLogitsThreads / 32];
   __shared__ int bi[kLogitsThreads / 32];
@@ -104,7 +133,7 @@ __global__ void __launch_bounds__(kLogitsThreads, 2) logits_kernel(const __grid_
   int at = 0x7fffffff;
   auto penalise = [&](float v, uint32_t u) -> float {
     v = v > 0.f ? v / r : v * r;
-    const uint32_t n = u & 0x7fffffffu;
+    const uint32_t n = u & (Counts::kTop - 1);
     return n ? v - (f * (float)n + pr) : v;
   };
   auto one_token = [&](int v, uint32_t u) {
@@ -122,15 +151,11 @@ __global__ void __launch_bounds__(kLogitsThreads, 2) logits_kernel(const __grid_
     const int n = max(0, min(kLogitsCounts, end - v0)), lo = v0 == 0 + head ? -head : 0;  // counts of [v0 + lo, v0 + n)
     if (p.T) {
       if (v0 != beg) __syncthreads();
-      for (int i = tid * 4; i < n + 4; i += kLogitsThreads * 4) *reinterpret_cast<uint4*>(cnt + i) = make_uint4(0, 0, 0, 0);
+      for (int i = tid; i * kPer16 < n + 4; i += kLogitsThreads) reinterpret_cast<uint4*>(cnt)[i] = make_uint4(0, 0, 0, 0);
       __syncthreads();
       auto count = [&](I x, int t) {
         const uint64_t id = (uint64_t)(int64_t)x - (uint64_t)(int64_t)(v0 + lo);
-        if (id < (uint64_t)(n - lo)) {
-          uint32_t* c = cnt + 4 + lo + (int)id;
-          if (t >= start) atomicAdd(c, 1u);
-          else atomicOr(c, 0x80000000u);
-        }
+        if (id < (uint64_t)(n - lo)) Counts::add(cnt, 4 + lo + (int)id, t >= start);
       };
 #pragma unroll
       for (int k = 0; k < kLogitsIds; ++k) count(ids[k], k * kLogitsThreads + tid);
@@ -138,7 +163,7 @@ __global__ void __launch_bounds__(kLogitsThreads, 2) logits_kernel(const __grid_
       for (int t = kLogitsIds * kLogitsThreads + tid; t < p.T; t += kLogitsThreads) count(__ldg(hist + t), t);
       __syncthreads();
     }
-    if (lo < 0 && tid < -lo) one_token(tid, p.T ? cnt[4 + lo + tid] : 0u);
+    if (lo < 0 && tid < -lo) one_token(tid, p.T ? Counts::get(cnt, 4 + lo + tid) : 0u);
     if (vec) {
       constexpr int kStep = kLogitsAhead * kLogitsThreads * 4;
       for (int i0 = 0; i0 < n; i0 += kStep) {
@@ -151,13 +176,13 @@ __global__ void __launch_bounds__(kLogitsThreads, 2) logits_kernel(const __grid_
         for (int k = 0; k < kLogitsAhead; ++k) {
           const int i = i0 + (k * kLogitsThreads + tid) * 4, v = v0 + i;
           if (i + 4 > n) {
-            for (int e = i; e < n; ++e) one_token(v0 + e, p.T ? cnt[4 + e] : 0u);
+            for (int e = i; e < n; ++e) one_token(v0 + e, p.T ? Counts::get(cnt, 4 + e) : 0u);
             continue;
           }
           float y[4];
           V4::open(now[k], y);
           if (p.T) {
-            const uint4 u = *reinterpret_cast<const uint4*>(cnt + 4 + i);
+            const uint4 u = Counts::get4(cnt, 4 + i);
             if (u.x | u.y | u.z | u.w) {
               if (u.x) y[0] = penalise(y[0], u.x);
               if (u.y) y[1] = penalise(y[1], u.y);
@@ -189,7 +214,7 @@ __global__ void __launch_bounds__(kLogitsThreads, 2) logits_kernel(const __grid_
       }
     } else {
 #pragma unroll 4
-      for (int i = tid; i < n; i += kLogitsThreads) one_token(v0 + i, p.T ? cnt[4 + i] : 0u);
+      for (int i = tid; i < n; i += kLogitsThreads) one_token(v0 + i, p.T ? Counts::get(cnt, 4 + i) : 0u);
     }
   }
   if (!p.best) {

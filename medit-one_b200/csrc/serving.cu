@@ -389,16 +389,20 @@ extern "C" int one_process_logits(const one_logits_rules* rules, const void* log
   while (ctas < 8 && (int64_t)batch * ctas < num_sms() && vocab > ctas * kLogitsThreads * 8) ctas *= 2;
   const int slice = ((vocab + ctas - 1) / ctas + 31) / 32 * 32;
   if ((int64_t)batch * ctas > 0x7fffffff) return fail(ONE_ERR_UNSUPPORTED, "process logits: too many rows");
-  const size_t smem = hist_len ? (size_t)std::min(slice, kLogitsCounts) * 4 + 32 : 0;
-  static std::atomic<bool> done[4][kMaxDevices];
-  auto run = [&](auto t, auto i, int at) -> int {
-    auto* kernel = logits_kernel<decltype(t), decltype(i)>;
-    const int rc = allow_smem(kernel, kLogitsCounts * 4 + 32, done[at]);
+  const bool wide = hist_len > 32767;  // a count may not fit 15 bits
+  const size_t smem = hist_len ? std::min<size_t>((size_t)slice * (wide ? 4 : 2), kLogitsBytes) + 32 : 0;
+  static std::atomic<bool> done[8][kMaxDevices];
+  auto run = [&](auto t, auto i, auto w) -> int {
+    using T = decltype(t);
+    using I = decltype(i);
+    auto* kernel = logits_kernel<T, I, decltype(w)::value != 0>;
+    const int rc = allow_smem(kernel, kLogitsBytes + 32, done[(sizeof(T) == 4) * 4 + (sizeof(I) == 8) * 2 + decltype(w)::value]);
     if (rc) return rc;
     return launched(launch_cluster(ctas, kernel, dim3((unsigned)batch * ctas), dim3(kLogitsThreads), smem, st, p, slice, ctas),
                     "process logits");
   };
-  const bool wide = x.history_bytes == 8;
-  if (dtype == ONE_DTYPE_BF16) return wide ? run(__nv_bfloat16(), int64_t(0), 0) : run(__nv_bfloat16(), int32_t(0), 1);
-  return wide ? run(float(0), int64_t(0), 2) : run(float(0), int32_t(0), 3);
+  auto by_counts = [&](auto t, auto i) { return wide ? run(t, i, Int<1>()) : run(t, i, Int<0>()); };
+  if (dtype == ONE_DTYPE_BF16)
+    return x.history_bytes == 8 ? by_counts(__nv_bfloat16(), int64_t(0)) : by_counts(__nv_bfloat16(), int32_t(0));
+  return x.history_bytes == 8 ? by_counts(float(0), int64_t(0)) : by_counts(float(0), int32_t(0));
 }

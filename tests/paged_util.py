@@ -1,4 +1,5 @@
 """A paged key-value cache on the CPU and the serving operators' formulas in 64 bits."""
+import collections
 import math
 
 import torch
@@ -94,9 +95,8 @@ def logits(x, history, starts, rep, pres, freq, bias, allowed):
         seen = sorted({i for i in ids if 0 <= i < V})
         for t in seen:
             z[b, t] = z[b, t] / float(rep[b]) if z[b, t] > 0 else z[b, t] * float(rep[b])
-        late = [i for i in ids[max(start, 0):] if 0 <= i < V]
-        for t in set(late):
-            z[b, t] -= float(freq[b]) * late.count(t) + float(pres[b])
+        for t, c in collections.Counter(i for i in ids[max(start, 0):] if 0 <= i < V).items():
+            z[b, t] -= float(freq[b]) * c + float(pres[b])
     if bias is not None:
         z += bias.double()
     if allowed is not None:

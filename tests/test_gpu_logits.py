@@ -31,7 +31,7 @@ def check_best(best, got):
 
 
 CASES = [(1, 1, 0), (3, 33, 5), (2, 1000, 1), (4, 32000, 300), (1, 50257, 5000), (5, 8192, 64), (2, 8193, 17),
-         (1, 160001, 40), (300, 70, 9)]
+         (1, 160001, 40), (300, 70, 9), (2, 40000, 32767), (1, 40000, 33000)]
 
 
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
@@ -88,6 +88,20 @@ def test_each_part_alone_and_nothing():
     ties[1, 0] = -0.0
     _, best = process_logits(ties.cuda(), return_argmax=True)
     assert best.tolist() == [12345, 0]
+
+
+def test_counts_past_15_and_16_bits():
+    from one.engine import process_logits
+    for n in (32767, 32768, 70000):
+        hist = torch.full((1, n), 5, dtype=torch.int32)
+        hist[0, 0] = 4  # before the output, beside the token that fills its count
+        x = torch.zeros(1, 64)
+        starts = torch.tensor([1], dtype=torch.int32)
+        out = process_logits(x.cuda(), hist.cuda(), starts.cuda(), frequency_penalty=1.0, presence_penalty=0.5,
+                             repetition_penalty=2.0).cpu()
+        want = torch.zeros(64)
+        want[5] = -(n - 1) - 0.5
+        assert torch.equal(out[0], want)
 
 
 def test_in_place_strided_rows_and_graph():
