@@ -393,8 +393,8 @@ struct PaBf16 {
     }
   }
 
-  // This warp's (m, l) [ROWS][2] and o [ROWS][DH] into shared memory.
-  ONE_DEVINL void leave(float* ml, float* so) {
+  // This warp's (m, l) [ROWS][2] and o [rows][DH] into shared memory.
+  ONE_DEVINL void leave(float* ml, float* so, int rows) {
     const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
 #pragma unroll
     for (int w = 0; w < (WIDE ? 2 : 1); ++w) {
@@ -405,6 +405,7 @@ struct PaBf16 {
         ml[2 * (r + 8 * w)] = m[w];
         ml[2 * (r + 8 * w) + 1] = t;
       }
+      if (r + 8 * w >= rows) continue;
 #pragma unroll
       for (int i = 0; i < NT; ++i)
 #pragma unroll
@@ -548,7 +549,7 @@ struct PaF32 {
     __syncwarp();
   }
 
-  ONE_DEVINL void leave(float* ml, float* so) {
+  ONE_DEVINL void leave(float* ml, float* so, int rows) {
     const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
     float t = l;
 #pragma unroll
@@ -560,7 +561,8 @@ struct PaF32 {
 #pragma unroll
     for (int g = 0; g < ROWS; ++g)
 #pragma unroll
-      for (int i = 0; i < VC; ++i) so[g * DH + lane + 32 * i] = o[g][i];
+      for (int i = 0; i < VC; ++i)
+        if (g < rows) so[g * DH + lane + 32 * i] = o[g][i];
   }
 };
 
@@ -592,11 +594,13 @@ struct PaSmem {
   static constexpr int kStage = E::kGroup * E::kGroups;                  // bytes per warp
   static constexpr int kStages = SPLIT ? E::kStages : E::kStagesFew;
   static constexpr int kWarp = kStage * kStages;
-  static constexpr int kML = kPaWarps * kWarp;                           // [warps][ROWS][2]
-  static constexpr int kFin = kML + kPaWarps * E::ROWS * 8;              // [ROWS][2]: m, 1 / l
+  static constexpr int kML = kPaWarps * kWarp;                           // [2][warps][ROWS][2]
+  static constexpr int kFin = kML + 2 * kPaWarps * E::ROWS * 8;          // [ROWS][2]: m, 1 / l
   static constexpr int kExtra = kFin + (E::ROWS * 8 + 15) / 16 * 16;
-  static constexpr int kSum = kExtra + kPaWarps * E::kExtra;             // [ROWS][DH]: this CTA's sums, for its cluster
-  static constexpr int kTotal = kSum + E::ROWS * E::DH * 4;
+  static constexpr int kSum = kExtra + kPaWarps * E::kExtra;
+  // of a cluster: this CTA's sums [ROWS][DH]; of a list: the warps' sums [1 or 2][warps][rows][DH] where they fit
+  static constexpr int kApart = 2 * kPaWarps * E::ROWS * E::DH * 4 < 9216 ? 2 * kPaWarps * E::ROWS * E::DH * 4 : 9216;
+  static constexpr int kTotal = kSum + (SPLIT ? kApart : E::ROWS * E::DH * 4);
   static constexpr int kPerSm = kSmPerSm / (kTotal + 1024) < 3 ? kSmPerSm / (kTotal + 1024) : 3;
   // a warp's sums fit the stage that it consumed last
   static_assert(kStage >= E::ROWS * E::DH * 4, "stage");
@@ -613,7 +617,6 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, SPLIT>::kPerSm) paged
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int TILE = E::TILE, GR = E::kGroups;
   uint8_t* ring = smem + warp * S::kWarp;
-  float* ml = reinterpret_cast<float*>(smem + S::kML);
   float* fin = reinterpret_cast<float*>(smem + S::kFin);
   uint8_t* extra = smem + S::kExtra + warp * E::kExtra;
   const PagedCache& c = p.c;
@@ -722,9 +725,17 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, SPLIT>::kPerSm) paged
   ask();
 #pragma unroll 1
   for (int i = 0; i < S::kStages - 1; ++i) copy();
-  // ---- the computing side, piece by piece
+  // ---- the computing side, piece by piece. At a piece's end the warps' sums go through shared memory. In
+  //      a list, where there is room for a piece's sums, the copies go on meanwhile, and where there is room
+  //      for two pieces' one barrier per piece is enough; otherwise the sums go where each warp consumed
+  //      last, the stage filled next. (64 ragged sequences of up to 4096 slots: 78.6 us with the copies
+  //      held up at each end, 74.9 as here; up to 1024: 36.8, 30.8.)
   E eng;
-  bool begun_inside = false;  // the piece does not start this CTA's share
+  bool begun_inside = false, copied = false;  // the piece does not start this CTA's share; its first tile is on its way
+  const int most = min(E::ROWS, p.G);
+  const bool apart = SPLIT && kPaWarps * most * E::DH * 4 <= S::kApart;
+  const bool twice = SPLIT && 2 * kPaWarps * most * E::DH * 4 <= S::kApart;
+  int parity = 0;
   do {
     const int kv = cur.kv, g0 = cur.gi * E::ROWS, rows = min(E::ROWS, p.G - g0);
     const int64_t hq0 = ((int64_t)cur.b * c.Hkv + kv) * p.G + g0;  // output row of this query-head tile
@@ -732,7 +743,8 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, SPLIT>::kPerSm) paged
     if (SPLIT && (cur.b >= c.B || last <= first)) break;  // lengths that changed during the call
     eng.begin(p, extra, (const T*)p.q + cur.b * p.q_bs + ((int64_t)kv * p.G + g0) * p.q_hs, rows);
     for (int tile = first; tile < last; ++tile) {
-      copy();
+      if (!copied) copy();
+      copied = false;
       cp_async_wait<S::kStages - 1>();
       uint32_t any = 0;
 #pragma unroll
@@ -742,11 +754,17 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, SPLIT>::kPerSm) paged
         eng.consume(p, ring + get, live[0], p.scores ? p.scores + hq0 * p.score_ld + tile * TILE + warp * (16 * GR) : nullptr, rows);
       __syncwarp();
       get = get + S::kStage == S::kWarp ? 0 : get + S::kStage;
+      if (apart && tile + 1 == last) {
+        copy();
+        copied = true;
+      }
     }
-    // the warps' sums go where each of them consumed last: the stage that is filled next
-    eng.leave(ml + warp * E::ROWS * 2, reinterpret_cast<float*>(ring + put));
+    float* so = reinterpret_cast<float*>(smem + (apart ? S::kSum : put));
+    const int so_warp = apart ? most * E::DH : S::kWarp / 4;
+    if (apart) so += parity * kPaWarps * so_warp;
+    float* ml = reinterpret_cast<float*>(smem + S::kML) + parity * kPaWarps * E::ROWS * 2;
+    eng.leave(ml + warp * E::ROWS * 2, so + warp * so_warp, rows);
     __syncthreads();
-    const float* so = reinterpret_cast<const float*>(smem + put);
     const bool whole = first == 0 && last == cur.tiles;
     if (SPLIT && first == 0 && threadIdx.x == 0) {  // which CTAs hold this segment: tiles from `left` on go to later ones
       const int more = (cur.tiles - left + share - 1) / share;
@@ -766,7 +784,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, SPLIT>::kPerSm) paged
       for (int k = 0; k < kPaWarps; ++k) {
         const float f = exp2f(ml[(k * E::ROWS + g) * 2] - Ms);
         L += f * ml[(k * E::ROWS + g) * 2 + 1];
-        const float4 x = *reinterpret_cast<const float4*>(so + k * (S::kWarp / 4) + g * E::DH + d);
+        const float4 x = *reinterpret_cast<const float4*>(so + k * so_warp + g * E::DH + d);
         a.x += f * x.x; a.y += f * x.y; a.z += f * x.z; a.w += f * x.w;
       }
       if (!SPLIT && p.cluster > 1) {
@@ -781,13 +799,10 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, SPLIT>::kPerSm) paged
           T* y = (T*)p.out + (hq0 + g) * c.Dh + d;
           st<T>(y, a.x * inv); st<T>(y + 1, a.y * inv); st<T>(y + 2, a.z * inv); st<T>(y + 3, a.w * inv);
         }
-        if (d == 0) {
-          fin[2 * g] = Ms;
-          fin[2 * g + 1] = inv;
-          if (SPLIT && p.mass) {
-            p.row_ml[2 * (hq0 + g)] = Ms;
-            p.row_ml[2 * (hq0 + g) + 1] = inv;
-          }
+        if (d == 0 && p.mass) {
+          float* x = SPLIT ? p.row_ml + 2 * (hq0 + g) : fin + 2 * g;
+          x[0] = Ms;
+          x[1] = inv;
         }
       } else {
         *reinterpret_cast<float4*>(p.part_o + (part * E::ROWS + g) * E::DH + d) = a;
@@ -797,7 +812,8 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, SPLIT>::kPerSm) paged
         }
       }
     }
-    __syncthreads();
+    if (twice) parity ^= 1;
+    else __syncthreads();
     const float* joint = fin;  // m, 1 / l of the whole segment
     if (!SPLIT && p.cluster > 1) {
       cluster_sync();
