@@ -108,22 +108,24 @@ ONE_DEVINL float2 mul2(float2 a, float2 b) {
 //
 // One thread per token, group of kAppendRows heads of its keys, queries or values, and 16-byte piece:
 // consecutive lanes read and write whole rows, the group's loads are in flight together and share cos
-// and sin. The piece half a row away, which the rotation needs, comes from its lane. For aligned rows
-// of a power of two of pieces; paged_append_any_kernel takes the rest. Sequence blockIdx.y.
+// and sin. The piece half a row away, which the rotation needs, comes from its lane (PAIR false: rows of
+// a power of two of pieces), or the thread has both (PAIR: halves of whole pieces).
+// paged_append_any_kernel takes the rest. Sequence blockIdx.y.
 //
-// 8 prompts of up to 4096 tokens, 12 heads x 64: 68 us with one row per thread and its two halves in one
-// lane, 54 as here, 51 with five CTAs per SM; without rotation it runs at the rate of a plain copy.
+// 8 prompts of up to 4096 tokens, 12 heads x 64: 68 us with one row per thread, 72 with pairs, 54 as here,
+// 51 with five CTAs per SM; without rotation it runs at the rate of a plain copy. 170 x 4 tokens of 367
+// heads x 80: 100 us one element at a time, 35 by halves.
 constexpr int kAppendRows = 4;
 
-template <typename T>
-__global__ void __launch_bounds__(256, 5) paged_append_kernel(const __grid_constant__ PagedAppendParams p) {
+template <typename T, bool PAIR>
+__global__ void __launch_bounds__(256, PAIR ? 3 : 5) paged_append_kernel(const __grid_constant__ PagedAppendParams p) {
   using P = Piece<T>;
   pdl_wait();
   const PagedCache& c = p.c;
-  const int pieces = c.Dh / P::N, hq = p.q ? p.Hq : 0, b = blockIdx.y;
+  const int pieces = c.Dh / P::N, units = PAIR ? pieces / 2 : pieces, half = PAIR ? c.Dh / 2 : 0, hq = p.q ? p.Hq : 0, b = blockIdx.y;
   const int kvg = (c.Hkv + kAppendRows - 1) / kAppendRows, qg = (hq + kAppendRows - 1) / kAppendRows, groups = 2 * kvg + qg;
-  const uint32_t i = blockIdx.x * blockDim.x + threadIdx.x, item = i / pieces;
-  const int piece = (int)(i - item * pieces), e = piece * P::N, t = (int)(item / groups);
+  const uint32_t i = blockIdx.x * blockDim.x + threadIdx.x, item = i / units;
+  const int piece = (int)(i - item * units), e = piece * P::N, t = (int)(item / groups);
   int g = (int)(item - (uint32_t)t * groups);
   if (t >= p.N) return;  // whole rows of lanes
   const T* from;
@@ -146,10 +148,13 @@ __global__ void __launch_bounds__(256, 5) paged_append_kernel(const __grid_const
   }
   const int r0 = g * kAppendRows, rows = min(kAppendRows, heads - r0);
   from += r0 * step + e;
-  uint4 x[kAppendRows];
+  uint4 x[kAppendRows], o[PAIR ? kAppendRows : 1];  // the other piece of a pair
 #pragma unroll
   for (int k = 0; k < kAppendRows; ++k)
-    if (k < rows) x[k] = *reinterpret_cast<const uint4*>(from + k * step);
+    if (k < rows) {
+      x[k] = *reinterpret_cast<const uint4*>(from + k * step);
+      if (PAIR) o[PAIR ? k : 0] = *reinterpret_cast<const uint4*>(from + k * step + half);
+    }
   T* y;
   int64_t ystep;
   if (kind == 1) {
@@ -162,38 +167,54 @@ __global__ void __launch_bounds__(256, 5) paged_append_kernel(const __grid_const
     y = (kind ? (T*)c.v + page * c.v_stride : (T*)c.k + page * c.k_stride) + (r0 * c.page_size + row) * c.Dh + e;
     ystep = c.page_size * c.Dh;
     if (kind == 0 && p.mass)
-      for (int k = piece; k < rows; k += pieces) p.mass[((int64_t)b * c.Hkv + r0 + k) * p.mass_width + slot] = 0.f;
+      for (int k = piece; k < rows; k += units) p.mass[((int64_t)b * c.Hkv + r0 + k) * p.mass_width + slot] = 0.f;
   }
   if (kind < 2 && p.cosv) {
     const int64_t at = b * p.cos_bs + (int64_t)t * c.Dh + e;
-    float2 cs[P::N / 2], sn[P::N / 2];
+    float2 cs[P::N / 2], sn[P::N / 2], cs2[PAIR ? P::N / 2 : 1], sn2[PAIR ? P::N / 2 : 1];
     P::open(__ldg(reinterpret_cast<const uint4*>((const T*)p.cosv + at)), cs);
     P::open(__ldg(reinterpret_cast<const uint4*>((const T*)p.sinv + at)), sn);
-    if (2 * piece < pieces) {
+    if constexpr (PAIR) {
+      P::open(__ldg(reinterpret_cast<const uint4*>((const T*)p.cosv + at + half)), cs2);
+      P::open(__ldg(reinterpret_cast<const uint4*>((const T*)p.sinv + at + half)), sn2);
+    }
+    if (PAIR || 2 * piece < pieces) {
 #pragma unroll
       for (int d = 0; d < P::N / 2; ++d) sn[d] = make_float2(-sn[d].x, -sn[d].y);
     }
     // the lanes of this row take this branch together
-    const uint32_t lanes = (0xffffffffu >> (32 - pieces)) << ((threadIdx.x & 31) & ~(pieces - 1));
+    const uint32_t lanes = PAIR ? 0u : (0xffffffffu >> (32 - pieces)) << ((threadIdx.x & 31) & ~(pieces - 1));
 #pragma unroll
     for (int k = 0; k < kAppendRows; ++k) {
       if (k >= rows) break;
-      uint4 o;
-      o.x = __shfl_xor_sync(lanes, x[k].x, pieces / 2);
-      o.y = __shfl_xor_sync(lanes, x[k].y, pieces / 2);
-      o.z = __shfl_xor_sync(lanes, x[k].z, pieces / 2);
-      o.w = __shfl_xor_sync(lanes, x[k].w, pieces / 2);
-      float2 u[P::N / 2], w[P::N / 2];
+      uint4 other;
+      if (PAIR) {
+        other = o[PAIR ? k : 0];
+      } else {
+        other.x = __shfl_xor_sync(lanes, x[k].x, pieces / 2);
+        other.y = __shfl_xor_sync(lanes, x[k].y, pieces / 2);
+        other.z = __shfl_xor_sync(lanes, x[k].z, pieces / 2);
+        other.w = __shfl_xor_sync(lanes, x[k].w, pieces / 2);
+      }
+      float2 u[P::N / 2], w[P::N / 2], r[P::N / 2];
       P::open(x[k], u);
-      P::open(o, w);
+      P::open(other, w);
 #pragma unroll
-      for (int d = 0; d < P::N / 2; ++d) u[d] = fma2(u[d], cs[d], mul2(w[d], sn[d]));
-      *reinterpret_cast<uint4*>(y + k * ystep) = P::close(u);
+      for (int d = 0; d < P::N / 2; ++d) r[d] = fma2(u[d], cs[d], mul2(w[d], sn[d]));
+      *reinterpret_cast<uint4*>(y + k * ystep) = P::close(r);
+      if constexpr (PAIR) {
+#pragma unroll
+        for (int d = 0; d < P::N / 2; ++d) r[d] = fma2(w[d], cs2[d], mul2(u[d], sn2[d]));
+        *reinterpret_cast<uint4*>(y + k * ystep + half) = P::close(r);
+      }
     }
   } else {
 #pragma unroll
     for (int k = 0; k < kAppendRows; ++k)
-      if (k < rows) *reinterpret_cast<uint4*>(y + k * ystep) = x[k];
+      if (k < rows) {
+        *reinterpret_cast<uint4*>(y + k * ystep) = x[k];
+        if (PAIR) *reinterpret_cast<uint4*>(y + k * ystep + half) = o[PAIR ? k : 0];
+      }
   }
 }
 
@@ -262,7 +283,8 @@ ONE_DEVINL uint32_t mass_key(float f) {
 // 51 in two, 70 in one). Otherwise one CTA writes the survivors' list and paged_move_kernel copies.
 // KPT > 0: a thread keeps the keys of candidates tid, tid + 512, .. in KPT registers, read together and
 // before the length is known. KPT = 0, for tables of more than 32768 slots: the masses are read again in
-// each pass.
+// each pass. Three CTAs per SM where registers allow it and nothing is moved (100 x 16 heads of 781 slots
+// to 200, 80 dims: 74.6 us in all with two, 70.3 with three).
 constexpr int kEvictThreads = 512;
 constexpr int kEvictWarps = kEvictThreads / 32;
 constexpr int kEvictList = 512;  // places listed at a time, one per thread
@@ -274,7 +296,7 @@ struct Int {
 };
 
 template <int KPT, bool MOVE>
-__global__ void __launch_bounds__(kEvictThreads, KPT > 16 ? 1 : 2)
+__global__ void __launch_bounds__(kEvictThreads, KPT > 16 ? 1 : KPT == 4 && !MOVE ? 3 : 2)
     paged_evict_kernel(const __grid_constant__ PagedEvictParams p, int parts, int pieces) {
   // digit counts [512][8], [4096], [2048]; the first part's room then holds the listed rows' addresses in
   // 16 bytes: [from, to][keys, values][places], from -1: nothing to copy

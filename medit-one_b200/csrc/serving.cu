@@ -300,26 +300,29 @@ extern "C" int one_paged_append(const one_paged_cache* cache, const one_paged_to
   }
   p.cosv = cosv; p.sinv = sinv; p.cos_bs = x.cos_batch == 1 ? 0 : (int64_t)n * dh; p.counts = x.counts;
   p.mass = cache->mass; p.mass_width = cache->mass_width; p.q_out = x.q_out; p.N = n; p.Hq = hq;
-  // 16-byte pieces need aligned rows and halves of whole pieces; anything else goes element by element
+  // 16-byte pieces need aligned rows of whole pieces, a power of two of them or two halves; anything else
+  // goes element by element
   const int64_t unit = 16 / elem_bytes(dtype);
   auto aligned = [&](const void* at, const int64_t* s) {
     return (reinterpret_cast<uintptr_t>(at) & 15) == 0 && s[0] % unit == 0 && s[1] % unit == 0 && s[2] % unit == 0;
   };
   const int pieces = dh % unit == 0 ? dh / (int)unit : 0;
-  const bool vec = pieces >= 2 && (pieces & (pieces - 1)) == 0 && aligned(k, p.ks) && aligned(v, p.vs) && (!q || aligned(q, p.qs)) &&
+  const bool vec = pieces >= 2 && pieces % 2 == 0 && aligned(k, p.ks) && aligned(v, p.vs) && (!q || aligned(q, p.qs)) &&
                    ((reinterpret_cast<uintptr_t>(x.q_out) | reinterpret_cast<uintptr_t>(cosv) | reinterpret_cast<uintptr_t>(sinv)) & 15) == 0;
+  const bool pair = (pieces & (pieces - 1)) != 0;
   const int64_t rows = 2 * (int64_t)hkv + (q ? hq : 0);
   auto groups = [](int64_t heads) { return (heads + kAppendRows - 1) / kAppendRows; };
-  const int64_t threads = vec ? n * (2 * groups(hkv) + groups(q ? hq : 0)) * pieces : n * rows * 32;
+  const int64_t threads = vec ? n * (2 * groups(hkv) + groups(q ? hq : 0)) * (pair ? pieces / 2 : pieces) : n * rows * 32;
   if (threads > 0x7fffffff) return fail(ONE_ERR_UNSUPPORTED, "paged append: too many rows");
   const dim3 grid((unsigned)((threads + 255) / 256), b);
   cudaStream_t st = (cudaStream_t)stream;
-  const bool bf = dtype == ONE_DTYPE_BF16;
-  return launched(vec ? bf ? launch(paged_append_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, p)
-                           : launch(paged_append_kernel<float>, grid, dim3(256), 0, st, p)
-                      : bf ? launch(paged_append_any_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, p)
-                           : launch(paged_append_any_kernel<float>, grid, dim3(256), 0, st, p),
-                  "paged append");
+  auto append = [&](auto t) {
+    using T = decltype(t);
+    return !vec   ? launch(paged_append_any_kernel<T>, grid, dim3(256), 0, st, p)
+           : pair ? launch(paged_append_kernel<T, true>, grid, dim3(256), 0, st, p)
+                  : launch(paged_append_kernel<T, false>, grid, dim3(256), 0, st, p);
+  };
+  return launched(dtype == ONE_DTYPE_BF16 ? append(__nv_bfloat16()) : append(float(0)), "paged append");
 }
 
 extern "C" int one_paged_evict(const one_paged_cache* cache, const int32_t* dst_table, int64_t dst_stride,

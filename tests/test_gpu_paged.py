@@ -199,7 +199,8 @@ def test_bad_pages_and_lengths_are_recorded():
 APPEND = [  # hkv, hq, dh, page, starts, n, counts
     (2, 4, 64, 16, [0, 5, 31], 1, None), (1, 0, 64, 16, [0, 40], 70, [70, 1]), (12, 12, 64, 16, [100] * 5, 1, None),
     (3, 3, 40, 7, [2, 0, 13], 9, [9, 0, 4]), (1, 5, 128, 1, [3], 20, None), (2, 2, 8, 3, [1, 1], 4, [2, 9]),
-    (2, 6, 24, 64, [0], 333, None), (7, 5, 16, 8, [3, 0], 11, [11, 2]), (4, 4, 32, 48, [47, 48], 2, [-1, 2]), (1, 1, 96, 16, [16], 5, [5]),
+    (2, 6, 24, 64, [0], 333, None), (3, 5, 80, 16, [0, 7], 40, [40, 3]), (5, 1, 48, 5, [2], 17, None), (2, 2, 112, 32, [9], 33, None),
+    (7, 5, 16, 8, [3, 0], 11, [11, 2]), (4, 4, 32, 48, [47, 48], 2, [-1, 2]), (1, 1, 96, 16, [16], 5, [5]),
 ]
 
 
