@@ -215,7 +215,7 @@ struct PaBf16 {
   static constexpr int kGroups = DH <= 64 ? 128 / DH : 1;  // 16-slot groups per warp and step
   static constexpr int TILE = 16 * kGroups * kPaWarps;
   static constexpr int kGroup = 64 * DH;               // bytes of a group's keys and values
-  static constexpr int kStages = 2, kStagesFew = 3;    // of a list, that fills the SMs; of clusters
+  static constexpr int kStages = 2, kStagesFew = 3;    // where CTAs fill the SMs; where they are few
   static constexpr int kExtra = 0;                     // further shared bytes per warp
   uint32_t qa[WIDE ? 2 : 1][KC][4];
   float o[NT][4];
@@ -589,10 +589,14 @@ ONE_DEVINL float4 cluster_ld4(const float* mine, int rank) {
   return v;
 }
 
-template <typename E, bool SPLIT>
+// What a CTA takes: a share of the list; a segment, or its share of a cluster's; the same with a deeper ring.
+enum PaMode { PA_LIST, PA_SEGMENT, PA_DEEP };
+
+template <typename E, PaMode MODE>
 struct PaSmem {
+  static constexpr bool SPLIT = MODE == PA_LIST;
   static constexpr int kStage = E::kGroup * E::kGroups;                  // bytes per warp
-  static constexpr int kStages = SPLIT ? E::kStages : E::kStagesFew;
+  static constexpr int kStages = MODE == PA_DEEP ? E::kStagesFew : E::kStages;
   static constexpr int kWarp = kStage * kStages;
   static constexpr int kML = kPaWarps * kWarp;                           // [2][warps][ROWS][2]
   static constexpr int kFin = kML + 2 * kPaWarps * E::ROWS * 8;          // [ROWS][2]: m, 1 / l
@@ -606,13 +610,15 @@ struct PaSmem {
   static_assert(kStage >= E::ROWS * E::DH * 4, "stage");
 };
 
-// SPLIT: CTA i takes the i-th share of the list. Otherwise a cluster of p.cluster CTAs (1 to 8) takes
-// each segment, in equal shares, and joins them through its shared memory: one launch, for small batches. RUN: pages hold a multiple of 16 slots and Dh is
-// E::DH, so that a group lies in one page and its copies need two addresses.
-template <typename E, bool RUN, bool SPLIT>
-__global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, SPLIT>::kPerSm) paged_attn_kernel(const __grid_constant__ PagedAttn p) {
+// PA_LIST: CTA i takes the i-th share of the list. Otherwise a cluster of p.cluster CTAs (1 to 8) takes
+// each segment, in equal shares, and joins them through its shared memory: one launch, for small batches.
+// RUN: pages hold a multiple of 16 slots and Dh is E::DH, so that a group lies in one page and its copies
+// need two addresses.
+template <typename E, bool RUN, PaMode MODE>
+__global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, MODE>::kPerSm) paged_attn_kernel(const __grid_constant__ PagedAttn p) {
   extern __shared__ __align__(16) uint8_t smem[];
-  using S = PaSmem<E, SPLIT>;
+  using S = PaSmem<E, MODE>;
+  constexpr bool SPLIT = S::SPLIT;
   using T = typename E::T;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int TILE = E::TILE, GR = E::kGroups;

@@ -177,30 +177,46 @@ struct PagedWs {
 
 int pad_dh(int dh) { return dh <= 32 ? 32 : dh <= 64 ? 64 : dh <= 96 ? 96 : 128; }
 
-template <typename E, bool RUN, bool SPLIT>
-int attend(PagedAttn& p, cudaStream_t st) {
+template <typename E, bool RUN, PaMode MODE>
+int attend(PagedAttn& p, int cluster, cudaStream_t st) {
+  constexpr bool SPLIT = MODE == PA_LIST;
   static std::atomic<bool> done[kMaxDevices];
-  int rc = allow_smem(paged_attn_kernel<E, RUN, SPLIT>, PaSmem<E, SPLIT>::kTotal, done);
+  int rc = allow_smem(paged_attn_kernel<E, RUN, MODE>, PaSmem<E, MODE>::kTotal, done);
   if (rc) return rc;
-  const int64_t segments = (int64_t)p.c.B * p.c.Hkv * p.hv_per_kv, slots = (int64_t)p.c.max_pages * p.c.page_size;
-  p.ranges = std::min(num_sms(), kMaxSms) * PaSmem<E, SPLIT>::kPerSm;
-  p.cluster = SPLIT ? 1 : paged_cluster(segments, slots);
-  rc = launched(launch_cluster(p.cluster, paged_attn_kernel<E, RUN, SPLIT>, dim3((unsigned)(SPLIT ? p.ranges : segments * p.cluster)),
-                               dim3(kPaWarps * 32), PaSmem<E, SPLIT>::kTotal, st, p),
+  const int64_t heads = (int64_t)p.c.B * p.c.Hkv, slots = (int64_t)p.c.max_pages * p.c.page_size;
+  p.ranges = std::min(num_sms(), kMaxSms) * PaSmem<E, MODE>::kPerSm;
+  p.cluster = SPLIT ? 1 : cluster;
+  rc = launched(launch_cluster(p.cluster, paged_attn_kernel<E, RUN, MODE>, dim3((unsigned)(SPLIT ? p.ranges : heads * p.hv_per_kv * cluster)),
+                               dim3(kPaWarps * 32), PaSmem<E, MODE>::kTotal, st, p),
                 "paged attention");
   if (rc || !SPLIT) return rc;
-  const int64_t heads = (int64_t)p.c.B * p.c.Hkv;
   const int mass_blocks = p.mass ? (int)((slots + kJoinSlots - 1) / kJoinSlots) : 0;
   return launched(launch(paged_join_kernel<E>, dim3((unsigned)(heads * (p.G + mass_blocks))), dim3(kJoinThreads), 0, st, p,
                          mass_blocks),
                   "paged attention join");
 }
 
+// A deeper ring costs the third CTA of an SM: taken where two per SM hold the grid at once, and clusters
+// of 4 and 8 are not placed as densely as that (36 of 8 are not, 32 are). bf16, slots as given, with the
+// deeper ring and without: 16 x 8 heads x 128, 1000 (pairs) 13.5 and 17.4 us; 37 x 8 x 128, 500 (single)
+// 12.7 and 16.6; 8 x 4 x 64, 4000 (32 clusters of 8) 10.5 and 11.6; 9 x 4 x 64, 4000 (36) 19.1 and 11.7;
+// 64 x 12 x 64, 128 (single, 768) 12.3 and 10.3; 149 x 16 x 64, 32 (2384) 26.7 and 20.5.
+bool paged_deep(int64_t segments, int cluster) { return segments * cluster <= (cluster > 2 ? 256 : 296); }
+
+template <typename E, bool RUN>
+int attend(PagedAttn& p, bool split, cudaStream_t st) {
+  const int64_t segments = (int64_t)p.c.B * p.c.Hkv * p.hv_per_kv;
+  const int cluster = paged_cluster(segments, (int64_t)p.c.max_pages * p.c.page_size);
+  if (split) return attend<E, RUN, PA_LIST>(p, cluster, st);
+  if constexpr (E::kStagesFew > E::kStages)
+    if (paged_deep(segments, cluster)) return attend<E, RUN, PA_DEEP>(p, cluster, st);
+  return attend<E, RUN, PA_SEGMENT>(p, cluster, st);
+}
+
 template <typename E>
 int attend(PagedAttn& p, bool split, cudaStream_t st) {
   const bool run = p.c.page_size % 16 == 0 && p.c.Dh == E::DH;
-  return split ? run ? attend<E, true, true>(p, st) : attend<E, false, true>(p, st)
-               : run ? attend<E, true, false>(p, st) : attend<E, false, false>(p, st);
+  return run ? attend<E, true>(p, split, st) : attend<E, false>(p, split, st);
 }
 
 }  // namespace

@@ -52,7 +52,11 @@ SHAPES = [  # hkv, group, dh, page, lengths
     (12, 1, 64, 16, [2049]), (1, 8, 64, 16, [20000, 3]), (1, 1, 16, 3, [0, 0]), (5, 4, 112, 24, [1500, 31, 600]),
     (16, 1, 64, 16, [(i * 97) % 701 for i in range(30)]), (10, 2, 32, 32, [(i * 331) % 1300 for i in range(50)]),
     (1, 4, 64, 16, [300]), (2, 9, 128, 16, [4096, 1]), (1, 2, 96, 16, [8192 * 3, 5, 0]),
+    (4, 1, 64, 16, [(i * 1000 + 700) % 4001 for i in range(9)]), (4, 2, 128, 16, [(i * 331) % 1001 for i in range(18)]),
 ]
+MANY = [(i * 89) % 261 for i in range(33)]  # more segments than are taken one by one with a deep ring
+SHAPES += [(10, g, dh, page, MANY) for g, dh, page in
+           [(1, 64, 16), (9, 64, 32), (2, 128, 16), (12, 128, 16), (3, 96, 16), (10, 96, 48), (1, 32, 16), (20, 32, 5), (2, 80, 16)]]
 
 
 @pytest.mark.parametrize("dt", [BF, F32], ids=["bf16", "fp32"])
