@@ -401,26 +401,29 @@ extern "C" int one_process_logits(const one_logits_rules* rules, const void* log
   p.bias = x.bias; p.bias_ld = x.bias_ld; p.mask = reinterpret_cast<const uint32_t*>(x.token_mask); p.mask_ld = x.mask_ld;
   p.out = out; p.out_ld = out_ld; p.best = best;
   cudaStream_t st = (cudaStream_t)stream;
-  // Enough CTAs per row (at most a portable cluster) to cover the SMs, each with a few tokens per thread;
-  // no more, since every CTA reads the row's whole history (256 rows of 32000 tokens, 2176 ids: 22.0 us
-  // with 1 CTA per row, 25.3 with 2, 32.9 with 4).
+  // CTAs per row (at most a portable cluster) until there are two per SM, each with a few tokens per thread;
+  // no more, since every CTA reads the row's whole history (256 rows of 32000 tokens, 2176 ids: 18.8 us
+  // with 1 CTA per row, 24.9 with 2; 148 rows, 500 ids: 14.1 and 10.6).
   int ctas = 1;
-  while (ctas < 8 && (int64_t)batch * ctas < num_sms() && vocab > ctas * kLogitsThreads * 8) ctas *= 2;
+  while (ctas < 8 && (int64_t)batch * ctas <= num_sms() && vocab > ctas * kLogitsThreads * 8) ctas *= 2;
   const int slice = ((vocab + ctas - 1) / ctas + 31) / 32 * 32;
   if ((int64_t)batch * ctas > 0x7fffffff) return fail(ONE_ERR_UNSUPPORTED, "process logits: too many rows");
   const bool wide = hist_len > 32767;  // a count may not fit 15 bits
   const size_t smem = hist_len ? std::min<size_t>((size_t)slice * (wide ? 4 : 2), kLogitsBytes) + 32 : 0;
-  static std::atomic<bool> done[8][kMaxDevices];
-  auto run = [&](auto t, auto i, auto w) -> int {
+  const bool full = (int64_t)batch * ctas > 2 * num_sms();
+  static std::atomic<bool> done[16][kMaxDevices];
+  auto run = [&](auto t, auto i, auto w, auto per_sm) -> int {
     using T = decltype(t);
     using I = decltype(i);
-    auto* kernel = logits_kernel<T, I, decltype(w)::value != 0>;
-    const int rc = allow_smem(kernel, kLogitsBytes + 32, done[(sizeof(T) == 4) * 4 + (sizeof(I) == 8) * 2 + decltype(w)::value]);
+    constexpr int WIDE = decltype(w)::value, PER_SM = decltype(per_sm)::value;
+    auto* kernel = logits_kernel<T, I, WIDE != 0, PER_SM>;
+    const int rc = allow_smem(kernel, kLogitsBytes + 32, done[(sizeof(T) == 4) * 8 + (sizeof(I) == 8) * 4 + WIDE * 2 + (PER_SM == 3)]);
     if (rc) return rc;
     return launched(launch_cluster(ctas, kernel, dim3((unsigned)batch * ctas), dim3(kLogitsThreads), smem, st, p, slice, ctas),
                     "process logits");
   };
-  auto by_counts = [&](auto t, auto i) { return wide ? run(t, i, Int<1>()) : run(t, i, Int<0>()); };
+  auto by_rows = [&](auto t, auto i, auto w) { return full ? run(t, i, w, Int<3>()) : run(t, i, w, Int<2>()); };
+  auto by_counts = [&](auto t, auto i) { return wide ? by_rows(t, i, Int<1>()) : by_rows(t, i, Int<0>()); };
   if (dtype == ONE_DTYPE_BF16)
     return x.history_bytes == 8 ? by_counts(__nv_bfloat16(), int64_t(0)) : by_counts(__nv_bfloat16(), int32_t(0));
   return x.history_bytes == 8 ? by_counts(float(0), int64_t(0)) : by_counts(float(0), int32_t(0));

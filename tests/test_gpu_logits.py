@@ -31,7 +31,7 @@ def check_best(best, got):
 
 
 CASES = [(1, 1, 0), (3, 33, 5), (2, 1000, 1), (4, 32000, 300), (1, 50257, 5000), (5, 8192, 64), (2, 8193, 17),
-         (1, 160001, 40), (300, 70, 9), (2, 40000, 32767), (1, 40000, 33000)]
+         (1, 160001, 40), (300, 70, 9), (2, 40000, 32767), (1, 40000, 33000), (148, 5001, 33)]
 
 
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
@@ -58,6 +58,11 @@ def test_process_logits(case, rows, ids, dt):
     ref = P.logits(x, hist, starts, *pen, bias, allowed.expand(B, V))
     check(out, ref, x, dt)
     check_best(best, out)
+
+
+@pytest.mark.parametrize("case,dt", [((297, 33001, 20), torch.bfloat16), ((299, 40, 32800), torch.float32)], ids=["slices", "ids"])
+def test_more_rows_than_fit_at_once(case, dt):
+    test_process_logits(case, True, torch.int32, dt)
 
 
 def test_each_part_alone_and_nothing():
