@@ -4,14 +4,17 @@
 //   o   = sum_t 2^(s_t - m) v_t / l    mass_t += 2^(s_t - m) / l, summed over a kv head's queries
 //
 // One pass over K and V with the running maximum and sum; parts of a sequence join by their (m, l, o).
-// HBM bounds it: every K and V row is read once, at 1 flop per byte and query head of a group.
+// HBM bounds it: every K and V row is read once, at 1 flop per byte and query head of a group. Measured, of
+// the measured copy rate: 64 ragged sequences up to 4096 slots, 12 heads x 64, bf16: 75 us, 84 %; 8 up to
+// 32768, 8 heads x 128 of 4 queries: 99 us, 89 %. Small batches are bound by a chain: lengths -> page
+// numbers -> rows -> softmax -> join, 4.3 us for one sequence of 200 slots.
 //
-// Partition. The work is the list of tiles (64 slots or more) of every (sequence, query-head tile) in order; a
-// grid that fills the GPU takes equal shares of that list, whatever the lengths, so a ragged batch
-// and a single long sequence keep all SMs busy. A share is a run of pieces of segments (a segment:
-// one sequence's tiles for one query-head tile). A piece that is its whole segment is finished on the
-// spot; the others leave (m, l, o) in the workspace, and paged_join_kernel joins them in a fixed
-// order (no atomics: equal inputs give equal bits).
+// Partition. Few or short segments (a segment: one sequence's tiles of 64 slots or more for one query-head
+// tile) have a cluster of CTAs each, and one launch. Otherwise the work is the list of all segments' tiles
+// in order; a grid that fills the GPU takes equal shares of that list, whatever the lengths, so a ragged
+// batch and a few long sequences keep all SMs busy. A share is a run of pieces of segments. A piece that
+// is its whole segment is finished on the spot; the others leave (m, l, o) in the workspace, and
+// paged_join_kernel joins them in a fixed order (no atomics: equal inputs give equal bits).
 //
 // Inside a CTA, each of four warps owns a quarter of a tile (groups of 16 slots) and a ring of stages
 // in shared memory that its own cp.async fill in the order of the matrix fragments: the ring needs no
@@ -147,7 +150,7 @@ ONE_DEVINL void mma_bf16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t
 // consecutive pieces, and D::at(row, piece), where a piece goes, keeps a 128-byte line of a row in one
 // 128-byte line of shared memory with its pieces permuted, which spreads the fragments' reads over
 // the banks. (Pieces that go to lines of their own are asked for one by one, and each 32-byte sector
-// twice: that read 1.5 times the bytes into the SMs and took 96 us where this takes 80, at 64 x 4096
+// twice: that read 1.5 times the bytes into the SMs and took 96 us where this took 80, at 64 x 4096
 // ragged tokens.) D::at is linear over exclusive or, so the unrolled loop splits it into a lane's
 // constant and a compile-time one.
 template <typename D, int CH>

@@ -148,8 +148,8 @@ int paged_cluster(int64_t segments, int64_t slots) {
 
 // Whether the segments are cut from a list. A cluster per segment has one launch and no second pass, but
 // at most 8 CTAs for a long sequence, and fewer than the SMs hold for a few. Both sides, per call: 8 x 3001
-// slots, 4 heads x 64 in fp32 (8 CTAs of 384 slots) 13.4 us by clusters, 15.3 from a list; 16 x 2500, 4 kv
-// heads (4 CTAs of 640 slots) 16.6 by clusters, 15.2 from a list.
+// slots, 4 heads x 64 in fp32 (8 CTAs of 384 slots) 13.6 us by clusters, 15.3 from a list; 16 x 2500, 4 kv
+// heads (4 CTAs of 640 slots) 16.6 by clusters, 14.4 from a list.
 bool paged_split(int64_t segments, int64_t slots) {
   const int64_t n = paged_cluster(segments, slots);
   return slots > kWhole * n;
