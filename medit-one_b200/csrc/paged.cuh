@@ -282,9 +282,12 @@ ONE_DEVINL uint32_t mass_key(float f) {
 // once (4 x 1040 slots to 1024, 12 heads x 64: 12.3 us in two launches, 10.3 in one; 16 x 8192 to 2048:
 // 51 in two, 70 in one). Otherwise one CTA writes the survivors' list and paged_move_kernel copies.
 // KPT > 0: a thread keeps the keys of candidates tid, tid + 512, .. in KPT registers, read together and
-// before the length is known. KPT = 0, for tables of more than 32768 slots: the masses are read again in
-// each pass. Three CTAs per SM where registers allow it and nothing is moved (100 x 16 heads of 781 slots
-// to 200, 80 dims: 74.6 us in all with two, 70.3 with three).
+// before the length is known; the smallest KPT that holds the table, since every pass goes over all of them
+// (200 x 16 heads of 4096 slots to 512: 251 us in all with 16, 218 with 8). KPT = 0, for tables of more than
+// 32768 slots: the masses are read again in each pass (16 x 12 heads of 30000 to 2048: 102 us, 84 with 64).
+// CTAs per SM as the keys' registers allow: 3 rather than 2 up to KPT = 8 (100 x 16 heads of 781 slots to
+// 200, 80 dims: 74.6 -> 70.3 us), 2 rather than 1 up to 32, which spills 8 bytes (16 x 12 heads of 16000 to
+// 2048: 60 us; with 64 keys and one CTA 78).
 constexpr int kEvictThreads = 512;
 constexpr int kEvictWarps = kEvictThreads / 32;
 constexpr int kEvictList = 512;  // places listed at a time, one per thread
@@ -296,7 +299,7 @@ struct Int {
 };
 
 template <int KPT, bool MOVE>
-__global__ void __launch_bounds__(kEvictThreads, KPT > 16 ? 1 : KPT == 4 && !MOVE ? 3 : 2)
+__global__ void __launch_bounds__(kEvictThreads, KPT > 32 ? 1 : KPT && KPT <= 8 && !MOVE ? 3 : 2)
     paged_evict_kernel(const __grid_constant__ PagedEvictParams p, int parts, int pieces) {
   // digit counts [512][8], [4096], [2048]; the first part's room then holds the listed rows' addresses in
   // 16 bytes: [from, to][keys, values][places], from -1: nothing to copy

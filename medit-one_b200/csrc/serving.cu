@@ -369,7 +369,13 @@ extern "C" int one_paged_evict(const one_paged_cache* cache, const int32_t* dst_
                                (int)parts, pieces)
                       : launch(paged_evict_kernel<KPT, false>, dim3((unsigned)heads), dim3(kEvictThreads), 0, st, p, 1, pieces);
   };
-  rc = launched(slots <= 2048 ? evict(Int<4>()) : slots <= 8192 ? evict(Int<16>()) : slots <= 32768 ? evict(Int<64>()) : evict(Int<0>()),
+  rc = launched(slots <= 1024    ? evict(Int<2>())
+                : slots <= 2048  ? evict(Int<4>())
+                : slots <= 4096  ? evict(Int<8>())
+                : slots <= 8192  ? evict(Int<16>())
+                : slots <= 16384 ? evict(Int<32>())
+                : slots <= 32768 ? evict(Int<64>())
+                                 : evict(Int<0>()),
                 "paged evict");
   if (rc || one_launch) return rc;
   return launched(launch(paged_move_kernel, dim3((unsigned)(per_bh * heads)), dim3(kMoveThreads), 0, st, p, (int)per_bh, pieces),

@@ -292,7 +292,7 @@ EVICT = [  # hkv, dh, page, lengths, budget, recent, sink
     (2, 64, 16, [40, 33, 32, 31, 0, 1], 32, 8, 4), (1, 64, 16, [1000], 999, 0, 0), (3, 32, 7, [200, 64, 70], 64, 64, 0),
     (1, 128, 48, [5000, 2], 100, 30, 70), (2, 8, 1, [9, 3], 1, 0, 0), (1, 40, 5, [300, 299], 128, 5, 1),
     (12, 64, 16, [2049, 2048, 500], 2048, 100, 4), (1, 16, 128, [70000], 1000, 100, 0), (1, 64, 16, [50], 60, 10, 0), (2, 32, 16, [48, 3], 70, 5, 64),
-    (2, 64, 16, [20000, 16384], 16000, 0, 0),
+    (2, 64, 16, [20000, 16384], 16000, 0, 0), (2, 16, 16, [3999, 0], 300, 9, 9), (1, 8, 16, [7777, 8000], 500, 3, 0), (1, 16, 32, [16000, 9000], 700, 0, 2),
 ]
 
 
@@ -338,6 +338,13 @@ def test_evict(case, kind, dt):
 
 
 # ------------------------------------------------------------------ together
+@pytest.mark.parametrize("kind,hkv,b,n,budget", [
+    ("ties", 50, 6, 1000, 250), ("odd", 25, 6, 2000, 700), ("distinct", 50, 6, 4090, 100), ("ties", 50, 6, 4500, 300),
+    ("odd", 10, 10, 9000, 900), ("distinct", 5, 6, 17000, 4000), ("ties", 5, 5, 33000, 3333)])
+def test_evict_more_than_fits_the_gpu_at_once(kind, hkv, b, n, budget):
+    test_evict((hkv, 16, 16, [n - 37 * i for i in range(b)], budget, 7, 3), kind, BF)
+
+
 def test_shared_prefix_pages_side_stream_and_graph():
     """Two sequences over the same prompt pages; a decode step (append, attention) captured and
     replayed on a side stream with lengths that move between replays; then an eviction, which only
