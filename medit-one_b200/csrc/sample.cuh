@@ -60,8 +60,10 @@ struct SampShared {
 };
 
 // Weight of a kept score for the top-p and sampling passes: exp(s - mx) in 2^-32 fixed point,
-// at least 1 (a kept token keeps a nonzero chance).
+// at least 1 (a kept token keeps a nonzero chance), but 0 for -inf: a masked token, or NaN, is never
+// drawn, whether or not the top-k reaches down to it.
 ONE_DEVINL unsigned long long samp_weight(float s, float mx) {
+  if (s == -INFINITY) return 0ull;
   const unsigned long long w = (unsigned long long)(expf(s - mx) * 4294967296.0f);
   return w ? w : 1ull;
 }
