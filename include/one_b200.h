@@ -229,9 +229,10 @@ int one_selftest_mean_division(const float* divisors, int32_t n, unsigned long l
  * then top-k (keep scores >= the k-th largest; top_k = 0: off), then top-p (keep the largest
  * tokens until their probability mass reaches top_p; top_p >= 1: off), then one draw from the
  * softmax of the kept scores. Ties at a top-k / top-p boundary are all kept. Scores of -inf and
- * NaN are never drawn; a row of nothing else gives token 0. The draw for sequence b uses the
- * Philox4x32-10 counter (offset, b) under key `seed`, so equal (seed, offset) give equal tokens.
- * vocab <= 49152; temperature > 0. out [batch] int32 (device).
+ * NaN are never drawn, a row of nothing else gives token 0; scores of +inf share the draw among
+ * themselves. The draw for sequence b uses the Philox4x32-10 counter (offset, b) under key `seed`,
+ * so equal (seed, offset) give equal tokens. vocab <= 49152; temperature > 0. out [batch] int32
+ * (device).
  * No counterpart in one_turbo: it replaces the sampling step of GenerationMixin.generate,
  * which the reference's generate() runs (one/modeling_one.py:845, README.md:73). */
 int one_sample_tokens(const void* logits, int32_t batch, int32_t vocab, int32_t ld, int32_t dtype, float temperature,

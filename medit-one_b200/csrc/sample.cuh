@@ -61,9 +61,10 @@ struct SampShared {
 
 // Weight of a kept score for the top-p and sampling passes: exp(s - mx) in 2^-32 fixed point,
 // at least 1 (a kept token keeps a nonzero chance), but 0 for -inf: a masked token, or NaN, is never
-// drawn, whether or not the top-k reaches down to it.
+// drawn, whether or not the top-k reaches down to it. Scores of +inf share the draw among themselves.
 ONE_DEVINL unsigned long long samp_weight(float s, float mx) {
   if (s == -INFINITY) return 0ull;
+  if (mx == INFINITY) return s == mx ? 1ull << 32 : 0ull;
   const unsigned long long w = (unsigned long long)(expf(s - mx) * 4294967296.0f);
   return w ? w : 1ull;
 }

@@ -312,8 +312,8 @@ def sample_tokens(logits: torch.Tensor, temperature: float = 1.0, top_k: int = 0
     """One token per row of logits [B, V] (CUDA, bf16 or fp32) drawn on the GPU
     (one_sample_tokens): scores / temperature, top-k, top-p, one draw from the softmax of the
     kept scores, as transformers' sampling loop warps its logits. Scores of -inf and NaN are never
-    drawn; a row of nothing else gives token 0. The draw of row b depends on (seed, offset, b) only.
-    Returns int32 [B] on the logits' device."""
+    drawn, a row of nothing else gives token 0; scores of +inf share the draw among themselves. The
+    draw of row b depends on (seed, offset, b) only. Returns int32 [B] on the logits' device."""
     if logits.dim() != 2 or not logits.is_cuda:
         raise C.OneError("sample_tokens takes CUDA logits [batch, vocab]")
     B, V = logits.shape

@@ -72,3 +72,35 @@ def test_scores_behind_the_mask_draw_as_they_did():
     for offset in range(4):
         a, b = (sample_tokens(t.cuda(), 1.0, 0, 1.0, seed=5, offset=offset).cpu() for t in (x, y))
         assert int((a != b).sum()) <= 1
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("T,k,p", WARPS)
+def test_scores_of_plus_infinity_take_the_draw(T, k, p, dt):
+    """A bias of +inf forces a token; several share the draw."""
+    from one.engine import sample_tokens
+    x = torch.randn(200, 32000, generator=torch.Generator().manual_seed(4))
+    x[:, 17000] = math.inf
+    x[:, 3] = -math.inf
+    x[100:, 31000] = math.inf
+    got = sample_tokens(x.to(dt).cuda(), T, k, p, seed=2, offset=7487565).cpu()
+    assert bool((got[:100] == 17000).all())
+    assert bool(((got[100:] == 17000) | (got[100:] == 31000)).all())
+    # 100 draws of two equal tokens: 5 standard deviations of a binomial
+    assert 25 <= int((got[100:] == 31000).sum()) <= 75
+
+
+def test_generate_is_forced_by_an_infinite_bias():
+    from one.configuration_one import tiny_config
+    from one.initialization import init_state_dict
+    from one.modeling_one import OneForCausalLM
+    cfg = tiny_config()
+    model = OneForCausalLM(cfg)
+    model.load_state_dict(init_state_dict(cfg, 0, torch.float32), strict=False)
+    model = model.to(torch.bfloat16).cuda()
+    ids = torch.randint(1, cfg.vocab_size, (3, 6), generator=torch.Generator().manual_seed(1)).cuda()
+    bias = torch.zeros(cfg.vocab_size)
+    bias[77] = math.inf
+    for sample in (False, True):
+        got = model.generate(ids, max_new_tokens=5, do_sample=sample, logit_bias=bias.cuda(), seed=1)
+        assert bool((got[:, 6:] == 77).all())
