@@ -247,10 +247,11 @@ class OneForCausalLM(OnePreTrainedModel, GenerationMixin):
         pad_token_id (eos when pad is unset), and generation stops when every sequence has
         finished. `seed` fixes the draws (default: drawn from torch's global generator).
 
-        repetition_penalty (over prompt and new tokens, as transformers'), presence_penalty and
-        frequency_penalty (over the new tokens), logit_bias (fp32 [V] or [B, V]) and token_mask
-        (one.engine.pack_token_mask's words, the same at every step) act on each step's logits before
-        the warpers or the argmax (one.engine.process_logits). They are taken from the call alone.
+        repetition_penalty (over prompt and new tokens, as transformers'; resolved as the arguments
+        above), presence_penalty and frequency_penalty (over the new tokens), logit_bias (fp32 [V] or
+        [B, V]) and token_mask (one.engine.pack_token_mask's words, the same at every step) act on each
+        step's logits before the warpers or the argmax (one.engine.process_logits). transformers'
+        configurations have no counterpart of the last four: they are taken from the call alone.
         Returns [B, S + new tokens]. Beam search, constraints and streaming are not supported."""
         unsupported = {k: v for k, v in kwargs.items()
                        if v is not None and not (k in ("num_beams", "num_return_sequences") and v == 1)
@@ -286,7 +287,7 @@ class OneForCausalLM(OnePreTrainedModel, GenerationMixin):
             return input_ids
         if do_sample and not temperature > 0:
             raise ValueError("do_sample=True needs temperature > 0")
-        rep = 1.0 if repetition_penalty is None else float(repetition_penalty)
+        rep = float(pick(repetition_penalty, "repetition_penalty", 1.0))
         pres, freq = float(presence_penalty or 0.0), float(frequency_penalty or 0.0)
         if not rep > 0:
             raise ValueError("repetition_penalty must be positive")
