@@ -268,14 +268,15 @@ typedef struct one_paged_cache {
 
 /* New tokens of a batch: keys k, values v [b, hkv, n, dh] and, optionally, queries q [b, hq, n, dh]
  * (element strides of batch, head and token; rows contiguous). cos, sin [cos_batch, n, dh]
- * (cos_batch = b, or 1 when shared), or NULL: no rotation. counts int32 [b], or NULL: n. */
+ * (cos_batch = b, or 1 when shared) in the cache's dtype, or in fp32 with tables_fp32 = 1; NULL: no
+ * rotation. counts int32 [b], or NULL: n. */
 typedef struct one_paged_tokens {
   const void *k, *v, *q;
   int64_t k_strides[3], v_strides[3], q_strides[3];
   const void *cos, *sin;
   const int32_t* counts;
   void* q_out;
-  int32_t n, hq, cos_batch, reserved;
+  int32_t n, hq, cos_batch, tables_fp32;
 } one_paged_tokens;
 
 /* New tokens into the cache. q and k are rotated as apply_rotary_pos_emb_flash does

@@ -48,7 +48,7 @@ struct PagedAppendParams {
   PagedCache c;
   const void *k, *v, *q;
   int64_t ks[3], vs[3], qs[3];  // element strides: batch, head, token
-  const void *cosv, *sinv;      // [cos_batch][N][Dh] or null
+  const void *cosv, *sinv;      // [cos_batch][N][Dh] or null, in the cache's type or fp32
   int64_t cos_bs;
   const int* counts;
   float* mass;
@@ -97,14 +97,23 @@ template <> struct Piece<float> {
     return make_uint4(__float_as_uint(v[0].x), __float_as_uint(v[0].y), __float_as_uint(v[1].x), __float_as_uint(v[1].y));
   }
 };
+// cos or sin, of type C, of a piece of T
+template <typename T, typename C>
+ONE_DEVINL void open_table(const C* at, float2 (&v)[Piece<T>::N / 2]) {
+  constexpr int N = Piece<C>::N / 2;  // pairs per load
+#pragma unroll
+  for (int i = 0; i < Piece<T>::N / 2; i += N)
+    Piece<C>::open(__ldg(reinterpret_cast<const uint4*>(at + 2 * i)), *reinterpret_cast<float2(*)[N]>(v + i));
+}
 ONE_DEVINL float2 mul2(float2 a, float2 b) {
   uint64_t d;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(f2_bits(a)), "l"(f2_bits(b)));
   return f2_from(d);
 }
 
-// New tokens into the pages, rotated: y = x cos + rotate_half(x) sin. A copy with two products per
-// element, bound by HBM (prompts) or by one round trip to it (single tokens).
+// New tokens into the pages, rotated: y = x cos + rotate_half(x) sin, in fp32 with one rounding; C is the
+// type of cos and sin, that of the tokens or fp32. A copy with two products per element, bound by HBM
+// (prompts) or by one round trip to it (single tokens).
 //
 // One thread per token, group of kAppendRows heads of its keys, queries or values, and 16-byte piece:
 // consecutive lanes read and write whole rows, the group's loads are in flight together and share cos
@@ -117,7 +126,7 @@ ONE_DEVINL float2 mul2(float2 a, float2 b) {
 // heads x 80: 100 us one element at a time, 35 by halves.
 constexpr int kAppendRows = 4;
 
-template <typename T, bool PAIR>
+template <typename T, typename C, bool PAIR>
 __global__ void __launch_bounds__(256, PAIR ? 3 : 5) paged_append_kernel(const __grid_constant__ PagedAppendParams p) {
   using P = Piece<T>;
   pdl_wait();
@@ -172,11 +181,11 @@ __global__ void __launch_bounds__(256, PAIR ? 3 : 5) paged_append_kernel(const _
   if (kind < 2 && p.cosv) {
     const int64_t at = b * p.cos_bs + (int64_t)t * c.Dh + e;
     float2 cs[P::N / 2], sn[P::N / 2], cs2[PAIR ? P::N / 2 : 1], sn2[PAIR ? P::N / 2 : 1];
-    P::open(__ldg(reinterpret_cast<const uint4*>((const T*)p.cosv + at)), cs);
-    P::open(__ldg(reinterpret_cast<const uint4*>((const T*)p.sinv + at)), sn);
+    open_table<T>((const C*)p.cosv + at, cs);
+    open_table<T>((const C*)p.sinv + at, sn);
     if constexpr (PAIR) {
-      P::open(__ldg(reinterpret_cast<const uint4*>((const T*)p.cosv + at + half)), cs2);
-      P::open(__ldg(reinterpret_cast<const uint4*>((const T*)p.sinv + at + half)), sn2);
+      open_table<T>((const C*)p.cosv + at + half, cs2);
+      open_table<T>((const C*)p.sinv + at + half, sn2);
     }
     if (PAIR || 2 * piece < pieces) {
 #pragma unroll
@@ -219,7 +228,7 @@ __global__ void __launch_bounds__(256, PAIR ? 3 : 5) paged_append_kernel(const _
 }
 
 // The same for rows of any alignment: one warp per row of q, k or v.
-template <typename T>
+template <typename T, typename C>
 __global__ void __launch_bounds__(256) paged_append_any_kernel(const __grid_constant__ PagedAppendParams p) {
   pdl_wait();
   const PagedCache& c = p.c;
@@ -246,7 +255,7 @@ __global__ void __launch_bounds__(256) paged_append_any_kernel(const __grid_cons
     float r = ld<T>(x + d);
     if (p.cosv && !is_v) {
       const float o = d < half ? -ld<T>(x + d + half) : ld<T>(x + d - half);
-      r = r * ld<T>((const T*)p.cosv + cs + d) + o * ld<T>((const T*)p.sinv + cs + d);
+      r = r * ld<C>((const C*)p.cosv + cs + d) + o * ld<C>((const C*)p.sinv + cs + d);
     }
     st<T>(y + d, r);
   }

@@ -332,13 +332,17 @@ extern "C" int one_paged_append(const one_paged_cache* cache, const one_paged_to
   if (threads > 0x7fffffff) return fail(ONE_ERR_UNSUPPORTED, "paged append: too many rows");
   const dim3 grid((unsigned)((threads + 255) / 256), b);
   cudaStream_t st = (cudaStream_t)stream;
-  auto append = [&](auto t) {
+  auto append = [&](auto t, auto c) {
     using T = decltype(t);
-    return !vec   ? launch(paged_append_any_kernel<T>, grid, dim3(256), 0, st, p)
-           : pair ? launch(paged_append_kernel<T, true>, grid, dim3(256), 0, st, p)
-                  : launch(paged_append_kernel<T, false>, grid, dim3(256), 0, st, p);
+    using C = decltype(c);
+    return !vec   ? launch(paged_append_any_kernel<T, C>, grid, dim3(256), 0, st, p)
+           : pair ? launch(paged_append_kernel<T, C, true>, grid, dim3(256), 0, st, p)
+                  : launch(paged_append_kernel<T, C, false>, grid, dim3(256), 0, st, p);
   };
-  return launched(dtype == ONE_DTYPE_BF16 ? append(__nv_bfloat16()) : append(float(0)), "paged append");
+  return launched(dtype == ONE_DTYPE_F32   ? append(float(0), float(0))
+                  : x.cos && x.tables_fp32 ? append(__nv_bfloat16(), float(0))
+                                           : append(__nv_bfloat16(), __nv_bfloat16()),
+                  "paged append");
 }
 
 extern "C" int one_paged_evict(const one_paged_cache* cache, const int32_t* dst_table, int64_t dst_stride,

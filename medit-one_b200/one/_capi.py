@@ -38,6 +38,7 @@ class OneConfigC(ctypes.Structure):
 # one_paged_cache, one_paged_tokens and one_logits_rules of include/one_b200.h.
 PAGED_CACHE = struct.Struct("=QQqqQqQQq7i4x").pack
 PAGED_TOKENS = struct.Struct("=QQQ9qQQQQiii4x").pack
+PAGED_TOKENS_FP32_TABLES = struct.Struct("=QQQ9qQQQQiiii").pack  # the same, ending with tables_fp32
 LOGITS_RULES = struct.Struct("=QqQQQQQqQqiifff4x").pack
 
 

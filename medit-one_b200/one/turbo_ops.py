@@ -236,6 +236,7 @@ def turbo_paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, 
     """New tokens into a paged cache. k, v [B, Hkv, N, Dh] (any strides) go to the slots lengths[b]
     .. lengths[b] + counts[b] - 1 (counts int32 [B], default N), k rotated by cos, sin [B or 1, N, Dh]
     (apply_rotary_pos_emb_flash in fp32, rounded once) when they are given; the slots' mass becomes 0.
+    cos and sin are taken in k's dtype or in fp32; other types become fp32.
     Returns q [B, Hq, N, Dh] rotated the same way, or None without q. The caller advances lengths."""
     dt = k.dtype
     dev, cache, (b, hkv, ps, dh, mp) = _paged(k_pages, v_pages, block_table, lengths, mass, dt)
@@ -275,15 +276,19 @@ def turbo_paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, 
         out = q.new_empty((b, hq, n, dh))
         optr, qptr, qs = out.data_ptr(), q.data_ptr(), q.stride()
     cosp = sinp = 0
+    pack, tables = C.PAGED_TOKENS, ()
     if cos is not None:
-        if cos.dtype is not dt or sin.dtype is not dt or not cos.is_contiguous() or not sin.is_contiguous():
-            cos, sin = cos.to(dt).contiguous(), sin.to(dt).contiguous()
+        if cos.dtype is not dt or sin.dtype is not dt:
+            cos, sin = cos.to(_F32), sin.to(_F32)
+            pack, tables = C.PAGED_TOKENS_FP32_TABLES, (1,)
+        if not cos.is_contiguous() or not sin.is_contiguous():
+            cos, sin = cos.contiguous(), sin.contiguous()
         cosp, sinp = cos.data_ptr(), sin.data_ptr()
     k, v = _rows_last(k), _rows_last(v)
     ks, vs = k.stride(), v.stride()
     _launch(C.LIB.one_paged_append, dev, cache,
-            C.PAGED_TOKENS(k.data_ptr(), v.data_ptr(), qptr, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], qs[0], qs[1], qs[2],
-                           cosp, sinp, cptr, optr, n, hq, cb))
+            pack(k.data_ptr(), v.data_ptr(), qptr, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], qs[0], qs[1], qs[2],
+                 cosp, sinp, cptr, optr, n, hq, cb, *tables))
     return out
 
 

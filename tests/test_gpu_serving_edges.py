@@ -50,3 +50,30 @@ def test_generate_takes_the_repetition_penalty_of_a_generation_config():
         model.generate(ids, max_new_tokens=2, repetition_penalty=0.0)
     model.generation_config = config
     assert torch.equal(model.generate(ids, max_new_tokens=16), want)
+
+
+# ------------------------------------------------------------------ rotation tables
+@pytest.mark.parametrize("tables", [F32, torch.float64, torch.float16, BF], ids=["fp32", "fp64", "fp16", "bf16"])
+@pytest.mark.parametrize("dt", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("dh,n,shared", [(64, 40, False), (80, 7, True), (40, 5, False), (128, 1, True), (8, 3, False)])
+def test_append_rotates_by_tables_of_any_type_in_fp32(dh, n, shared, dt, tables):
+    """Two products of fp32 factors and their sum, one rounding: 2^-22 of the products' magnitudes
+    (three roundings, and one of the tables for fp64), half a step of the result."""
+    gen = torch.Generator().manual_seed(dh + n)
+    hkv, hq, page, start = 2, 3, 16, [5, 0]
+    k, v, table, _ = P.make_cache([s + n for s in start], hkv, dh, page, dt, gen, junk=0.0)
+    new = [torch.randn(2, h, n, dh, generator=gen).to(dt) for h in (hkv, hkv, hq)]
+    ang = 6.28 * torch.rand(1 if shared else 2, n, dh, generator=gen, dtype=torch.float64)
+    cos, sin = ang.cos().to(tables), ang.sin().to(tables)
+    dk, dv, dtab, dl = k.cuda(), v.cuda(), table.cuda(), torch.tensor(start, dtype=torch.int32).cuda()
+    got = ops().turbo_paged_append(new[0].cuda(), new[1].cuda(), dk, dv, dtab, dl, cos=cos.cuda(), sin=sin.cuda(), q=new[2].cuda())
+    u, h = torch.finfo(dt).eps / 2, dh // 2
+
+    def check(x, src):
+        want, a = P.rotate(src, cos, sin), src.double().abs()
+        mag = a * cos.double().abs()[:, None] + torch.cat([a[..., h:], a[..., :h]], -1) * sin.double().abs()[:, None]
+        err = (x.cpu().double() - want).abs() - u * want.abs() - 2.0 ** -22 * mag
+        assert bool((err <= 0).all()), float(err.max())
+
+    check(got, new[2])
+    check(torch.stack([P.rows(dk.cpu(), table, b, s + n)[:, s:] for b, s in enumerate(start)]), new[0])
