@@ -228,6 +228,32 @@ def _rows_last(t):
     return t if t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
 
 
+def _span(t):
+    """[first, last) byte of a tensor with elements."""
+    at, es = t.data_ptr(), t.element_size()
+    return at, at + es * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+
+
+def _row_starts(t):
+    at = torch.zeros(1, dtype=torch.int64)
+    for n, s in zip(t.shape[:-1], t.stride()[:-1]):
+        at = (at[:, None] + s * torch.arange(n)).flatten()
+    return t.data_ptr() + t.element_size() * at
+
+
+def _rows_overlap(x, y):
+    """Whether rows (along the last dimension, each contiguous) of two tensors share memory."""
+    if not x.numel() or not y.numel():
+        return False
+    (x0, x1), (y0, y1) = _span(x), _span(y)
+    if x0 >= y1 or y0 >= x1:
+        return False
+    xs, ys = _row_starts(x), _row_starts(y).sort().values
+    wx, wy = x.shape[-1] * x.element_size(), y.shape[-1] * y.element_size()
+    i = torch.searchsorted(ys, xs - wy, right=True)  # the first row of y that ends behind the start of x's
+    return bool(((i < ys.numel()) & (ys[i.clamp(max=ys.numel() - 1)] < xs + wx)).any())
+
+
 def turbo_paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                        block_table: torch.Tensor, lengths: torch.Tensor, cos: Optional[torch.Tensor] = None,
                        sin: Optional[torch.Tensor] = None, q: Optional[torch.Tensor] = None,
@@ -314,11 +340,11 @@ def turbo_paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch
         raise ValueError("all tensors must be on one device")
     if out is not None and (out.shape != shape or out.dtype is not dt or not out.is_contiguous()):
         raise ValueError(f"out must be contiguous {tuple(shape)} in {dt}")
-    if out is q:
-        raise ValueError("out must not be q")
+    q = _rows_last(q)
+    if out is not None and _rows_overlap(q, out):
+        raise ValueError("out must not overlap q")
     _cuda(dev, q)
     hq = shape[1]
-    q = _rows_last(q)
     if out is None:
         out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(shape)
     nws = _attention_workspace(b, hq, hkv, dh, ps, mp, C.dtype_code(dt), mass is not None)

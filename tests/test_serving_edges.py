@@ -22,3 +22,22 @@ def test_packed_tokens_with_fp32_tables():
     plain, fp32 = C.PAGED_TOKENS(*range(1, 20)), C.PAGED_TOKENS_FP32_TABLES(*range(1, 20), 1)
     assert len(plain) == len(fp32) == ctypes.sizeof(Tokens) and Tokens.reserved.offset == len(plain) - 4
     assert plain[-4:] == bytes(4) and fp32 == plain[:-4] + (1).to_bytes(4, "little")
+
+
+def test_attention_refuses_an_out_that_overlaps_q():
+    k, v, t, n = cache()
+    buf = torch.zeros(4096, dtype=torch.bfloat16)
+    q = buf[:512].view(2, 4, 1, 64)
+    f = T.turbo_paged_attention
+    overlap(f, q, k, v, t, n, out=q.view(2, 4, 1, 64))
+    overlap(f, q, k, v, t, n, out=buf[8:520].view(2, 4, 1, 64))
+    overlap(f, q, k, v, t, n, out=buf[504:1016].view(2, 4, 1, 64))
+    rows = buf.view(2, 4, 8, 64)[:, :, 1:2]  # rows of a wider projection
+    overlap(f, rows, k, v, t, n, out=buf[:512].view(2, 4, 1, 64))
+    for out in (buf[512:1024], buf[3584:]):  # beside q, and behind its rows
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            f(q, k, v, t, n, out=out.view(2, 4, 1, 64))
+    apart = buf.as_strided((2, 4, 1, 64), (2048, 64, 64, 1))  # rows 0 .. 255 and 2048 .. 2303
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        f(apart, k, v, t, n, out=buf[256:768].view(2, 4, 1, 64))
+    overlap(f, apart, k, v, t, n, out=buf[1600:2112].view(2, 4, 1, 64))
