@@ -336,9 +336,9 @@ typedef struct one_logits_rules {
  * on and the row's penalties r, p, f,
  *   z = x; z = z > 0 ? z / r : z * r if the token stands anywhere in the history;
  *   z -= f * c + (c > 0 ? p : 0); z += bias; z = -inf where the token's mask bit is 0.
- * out fp32 [batch][out_ld] (may be the logits themselves when they are fp32). best int32 [batch] or
- * NULL: the token of the largest score, the lowest among equals; NaN is never chosen; 0 when nothing
- * is left. Replaces transformers' RepetitionPenaltyLogitsProcessor and its like in
+ * out fp32 [batch][out_ld] (may be the logits themselves when they are fp32; must not overlap them
+ * otherwise). best int32 [batch] or NULL: the token of the largest score, the lowest among equals; NaN
+ * is never chosen; 0 when nothing is left. Replaces transformers' RepetitionPenaltyLogitsProcessor and its like in
  * GenerationMixin.generate (one/modeling_one.py:845). */
 int one_process_logits(const one_logits_rules* rules, const void* logits, int64_t ld, int32_t batch, int32_t vocab,
                        int32_t dtype, float* out, int64_t out_ld, int32_t* best, void* stream);

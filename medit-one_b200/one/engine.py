@@ -19,7 +19,7 @@ import torch
 
 from . import _capi as C
 from .initialization import param_specs
-from .turbo_ops import _launch
+from .turbo_ops import _launch, _rows_overlap
 
 
 def rope_inv_freq(head_dim: int, theta: float) -> torch.Tensor:
@@ -373,13 +373,15 @@ def process_logits(logits: torch.Tensor, history: Optional[torch.Tensor] = None,
     (repetition_penalty r); z -= frequency_penalty * c + presence_penalty * (c > 0); z += bias (fp32
     [V] or [B, V]); z = -inf where token_mask (pack_token_mask's words, [W] or [B, W]) has a 0. Each
     penalty is a number or fp32 [B]. Returns the scores fp32 [B, V] (`out`, which may be the logits
-    when they are fp32), and with return_argmax also int32 [B]: the token of the largest score, the
-    lowest among equals; NaN is never chosen; 0 when nothing is left."""
+    when they are fp32 and must not overlap them otherwise), and with return_argmax also int32 [B]: the
+    token of the largest score, the lowest among equals; NaN is never chosen; 0 when nothing is left."""
     shape = logits.shape
     if len(shape) != 2:
         raise C.OneError("process_logits takes logits [batch, vocab]")
     B, V = shape
     dev = logits.get_device()
+    if V > 1 and logits.stride(1) != 1:
+        logits = logits.contiguous()
     used = []
     rep, rep1 = _penalty(repetition_penalty, "repetition_penalty", B, used)
     pres, pres1 = _penalty(presence_penalty, "presence_penalty", B, used)
@@ -410,6 +412,10 @@ def process_logits(logits: torch.Tensor, history: Optional[torch.Tensor] = None,
     if out is not None:
         if out.shape != shape or out.dtype is not torch.float32 or (V > 1 and out.stride(1) != 1):
             raise C.OneError(f"out must be fp32 [{B}, {V}] with contiguous rows")
+        in_place = (out.data_ptr() == logits.data_ptr() and logits.dtype is torch.float32
+                    and (B == 1 or out.stride(0) == logits.stride(0)))
+        if not in_place and _rows_overlap(logits, out):
+            raise C.OneError("out must be the logits in place or not overlap them")
         used.append(out)
     code = C.dtype_code(logits.dtype)
     if dev < 0:
@@ -417,8 +423,6 @@ def process_logits(logits: torch.Tensor, history: Optional[torch.Tensor] = None,
     for t in used:
         if t.get_device() != dev:
             raise C.OneError(f"all tensors must be on one device, got {logits.device} and {t.device}")
-    if V > 1 and logits.stride(1) != 1:
-        logits = logits.contiguous()
     if out is None:
         out = logits.new_empty(shape, dtype=torch.float32)
     best, best_ptr = None, 0

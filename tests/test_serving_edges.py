@@ -41,3 +41,16 @@ def test_attention_refuses_an_out_that_overlaps_q():
     with pytest.raises(RuntimeError, match="no CPU path"):
         f(apart, k, v, t, n, out=buf[256:768].view(2, 4, 1, 64))
     overlap(f, apart, k, v, t, n, out=buf[1600:2112].view(2, 4, 1, 64))
+
+
+def test_logits_refuse_an_out_that_overlaps_them_otherwise_than_in_place():
+    buf = torch.zeros(3, 100)
+    x = buf[:, :40]
+    overlap(process_logits, x, out=buf[:, 1:41])
+    overlap(process_logits, x, out=buf[:, 39:79])
+    overlap(process_logits, buf[:2, :40], out=buf[1:, :40])
+    half = buf.view(torch.bfloat16)  # the same bytes, read as 200 a row
+    overlap(process_logits, half[:, :40], out=buf[:, :40])
+    for out in (x, buf[:, 40:80], buf[:, :40].view(3, 40), torch.zeros(3, 40)):  # in place, between the rows, elsewhere
+        with pytest.raises(C.OneError, match="CUDA"):
+            process_logits(x, out=out)
