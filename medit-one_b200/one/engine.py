@@ -380,7 +380,7 @@ def process_logits(logits: torch.Tensor, history: Optional[torch.Tensor] = None,
         raise C.OneError("process_logits takes logits [batch, vocab]")
     B, V = shape
     dev = logits.get_device()
-    if V > 1 and logits.stride(1) != 1:
+    if (V > 1 and logits.stride(1) != 1) or (B > 1 and logits.stride(0) < V):  # rows that are not whole or not apart
         logits = logits.contiguous()
     used = []
     rep, rep1 = _penalty(repetition_penalty, "repetition_penalty", B, used)
@@ -394,7 +394,7 @@ def process_logits(logits: torch.Tensor, history: Optional[torch.Tensor] = None,
         if len(hshape) != 2 or hshape[0] != B or history.dtype not in (torch.int32, torch.int64):
             raise C.OneError(f"history must be int32 or int64 [{B}, T]")
         T, hb = hshape[1], history.element_size()
-        if T > 1 and history.stride(1) != 1:
+        if (T > 1 and history.stride(1) != 1) or (B > 1 and history.stride(0) < T):
             history = history.contiguous()
         hld = history.stride(0) if B > 1 else T
         hptr = history.data_ptr()

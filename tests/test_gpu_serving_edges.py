@@ -77,3 +77,19 @@ def test_append_rotates_by_tables_of_any_type_in_fp32(dh, n, shared, dt, tables)
 
     check(got, new[2])
     check(torch.stack([P.rows(dk.cpu(), table, b, s + n)[:, s:] for b, s in enumerate(start)]), new[0])
+
+
+@pytest.mark.parametrize("dt", [BF, F32], ids=["bf16", "fp32"])
+def test_logits_and_history_shared_by_the_rows(dt):
+    from one.engine import process_logits
+    gen = torch.Generator().manual_seed(2)
+    x = torch.randn(1, 777, generator=gen).to(dt)
+    hist = torch.randint(0, 777, (1, 30), generator=gen)
+    rep = torch.tensor([1.5, 1.0, 2.0, 0.5])
+    dx, dh, dr = x.cuda(), hist.cuda(), rep.cuda()
+    want = process_logits(dx.repeat(4, 1), dh.repeat(4, 1), repetition_penalty=dr)
+    assert torch.equal(process_logits(dx.expand(4, -1), dh.expand(4, -1), repetition_penalty=dr), want)
+    assert torch.equal(process_logits(dx.repeat(4, 1), dh.expand(4, -1), repetition_penalty=dr), want)
+    one = torch.tensor([[5]], device="cuda")
+    want = process_logits(dx.repeat(4, 1), one.repeat(4, 1), repetition_penalty=dr)
+    assert torch.equal(process_logits(dx.expand(4, -1), one.expand(4, -1), repetition_penalty=dr), want)
