@@ -429,6 +429,8 @@ def process_logits(logits: torch.Tensor, history: Optional[torch.Tensor] = None,
     if return_argmax:
         best = logits.new_empty((B,), dtype=torch.int32)
         best_ptr = best.data_ptr()
+    if B == 0:
+        return (out, best) if return_argmax else out
     rules = C.LOGITS_RULES(hptr, hld, sptr, rep, pres, freq, bptr, bld, mptr, mld, T, hb, rep1, pres1, freq1)
     _launch(C.LIB.one_process_logits, dev, rules, logits.data_ptr(), logits.stride(0) if B > 1 else V, B, V, code,
             out.data_ptr(), out.stride(0) if B > 1 else V, best_ptr)

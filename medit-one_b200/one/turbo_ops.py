@@ -301,6 +301,8 @@ def turbo_paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, 
         q = _rows_last(q)
         out = q.new_empty((b, hq, n, dh))
         optr, qptr, qs = out.data_ptr(), q.data_ptr(), q.stride()
+    if b == 0 or n == 0:
+        return out
     cosp = sinp = 0
     pack, tables = C.PAGED_TOKENS, ()
     if cos is not None:
@@ -347,6 +349,8 @@ def turbo_paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch
     hq = shape[1]
     if out is None:
         out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(shape)
+    if b == 0:
+        return out
     nws = _attention_workspace(b, hq, hkv, dh, ps, mp, C.dtype_code(dt), mass is not None)
     ws = q.new_empty(nws, dtype=torch.uint8) if nws else None
     qs = q.stride()
@@ -378,13 +382,15 @@ def turbo_paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table:
     width = dp * ps
     if width < budget:
         raise ValueError(f"dst_block_table holds {width} slots, fewer than the budget {budget}")
-    if d.data_ptr() == block_table.data_ptr():
+    if b and d.data_ptr() == block_table.data_ptr():
         raise ValueError("survivors go to other pages: dst_block_table is block_table")
     if d.get_device() != dev:
         raise ValueError("all tensors must be on one device")
     _cuda(dev, k_pages)
     mass_out = mass.new_empty((b, hkv, width))
     kept = d.new_empty((b, hkv, budget))
+    if b == 0:
+        return mass_out, kept
     _launch(C.LIB.one_paged_evict, dev, cache, d.data_ptr(), d.stride(0) if b > 1 else dp, dp, budget, recent, sink,
             mass_out.data_ptr(), width, kept.data_ptr())
     return mass_out, kept

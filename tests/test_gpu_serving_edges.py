@@ -93,3 +93,32 @@ def test_logits_and_history_shared_by_the_rows(dt):
     one = torch.tensor([[5]], device="cuda")
     want = process_logits(dx.repeat(4, 1), one.repeat(4, 1), repetition_penalty=dr)
     assert torch.equal(process_logits(dx.expand(4, -1), one.expand(4, -1), repetition_penalty=dr), want)
+
+
+# ------------------------------------------------------------------ empty, shared rows
+@pytest.mark.parametrize("dt", [BF, F32], ids=["bf16", "fp32"])
+def test_empty_batches_and_no_new_tokens(dt):
+    from one.engine import process_logits
+    gen = torch.Generator().manual_seed(1)
+    k, v, table, ln = (x.cuda() for x in P.make_cache([20, 3], 2, 64, 16, dt, gen, junk=0.0))
+    before, mass = k.clone(), torch.rand(2, 2, 32, device="cuda")
+    m0 = mass.clone()
+    q = torch.randn(2, 4, 0, 64, device="cuda").to(dt)
+    got = ops().turbo_paged_append(q[:, :2], q[:, :2], k, v, table, ln, q=q, mass=mass)
+    assert got.shape == (2, 4, 0, 64) and got.dtype == dt
+    assert ops().turbo_paged_append(q[:, :2], q[:, :2], k, v, table, ln) is None
+    cos = torch.zeros(1, 0, 64, device="cuda")
+    assert ops().turbo_paged_append(q[:, :2], q[:, :2], k, v, table, ln, cos=cos, sin=cos, q=q).shape == q.shape
+    none, zero = table[:0], ln[:0]
+    one = torch.randn(0, 4, 1, 64, device="cuda").to(dt)
+    assert ops().turbo_paged_append(one[:, :2], one[:, :2], k, v, none, zero, q=one).shape == one.shape
+    assert ops().turbo_paged_attention(one, k, v, none, zero, mass=mass[:0]).shape == one.shape
+    out = torch.empty_like(one)
+    assert ops().turbo_paged_attention(one, k, v, none, zero, out=out) is out
+    mo, kept = ops().turbo_paged_evict(k, v, none, none, zero, mass[:0], 32)
+    assert mo.shape == (0, 2, 32) and kept.shape == (0, 2, 32) and kept.dtype == torch.int32
+    x = torch.zeros(0, 100, device="cuda").to(dt)
+    s, best = process_logits(x, torch.zeros(0, 5, dtype=torch.int64, device="cuda"), repetition_penalty=1.5, return_argmax=True)
+    assert s.shape == (0, 100) and s.dtype == F32 and best.shape == (0,) and best.dtype == torch.int32
+    assert process_logits(x).shape == (0, 100)
+    assert torch.equal(k, before) and torch.equal(mass, m0)

@@ -54,3 +54,12 @@ def test_logits_refuse_an_out_that_overlaps_them_otherwise_than_in_place():
     for out in (x, buf[:, 40:80], buf[:, :40].view(3, 40), torch.zeros(3, 40)):  # in place, between the rows, elsewhere
         with pytest.raises(C.OneError, match="CUDA"):
             process_logits(x, out=out)
+
+
+def test_empty_inputs_have_no_cpu_path_either():
+    k, v, t, n = cache()
+    q = torch.zeros(0, 4, 1, 64, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        T.turbo_paged_attention(q, k, v, t[:0], n[:0])
+    with pytest.raises(C.OneError, match="CUDA"):
+        process_logits(torch.zeros(0, 10))
