@@ -59,7 +59,7 @@ ONE_DEVINL int pa_tiles(const PagedCache& c, int b) {
   return (paged_length(c, b, SITE_PAGED_ATTN) + TILE - 1) / TILE;
 }
 
-// Tiles in the list (the host bounds them to 2^31). Every warp computes them for itself.
+// Tiles in the list (the host keeps them, rounded up to shares, below 2^31). Every warp computes them for itself.
 template <int TILE>
 ONE_DEVINL int pa_total(const PagedAttn& p) {
   int n = 0;

@@ -241,7 +241,8 @@ extern "C" int one_paged_attention(const one_paged_cache* cache, const void* q, 
   float* mass = cache->mass;
   if (hq < 1 || hq % hkv) return fail(ONE_ERR_INVALID, "paged attention: the query heads must be a multiple of the kv heads");
   const int64_t slots = (int64_t)cache->max_pages * page_size;
-  if ((int64_t)b * hq > 0x3fffffff || (int64_t)b * hq * (slots / 64 + 1) > 0x7fffffff)
+  // tiles, and the list's length rounded up to equal shares, in 31 bits
+  if ((int64_t)b * hq > 0x3fffffff || (int64_t)b * hq * (slots / 64 + 1) > 0x7fffffff - kMaxSms * kPaPerSm)
     return fail(ONE_ERR_UNSUPPORTED, "paged attention: too many rows");
   const size_t need = one_paged_attention_workspace_bytes(b, hq, hkv, dh, page_size, cache->max_pages, dtype, mass != nullptr);
   if (need && (!workspace || workspace_bytes < need)) return fail(ONE_ERR_INVALID, "workspace too small");

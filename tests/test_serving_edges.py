@@ -63,3 +63,13 @@ def test_empty_inputs_have_no_cpu_path_either():
         T.turbo_paged_attention(q, k, v, t[:0], n[:0])
     with pytest.raises(C.OneError, match="CUDA"):
         process_logits(torch.zeros(0, 10))
+
+
+@pytest.mark.skipif(cuda_ok(), reason="its addresses are no memory: where the call were not refused it must not launch")
+def test_attention_refuses_lists_that_its_shares_would_carry_past_31_bits():
+    """2^31 - 383 tiles rounded up to equal shares pass 2^31."""
+    heads, tiles = 255, 8421503
+    big = dict(CACHE, B=heads, hkv=1, ps=64, mp=tiles, ts=tiles, ks=64 * 64, vs=64 * 64)
+    call = lambda **c: C.LIB.one_paged_attention(cache_of(c), A, 64, 64, 1, 0.1, B_, A, 1 << 40, 0)
+    assert heads * (tiles + 1) <= 0x7fffffff and heads * tiles + 443 > 0x7fffffff
+    assert call(**big) == C.ONE_ERR_UNSUPPORTED
