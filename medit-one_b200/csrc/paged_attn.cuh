@@ -220,6 +220,7 @@ struct PaBf16 {
   static constexpr int kGroup = 64 * DH;               // bytes of a group's keys and values
   static constexpr int kStages = 2, kStagesFew = 3;    // where CTAs fill the SMs; where they are few
   static constexpr int kExtra = 0;                     // further shared bytes per warp
+  ONE_DEVINL static float weight(float x) { return ex2_approx(x); }  // 2^x as consume computes it
   uint32_t qa[WIDE ? 2 : 1][KC][4];
   float o[NT][4];
   float m[2], l[2];  // rows r and r + 8
@@ -437,6 +438,7 @@ struct PaF32 {
   static constexpr int kValues = 64 * DH;
   static constexpr int kStages = DH == 32 ? 4 : DH == 96 ? 2 : 3, kStagesFew = kStages;
   static constexpr int kExtra = ROWS * DH * 4 + 16 * ROWS * 4;  // q [ROWS][DH], weights [16][ROWS]
+  ONE_DEVINL static float weight(float x) { return exp2f(x); }   // 2^x as consume computes it
   float o[ROWS][VC];
   float m, l;  // of head c
   float *qs, *ps;
@@ -880,7 +882,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, MODE>::kPerSm) paged_
       float* mass = p.mass + ((int64_t)cur.b * c.Hkv + kv) * p.mass_width;
       for (int t = first * TILE + threadIdx.x; t < min(last * TILE, cur.len); t += blockDim.x) {
         float a = 0.f;
-        for (int g = 0; g < rows; ++g) a += ex2_approx(p.scores[(hq0 + g) * p.score_ld + t] - joint[2 * g]) * joint[2 * g + 1];
+        for (int g = 0; g < rows; ++g) a += E::weight(p.scores[(hq0 + g) * p.score_ld + t] - joint[2 * g]) * joint[2 * g + 1];
         mass[t] += a;
       }
     }
@@ -1005,10 +1007,10 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
       for (int g = 0; g < gn; ++g) {
         const float4 s = *reinterpret_cast<const float4*>(p.scores + (row0 + gb + g) * p.score_ld + t);
         const float M = fin[0][g], inv = fin[1][g];
-        add[0] += ex2_approx(s.x - M) * inv;
-        add[1] += ex2_approx(s.y - M) * inv;
-        add[2] += ex2_approx(s.z - M) * inv;
-        add[3] += ex2_approx(s.w - M) * inv;
+        add[0] += E::weight(s.x - M) * inv;
+        add[1] += E::weight(s.y - M) * inv;
+        add[2] += E::weight(s.z - M) * inv;
+        add[3] += E::weight(s.w - M) * inv;
       }
     }
   }

@@ -122,3 +122,27 @@ def test_empty_batches_and_no_new_tokens(dt):
     assert s.shape == (0, 100) and s.dtype == F32 and best.shape == (0,) and best.dtype == torch.int32
     assert process_logits(x).shape == (0, 100)
     assert torch.equal(k, before) and torch.equal(mass, m0)
+
+
+# ------------------------------------------------------------------ weights
+@pytest.mark.parametrize("hkv,g,n", [(1, 1, 40), (1, 4, 300), (2, 3, 9000), (40, 1, 2000)])
+def test_fp32_weights_below_the_normal_range(hkv, g, n):
+    """A slot 2^130 times lighter than the heaviest adds 2^-130 (a denormal) to its mass."""
+    k = torch.zeros(1, hkv, n, 64)
+    k[..., 0] = -130.0
+    k[:, :, 3, 0] = 0.0
+    page = 16
+    pages = -(-n // page)
+    pool = torch.zeros(pages, hkv, page, 64)
+    kp = torch.nn.functional.pad(k, (0, 0, 0, pages * page - n)).view(hkv, pages, page, 64).transpose(0, 1).contiguous().cuda()
+    q = torch.zeros(1, hkv * g, 1, 64)
+    q[..., 0] = 1.0
+    mass = torch.zeros(1, hkv, pages * page, device="cuda")
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").view(1, -1)
+    ops().turbo_paged_attention(q.cuda(), kp, pool.cuda(), table, torch.tensor([n], dtype=torch.int32, device="cuda"),
+                                scale_factor=math.log(2.0), mass=mass)
+    got = mass.cpu().double()[0, :, :n]
+    want = torch.full((hkv, n), g * 2.0 ** -130, dtype=torch.float64)
+    want[:, 3] = g
+    # one step of the denormals; an exponent of 130 is off by 130 * 2^-23 at most, the weight by 2^-16 of itself
+    assert bool(((got - want).abs() <= g * 2.0 ** -149 + 2.0 ** -15 * want).all())
