@@ -295,8 +295,9 @@ ONE_DEVINL uint32_t mass_key(float f) {
 // (200 x 16 heads of 4096 slots to 512: 251 us in all with 16, 218 with 8). KPT = 0, for tables of more than
 // 32768 slots: the masses are read again in each pass (16 x 12 heads of 30000 to 2048: 102 us, 84 with 64).
 // CTAs per SM as the keys' registers allow: 3 rather than 2 up to KPT = 8 (100 x 16 heads of 781 slots to
-// 200, 80 dims: 74.6 -> 70.3 us), 2 rather than 1 up to 32, which spills 8 bytes (16 x 12 heads of 16000 to
-// 2048: 60 us; with 64 keys and one CTA 78).
+// 200, 80 dims: 74.6 -> 70.3 us), 2 rather than 1 up to 32 (16 x 12 heads of 16000 to 2048: 60 us; with 64
+// keys and one CTA 78), although the 64 registers of two spill: 8 bytes with KPT = 32, and with MOVE 176
+// (KPT = 32) and 48 (KPT = 16).
 constexpr int kEvictThreads = 512;
 constexpr int kEvictWarps = kEvictThreads / 32;
 constexpr int kEvictList = 512;  // places listed at a time, one per thread

@@ -365,7 +365,9 @@ extern "C" int one_paged_evict(const one_paged_cache* cache, const int32_t* dst_
   cudaStream_t st = (cudaStream_t)stream;
   const int64_t slots = (int64_t)cache->max_pages * page_size, heads = (int64_t)b * hkv;
   const int64_t parts = (budget + 255) / 256, per_bh = (mass_out_width + kMovePlaces - 1) / kMovePlaces;
-  const bool one_launch = heads * parts <= 2 * num_sms();  // two CTAs per SM
+  // where the CTAs fit the SMs at once: two per SM, one of those that hold 64 keys per thread (192 CTAs of
+  // those, 48 heads of 30000 slots to 1000: 49 us in one launch, 29 in two; device times)
+  const bool one_launch = heads * parts <= (slots > 16384 && slots <= 32768 ? 1 : 2) * num_sms();
   if (heads * std::max(parts, per_bh) > 0x7fffffff) return fail(ONE_ERR_UNSUPPORTED, "paged evict: too many rows");
   const int pieces = dh * elem_bytes(dtype) / 16;
   auto evict = [&](auto keys) {
