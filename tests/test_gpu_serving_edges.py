@@ -146,3 +146,98 @@ def test_fp32_weights_below_the_normal_range(hkv, g, n):
     want[:, 3] = g
     # one step of the denormals; an exponent of 130 is off by 130 * 2^-23 at most, the weight by 2^-16 of itself
     assert bool(((got - want).abs() <= g * 2.0 ** -149 + 2.0 ** -15 * want).all())
+
+
+WIDE = [([200], 1, 1, 64, 16), ([0, 700, 33], 4, 3, 64, 16), ([1500, 2, 90, 0], 2, 8, 128, 48), ([5], 1, 20, 32, 7)]
+
+
+@pytest.mark.parametrize("dt", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("with_mass", [False, True], ids=["plain", "mass"])
+@pytest.mark.parametrize("lens,hkv,g,dh,page", WIDE)
+def test_attention_in_a_table_for_32768_slots(lens, hkv, g, dh, page, with_mass, dt):
+    from test_gpu_paged import check_attention, cuda
+    gen = torch.Generator().manual_seed(9)
+    k, v, table, ln = P.make_cache(lens, hkv, dh, page, dt, gen, width=32768 // page)
+    q = torch.randn(len(lens), hkv * g, 1, dh, generator=gen).to(dt)
+    mass0 = torch.rand(len(lens), hkv, table.shape[1] * page, generator=gen) if with_mass else None
+    dq, dk, dv, dtab, dl, dm = cuda(q, k, v, table, ln, mass0)
+    got = ops().turbo_paged_attention(dq, dk, dv, dtab, dl, mass=dm)
+    check_attention(got, q, k, v, table, ln, dh ** -0.5, dt, dm, mass0)
+    if with_mass:
+        for b, n in enumerate(lens):
+            assert torch.equal(dm[b, :, n:].cpu(), mass0[b, :, n:])
+
+
+@pytest.mark.parametrize("width", [4096, 32768, 40000], ids=str)
+@pytest.mark.parametrize("b,hkv", [(2, 3), (20, 40)])
+def test_evict_and_append_in_a_wide_table(b, hkv, width):
+    gen = torch.Generator().manual_seed(b)
+    page, dh, budget, recent, sink = 16, 16, 100, 20, 4
+    lens = [(130 + 37 * i) % 300 for i in range(b)]
+    k, v, table, ln = P.make_cache([n + 1 for n in lens], hkv, dh, page, BF, gen, width=width // page, spare=b * 7, junk=3.0)
+    free = [p for p in range(k.shape[0]) if p not in set(table.flatten().tolist())]
+    to = torch.full((b, width // page), -1, dtype=torch.int32)
+    for i in range(b):
+        to[i, :7] = torch.tensor(free[7 * i:7 * i + 7], dtype=torch.int32)
+    mass = torch.rand(b, hkv, width, generator=gen)
+    dk, dv, dtab, dto, dm = (x.cuda() for x in (k, v, table, to, mass))
+    dl = torch.tensor(lens, dtype=torch.int32).cuda()
+    new = torch.randn(b, hkv, 1, dh, generator=gen).to(BF)
+    ops().turbo_paged_append(new.cuda(), new.cuda(), dk, dv, dtab, dl, mass=dm)
+    for i, n in enumerate(lens):
+        assert torch.equal(dk[int(table[i, n // page]), :, n % page].cpu(), new[i, :, 0])
+        mass[i, :, n] = 0
+    assert torch.equal(dm.cpu(), mass)
+    mo, kept = ops().turbo_paged_evict(dk, dv, dtab, dto, dl + 1, dm, budget, recent=recent, sink=sink)
+    ck, src = dk.cpu(), kept.cpu()
+    assert mo.shape == (b, hkv, width) and float(mo[..., budget:].abs().max()) == 0.0
+    for i, n in enumerate(lens):
+        for h in range(hkv):
+            s = P.evict(mass[i, h], n + 1, budget, recent, sink)
+            assert src[i, h].tolist() == s + [-1] * (budget - len(s))
+            s, d = torch.tensor(s), torch.arange(len(s))
+            assert torch.equal(ck[to[i].long()[d // page], h, d % page], ck[table[i].long()[s // page], h, s % page])
+            assert torch.equal(mo[i, h, :len(s)].cpu(), mass[i, h][s])
+
+
+FIRST = """
+import sys
+sys.path[:0] = sys.argv[1:3]
+import torch
+import paged_util as P
+from one import turbo_ops as T
+from one.engine import process_logits
+gen = torch.Generator().manual_seed(0)
+k, v, t, n = (x.cuda() for x in P.make_cache([900, 40], 2, 64, 16, torch.bfloat16, gen, spare=80, junk=0.0))
+free = [p for p in range(k.shape[0]) if p not in set(t.flatten().tolist())]
+to = torch.tensor(free[:16], dtype=torch.int32).view(2, 8).cuda()
+q = torch.randn(2, 4, 1, 64, generator=gen).bfloat16().cuda()
+mass = torch.rand(2, 2, t.shape[1] * 16, device="cuda")
+x, hist = torch.randn(2, 5000, device="cuda"), torch.randint(0, 5000, (2, 9), device="cuda")
+long = torch.arange(4, dtype=torch.int32, device="cuda").repeat(2, 512)
+m = torch.tensor([20000, 5], dtype=torch.int32, device="cuda")
+last = n - 1
+calls = [lambda: T.turbo_paged_append(q[:, :2], q[:, :2], k, v, t, last, q=q),
+         lambda: T.turbo_paged_attention(q, k, v, t, n, mass=mass.clone()),
+         lambda: T.turbo_paged_attention(q, k, v, long, m),
+         lambda: T.turbo_paged_evict(k, v, t, to, n, mass, 128)[1],
+         lambda: process_logits(x, hist, repetition_penalty=1.5)]
+torch.cuda.synchronize()
+graphs = []
+for f in calls:
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = f()
+    graphs.append((g, got))
+for (g, got), f in zip(graphs, calls):
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, f())
+assert T.ops_error() == (0, 0)
+print("captured")
+"""
+
+
+def test_the_first_call_of_a_process_may_be_captured():
+    done = subprocess.run([sys.executable, "-c", FIRST, PKG, os.path.join(REPO, "tests")], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "captured" in done.stdout, done.stderr[-2000:]
