@@ -250,9 +250,9 @@ int one_sample_tokens(const void* logits, int32_t batch, int32_t vocab, int32_t 
  * order: slot t of sequence i is row t % page_size of page block_table[i][t / page_size]. Entries
  * past a sequence's last used page are not read. Sequences may share pages that are only read.
  * lengths int32 [b]: slots in use (0 allowed); no call writes it, so the layers of a model share it
- * and a call can be repeated. A page number outside [0, num_pages) where one is used, a length below
- * 0 or beyond the table's slots: the rows are neither read nor written, and the error record
- * (one_ops_error) holds code 2. mass fp32 [b][hkv][mass_width], mass_width >= max_pages * page_size:
+ * and a call can be repeated. A page number outside [0, num_pages) where one is used: its rows are
+ * neither read nor written; a length below 0 or beyond the table's slots: counts as 0 or as all of
+ * them (append: stores nothing there). The error record (one_ops_error) then holds code 2. mass fp32 [b][hkv][mass_width], mass_width >= max_pages * page_size:
  * the attention weight that each slot has received; NULL where it is not kept. */
 typedef struct one_paged_cache {
   void* k_pages;

@@ -122,8 +122,10 @@ ONE_DEVINL float2 mul2(float2 a, float2 b) {
 // paged_append_any_kernel takes the rest. Sequence blockIdx.y.
 //
 // 8 prompts of up to 4096 tokens, 12 heads x 64: 68 us with one row per thread, 72 with pairs, 54 as here,
-// 51 with five CTAs per SM; without rotation it runs at the rate of a plain copy. 170 x 4 tokens of 367
-// heads x 80: 100 us one element at a time, 35 by halves.
+// 51 with five CTAs per SM (73 % of the copy rate; two thirds of the issue slots are taken, and what the
+// warps wait for most is loads: cos and sin are asked for only when the page is known); without rotation it
+// runs at the rate of a plain copy. 170 x 4 tokens of 367 heads x 80: 100 us one element at a time, 35 by
+// halves.
 constexpr int kAppendRows = 4;
 
 template <typename T, typename C, bool PAIR>

@@ -4,10 +4,11 @@
 //   o   = sum_t 2^(s_t - m) v_t / l    mass_t += 2^(s_t - m) / l, summed over a kv head's queries
 //
 // One pass over K and V with the running maximum and sum; parts of a sequence join by their (m, l, o).
-// HBM bounds it: every K and V row is read once, at 1 flop per byte and query head of a group. Measured, of
-// the measured copy rate: 64 ragged sequences up to 4096 slots, 12 heads x 64, bf16: 75 us, 84 %; 8 up to
-// 32768, 8 heads x 128 of 4 queries: 99 us, 89 %. Small batches are bound by a chain: lengths -> page
-// numbers -> rows -> softmax -> join, 4.3 us for one sequence of 200 slots.
+// HBM bounds it: every K and V row is read once per query-head tile (up to 16 query heads in bf16, 4 in
+// fp32), at 1 flop per byte and query head. Measured, of the measured copy rate: 64 ragged sequences up to
+// 4096 slots, 12 heads x 64, bf16: 75 us, 84 %; 8 up to 32768, 8 heads x 128 of 4 queries: 98 us, 90 %, of
+// 32 queries, two tiles: 184 us. Small batches are bound by a chain: lengths -> page numbers -> rows ->
+// softmax -> join, 5 us for one sequence of 200 slots, one call after the other.
 //
 // Partition. Few or short segments (a segment: one sequence's tiles of 64 slots or more for one query-head
 // tile) have a cluster of CTAs each, and one launch. Otherwise the work is the list of all segments' tiles

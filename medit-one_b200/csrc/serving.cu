@@ -146,10 +146,17 @@ int paged_cluster(int64_t segments, int64_t slots) {
   return n;
 }
 
-// Whether the segments are cut from a list. A cluster per segment has one launch and no second pass, but
-// at most 8 CTAs for a long sequence, and fewer than the SMs hold for a few. Both sides, per call: 8 x 3001
-// slots, 4 heads x 64 in fp32 (8 CTAs of 384 slots) 13.6 us by clusters, 15.3 from a list; 16 x 2500, 4 kv
-// heads (4 CTAs of 640 slots) 16.6 by clusters, 14.4 from a list.
+// Whether the segments are cut from a list. A cluster per segment has one launch and no second pass, but at
+// most 8 CTAs for a long sequence, shares as uneven as the lengths, and with weights a second look at the
+// scores by the CTAs that hold them alone. The list gains with few segments, uneven lengths and weights,
+// clusters with many even segments; 512 slots per CTA lie between. Us per call, by clusters and from a list
+// (one after the other in a graph, 64 dims, bf16 unless said):
+//   12 heads of one sequence (8 CTAs each): 1000 slots 6.4, 6.6; 2500 8.3, 7.5; 4000 9.3, 7.8; 8000 13.8, 9.9
+//   16 x 4 heads x 3 queries (4 CTAs each): 1600 slots 9.7, 10.1; 2500 13.4, 14.4; 3500 16.2, 17.3
+//     with weights: 1200 11.3, 11.5; 1600 13.4, 11.7; 2500 20.4, 17.4; fp32 1200 16.3, 18.0; 2500 25.7, 24.6
+//   16 x 12 heads (1 CTA each), ragged up to 500: 7.2, 9.4; 700 9.2, 9.6; 1024 11.8, 10.3; 2048 23.5, 16.4
+//   64 x 12 heads, ragged up to 700: 20.4, 22.6; 1024 27.3, 27.9; 2048 46.6, 45.4; 4096 86.7, 73.0; all of
+//     700: 28.0, 31.7
 bool paged_split(int64_t segments, int64_t slots) {
   const int64_t n = paged_cluster(segments, slots);
   return slots > kWhole * n;
@@ -197,10 +204,11 @@ int attend(PagedAttn& p, int cluster, cudaStream_t st) {
 }
 
 // A deeper ring costs the third CTA of an SM: taken where two per SM hold the grid at once, and clusters
-// of 4 and 8 are not placed as densely as that (36 of 8 are not, 32 are). bf16, slots as given, with the
-// deeper ring and without: 16 x 8 heads x 128, 1000 (pairs) 13.5 and 17.4 us; 37 x 8 x 128, 500 (single)
-// 12.7 and 16.6; 8 x 4 x 64, 4000 (32 clusters of 8) 10.5 and 11.6; 9 x 4 x 64, 4000 (36) 19.1 and 11.7;
-// 64 x 12 x 64, 128 (single, 768) 12.3 and 10.3; 149 x 16 x 64, 32 (2384) 26.7 and 20.5.
+// of 4 and 8 are not placed as densely as that (36 of 8 are not, 32 are). bf16, slots as given, us per call
+// one after the other in a graph, with the deeper ring and without: 16 x 8 heads x 128, 1000 (256 CTAs in
+// pairs) 15.7, 17.3; 37 x 8 x 128, 500 (296 single) 16.0, 17.2; 24 x 12 x 64, 500 (288) 10.3, 11.0; 26 x 12
+// x 64, 500 (312) 16.0, 11.6; 8 x 4 x 64, 4000 (32 clusters of 8) 11.6, 12.6; 9 x 4 x 64, 4000 (36) 21.4,
+// 13.4; 64 x 12 x 64, 128 (768) 10.1, 8.0; 149 x 16 x 64, 32 (2384) 24.7, 18.3.
 bool paged_deep(int64_t segments, int cluster) { return segments * cluster <= (cluster > 2 ? 256 : 296); }
 
 template <typename E, bool RUN>
@@ -416,7 +424,7 @@ extern "C" int one_process_logits(const one_logits_rules* rules, const void* log
   cudaStream_t st = (cudaStream_t)stream;
   // CTAs per row (at most a portable cluster) until there are two per SM, each with a few tokens per thread;
   // no more, since every CTA reads the row's whole history (256 rows of 32000 tokens, 2176 ids: 18.8 us
-  // with 1 CTA per row, 24.9 with 2; 148 rows, 500 ids: 14.1 and 10.6).
+  // with 1 CTA per row, 24.9 with 2; 148 rows, 500 ids: 14.1 and 10.6; calls back to back).
   int ctas = 1;
   while (ctas < 8 && (int64_t)batch * ctas <= num_sms() && vocab > ctas * kLogitsThreads * 8) ctas *= 2;
   const int slice = ((vocab + ctas - 1) / ctas + 31) / 32 * 32;
