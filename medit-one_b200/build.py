@@ -12,13 +12,15 @@ import hashlib
 import os
 import subprocess
 import sys
+import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "one", "libone_b200.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-lineinfo",
-         "-Xcompiler", "-fPIC", "-shared", "-diag-suppress=177"]
+         "-Xcompiler", "-fPIC", "-diag-suppress=177"]
+UNITS = ["engine", "linear_moe_noalloc", "serving"]  # compiled side by side, one library
 
 
 def _sources():
@@ -36,16 +38,26 @@ def _digest():
     return h.hexdigest()
 
 
+def _run_all(cmds, verbose):
+    """Runs the commands side by side; raises for the first that fails."""
+    if verbose:
+        print("\n".join(" ".join(c) for c in cmds), flush=True)
+    running = [subprocess.Popen(c) for c in cmds]
+    codes = [p.wait() for p in running]
+    for c, rc in zip(cmds, codes):
+        if rc:
+            raise subprocess.CalledProcessError(rc, c)
+
+
 def build(force: bool = False, verbose: bool = True) -> str:
     stamp = OUT + ".sha256"
     dig = _digest()
     if not force and os.path.exists(OUT) and os.path.exists(stamp) and open(stamp).read().strip() == dig:
         return OUT
-    cmd = [NVCC, *FLAGS, "-o", OUT, os.path.join(CSRC, "engine.cu"), os.path.join(CSRC, "linear_moe_noalloc.cu"),
-           os.path.join(CSRC, "serving.cu")]
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    subprocess.run(cmd, check=True)
+    with tempfile.TemporaryDirectory() as tmp:
+        objects = {os.path.join(tmp, name + ".o"): os.path.join(CSRC, name + ".cu") for name in UNITS}
+        _run_all([[NVCC, *FLAGS, "-c", "-o", obj, src] for obj, src in objects.items()], verbose)
+        _run_all([[NVCC, *FLAGS, "-shared", "-o", OUT, *objects]], verbose)
     with open(stamp, "w") as fh:
         fh.write(dig)
     return OUT
