@@ -311,6 +311,54 @@ int one_paged_evict(const one_paged_cache* cache, const int32_t* dst_table, int6
                     int32_t budget, int32_t recent, int32_t sink, float* mass_out, int64_t mass_out_width, int32_t* kept,
                     void* stream);
 
+/* The same operators over a paged cache held in 4 or 8 bits. A row of dh values is cut into groups of
+ * 32 (the last may be shorter), each standing for scale * code: scale = bf16(max |x| / m), m = 7 (4
+ * bits) or 127 (8 bits), code = x / scale to the nearest whole number, halves to the even one, x the
+ * value in fp32 (a rotated key: rounded to it once). Scales below 2^-100 are held as 0, with codes of
+ * 0; a group with an infinity or NaN has the scale NaN, and codes of 0: it reads as NaN.
+ *
+ * k_pages, v_pages hold num_pages pages uint8 [hkv][page_size][dh * bits / 8]: a byte is code + 128 (8
+ * bits), or code + 8 of an even dim in its low half and of the next dim in its high half (4 bits).
+ * scales holds num_pages pages bf16 [hkv][page_size][2][ceil(dh / 32)]: a slot's scales of the key, then
+ * of the value. Pages lie k_page_stride, v_page_stride bytes and scale_page_stride elements apart (no
+ * less than their size, at most 2^31 - 1); codes start on 8-byte boundaries, scales on 4-byte ones. dh a
+ * multiple of 16, at most 128; any page_size. Everything else as in one_paged_cache. */
+typedef struct one_paged_quant_cache {
+  void* k_pages;
+  void* v_pages;
+  void* scales;
+  int64_t k_page_stride, v_page_stride, scale_page_stride;
+  const int32_t* block_table;
+  int64_t table_stride;
+  const int32_t* lengths;
+  float* mass;
+  int64_t mass_width;
+  int32_t num_pages, page_size, max_pages, b, hkv, dh, bits, reserved;
+} one_paged_quant_cache;
+
+/* New tokens into the cache, quantised as they are written: as one_paged_append, of tokens in `dtype`. */
+int one_paged_quant_append(const one_paged_quant_cache* cache, const one_paged_tokens* tokens, int32_t dtype, void* stream);
+
+/* The cache's values, dense: k, v [b, hkv, n, dh] in dtype (16-byte boundaries) receive scale * code,
+ * rounded once, of the slots starts[i] .. starts[i] + n - 1 of sequence i (starts int32 [b], not
+ * negative, or NULL: 0); slots from lengths[i] on read as zeros, and so do slots without a page, which
+ * are recorded. */
+int one_paged_quant_read(const one_paged_quant_cache* cache, const int32_t* starts, int32_t n, int32_t dtype, void* k, void* v,
+                         void* stream);
+
+/* Attention of one new token per sequence, q and out in dtype: as one_paged_attention over the values that
+ * the cache stands for. */
+size_t one_paged_quant_attention_workspace_bytes(int32_t b, int32_t hq, int32_t hkv, int32_t dh, int32_t page_size,
+                                                 int32_t max_pages, int32_t dtype, int32_t with_mass);
+int one_paged_quant_attention(const one_paged_quant_cache* cache, const void* q, int64_t q_batch_stride,
+                              int64_t q_head_stride, int32_t hq, float scale, int32_t dtype, void* out, void* workspace,
+                              size_t workspace_bytes, void* stream);
+
+/* Eviction by accumulated attention weight: as one_paged_evict; codes and scales move as they are. */
+int one_paged_quant_evict(const one_paged_quant_cache* cache, const int32_t* dst_table, int64_t dst_stride,
+                          int32_t dst_max_pages, int32_t budget, int32_t recent, int32_t sink, float* mass_out,
+                          int64_t mass_out_width, int32_t* kept, void* stream);
+
 /* What one_process_logits does to a row. history [batch][history_ld]: history_len ids of
  * history_bytes = 4 or 8 bytes; ids outside [0, vocab) are padding; NULL: none. output_starts int32
  * [batch], or NULL: 0. repetition, presence, frequency: fp32 [batch], or NULL for the scalar of the

@@ -20,7 +20,7 @@ OUT = os.path.join(HERE, "one", "libone_b200.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-lineinfo",
          "-Xcompiler", "-fPIC", "-diag-suppress=177"]
-UNITS = ["engine", "linear_moe_noalloc", "serving"]  # compiled side by side, one library
+UNITS = ["engine", "linear_moe_noalloc", "serving", "serving_quant"]  # compiled side by side, one library
 
 
 def _sources():

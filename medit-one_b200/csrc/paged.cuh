@@ -15,7 +15,10 @@
 
 namespace one {
 
-enum : int { SITE_PAGED_ATTN = 41, SITE_PAGED_APPEND = 42, SITE_PAGED_EVICT = 43 };
+enum : int {
+  SITE_PAGED_ATTN = 41, SITE_PAGED_APPEND = 42, SITE_PAGED_EVICT = 43,
+  SITE_QUANT_APPEND = 44, SITE_QUANT_READ = 45, SITE_QUANT_ATTN = 46, SITE_QUANT_EVICT = 47
+};
 
 struct PagedCache {
   void* k;
@@ -59,17 +62,18 @@ struct PagedAppendParams {
 
 // The page and the row in it (head 0) of token t of sequence b; false: the token is not stored. A slot
 // beyond the table and a page outside the pool are recorded.
-ONE_DEVINL bool append_place(const PagedAppendParams& p, int b, int t, int64_t& slot, int& page, int& row) {
+ONE_DEVINL bool append_place(const PagedAppendParams& p, int b, int t, int64_t& slot, int& page, int& row,
+                             int site = SITE_PAGED_APPEND) {
   const PagedCache& c = p.c;
   if (p.counts && t >= p.counts[b]) return false;
   const int len = c.lengths[b];
   slot = (int64_t)len + t;
   if (len < 0 || slot >= (int64_t)c.max_pages * c.page_size) {
-    set_err(c.err, ERR_BAD_ARG, SITE_PAGED_APPEND);
+    set_err(c.err, ERR_BAD_ARG, site);
     return false;
   }
   const int index = (int)slot / c.page_size;
-  page = paged_page(c, c.table, b * c.table_stride, index, SITE_PAGED_APPEND);
+  page = paged_page(c, c.table, b * c.table_stride, index, site);
   row = (int)slot - index * c.page_size;
   return page >= 0;
 }
@@ -273,6 +277,9 @@ struct PagedEvictParams {
   float* mass_out;
   int64_t out_width;
   int* kept;  // [B][Hkv][budget]
+  uint32_t* scales;  // of a quantised cache: `words` words per row, pages s_stride words apart
+  int64_t s_stride;
+  int words;
 };
 
 // Rank of a mass, larger first: order-preserving bits of the float, -0 as 0, NaN below all.
@@ -310,7 +317,7 @@ struct Int {
   static constexpr int value = N;
 };
 
-template <int KPT, bool MOVE>
+template <int KPT, bool MOVE, typename U = uint4>
 __global__ void __launch_bounds__(kEvictThreads, KPT > 32 ? 1 : KPT && KPT <= 8 && !MOVE ? 3 : 2)
     paged_evict_kernel(const __grid_constant__ PagedEvictParams p, int parts, int pieces) {
   // digit counts [512][8], [4096], [2048]; the first part's room then holds the listed rows' addresses in
@@ -319,6 +326,11 @@ __global__ void __launch_bounds__(kEvictThreads, KPT > 32 ? 1 : KPT && KPT <= 8 
   static_assert(sizeof(int64_t) * 4 * kEvictList <= 4 * 4096, "addresses");
   int64_t* from = reinterpret_cast<int64_t*>(hist);
   int64_t* to = from + 2 * kEvictList;
+  constexpr bool SCALES = sizeof(U) == 8;  // a cache in 4 or 8 bits: rows of 8-byte units, and scales
+  constexpr int SITE = SCALES ? SITE_QUANT_EVICT : SITE_PAGED_EVICT;
+  // the third part's: the listed rows' scales, in words
+  int64_t* from_s = reinterpret_cast<int64_t*>(hist + 8192);
+  static_assert(sizeof(int64_t) * 2 * kEvictList <= 4 * 2048, "addresses");
   __shared__ int wsum[kEvictWarps];
   __shared__ uint32_t sh_digit[3];
   __shared__ int sh_above[3];
@@ -339,7 +351,7 @@ __global__ void __launch_bounds__(kEvictThreads, KPT > 32 ? 1 : KPT && KPT <= 8 
   uint32_t key[KPT ? KPT : 1];
 #pragma unroll
   for (int k = 0; k < KPT; ++k) key[k] = __float_as_uint(__ldg(mass + min(k * kEvictThreads + tid, slots - 1)));
-  const int n = paged_length(c, b, SITE_PAGED_EVICT), all = min(n, p.budget);
+  const int n = paged_length(c, b, SITE), all = min(n, p.budget);
   // this part's places; the last part also clears the masses behind the survivors
   const int per = (p.budget + parts - 1) / parts, beg = min(part * per, p.budget), end = min(beg + per, p.budget);
   int* kept = p.kept + bh * p.budget;
@@ -469,10 +481,10 @@ __global__ void __launch_bounds__(kEvictThreads, KPT > 32 ? 1 : KPT && KPT <= 8 
       w += v[k];
     }
   }
-  uint4* kp = (uint4*)c.k;
-  uint4* vp = (uint4*)c.v;
-  const int per16 = c.Dh / pieces, head = h * c.page_size;  // elements of 16 bytes; the head's first row in a page
-  const int64_t ks = c.k_stride / per16, vs = c.v_stride / per16;
+  U* kp = (U*)c.k;
+  U* vp = (U*)c.v;
+  const int unit = SCALES ? sizeof(U) : c.Dh / pieces, head = h * c.page_size;  // elements of a unit; the head's first row in a page
+  const int64_t ks = c.k_stride / unit, vs = c.v_stride / unit;
   const int step = MOVE ? kEvictList : p.budget;
   for (int lo = beg; lo < min(end, all); lo += step) {
     const int hi = MOVE ? min(lo + step, min(end, all)) : all;
@@ -519,19 +531,28 @@ __global__ void __launch_bounds__(kEvictThreads, KPT > 32 ? 1 : KPT && KPT <= 8 
       const int i = lo + tid, src = list[tid], si = src / c.page_size, di = i / c.page_size;
       kept[i] = src;
       mass_out[i] = row_mass[src];
-      const int ps = paged_page(c, c.table, b * c.table_stride, si, SITE_PAGED_EVICT);
-      const int pd = paged_page(c, p.dst, b * p.dst_stride, di, SITE_PAGED_EVICT);
+      const int ps = paged_page(c, c.table, b * c.table_stride, si, SITE);
+      const int pd = paged_page(c, p.dst, b * p.dst_stride, di, SITE);
       const bool there = ps >= 0 && pd >= 0;
       const int64_t sr = (int64_t)(head + src - si * c.page_size) * pieces, dr = (int64_t)(head + i - di * c.page_size) * pieces;
       from[tid] = there ? ps * ks + sr : -1;
       from[kEvictList + tid] = there ? ps * vs + sr : -1;
       to[tid] = pd * ks + dr;
       to[kEvictList + tid] = pd * vs + dr;
+      if (SCALES) {
+        from_s[tid] = ps * p.s_stride + (int64_t)(head + src - si * c.page_size) * p.words;
+        from_s[kEvictList + tid] = pd * p.s_stride + (int64_t)(head + i - di * c.page_size) * p.words;
+      }
     }
     __syncthreads();
+    if (SCALES)
+      for (int e = tid; e < (hi - lo) * p.words; e += kEvictThreads) {
+        const int place = e / p.words, w = e - place * p.words;
+        if (from[place] >= 0) p.scales[from_s[kEvictList + place] + w] = p.scales[from_s[place] + w];
+      }
     const int count = (hi - lo) * pieces;
     for (int e0 = tid; e0 < count; e0 += kEvictAhead * kEvictThreads) {
-      uint4 a[kEvictAhead], v[kEvictAhead];
+      U a[kEvictAhead], v[kEvictAhead];
       int place[kEvictAhead];
 #pragma unroll
       for (int k = 0; k < kEvictAhead; ++k) {
@@ -562,8 +583,12 @@ constexpr int kMovePlaces = 64;
 constexpr int kMoveAhead = 4;
 constexpr int kMoveThreads = 128;
 
+template <typename U = uint4>
 __global__ void __launch_bounds__(kMoveThreads) paged_move_kernel(const __grid_constant__ PagedEvictParams p, int per_bh, int pieces) {
-  __shared__ int64_t from[2][kMovePlaces], to[2][kMovePlaces];  // 16-byte units; -1: nothing to copy
+  constexpr bool SCALES = sizeof(U) == 8;
+  constexpr int SITE = SCALES ? SITE_QUANT_EVICT : SITE_PAGED_EVICT;
+  __shared__ int64_t from[2][kMovePlaces], to[2][kMovePlaces];  // units of U; -1: nothing to copy
+  __shared__ int64_t from_s[SCALES ? kMovePlaces : 1], to_s[SCALES ? kMovePlaces : 1];  // the rows' scales, in words
   pdl_wait();
   const PagedCache& c = p.c;
   const int tid = threadIdx.x;
@@ -574,26 +599,34 @@ __global__ void __launch_bounds__(kMoveThreads) paged_move_kernel(const __grid_c
     const int src = i < p.budget ? p.kept[bh * p.budget + i] : -1;
     int ps = -1, pd = -1;
     if (src >= 0) {
-      ps = paged_page(c, c.table, b * c.table_stride, src / c.page_size, SITE_PAGED_EVICT);
-      pd = paged_page(c, p.dst, b * p.dst_stride, (int)i / c.page_size, SITE_PAGED_EVICT);
+      ps = paged_page(c, c.table, b * c.table_stride, src / c.page_size, SITE);
+      pd = paged_page(c, p.dst, b * p.dst_stride, (int)i / c.page_size, SITE);
     }
     const bool there = ps >= 0 && pd >= 0;
-    const int64_t row = (int64_t)c.Dh, per16 = row / pieces;  // elements of a row; of 16 bytes
-    const int64_t so = ((int64_t)h * c.page_size + src % c.page_size) * row;
-    const int64_t dt = ((int64_t)h * c.page_size + (int)i % c.page_size) * row;
-    from[0][tid] = there ? (ps * c.k_stride + so) / per16 : -1;
-    from[1][tid] = there ? (ps * c.v_stride + so) / per16 : -1;
-    to[0][tid] = there ? (pd * c.k_stride + dt) / per16 : -1;
-    to[1][tid] = there ? (pd * c.v_stride + dt) / per16 : -1;
+    const int64_t unit = SCALES ? sizeof(U) : c.Dh / pieces;  // elements of a unit
+    const int64_t sr = (int64_t)h * c.page_size + src % c.page_size, dr = (int64_t)h * c.page_size + (int)i % c.page_size;
+    from[0][tid] = there ? ps * c.k_stride / unit + sr * pieces : -1;
+    from[1][tid] = there ? ps * c.v_stride / unit + sr * pieces : -1;
+    to[0][tid] = there ? pd * c.k_stride / unit + dr * pieces : -1;
+    to[1][tid] = there ? pd * c.v_stride / unit + dr * pieces : -1;
+    if constexpr (SCALES) {
+      from_s[tid] = there ? ps * p.s_stride + sr * p.words : -1;
+      to_s[tid] = there ? pd * p.s_stride + dr * p.words : -1;
+    }
     if (i < p.out_width) p.mass_out[bh * p.out_width + i] = src < 0 ? 0.f : p.mass[bh * p.mass_width + src];
   }
   __syncthreads();
   if (i0 >= p.budget) return;
-  uint4* kp = (uint4*)c.k;
-  uint4* vp = (uint4*)c.v;
+  if constexpr (SCALES)
+    for (int e = tid; e < kMovePlaces * p.words; e += blockDim.x) {
+      const int place = e / p.words, w = e - place * p.words;
+      if (from_s[place] >= 0) p.scales[to_s[place] + w] = p.scales[from_s[place] + w];
+    }
+  U* kp = (U*)c.k;
+  U* vp = (U*)c.v;
   const int all = kMovePlaces * pieces;
   for (int e0 = tid; e0 < all; e0 += kMoveAhead * blockDim.x) {
-    uint4 a[kMoveAhead], v[kMoveAhead];
+    U a[kMoveAhead], v[kMoveAhead];
 #pragma unroll
     for (int k = 0; k < kMoveAhead; ++k) {
       const int e = e0 + k * blockDim.x, place = e / pieces;

@@ -1,4 +1,5 @@
-// How the attention of one new token over a paged cache is cut: clusters or a list, workspace, launches.
+// Host side of the operators over a paged cache: checks, the cut of the attention into clusters or a list, its
+// workspace, launches.
 #pragma once
 
 #include "paged_attn.cuh"
@@ -6,6 +7,25 @@
 
 namespace one {
 namespace {
+
+// What the operators over a paged cache of either kind ask of its table and sizes; head_dim in units of `dims`.
+template <typename S>
+int check_table(PagedCache& c, const S* x, int dims) {
+  if (!x || !x->k_pages || !x->v_pages || !x->block_table || !x->lengths)
+    return fail(ONE_ERR_INVALID, "paged cache: null argument");
+  if (x->num_pages < 1 || x->page_size < 1 || x->max_pages < 1 || x->b < 1 || x->hkv < 1 || x->dh < 1)
+    return fail(ONE_ERR_INVALID, "paged cache: sizes must be positive");
+  if (x->dh > 128 || x->dh % dims) return fail(ONE_ERR_UNSUPPORTED, "paged cache: head_dim a multiple of %d, at most 128", dims);
+  if (x->b > 65535 || x->hkv > 65535) return fail(ONE_ERR_UNSUPPORTED, "paged cache: at most 65535 sequences and heads");
+  if ((int64_t)x->max_pages * x->page_size > 0x3fffffff)
+    return fail(ONE_ERR_UNSUPPORTED, "paged cache: at most 2^30 - 1 slots per sequence");
+  if (x->table_stride < x->max_pages) return fail(ONE_ERR_INVALID, "paged cache: block table rows overlap");
+  if (x->mass && x->mass_width < (int64_t)x->max_pages * x->page_size)
+    return fail(ONE_ERR_INVALID, "paged cache: mass rows are shorter than the block table's slots");
+  c.table = x->block_table; c.table_stride = x->table_stride; c.lengths = x->lengths;
+  c.num_pages = x->num_pages; c.page_size = x->page_size; c.max_pages = x->max_pages; c.B = x->b; c.Hkv = x->hkv; c.Dh = x->dh;
+  return ONE_OK;
+}
 
 constexpr int kMaxTile = 256;  // slots of the largest tile
 constexpr int kWhole = 512;    // slots that one CTA takes rather than split them
@@ -97,6 +117,45 @@ template <typename E>
 int attend(PagedAttn& p, bool split, cudaStream_t st) {
   const bool run = p.c.page_size % 16 == 0 && p.c.Dh == E::DH;
   return run ? attend<E, true>(p, split, st) : attend<E, false>(p, split, st);
+}
+
+// Eviction over a cache of either kind, in p.c: `pieces` units of U per row.
+template <typename U, typename S>
+int evict(PagedEvictParams& p, const S* cache, int pieces, const int32_t* dst_table, int64_t dst_stride, int32_t dst_max_pages,
+          int32_t budget, int32_t recent, int32_t sink, float* mass_out, int64_t mass_out_width, int32_t* kept, cudaStream_t st) {
+  if (!dst_table || !mass_out || !kept) return fail(ONE_ERR_INVALID, "paged evict: null argument");
+  const int b = cache->b, hkv = cache->hkv, page_size = cache->page_size;
+  if (budget < 1 || recent < 0 || sink < 0 || (int64_t)recent + sink > budget)
+    return fail(ONE_ERR_INVALID, "paged evict: 1 <= budget, 0 <= recent, sink and recent + sink <= budget");
+  if (dst_max_pages < 1 || dst_stride < dst_max_pages || (int64_t)dst_max_pages * page_size < budget)
+    return fail(ONE_ERR_INVALID, "paged evict: the destination pages hold fewer slots than the budget");
+  if (mass_out_width < budget) return fail(ONE_ERR_INVALID, "paged evict: mass rows are too short");
+  if (mass_out_width > 0x3fffffff) return fail(ONE_ERR_UNSUPPORTED, "paged evict: too many rows");
+  p.dst = dst_table; p.dst_stride = dst_stride; p.mass = cache->mass; p.mass_width = cache->mass_width;
+  p.budget = budget; p.recent = recent; p.sink = sink; p.mass_out = mass_out; p.out_width = mass_out_width; p.kept = kept;
+  const int64_t slots = (int64_t)cache->max_pages * page_size, heads = (int64_t)b * hkv;
+  const int64_t parts = (budget + 255) / 256, per_bh = (mass_out_width + kMovePlaces - 1) / kMovePlaces;
+  // where the CTAs fit the SMs at once: two per SM, one of those that hold 64 keys per thread (192 CTAs of
+  // those, 48 heads of 30000 slots to 1000: 49 us in one launch, 29 in two; device times)
+  const bool one_launch = heads * parts <= (slots > 16384 && slots <= 32768 ? 1 : 2) * num_sms();
+  if (heads * std::max(parts, per_bh) > 0x7fffffff) return fail(ONE_ERR_UNSUPPORTED, "paged evict: too many rows");
+  auto select = [&](auto keys) {
+    constexpr int KPT = decltype(keys)::value;
+    return one_launch ? launch(paged_evict_kernel<KPT, true, U>, dim3((unsigned)(heads * parts)), dim3(kEvictThreads), 0, st, p,
+                               (int)parts, pieces)
+                      : launch(paged_evict_kernel<KPT, false>, dim3((unsigned)heads), dim3(kEvictThreads), 0, st, p, 1, pieces);
+  };
+  const int rc = launched(slots <= 1024    ? select(Int<2>())
+                          : slots <= 2048  ? select(Int<4>())
+                          : slots <= 4096  ? select(Int<8>())
+                          : slots <= 8192  ? select(Int<16>())
+                          : slots <= 16384 ? select(Int<32>())
+                          : slots <= 32768 ? select(Int<64>())
+                                           : select(Int<0>()),
+                          "paged evict");
+  if (rc || one_launch) return rc;
+  return launched(launch(paged_move_kernel<U>, dim3((unsigned)(per_bh * heads)), dim3(kMoveThreads), 0, st, p, (int)per_bh, pieces),
+                  "paged move");
 }
 
 }  // namespace

@@ -12,16 +12,9 @@ namespace {
 
 // What every operator over a cache asks of it.
 int check_cache(PagedCache& c, const one_paged_cache* x) {
-  if (!x || !x->k_pages || !x->v_pages || !x->block_table || !x->lengths)
-    return fail(ONE_ERR_INVALID, "paged cache: null argument");
+  int rc = check_table(c, x, 8);
+  if (rc) return rc;
   if (x->dtype != ONE_DTYPE_BF16 && x->dtype != ONE_DTYPE_F32) return fail(ONE_ERR_INVALID, "paged cache: dtype");
-  if (x->num_pages < 1 || x->page_size < 1 || x->max_pages < 1 || x->b < 1 || x->hkv < 1 || x->dh < 1)
-    return fail(ONE_ERR_INVALID, "paged cache: sizes must be positive");
-  if (x->dh > 128 || x->dh % 8) return fail(ONE_ERR_UNSUPPORTED, "paged cache: head_dim a multiple of 8, at most 128");
-  if (x->b > 65535 || x->hkv > 65535) return fail(ONE_ERR_UNSUPPORTED, "paged cache: at most 65535 sequences and heads");
-  if ((int64_t)x->max_pages * x->page_size > 0x3fffffff)
-    return fail(ONE_ERR_UNSUPPORTED, "paged cache: at most 2^30 - 1 slots per sequence");
-  if (x->table_stride < x->max_pages) return fail(ONE_ERR_INVALID, "paged cache: block table rows overlap");
   const int64_t page = (int64_t)x->hkv * x->page_size * x->dh, es = elem_bytes(x->dtype);
   const int64_t ks = x->k_page_stride, vs = x->v_page_stride;
   if (ks > 0x7fffffff || vs > 0x7fffffff || page > 0x7fffffff)
@@ -29,11 +22,7 @@ int check_cache(PagedCache& c, const one_paged_cache* x) {
   if (ks < page || vs < page) return fail(ONE_ERR_INVALID, "paged cache: pages overlap");
   if (((reinterpret_cast<uintptr_t>(x->k_pages) | reinterpret_cast<uintptr_t>(x->v_pages)) & 15) || ks * es % 16 || vs * es % 16)
     return fail(ONE_ERR_INVALID, "paged cache: pages must start on 16-byte boundaries");
-  if (x->mass && x->mass_width < (int64_t)x->max_pages * x->page_size)
-    return fail(ONE_ERR_INVALID, "paged cache: mass rows are shorter than the block table's slots");
   c.k = x->k_pages; c.v = x->v_pages; c.k_stride = ks; c.v_stride = vs;
-  c.table = x->block_table; c.table_stride = x->table_stride; c.lengths = x->lengths;
-  c.num_pages = x->num_pages; c.page_size = x->page_size; c.max_pages = x->max_pages; c.B = x->b; c.Hkv = x->hkv; c.Dh = x->dh;
   c.err = reinterpret_cast<DevErr*>(one_ops_err_record());
   return ONE_OK;
 }
@@ -169,43 +158,11 @@ extern "C" int one_paged_evict(const one_paged_cache* cache, const int32_t* dst_
                                int32_t dst_max_pages, int32_t budget, int32_t recent, int32_t sink, float* mass_out,
                                int64_t mass_out_width, int32_t* kept, void* stream) {
   PagedEvictParams p = {};
-  if (!dst_table || !mass_out || !kept || !cache || !cache->mass) return fail(ONE_ERR_INVALID, "paged evict: null argument");
-  int rc = check_cache(p.c, cache);
-  if (rc) return rc;
-  const int b = cache->b, hkv = cache->hkv, dh = cache->dh, dtype = cache->dtype, page_size = cache->page_size;
-  if (budget < 1 || recent < 0 || sink < 0 || (int64_t)recent + sink > budget)
-    return fail(ONE_ERR_INVALID, "paged evict: 1 <= budget, 0 <= recent, sink and recent + sink <= budget");
-  if (dst_max_pages < 1 || dst_stride < dst_max_pages || (int64_t)dst_max_pages * page_size < budget)
-    return fail(ONE_ERR_INVALID, "paged evict: the destination pages hold fewer slots than the budget");
-  if (mass_out_width < budget) return fail(ONE_ERR_INVALID, "paged evict: mass rows are too short");
-  if (mass_out_width > 0x3fffffff) return fail(ONE_ERR_UNSUPPORTED, "paged evict: too many rows");
-  p.dst = dst_table; p.dst_stride = dst_stride; p.mass = cache->mass; p.mass_width = cache->mass_width;
-  p.budget = budget; p.recent = recent; p.sink = sink; p.mass_out = mass_out; p.out_width = mass_out_width; p.kept = kept;
-  cudaStream_t st = (cudaStream_t)stream;
-  const int64_t slots = (int64_t)cache->max_pages * page_size, heads = (int64_t)b * hkv;
-  const int64_t parts = (budget + 255) / 256, per_bh = (mass_out_width + kMovePlaces - 1) / kMovePlaces;
-  // where the CTAs fit the SMs at once: two per SM, one of those that hold 64 keys per thread (192 CTAs of
-  // those, 48 heads of 30000 slots to 1000: 49 us in one launch, 29 in two; device times)
-  const bool one_launch = heads * parts <= (slots > 16384 && slots <= 32768 ? 1 : 2) * num_sms();
-  if (heads * std::max(parts, per_bh) > 0x7fffffff) return fail(ONE_ERR_UNSUPPORTED, "paged evict: too many rows");
-  const int pieces = dh * elem_bytes(dtype) / 16;
-  auto evict = [&](auto keys) {
-    constexpr int KPT = decltype(keys)::value;
-    return one_launch ? launch(paged_evict_kernel<KPT, true>, dim3((unsigned)(heads * parts)), dim3(kEvictThreads), 0, st, p,
-                               (int)parts, pieces)
-                      : launch(paged_evict_kernel<KPT, false>, dim3((unsigned)heads), dim3(kEvictThreads), 0, st, p, 1, pieces);
-  };
-  rc = launched(slots <= 1024    ? evict(Int<2>())
-                : slots <= 2048  ? evict(Int<4>())
-                : slots <= 4096  ? evict(Int<8>())
-                : slots <= 8192  ? evict(Int<16>())
-                : slots <= 16384 ? evict(Int<32>())
-                : slots <= 32768 ? evict(Int<64>())
-                                 : evict(Int<0>()),
-                "paged evict");
-  if (rc || one_launch) return rc;
-  return launched(launch(paged_move_kernel, dim3((unsigned)(per_bh * heads)), dim3(kMoveThreads), 0, st, p, (int)per_bh, pieces),
-                  "paged move");
+  if (!cache || !cache->mass) return fail(ONE_ERR_INVALID, "paged evict: null argument");
+  const int rc = check_cache(p.c, cache);
+  return rc ? rc
+            : evict<uint4>(p, cache, cache->dh * elem_bytes(cache->dtype) / 16, dst_table, dst_stride, dst_max_pages, budget,
+                           recent, sink, mass_out, mass_out_width, kept, (cudaStream_t)stream);
 }
 
 extern "C" int one_process_logits(const one_logits_rules* rules, const void* logits, int64_t ld, int32_t batch,

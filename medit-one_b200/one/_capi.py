@@ -37,6 +37,7 @@ class OneConfigC(ctypes.Structure):
 # The serving operators' structures, packed per call (struct modules pack faster than ctypes fields):
 # one_paged_cache, one_paged_tokens and one_logits_rules of include/one_b200.h.
 PAGED_CACHE = struct.Struct("=QQqqQqQQq7i4x").pack
+PAGED_QUANT_CACHE = struct.Struct("=QQQqqqQqQQq7i4x").pack  # one_paged_quant_cache
 PAGED_TOKENS = struct.Struct("=QQQ9qQQQQiii4x").pack
 PAGED_TOKENS_FP32_TABLES = struct.Struct("=QQQ9qQQQQiiii").pack  # the same, ending with tables_fp32
 LOGITS_RULES = struct.Struct("=QqQQQQQqQqiifff4x").pack
@@ -89,6 +90,13 @@ SIGNATURES = {
                                     c_void_p]),
     "one_paged_evict": (c_int, [c_void_p, c_void_p, c_int64, c_int32, c_int32, c_int32, c_int32, c_void_p, c_int64,
                                 c_void_p, c_void_p]),
+    "one_paged_quant_append": (c_int, [c_void_p, c_void_p, c_int32, c_void_p]),
+    "one_paged_quant_read": (c_int, [c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_void_p, c_void_p]),
+    "one_paged_quant_attention_workspace_bytes": (c_size_t, [c_int32] * 8),
+    "one_paged_quant_attention": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int32, c_float, c_int32, c_void_p, c_void_p,
+                                          c_size_t, c_void_p]),
+    "one_paged_quant_evict": (c_int, [c_void_p, c_void_p, c_int64, c_int32, c_int32, c_int32, c_int32, c_void_p, c_int64,
+                                      c_void_p, c_void_p]),
     "one_process_logits": (c_int, [c_void_p, c_void_p, c_int64, c_int32, c_int32, c_int32, c_void_p, c_int64, c_void_p,
                                    c_void_p]),
 }

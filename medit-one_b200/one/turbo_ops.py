@@ -169,26 +169,17 @@ def _page_stride(p, n, inner):
     return s[0] if n > 1 else p.shape[1] * inner[0]
 
 
-def _paged(k_pages, v_pages, block_table, lengths, mass, dtype):
-    """Checks a cache and packs it for the C entry points: (device, packed, (B, Hkv, page_size, Dh, max_pages))."""
-    shape = k_pages.shape
-    if len(shape) != 4 or v_pages.shape != shape:
-        raise ValueError("k_pages and v_pages must have the same shape [num_pages, Hkv, page_size, Dh]")
+def _table(dev, block_table, lengths, mass, hkv, ps):
+    """Checks what says where a batch's slots lie: (B, max_pages, row stride of the table, address of mass, its width)."""
     tshape = block_table.shape
     if len(tshape) != 2 or lengths.shape != tshape[:1]:
         raise ValueError("block_table must be [B, max_pages] and lengths [B]")
     if block_table.dtype is not _I32 or lengths.dtype is not _I32:
         raise ValueError("block_table and lengths must be int32")
-    if k_pages.dtype is not dtype or v_pages.dtype is not dtype:
-        raise ValueError("the cache and the new tokens must have one dtype")
-    n, hkv, ps, dh = shape
     b, mp = tshape
-    inner = (ps * dh, dh, 1)
-    ks, vs = _page_stride(k_pages, n, inner), _page_stride(v_pages, n, inner)
     ts, tc = block_table.stride()
     if (mp > 1 and tc != 1) or not lengths.is_contiguous():
         raise ValueError("block_table rows and lengths must be contiguous")
-    dev = k_pages.get_device()
     mptr = mw = 0
     if mass is not None:
         mshape = mass.shape
@@ -199,12 +190,33 @@ def _paged(k_pages, v_pages, block_table, lengths, mass, dtype):
         mptr, mw = mass.data_ptr(), mshape[2]
         if mass.get_device() != dev:
             raise ValueError("all tensors must be on one device")
-    if v_pages.get_device() != dev or block_table.get_device() != dev or lengths.get_device() != dev:
+    if block_table.get_device() != dev or lengths.get_device() != dev:
         raise ValueError("all tensors must be on one device")
-    code = C.dtype_code(dtype) if C is not None else 0
-    packed = C.PAGED_CACHE(k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, block_table.data_ptr(), ts if b > 1 else mp,
-                           lengths.data_ptr(), mptr, mw, n, ps, mp, b, hkv, dh, code) if C is not None else b""
+    return b, mp, ts if b > 1 else mp, mptr, mw
+
+
+def _paged(k_pages, v_pages, block_table, lengths, mass, dtype):
+    """Checks a cache and packs it for the C entry points: (device, packed, (B, Hkv, page_size, Dh, max_pages))."""
+    shape = k_pages.shape
+    if len(shape) != 4 or v_pages.shape != shape:
+        raise ValueError("k_pages and v_pages must have the same shape [num_pages, Hkv, page_size, Dh]")
+    if k_pages.dtype is not dtype or v_pages.dtype is not dtype:
+        raise ValueError("the cache and the new tokens must have one dtype")
+    n, hkv, ps, dh = shape
+    inner = (ps * dh, dh, 1)
+    ks, vs = _page_stride(k_pages, n, inner), _page_stride(v_pages, n, inner)
+    dev = k_pages.get_device()
+    if v_pages.get_device() != dev:
+        raise ValueError("all tensors must be on one device")
+    b, mp, ts, mptr, mw = _table(dev, block_table, lengths, mass, hkv, ps)
+    code = _code(dtype)
+    packed = C.PAGED_CACHE(k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, block_table.data_ptr(), ts, lengths.data_ptr(),
+                           mptr, mw, n, ps, mp, b, hkv, dh, code) if C is not None else b""
     return dev, packed, (b, hkv, ps, dh, mp)
+
+
+def _code(dtype):
+    return C.dtype_code(dtype) if C is not None else 0
 
 
 def _cuda(dev, first):
@@ -254,18 +266,10 @@ def _rows_overlap(x, y):
     return bool(((i < ys.numel()) & (ys[i.clamp(max=ys.numel() - 1)] < xs + wx)).any())
 
 
-def turbo_paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
-                       block_table: torch.Tensor, lengths: torch.Tensor, cos: Optional[torch.Tensor] = None,
-                       sin: Optional[torch.Tensor] = None, q: Optional[torch.Tensor] = None,
-                       counts: Optional[torch.Tensor] = None, mass: Optional[torch.Tensor] = None
-                       ) -> Optional[torch.Tensor]:
-    """New tokens into a paged cache. k, v [B, Hkv, N, Dh] (any strides) go to the slots lengths[b]
-    .. lengths[b] + counts[b] - 1 (counts int32 [B], default N), k rotated by cos, sin [B or 1, N, Dh]
-    (apply_rotary_pos_emb_flash in fp32, rounded once) when they are given; the slots' mass becomes 0.
-    cos and sin are taken in k's dtype or in fp32; other types become fp32.
-    Returns q [B, Hq, N, Dh] rotated the same way, or None without q. The caller advances lengths."""
+def _append(dev, cache, dims, k, v, cos, sin, q, counts, quant=None):
+    """New tokens into a cache that _paged or, with the tokens' dtype code, _paged_quant has packed."""
+    b, hkv, ps, dh, mp = dims
     dt = k.dtype
-    dev, cache, (b, hkv, ps, dh, mp) = _paged(k_pages, v_pages, block_table, lengths, mass, dt)
     shape = k.shape
     if len(shape) != 4 or v.shape != shape or shape[0] != b or shape[1] != hkv or shape[3] != dh:
         raise ValueError(f"k and v must be [{b}, {hkv}, N, {dh}], got {tuple(k.shape)} and {tuple(v.shape)}")
@@ -314,28 +318,39 @@ def turbo_paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, 
         cosp, sinp = cos.data_ptr(), sin.data_ptr()
     k, v = _rows_last(k), _rows_last(v)
     ks, vs = k.stride(), v.stride()
-    _launch(C.LIB.one_paged_append, dev, cache,
-            pack(k.data_ptr(), v.data_ptr(), qptr, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], qs[0], qs[1], qs[2],
-                 cosp, sinp, cptr, optr, n, hq, cb, *tables))
+    tokens = pack(k.data_ptr(), v.data_ptr(), qptr, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], qs[0], qs[1], qs[2],
+                  cosp, sinp, cptr, optr, n, hq, cb, *tables)
+    if quant is None:
+        _launch(C.LIB.one_paged_append, dev, cache, tokens)
+    else:
+        _launch(C.LIB.one_paged_quant_append, dev, cache, tokens, quant)
     return out
 
 
+def turbo_paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                       block_table: torch.Tensor, lengths: torch.Tensor, cos: Optional[torch.Tensor] = None,
+                       sin: Optional[torch.Tensor] = None, q: Optional[torch.Tensor] = None,
+                       counts: Optional[torch.Tensor] = None, mass: Optional[torch.Tensor] = None
+                       ) -> Optional[torch.Tensor]:
+    """New tokens into a paged cache. k, v [B, Hkv, N, Dh] (any strides) go to the slots lengths[b]
+    .. lengths[b] + counts[b] - 1 (counts int32 [B], default N), k rotated by cos, sin [B or 1, N, Dh]
+    (apply_rotary_pos_emb_flash in fp32, rounded once) when they are given; the slots' mass becomes 0.
+    cos and sin are taken in k's dtype or in fp32; other types become fp32.
+    Returns q [B, Hq, N, Dh] rotated the same way, or None without q. The caller advances lengths."""
+    return _append(*_paged(k_pages, v_pages, block_table, lengths, mass, k.dtype), k, v, cos, sin, q, counts)
+
+
 @functools.lru_cache(maxsize=1024)
-def _attention_workspace(*sizes):
+def _attention_workspace(quantised, *sizes):
+    if quantised:
+        return C.LIB.one_paged_quant_attention_workspace_bytes(*sizes)
     return C.LIB.one_paged_attention_workspace_bytes(*sizes)
 
 
-def turbo_paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
-                          lengths: torch.Tensor, scale_factor: Optional[float] = None,
-                          mass: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """Attention of one new token per sequence, q [B, Hq, 1, Dh], over the cached slots below
-    lengths[b]: softmax(q k^T * scale) v with an fp32 softmax, scale 1/sqrt(Dh) by default. Hq is a
-    multiple of Hkv: query head j reads kv head j // (Hq // Hkv). A sequence without slots gives
-    zeros. mass grows by the softmax weights, summed over each kv head's query heads; that takes a
-    workspace of 4 bytes per query head and slot of the table. `out` must not overlap q."""
-    dt = q.dtype
-    dev, cache, (b, hkv, ps, dh, mp) = _paged(k_pages, v_pages, block_table, lengths, mass, dt)
-    shape = q.shape
+def _attend(dev, cache, dims, q, scale_factor, mass, out, quant=None):
+    """Attention over a cache that _paged or, with the dtype code of q, _paged_quant has packed."""
+    b, hkv, ps, dh, mp = dims
+    dt, shape = q.dtype, q.shape
     if len(shape) != 4 or shape[0] != b or shape[2] != 1 or shape[3] != dh or shape[1] % hkv:
         raise ValueError(f"q must be [{b}, a multiple of {hkv}, 1, {dh}], got {tuple(shape)}")
     if q.get_device() != dev or (out is not None and out.get_device() != dev):
@@ -351,12 +366,55 @@ def turbo_paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch
         out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(shape)
     if b == 0:
         return out
-    nws = _attention_workspace(b, hq, hkv, dh, ps, mp, C.dtype_code(dt), mass is not None)
+    nws = _attention_workspace(quant is not None, b, hq, hkv, dh, ps, mp, C.dtype_code(dt), mass is not None)
     ws = q.new_empty(nws, dtype=torch.uint8) if nws else None
     qs = q.stride()
-    _launch(C.LIB.one_paged_attention, dev, cache, q.data_ptr(), qs[0], qs[1], hq,
-            dh ** -0.5 if scale_factor is None else float(scale_factor), out.data_ptr(), ws.data_ptr() if nws else 0, nws)
+    scale = dh ** -0.5 if scale_factor is None else float(scale_factor)
+    wptr = ws.data_ptr() if nws else 0
+    if quant is None:
+        _launch(C.LIB.one_paged_attention, dev, cache, q.data_ptr(), qs[0], qs[1], hq, scale, out.data_ptr(), wptr, nws)
+    else:
+        _launch(C.LIB.one_paged_quant_attention, dev, cache, q.data_ptr(), qs[0], qs[1], hq, scale, quant, out.data_ptr(), wptr,
+                nws)
     return out
+
+
+def turbo_paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
+                          lengths: torch.Tensor, scale_factor: Optional[float] = None,
+                          mass: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of one new token per sequence, q [B, Hq, 1, Dh], over the cached slots below
+    lengths[b]: softmax(q k^T * scale) v with an fp32 softmax, scale 1/sqrt(Dh) by default. Hq is a
+    multiple of Hkv: query head j reads kv head j // (Hq // Hkv). A sequence without slots gives
+    zeros. mass grows by the softmax weights, summed over each kv head's query heads; that takes a
+    workspace of 4 bytes per query head and slot of the table. `out` must not overlap q."""
+    return _attend(*_paged(k_pages, v_pages, block_table, lengths, mass, q.dtype), q, scale_factor, mass, out)
+
+
+def _evict(dev, cache, dims, block_table, d, mass, budget, recent, sink, quantised=False):
+    """Eviction from a cache that _paged or _paged_quant has packed, into the pages of table d."""
+    b, hkv, ps, dh, mp = dims
+    budget, recent, sink = int(budget), int(recent), int(sink)
+    if budget < 1 or recent < 0 or sink < 0 or recent + sink > budget:
+        raise ValueError("1 <= budget, 0 <= recent, 0 <= sink and recent + sink <= budget")
+    dshape = d.shape
+    if len(dshape) != 2 or d.dtype is not _I32 or dshape[0] != b or (dshape[1] > 1 and d.stride(1) != 1):
+        raise ValueError(f"dst_block_table must be int32 [{b}, dst pages] with contiguous rows")
+    dp = dshape[1]
+    width = dp * ps
+    if width < budget:
+        raise ValueError(f"dst_block_table holds {width} slots, fewer than the budget {budget}")
+    if b and d.data_ptr() == block_table.data_ptr():
+        raise ValueError("survivors go to other pages: dst_block_table is block_table")
+    if d.get_device() != dev:
+        raise ValueError("all tensors must be on one device")
+    _cuda(dev, d)
+    mass_out = mass.new_empty((b, hkv, width))
+    kept = d.new_empty((b, hkv, budget))
+    if b == 0:
+        return mass_out, kept
+    _launch(C.LIB.one_paged_quant_evict if quantised else C.LIB.one_paged_evict, dev, cache, d.data_ptr(),
+            d.stride(0) if b > 1 else dp, dp, budget, recent, sink, mass_out.data_ptr(), width, kept.data_ptr())
+    return mass_out, kept
 
 
 def turbo_paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
@@ -370,30 +428,110 @@ def turbo_paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table:
     slots, then -1). The caller goes on with dst_block_table and lengths.clamp(max=budget)."""
     if mass is None:
         raise ValueError("eviction goes by mass")
-    dev, cache, (b, hkv, ps, dh, mp) = _paged(k_pages, v_pages, block_table, lengths, mass, k_pages.dtype)
-    budget, recent, sink = int(budget), int(recent), int(sink)
-    if budget < 1 or recent < 0 or sink < 0 or recent + sink > budget:
-        raise ValueError("1 <= budget, 0 <= recent, 0 <= sink and recent + sink <= budget")
-    d = dst_block_table
-    dshape = d.shape
-    if len(dshape) != 2 or d.dtype is not _I32 or dshape[0] != b or (dshape[1] > 1 and d.stride(1) != 1):
-        raise ValueError(f"dst_block_table must be int32 [{b}, dst pages] with contiguous rows")
-    dp = dshape[1]
-    width = dp * ps
-    if width < budget:
-        raise ValueError(f"dst_block_table holds {width} slots, fewer than the budget {budget}")
-    if b and d.data_ptr() == block_table.data_ptr():
-        raise ValueError("survivors go to other pages: dst_block_table is block_table")
-    if d.get_device() != dev:
+    return _evict(*_paged(k_pages, v_pages, block_table, lengths, mass, k_pages.dtype), block_table, dst_block_table, mass,
+                  budget, recent, sink)
+
+
+# ------------------------------------------------------------------ the same cache in 4 or 8 bits
+# k_pages, v_pages uint8 [num_pages, Hkv, page_size, Dh / 2 (4 bits) or Dh (8 bits)], scales bf16
+# [num_pages, Hkv, page_size, 2, ceil(Dh / 32)] (a slot's scales of the key, then of the value); Dh a
+# multiple of 16, at most 128. Every 32 values of a row (the last ones may be fewer) stand for scale *
+# code: scale = bf16(max |x| / m), m = 7 (4 bits) or 127 (8 bits), code = x / scale to the nearest whole
+# number, halves to the even one; x is the value in fp32. Scales below 2^-100 are held as 0; a group with
+# an infinity or NaN has the scale NaN and reads as NaN. A byte holds code + 128, or two codes, 8 added to
+# each, the even dim in the low half. Tables, lengths and masses are those of the cache above.
+
+
+def turbo_paged_quant_pools(num_pages: int, num_kv_heads: int, page_size: int, head_dim: int, bits: int = 4,
+                            device="cuda") -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Pools of a quantised cache, (k_pages, v_pages, scales), not initialised."""
+    if bits not in (4, 8) or head_dim < 16 or head_dim > 128 or head_dim % 16:
+        raise ValueError("4 or 8 bits, and a head_dim that is a multiple of 16, at most 128")
+    shape = (num_pages, num_kv_heads, page_size)
+    k, v = (torch.empty(*shape, head_dim * bits // 8, dtype=torch.uint8, device=device) for _ in range(2))
+    return k, v, torch.empty(*shape, 2, (head_dim + 31) // 32, dtype=torch.bfloat16, device=device)
+
+
+def _paged_quant(k_pages, v_pages, scales, block_table, lengths, mass, dh):
+    """As _paged for a cache in 4 or 8 bits; dh None: whatever the rows hold."""
+    shape, sshape = k_pages.shape, scales.shape
+    if len(shape) != 4 or v_pages.shape != shape:
+        raise ValueError("k_pages and v_pages must have the same shape [num_pages, Hkv, page_size, Dh * bits / 8]")
+    if k_pages.dtype is not torch.uint8 or v_pages.dtype is not torch.uint8 or scales.dtype is not torch.bfloat16:
+        raise ValueError("k_pages and v_pages must be uint8 and scales bf16")
+    n, hkv, ps, row = shape
+    groups = sshape[-1] if len(sshape) == 5 else 0
+    if dh is None:
+        dh = 2 * row if groups == (2 * row + 31) // 32 else row
+    bits = 4 if dh == 2 * row else 8
+    if dh != row * 8 // bits or sshape != (n, hkv, ps, 2, (dh + 31) // 32):
+        raise ValueError(f"rows of {row} bytes hold head_dim {2 * row} or {row}, and scales must be [{n}, {hkv}, {ps}, 2, "
+                         f"ceil(head_dim / 32)]; got head_dim {dh} and {tuple(sshape)}")
+    inner = (ps * row, row, 1)
+    ks, vs = _page_stride(k_pages, n, inner), _page_stride(v_pages, n, inner)
+    ss = _page_stride(scales, n, (ps * 2 * groups, 2 * groups, groups, 1))
+    dev = k_pages.get_device()
+    if v_pages.get_device() != dev or scales.get_device() != dev:
         raise ValueError("all tensors must be on one device")
+    b, mp, ts, mptr, mw = _table(dev, block_table, lengths, mass, hkv, ps)
+    packed = C.PAGED_QUANT_CACHE(k_pages.data_ptr(), v_pages.data_ptr(), scales.data_ptr(), ks, vs, ss, block_table.data_ptr(),
+                                 ts, lengths.data_ptr(), mptr, mw, n, ps, mp, b, hkv, dh, bits) if C is not None else b""
+    return dev, packed, (b, hkv, ps, dh, mp)
+
+
+def turbo_paged_quant_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                             scales: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
+                             cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None,
+                             q: Optional[torch.Tensor] = None, counts: Optional[torch.Tensor] = None,
+                             mass: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """turbo_paged_append into a cache in 4 or 8 bits: keys, rotated when cos and sin are given, and
+    values are quantised as they are written."""
+    return _append(*_paged_quant(k_pages, v_pages, scales, block_table, lengths, mass, k.shape[-1]), k, v, cos, sin, q, counts,
+                   quant=_code(k.dtype))
+
+
+def turbo_paged_quant_read(k_pages: torch.Tensor, v_pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor,
+                           lengths: torch.Tensor, n: int, head_dim: int, starts: Optional[torch.Tensor] = None,
+                           dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The keys and values that the cache stands for, dense: k, v [B, Hkv, n, head_dim] of the slots
+    starts[b] .. starts[b] + n - 1 (starts int32 [B], default 0), scale * code rounded once to dtype (bf16
+    or fp32). Slots from lengths[b] on read as zeros."""
+    head_dim, n = int(head_dim), int(n)
+    dev, cache, (b, hkv, ps, dh, mp) = _paged_quant(k_pages, v_pages, scales, block_table, lengths, None, head_dim)
+    if n < 0:
+        raise ValueError("n must not be negative")
+    sptr = 0
+    if starts is not None:
+        if starts.dtype is not _I32 or starts.shape != (b,) or not starts.is_contiguous():
+            raise ValueError(f"starts must be int32 [{b}]")
+        if starts.get_device() != dev:
+            raise ValueError("all tensors must be on one device")
+        sptr = starts.data_ptr()
+    code = _code(dtype)
     _cuda(dev, k_pages)
-    mass_out = mass.new_empty((b, hkv, width))
-    kept = d.new_empty((b, hkv, budget))
-    if b == 0:
-        return mass_out, kept
-    _launch(C.LIB.one_paged_evict, dev, cache, d.data_ptr(), d.stride(0) if b > 1 else dp, dp, budget, recent, sink,
-            mass_out.data_ptr(), width, kept.data_ptr())
-    return mass_out, kept
+    k, v = (scales.new_empty((b, hkv, n, dh), dtype=dtype) for _ in range(2))
+    if b and n:
+        _launch(C.LIB.one_paged_quant_read, dev, cache, sptr, n, code, k.data_ptr(), v.data_ptr())
+    return k, v
+
+
+def turbo_paged_quant_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, scales: torch.Tensor,
+                                block_table: torch.Tensor, lengths: torch.Tensor, scale_factor: Optional[float] = None,
+                                mass: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """turbo_paged_attention over the values that a cache in 4 or 8 bits stands for; q and the result
+    in bf16 or fp32."""
+    return _attend(*_paged_quant(k_pages, v_pages, scales, block_table, lengths, mass, q.shape[-1]), q, scale_factor, mass, out,
+                   quant=_code(q.dtype))
+
+
+def turbo_paged_quant_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor,
+                            dst_block_table: torch.Tensor, lengths: torch.Tensor, mass: torch.Tensor, budget: int,
+                            recent: int = 0, sink: int = 0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """turbo_paged_evict from a cache in 4 or 8 bits; codes and scales move as they are."""
+    if mass is None:
+        raise ValueError("eviction goes by mass")
+    return _evict(*_paged_quant(k_pages, v_pages, scales, block_table, lengths, mass, None), block_table, dst_block_table, mass,
+                  budget, recent, sink, quantised=True)
 
 
 class TurboFlashAttention(torch.nn.Module):
