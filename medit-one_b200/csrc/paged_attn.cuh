@@ -53,6 +53,11 @@ struct PagedAttn {
   int2* parts;            // [B * Hkv * hv_per_kv]: first CTA of a segment; last << 1 | (its first part is slot 1)
   int ranges;             // CTAs that share the list
   int cluster;            // CTAs per segment, where there is no list
+  // of a cache in 4 or 8 bits:
+  const uint8_t* scales;
+  int64_t s_stride;       // bytes from one page's scales to the next's
+  int row;                // bytes of a row of codes
+  int run, vec16;         // groups of 16 slots may be copied as they lie; rows are whole 16-byte pieces
 };
 
 template <int TILE>
@@ -212,6 +217,8 @@ struct PaCopy {
 template <int DH_, bool WIDE>
 struct PaBf16 {
   using T = __nv_bfloat16;
+  using Cell = T;                                      // of the cache
+  static constexpr bool kQuant = false;
   static constexpr int DH = DH_, ROWS = WIDE ? 16 : 8;
   static constexpr int KC = DH / 32;                   // 16-byte chunks of a key row per lane
   static constexpr int VC = DH / 64, VH = DH % 64 / 32;  // 16-byte and 8-byte pieces of a value row per lane
@@ -432,6 +439,8 @@ struct PaBf16 {
 template <int DH_, int ROWS_>
 struct PaF32 {
   using T = float;
+  using Cell = T;
+  static constexpr bool kQuant = false;
   static constexpr int DH = DH_, ROWS = ROWS_;
   static constexpr int KC = DH / 16, VC = DH / 32, CH = DH / 4;
   static constexpr int kGroups = 1, TILE = 16 * kPaWarps;
@@ -608,12 +617,15 @@ struct PaSmem {
   static constexpr int kFin = kML + 2 * kPaWarps * E::ROWS * 8;          // [ROWS][2]: m, 1 / l
   static constexpr int kExtra = kFin + (E::ROWS * 8 + 15) / 16 * 16;
   static constexpr int kSum = kExtra + kPaWarps * E::kExtra;
+  // a warp's sums fit the stage that it consumed last, or at least its ring
+  static constexpr int kSums = E::ROWS * E::DH * 4;
+  static constexpr bool kInStage = kStage >= kSums;
+  static_assert(kInStage || kWarp >= kSums, "ring");
   // of a cluster: this CTA's sums [ROWS][DH]; of a list: the warps' sums [1 or 2][warps][rows][DH] where they fit
-  static constexpr int kApart = 2 * kPaWarps * E::ROWS * E::DH * 4 < 9216 ? 2 * kPaWarps * E::ROWS * E::DH * 4 : 9216;
+  static constexpr int kLeast = kInStage ? 0 : kPaWarps * kSums, kMost = kLeast > 9216 ? kLeast : 9216;
+  static constexpr int kApart = 2 * kPaWarps * kSums < kMost ? 2 * kPaWarps * kSums : kMost;
   static constexpr int kTotal = kSum + (SPLIT ? kApart : E::ROWS * E::DH * 4);
   static constexpr int kPerSm = kSmPerSm / (kTotal + 1024) < 3 ? kSmPerSm / (kTotal + 1024) : 3;
-  // a warp's sums fit the stage that it consumed last
-  static_assert(kStage >= E::ROWS * E::DH * 4, "stage");
 };
 
 // PA_LIST: CTA i takes the i-th share of the list. Otherwise a cluster of p.cluster CTAs (1 to 8) takes
@@ -626,6 +638,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, MODE>::kPerSm) paged_
   using S = PaSmem<E, MODE>;
   constexpr bool SPLIT = S::SPLIT;
   using T = typename E::T;
+  using Cell = typename E::Cell;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int TILE = E::TILE, GR = E::kGroups;
   uint8_t* ring = smem + warp * S::kWarp;
@@ -656,7 +669,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, MODE>::kPerSm) paged_
   // ---- the copying side: page numbers are asked for one tile ahead of the copies. RUN: one per group;
   //      otherwise lane t and lane 16 + t look slot t up.
   PaCursor<TILE> src = cur;
-  int to_copy = left, pg[GR], row[GR];  // page and first element in its head of each group
+  int to_copy = left, pg[GR], row[GR];  // page and first element (kQuant: row) in its head of each group
   uint32_t live[S::kStages][GR];        // slots in use of the tiles in the ring, the oldest first
 #pragma unroll
   for (int k = 0; k < S::kStages; ++k)
@@ -664,12 +677,15 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, MODE>::kPerSm) paged_
     for (int g = 0; g < GR; ++g) live[k][g] = 0;
   const int mine = warp * (16 * GR) + (RUN ? 0 : lane & 15);
   const int* table;          // of the segment being copied:
-  const T *keys, *values;    // its block table, and its head in page 0 (RUN: this lane's first piece)
+  const Cell *keys, *values; // its block table, and its head in page 0 (RUN: this lane's first piece)
+  const uint8_t* scales = nullptr;
+  const int cells = E::kQuant ? p.row : c.Dh;  // of a row
   auto segment = [&] {
-    const int64_t head = (int64_t)src.kv * c.page_size * c.Dh + (RUN ? lane * (int)(16 / sizeof(T)) : 0);
+    const int64_t head = (int64_t)src.kv * c.page_size * cells + (RUN ? lane * (int)(16 / sizeof(Cell)) : 0);
     table = c.table + src.b * c.table_stride;
-    keys = (const T*)c.k + head;
-    values = (const T*)c.v + head;
+    keys = (const Cell*)c.k + head;
+    values = (const Cell*)c.v + head;
+    if constexpr (E::kQuant) scales = p.scales + (int64_t)src.kv * c.page_size * E::SR + (RUN ? lane * 16 : 0);
   };
   int ahead = src.len - src.tile * TILE - mine;  // slots from this warp's first one to the end
   auto ask = [&] {
@@ -679,7 +695,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, MODE>::kPerSm) paged_
       pg[g] = -1;
       if (ahead > 16 * g) {
         const int t = t0 + 16 * g, index = (int)(((uint64_t)(uint32_t)t * p.div_m) >> p.div_s);
-        row[g] = (t - index * c.page_size) * c.Dh;
+        row[g] = (t - index * c.page_size) * (E::kQuant ? 1 : c.Dh);
         pg[g] = table[index];
       }
     }
@@ -698,7 +714,24 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, MODE>::kPerSm) paged_
         uint32_t& alive = live[S::kStages - 1][g];
         const bool good = (uint32_t)pg[g] < (uint32_t)c.num_pages;
         if (!good && ahead > 16 * g) set_err(c.err, ERR_BAD_ARG, SITE_PAGED_ATTN);
-        if (RUN) {
+        if constexpr (E::kQuant) {
+          const uint32_t at = smem_u32(to);
+          if (RUN) {
+            alive = 0;
+            if (good) {
+              const uint8_t* kp = keys + ((int64_t)pg[g] * ks + row[g] * p.row);
+              const uint8_t* vp = values + ((int64_t)pg[g] * vs + row[g] * p.row);
+              const uint8_t* sp = scales + ((int64_t)pg[g] * p.s_stride + row[g] * E::SR);
+              const int n = min(ahead - 16 * g, 16);
+              alive = (1u << n) - 1;
+              if (n == 16) E::template copy<true>(at, kp, vp, sp, 16);
+              else E::template copy<false>(at, kp, vp, sp, n);
+            }
+          } else {
+            alive = __ballot_sync(0xffffffffu, good) & 0xffffu;
+            if (alive) E::copy_any(at, p, keys, values, scales, good ? pg[g] : -1, row[g]);
+          }
+        } else if (RUN) {
           alive = 0;
           if (good) {
             const uint8_t* kp = (const uint8_t*)(keys + ((int64_t)pg[g] * ks + row[g]));
@@ -771,7 +804,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, MODE>::kPerSm) paged_
         copied = true;
       }
     }
-    float* so = reinterpret_cast<float*>(smem + (apart ? S::kSum : put));
+    float* so = reinterpret_cast<float*>(smem + (apart ? S::kSum : S::kInStage ? put : 0));
     const int so_warp = apart ? most * E::DH : S::kWarp / 4;
     if (apart) so += parity * kPaWarps * so_warp;
     float* ml = reinterpret_cast<float*>(smem + S::kML) + parity * kPaWarps * E::ROWS * 2;

@@ -56,6 +56,13 @@ bool paged_split(int64_t segments, int64_t slots) {
 
 size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
+// t / page_size for t < 2^31 as a product and a shift.
+void paged_divisor(PagedAttn& p, int page_size) {
+  while ((1 << p.div_s) < page_size) ++p.div_s;
+  p.div_m = (uint32_t)((1ull << (31 + p.div_s)) / page_size + 1);
+  p.div_s += 31;
+}
+
 // Query heads that one pass over a kv head's cache serves.
 int paged_rows(int dtype, int G) { return dtype == ONE_DTYPE_F32 ? (G > 1 ? 4 : 1) : G > 8 ? 16 : 8; }
 
@@ -75,6 +82,44 @@ struct PagedWs {
 };
 
 int pad_dh(int dh) { return dh <= 32 ? 32 : dh <= 64 ? 64 : dh <= 96 ? 96 : 128; }
+
+// What the attention over a cache of either kind, in p.c, asks of its arguments, and its plan; `rows` query
+// heads per pass. need: workspace bytes.
+template <typename S>
+int plan_attention(PagedAttn& p, bool& split, const S* cache, const void* q, int64_t q_bs, int64_t q_hs, int hq, int rows,
+                   float scale, void* out, void* workspace, size_t workspace_bytes, size_t need) {
+  const int b = cache->b, hkv = cache->hkv, dh = cache->dh, page_size = cache->page_size;
+  float* mass = cache->mass;
+  const int64_t slots = (int64_t)cache->max_pages * page_size;
+  // tiles, and the list's length rounded up to equal shares, in 31 bits
+  if ((int64_t)b * hq > 0x3fffffff || (int64_t)b * hq * (slots / 64 + 1) > 0x7fffffff - kMaxSms * kPaPerSm)
+    return fail(ONE_ERR_UNSUPPORTED, "paged attention: too many rows");
+  if (need && (!workspace || workspace_bytes < need)) return fail(ONE_ERR_INVALID, "workspace too small");
+  p.q = q; p.q_bs = q_bs; p.q_hs = q_hs; p.G = hq / hkv;
+  p.hv_per_kv = (p.G + rows - 1) / rows;
+  p.q_vec = (reinterpret_cast<uintptr_t>(q) & 15) == 0 && q_bs % 8 == 0 && q_hs % 8 == 0;
+  paged_divisor(p, page_size);
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.mass = mass; p.mass_width = cache->mass_width; p.out = out;
+  const PagedWs w(b, hq, rows, pad_dh(dh), slots, mass != nullptr);
+  uint8_t* ws = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(workspace) + 255) & ~uintptr_t(255));
+  p.part_ml = reinterpret_cast<float*>(ws + w.part_ml);
+  p.part_o = reinterpret_cast<float*>(ws + w.part_o);
+  p.row_ml = reinterpret_cast<float*>(ws + w.row_ml);
+  p.parts = reinterpret_cast<int2*>(ws + w.segs);
+  p.scores = mass ? reinterpret_cast<float*>(ws + w.scores) : nullptr;
+  p.score_ld = w.score_ld;
+  split = paged_split((int64_t)b * hkv * p.hv_per_kv, slots) || (mass && p.hv_per_kv > 1);
+  return ONE_OK;
+}
+
+size_t attention_bytes(int b, int hq, int hkv, int dh, int rows, int page_size, int max_pages, bool with_mass) {
+  if (b < 1 || hq < 1 || hkv < 1 || dh < 1 || page_size < 1 || max_pages < 1) return 0;
+  const int64_t slots = (int64_t)max_pages * page_size;
+  const int tiles = (hq / hkv + rows - 1) / rows;
+  if (!with_mass && !paged_split((int64_t)b * hkv * tiles, slots)) return 0;
+  return PagedWs(b, hq, rows, pad_dh(dh), slots, with_mass).total + 256;
+}
 
 template <typename E, bool RUN, PaMode MODE>
 int attend(PagedAttn& p, int cluster, cudaStream_t st) {
@@ -115,7 +160,7 @@ int attend(PagedAttn& p, bool split, cudaStream_t st) {
 
 template <typename E>
 int attend(PagedAttn& p, bool split, cudaStream_t st) {
-  const bool run = p.c.page_size % 16 == 0 && p.c.Dh == E::DH;
+  const bool run = p.c.page_size % 16 == 0 && p.c.Dh == E::DH && (!E::kQuant || p.run);
   return run ? attend<E, true>(p, split, st) : attend<E, false>(p, split, st);
 }
 

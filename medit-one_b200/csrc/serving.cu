@@ -31,11 +31,8 @@ int check_cache(PagedCache& c, const one_paged_cache* x) {
 
 extern "C" size_t one_paged_attention_workspace_bytes(int32_t b, int32_t hq, int32_t hkv, int32_t dh, int32_t page_size,
                                                       int32_t max_pages, int32_t dtype, int32_t with_mass) {
-  if (b < 1 || hq < 1 || hkv < 1 || dh < 1 || page_size < 1 || max_pages < 1) return 0;
-  const int64_t slots = (int64_t)max_pages * page_size;
-  const int rows = paged_rows(dtype, hq / hkv), tiles = (hq / hkv + rows - 1) / rows;
-  if (!with_mass && !paged_split((int64_t)b * hkv * tiles, slots)) return 0;
-  return PagedWs(b, hq, rows, pad_dh(dh), slots, with_mass != 0).total + 256;
+  if (hq < 1 || hkv < 1) return 0;
+  return attention_bytes(b, hq, hkv, dh, paged_rows(dtype, hq / hkv), page_size, max_pages, with_mass != 0);
 }
 
 extern "C" int one_paged_attention(const one_paged_cache* cache, const void* q, int64_t q_batch_stride,
@@ -45,33 +42,13 @@ extern "C" int one_paged_attention(const one_paged_cache* cache, const void* q, 
   PagedAttn p = {};
   int rc = check_cache(p.c, cache);
   if (rc) return rc;
-  const int b = cache->b, hkv = cache->hkv, dh = cache->dh, dtype = cache->dtype, page_size = cache->page_size;
-  float* mass = cache->mass;
+  const int b = cache->b, hkv = cache->hkv, dh = cache->dh, dtype = cache->dtype;
   if (hq < 1 || hq % hkv) return fail(ONE_ERR_INVALID, "paged attention: the query heads must be a multiple of the kv heads");
-  const int64_t slots = (int64_t)cache->max_pages * page_size;
-  // tiles, and the list's length rounded up to equal shares, in 31 bits
-  if ((int64_t)b * hq > 0x3fffffff || (int64_t)b * hq * (slots / 64 + 1) > 0x7fffffff - kMaxSms * kPaPerSm)
-    return fail(ONE_ERR_UNSUPPORTED, "paged attention: too many rows");
-  const size_t need = one_paged_attention_workspace_bytes(b, hq, hkv, dh, page_size, cache->max_pages, dtype, mass != nullptr);
-  if (need && (!workspace || workspace_bytes < need)) return fail(ONE_ERR_INVALID, "workspace too small");
-  p.q = q; p.q_bs = q_batch_stride; p.q_hs = q_head_stride; p.G = hq / hkv;
-  const int rows = paged_rows(dtype, p.G);
-  p.hv_per_kv = (p.G + rows - 1) / rows;
-  p.q_vec = (reinterpret_cast<uintptr_t>(q) & 15) == 0 && q_batch_stride % 8 == 0 && q_head_stride % 8 == 0;
-  while ((1 << p.div_s) < page_size) ++p.div_s;
-  p.div_m = (uint32_t)((1ull << (31 + p.div_s)) / page_size + 1);
-  p.div_s += 31;
-  p.scale_log2 = scale * 1.4426950408889634f;
-  p.mass = mass; p.mass_width = cache->mass_width; p.out = out;
-  const PagedWs w(b, hq, rows, pad_dh(dh), slots, mass != nullptr);
-  uint8_t* ws = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(workspace) + 255) & ~uintptr_t(255));
-  p.part_ml = reinterpret_cast<float*>(ws + w.part_ml);
-  p.part_o = reinterpret_cast<float*>(ws + w.part_o);
-  p.row_ml = reinterpret_cast<float*>(ws + w.row_ml);
-  p.parts = reinterpret_cast<int2*>(ws + w.segs);
-  p.scores = mass ? reinterpret_cast<float*>(ws + w.scores) : nullptr;
-  p.score_ld = w.score_ld;
-  const bool split = paged_split((int64_t)b * hkv * p.hv_per_kv, slots) || (mass && p.hv_per_kv > 1);
+  const size_t need = one_paged_attention_workspace_bytes(b, hq, hkv, dh, cache->page_size, cache->max_pages, dtype, cache->mass != nullptr);
+  const int rows = paged_rows(dtype, hq / hkv);
+  bool split;
+  rc = plan_attention(p, split, cache, q, q_batch_stride, q_head_stride, hq, rows, scale, out, workspace, workspace_bytes, need);
+  if (rc) return rc;
   cudaStream_t st = (cudaStream_t)stream;
   const int d = pad_dh(dh);
   if (dtype == ONE_DTYPE_F32) {

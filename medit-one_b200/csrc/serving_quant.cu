@@ -93,35 +93,57 @@ extern "C" int one_paged_quant_read(const one_paged_quant_cache* cache, const in
   return launched(dtype == ONE_DTYPE_F32 ? read(float(0)) : read(__nv_bfloat16()), "paged read");
 }
 
+namespace {
+
+// Query heads that one pass over a kv head's cache serves.
+int quant_rows(int dtype, int G) { return dtype != ONE_DTYPE_F32 && G > 8 ? 16 : 8; }
+
+template <int BITS>
+int attend_bits(PagedAttn& p, bool split, int dtype, int rows, cudaStream_t st) {
+  auto dims = [&](auto dh) -> int {
+    constexpr int DH = decltype(dh)::value;
+    return dtype == ONE_DTYPE_F32 ? attend<PaQuant<DH, BITS, PQ_PAIR>>(p, split, st)
+           : rows == 16           ? attend<PaQuant<DH, BITS, PQ_16>>(p, split, st)
+                                  : attend<PaQuant<DH, BITS, PQ_8>>(p, split, st);
+  };
+  switch (pad_dh(p.c.Dh)) {
+    case 32: return dims(Int<32>());
+    case 64: return dims(Int<64>());
+    case 96: return dims(Int<96>());
+    default: return dims(Int<128>());
+  }
+}
+
+}  // namespace
+
 extern "C" size_t one_paged_quant_attention_workspace_bytes(int32_t b, int32_t hq, int32_t hkv, int32_t dh, int32_t page_size,
                                                             int32_t max_pages, int32_t dtype, int32_t with_mass) {
-  if (b < 1 || hq < 1 || hkv < 1 || dh < 1 || page_size < 1 || max_pages < 1) return 0;
-  return with_mass ? (size_t)b * hq * max_pages * page_size * 4 : 0;
+  if (hq < 1 || hkv < 1) return 0;
+  return attention_bytes(b, hq, hkv, dh, quant_rows(dtype, hq / hkv), page_size, max_pages, with_mass != 0);
 }
 
 extern "C" int one_paged_quant_attention(const one_paged_quant_cache* cache, const void* q, int64_t q_batch_stride,
                                          int64_t q_head_stride, int32_t hq, float scale, int32_t dtype, void* out,
                                          void* workspace, size_t workspace_bytes, void* stream) {
   if (!q || !out) return fail(ONE_ERR_INVALID, "paged attention: null argument");
-  QuantAttnParams p = {};
-  int rc = check_quant(p.m, cache);
+  PagedQuant m = {};
+  int rc = check_quant(m, cache);
   if (!rc) rc = check_dtype(dtype);
   if (rc) return rc;
   const int b = cache->b, hkv = cache->hkv, dh = cache->dh;
   if (hq < 1 || hq % hkv) return fail(ONE_ERR_INVALID, "paged attention: the query heads must be a multiple of the kv heads");
-  const int64_t slots = (int64_t)cache->max_pages * cache->page_size;
-  if ((int64_t)b * hq > 0x3fffffff) return fail(ONE_ERR_UNSUPPORTED, "paged attention: too many rows");
+  const int rows = quant_rows(dtype, hq / hkv);
   const size_t need = one_paged_quant_attention_workspace_bytes(b, hq, hkv, dh, cache->page_size, cache->max_pages, dtype, cache->mass != nullptr);
-  if (need && (!workspace || workspace_bytes < need)) return fail(ONE_ERR_INVALID, "workspace too small");
-  p.q = q; p.q_bs = q_batch_stride; p.q_hs = q_head_stride; p.G = hq / hkv; p.scale_log2 = scale * 1.4426950408889634f;
-  p.mass = cache->mass; p.mass_width = cache->mass_width; p.out = out;
-  p.scores = cache->mass ? (float*)workspace : nullptr; p.score_ld = slots;
-  auto run = [&](auto t) {
-    using T = decltype(t);
-    return cache->bits == 4 ? launch(quant_attn_kernel<T, 4>, dim3((unsigned)(b * hkv)), dim3(128), 0, (cudaStream_t)stream, p)
-                            : launch(quant_attn_kernel<T, 8>, dim3((unsigned)(b * hkv)), dim3(128), 0, (cudaStream_t)stream, p);
-  };
-  return launched(dtype == ONE_DTYPE_F32 ? run(float(0)) : run(__nv_bfloat16()), "paged attention");
+  PagedAttn p = {};
+  p.c = m.c; p.scales = (const uint8_t*)m.scales; p.s_stride = 2 * m.s_stride; p.row = m.row;
+  const int64_t at = reinterpret_cast<uintptr_t>(m.c.k) | reinterpret_cast<uintptr_t>(m.c.v) | m.c.k_stride | m.c.v_stride;
+  p.vec16 = ((at | m.row) & 15) == 0;
+  p.run = ((at | reinterpret_cast<uintptr_t>(m.scales) | p.s_stride) & 15) == 0;
+  bool split;
+  rc = plan_attention(p, split, cache, q, q_batch_stride, q_head_stride, hq, rows, scale, out, workspace, workspace_bytes, need);
+  if (rc) return rc;
+  return cache->bits == 4 ? attend_bits<4>(p, split, dtype, rows, (cudaStream_t)stream)
+                          : attend_bits<8>(p, split, dtype, rows, (cudaStream_t)stream);
 }
 
 extern "C" int one_paged_quant_evict(const one_paged_quant_cache* cache, const int32_t* dst_table, int64_t dst_stride,
