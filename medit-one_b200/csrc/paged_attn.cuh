@@ -31,7 +31,7 @@ namespace one {
 constexpr int kPaWarps = 4;
 constexpr size_t kSmPerSm = 228 * 1024;    // shared memory of an SM, 1 KB of it per CTA reserved
 constexpr int kMaxSms = 160;            // SMs that share a list, at most
-constexpr int kPaPerSm = 3;             // CTAs of these kernels on an SM, at most
+constexpr int kPaPerSm = 5;             // CTAs of these kernels on an SM, at most
 
 struct PagedAttn {
   PagedCache c;
@@ -65,11 +65,17 @@ ONE_DEVINL int pa_tiles(const PagedCache& c, int b) {
   return (paged_length(c, b, SITE_PAGED_ATTN) + TILE - 1) / TILE;
 }
 
-// Tiles in the list (the host keeps them, rounded up to shares, below 2^31). Every warp computes them for itself.
-template <int TILE>
+// Units of the list (the host keeps them, rounded up to shares, below 2^31): a segment's tiles, and MORE for
+// a segment's begin and end. Every warp computes them for itself.
+template <int TILE, int MORE>
+ONE_DEVINL int pa_units(const PagedCache& c, int b) {
+  const int n = pa_tiles<TILE>(c, b);
+  return MORE && n ? n + MORE : n;
+}
+template <int TILE, int MORE>
 ONE_DEVINL int pa_total(const PagedAttn& p) {
   int n = 0;
-  for (int b = threadIdx.x & 31; b < p.c.B; b += 32) n += pa_tiles<TILE>(p.c, b);
+  for (int b = threadIdx.x & 31; b < p.c.B; b += 32) n += pa_units<TILE, MORE>(p.c, b);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
   return n * p.c.Hkv * p.hv_per_kv;
@@ -77,17 +83,18 @@ ONE_DEVINL int pa_total(const PagedAttn& p) {
 
 // A place in the list: tile `tile` of query-head tile gi of kv head kv of sequence b; the heads' tiles
 // of a sequence follow one another, ng query-head tiles per kv head.
-template <int TILE>
+template <int TILE, int MORE = 0>
 struct PaCursor {
   int b, kv, gi, tile, tiles, len;
   ONE_DEVINL void load(const PagedCache& c) {
     len = b < c.B ? paged_length(c, b, SITE_PAGED_ATTN) : 0;
     tiles = (len + TILE - 1) / TILE;
   }
-  ONE_DEVINL void seek(const PagedCache& c, int ng, int w) {
+  // To unit w; returns how many of the segment's first MORE units are left.
+  ONE_DEVINL int seek(const PagedCache& c, int ng, int w) {
     const int HV = c.Hkv * ng, lane = threadIdx.x & 31;
     for (int base = 0; base < c.B; base += 32) {
-      const int n = base + lane < c.B ? pa_tiles<TILE>(c, base + lane) : 0;
+      const int n = base + lane < c.B ? pa_units<TILE, MORE>(c, base + lane) : 0;
       int incl = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -100,16 +107,17 @@ struct PaCursor {
         b = base + src;
         w -= HV * __shfl_sync(0xffffffffu, incl - n, src);
         load(c);
-        const int hv = w / tiles;
-        tile = w - hv * tiles;
+        const int hv = w / (tiles + MORE), at = w - hv * (tiles + MORE) - MORE;
+        tile = max(at, 0);
         kv = hv / ng;
         gi = hv - kv * ng;
-        return;
+        return max(-at, 0);
       }
       w -= HV * __shfl_sync(0xffffffffu, incl, 31);
     }
     b = c.B;
     kv = gi = tile = tiles = len = 0;
+    return 0;
   }
   // Returns whether this is another segment.
   ONE_DEVINL bool next(const PagedCache& c, int ng) {
@@ -228,6 +236,8 @@ struct PaBf16 {
   static constexpr int kGroup = 64 * DH;               // bytes of a group's keys and values
   static constexpr int kStages = 2, kStagesFew = 3;    // where CTAs fill the SMs; where they are few
   static constexpr int kExtra = 0;                     // further shared bytes per warp
+  static constexpr int kMaxPerSm = 3;                  // CTAs on an SM, at most
+  static constexpr int kSegmentUnits = 0;              // tiles that a segment's begin and end take in a list
   ONE_DEVINL static float weight(float x) { return ex2_approx(x); }  // 2^x as consume computes it
   uint32_t qa[WIDE ? 2 : 1][KC][4];
   float o[NT][4];
@@ -448,6 +458,7 @@ struct PaF32 {
   static constexpr int kValues = 64 * DH;
   static constexpr int kStages = DH == 32 ? 4 : DH == 96 ? 2 : 3, kStagesFew = kStages;
   static constexpr int kExtra = ROWS * DH * 4 + 16 * ROWS * 4;  // q [ROWS][DH], weights [16][ROWS]
+  static constexpr int kMaxPerSm = 3, kSegmentUnits = 0;
   ONE_DEVINL static float weight(float x) { return exp2f(x); }   // 2^x as consume computes it
   float o[ROWS][VC];
   float m, l;  // of head c
@@ -625,7 +636,7 @@ struct PaSmem {
   static constexpr int kLeast = kInStage ? 0 : kPaWarps * kSums, kMost = kLeast > 9216 ? kLeast : 9216;
   static constexpr int kApart = 2 * kPaWarps * kSums < kMost ? 2 * kPaWarps * kSums : kMost;
   static constexpr int kTotal = kSum + (SPLIT ? kApart : E::ROWS * E::DH * 4);
-  static constexpr int kPerSm = kSmPerSm / (kTotal + 1024) < 3 ? kSmPerSm / (kTotal + 1024) : 3;
+  static constexpr int kPerSm = kSmPerSm / (kTotal + 1024) < E::kMaxPerSm ? kSmPerSm / (kTotal + 1024) : E::kMaxPerSm;
 };
 
 // PA_LIST: CTA i takes the i-th share of the list. Otherwise a cluster of p.cluster CTAs (1 to 8) takes
@@ -648,15 +659,17 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, MODE>::kPerSm) paged_
   const int ng = p.hv_per_kv;
   pdl_wait();
   pdl_launch_dependents();
-  PaCursor<TILE> cur;
-  int left, share = 0;  // tiles to do; a full share
+  constexpr int MORE = SPLIT ? E::kSegmentUnits : 0;
+  PaCursor<TILE, MORE> cur;
+  int left, share = 0;  // units to do; a full share
   if (SPLIT) {
-    const int total = pa_total<TILE>(p);
+    const int total = pa_total<TILE, MORE>(p);
     share = max(1, (total + p.ranges - 1) / p.ranges);
     const long long w0 = (long long)share * blockIdx.x;
     if (w0 >= total) return;
     left = min(share, total - (int)w0);
-    cur.seek(c, ng, (int)w0);
+    left -= cur.seek(c, ng, (int)w0);
+    if (MORE && left <= 0) return;  // the share ends before the segment's first tile
   } else {
     const int seg = blockIdx.x / p.cluster, rank = blockIdx.x % p.cluster, HV = c.Hkv * ng;
     cur.b = seg / HV;
@@ -667,10 +680,17 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, MODE>::kPerSm) paged_
     left = (int)((int64_t)cur.tiles * (rank + 1) / p.cluster) - cur.tile;
   }
   // ---- the copying side: page numbers are asked for one tile ahead of the copies. RUN: one per group;
-  //      otherwise lane t and lane 16 + t look slot t up.
-  PaCursor<TILE> src = cur;
+  //      otherwise lane t and lane 16 + t look slot t up. LOOK, which is RUN of a quantised cache, whose
+  //      groups are a quarter as long: lane i has those of the i-th group from tile `look` of the segment on,
+  //      so that one look serves 32 groups.
+  constexpr bool LOOK = RUN && E::kQuant;
+  PaCursor<TILE, MORE> src = cur;
   int to_copy = left, pg[GR], row[GR];  // page and first element (kQuant: row) in its head of each group
-  uint32_t live[S::kStages][GR];        // slots in use of the tiles in the ring, the oldest first
+  uint32_t live[S::kStages][GR];        // slots in use of the tiles in the ring, the oldest first (not LOOK)
+  uint32_t dead = 0;                    // LOOK: a bit per group without a page of the tiles in the ring, the newest last
+  static_assert(!LOOK || S::kStages * GR <= 32, "bits");
+  int look = 0, looked = 0;
+  uint32_t k_at = 0, v_at = 0, s_at = 0;  // of this lane's group, in 16 bytes
 #pragma unroll
   for (int k = 0; k < S::kStages; ++k)
 #pragma unroll
@@ -689,6 +709,20 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, MODE>::kPerSm) paged_
   };
   int ahead = src.len - src.tile * TILE - mine;  // slots from this warp's first one to the end
   auto ask = [&] {
+    if constexpr (LOOK) {
+      if (src.tile - look < 32 / GR && looked != 0) return;
+      look = src.tile;
+      looked = 1;
+      const int t = (look + lane / GR) * TILE + warp * (16 * GR) + lane % GR * 16;
+      pg[0] = -1;
+      row[0] = -1;
+      if (t < src.len) {
+        const int index = (int)(((uint64_t)(uint32_t)t * p.div_m) >> p.div_s);
+        row[0] = t - index * c.page_size;
+        pg[0] = table[index];
+      }
+      return;
+    } else {
     const int t0 = src.len - ahead;
 #pragma unroll
     for (int g = 0; g < GR; ++g) {
@@ -699,10 +733,55 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, MODE>::kPerSm) paged_
         pg[g] = table[index];
       }
     }
+    }
   };
   const int ks = (int)c.k_stride, vs = (int)c.v_stride;
   uint32_t put = 0, get = 0;  // byte offsets of stages
   auto copy = [&] {
+    if constexpr (LOOK) {
+      dead <<= GR;
+      if (to_copy > 0) {
+        if (looked == 1) {  // the page numbers have come
+          looked = 2;
+          const bool good = (uint32_t)pg[0] < (uint32_t)c.num_pages;
+          if (!good && row[0] >= 0) set_err(c.err, ERR_BAD_ARG, SITE_QUANT_ATTN);
+          const int64_t n = good ? pg[0] : 0, r = good ? row[0] : 0;
+          k_at = good ? (uint32_t)((n * ks + r * p.row) >> 4) : 0xffffffffu;
+          v_at = (uint32_t)((n * vs + r * p.row) >> 4);
+          s_at = (uint32_t)((n * p.s_stride + r * E::SR) >> 4);
+        }
+#pragma unroll
+        for (int g = 0; g < GR; ++g) {
+          const int n = ahead - 16 * g;
+          const int from = (src.tile - look) * GR + g;
+          const uint32_t k16 = __shfl_sync(0xffffffffu, k_at, from), v16 = __shfl_sync(0xffffffffu, v_at, from);
+          const uint32_t s16 = __shfl_sync(0xffffffffu, s_at, from);
+          const uint32_t to = smem_u32(ring) + put + g * E::kGroup;
+          const uint8_t *kp = keys + (uint64_t)k16 * 16, *vp = values + (uint64_t)v16 * 16, *sp = scales + (uint64_t)s16 * 16;
+          if (n >= 16 && k16 != 0xffffffffu) {
+            E::template copy<true>(to, kp, vp, sp, 16);
+          } else if (n > 0 && k16 != 0xffffffffu) {
+            E::template copy<false>(to, kp, vp, sp, n);
+          } else {  // zeros: scales must be finite where the weights are 0
+            E::template copy<false>(to, keys, values, scales, 0);
+            dead |= 1u << g;
+          }
+        }
+        if (--to_copy > 0) {
+          ahead -= TILE;
+          if (src.next(c, ng)) {
+            to_copy -= MORE;
+            segment();
+            looked = 0;
+            ahead = src.len - src.tile * TILE - mine;
+          }
+          ask();
+        }
+      }
+      cp_async_commit();
+      put = put + S::kStage == S::kWarp ? 0 : put + S::kStage;
+      return;
+    } else {
 #pragma unroll
     for (int k = 0; k + 1 < S::kStages; ++k)
 #pragma unroll
@@ -715,22 +794,8 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, MODE>::kPerSm) paged_
         const bool good = (uint32_t)pg[g] < (uint32_t)c.num_pages;
         if (!good && ahead > 16 * g) set_err(c.err, ERR_BAD_ARG, SITE_PAGED_ATTN);
         if constexpr (E::kQuant) {
-          const uint32_t at = smem_u32(to);
-          if (RUN) {
-            alive = 0;
-            if (good) {
-              const uint8_t* kp = keys + ((int64_t)pg[g] * ks + row[g] * p.row);
-              const uint8_t* vp = values + ((int64_t)pg[g] * vs + row[g] * p.row);
-              const uint8_t* sp = scales + ((int64_t)pg[g] * p.s_stride + row[g] * E::SR);
-              const int n = min(ahead - 16 * g, 16);
-              alive = (1u << n) - 1;
-              if (n == 16) E::template copy<true>(at, kp, vp, sp, 16);
-              else E::template copy<false>(at, kp, vp, sp, n);
-            }
-          } else {
-            alive = __ballot_sync(0xffffffffu, good) & 0xffffu;
-            if (alive) E::copy_any(at, p, keys, values, scales, good ? pg[g] : -1, row[g]);
-          }
+          alive = __ballot_sync(0xffffffffu, good) & 0xffffu;
+          E::copy_any(smem_u32(to), p, keys, values, scales, good ? pg[g] : -1, row[g]);
         } else if (RUN) {
           alive = 0;
           if (good) {
@@ -756,6 +821,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, MODE>::kPerSm) paged_
       if (--to_copy > 0) {
         ahead -= TILE;
         if (src.next(c, ng)) {
+          to_copy -= MORE;
           segment();
           ahead = src.len - src.tile * TILE - mine;
         }
@@ -764,6 +830,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, MODE>::kPerSm) paged_
     }
     cp_async_commit();
     put = put + S::kStage == S::kWarp ? 0 : put + S::kStage;
+    }
   };
   segment();
   if (to_copy == 0) ahead = 0;
@@ -791,12 +858,21 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, MODE>::kPerSm) paged_
       if (!copied) copy();
       copied = false;
       cp_async_wait<S::kStages - 1>();
-      uint32_t any = 0;
+      if constexpr (LOOK) {
+        const int n = cur.len - tile * TILE - warp * (16 * GR);
 #pragma unroll
-      for (int g = 0; g < GR; ++g) any |= live[0][g];
+        for (int g = 0; g < GR; ++g)
+          live[0][g] = dead >> ((S::kStages - 1) * GR + g) & 1 ? 0 : n - 16 * g >= 16 ? 0xffffu : n > 16 * g ? (1u << (n - 16 * g)) - 1 : 0;
+      }
+      uint32_t any = 0, all = 0xffffu;
+#pragma unroll
+      for (int g = 0; g < GR; ++g) any |= live[0][g], all &= live[0][g];
       __syncwarp();
-      if (any || p.scores)
-        eng.consume(p, ring + get, live[0], p.scores ? p.scores + hq0 * p.score_ld + tile * TILE + warp * (16 * GR) : nullptr, rows);
+      float* scores = p.scores ? p.scores + hq0 * p.score_ld + tile * TILE + warp * (16 * GR) : nullptr;
+      if (any || p.scores) {
+        if constexpr (E::kQuant) eng.consume(p, ring + get, live[0], all == 0xffffu, scores, rows);
+        else eng.consume(p, ring + get, live[0], scores, rows);
+      }
       __syncwarp();
       get = get + S::kStage == S::kWarp ? 0 : get + S::kStage;
       if (apart && tile + 1 == last) {
@@ -924,7 +1000,10 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, MODE>::kPerSm) paged_
     begun_inside = true;
     left -= last - first;
     cur.tile = last - 1;
-    if (left > 0) cur.next(c, ng);
+    if (left > 0) {
+      cur.next(c, ng);
+      left -= MORE;
+    }
   } while (left > 0);
 }
 
@@ -940,7 +1019,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
   using T = typename E::T;
   constexpr int ROWS = E::ROWS, DH = E::DH;
   __shared__ float4 red[kJoinThreads];
-  __shared__ float weight[kMaxSms * kPaPerSm];  // 2^(m - M) of each part
+  __shared__ float weight[kMaxSms * E::kMaxPerSm];  // 2^(m - M) of each part
   __shared__ float fin[2][128];                 // M and 1 / l of a kv head's query heads
   const PagedCache& c = p.c;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;

@@ -69,8 +69,8 @@ int paged_rows(int dtype, int G) { return dtype == ONE_DTYPE_F32 ? (G > 1 ? 4 : 
 struct PagedWs {
   size_t part_ml, part_o, row_ml, segs, scores, total;
   int64_t score_ld;
-  PagedWs(int b, int hq, int rows, int dh_pad, int64_t slots, bool mass) {
-    const size_t parts = 2 * (size_t)kMaxSms * kPaPerSm * rows;
+  PagedWs(int b, int hq, int rows, int dh_pad, int64_t slots, bool mass, int per_sm) {
+    const size_t parts = 2 * (size_t)kMaxSms * per_sm * rows;
     part_ml = 0;
     part_o = align256(parts * 8);
     row_ml = part_o + align256(parts * dh_pad * 4);
@@ -84,15 +84,15 @@ struct PagedWs {
 int pad_dh(int dh) { return dh <= 32 ? 32 : dh <= 64 ? 64 : dh <= 96 ? 96 : 128; }
 
 // What the attention over a cache of either kind, in p.c, asks of its arguments, and its plan; `rows` query
-// heads per pass. need: workspace bytes.
+// heads per pass, at most per_sm CTAs on an SM, `units` as E::kSegmentUnits. need: workspace bytes.
 template <typename S>
-int plan_attention(PagedAttn& p, bool& split, const S* cache, const void* q, int64_t q_bs, int64_t q_hs, int hq, int rows,
+int plan_attention(PagedAttn& p, bool& split, const S* cache, const void* q, int64_t q_bs, int64_t q_hs, int hq, int rows, int per_sm, int units,
                    float scale, void* out, void* workspace, size_t workspace_bytes, size_t need) {
   const int b = cache->b, hkv = cache->hkv, dh = cache->dh, page_size = cache->page_size;
   float* mass = cache->mass;
   const int64_t slots = (int64_t)cache->max_pages * page_size;
-  // tiles, and the list's length rounded up to equal shares, in 31 bits
-  if ((int64_t)b * hq > 0x3fffffff || (int64_t)b * hq * (slots / 64 + 1) > 0x7fffffff - kMaxSms * kPaPerSm)
+  // tiles and a segment's further units, and the list's length rounded up to equal shares, in 31 bits
+  if ((int64_t)b * hq > 0x3fffffff || (int64_t)b * hq * (slots / 64 + 1 + units) > 0x7fffffff - kMaxSms * per_sm)
     return fail(ONE_ERR_UNSUPPORTED, "paged attention: too many rows");
   if (need && (!workspace || workspace_bytes < need)) return fail(ONE_ERR_INVALID, "workspace too small");
   p.q = q; p.q_bs = q_bs; p.q_hs = q_hs; p.G = hq / hkv;
@@ -101,7 +101,7 @@ int plan_attention(PagedAttn& p, bool& split, const S* cache, const void* q, int
   paged_divisor(p, page_size);
   p.scale_log2 = scale * 1.4426950408889634f;
   p.mass = mass; p.mass_width = cache->mass_width; p.out = out;
-  const PagedWs w(b, hq, rows, pad_dh(dh), slots, mass != nullptr);
+  const PagedWs w(b, hq, rows, pad_dh(dh), slots, mass != nullptr, per_sm);
   uint8_t* ws = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(workspace) + 255) & ~uintptr_t(255));
   p.part_ml = reinterpret_cast<float*>(ws + w.part_ml);
   p.part_o = reinterpret_cast<float*>(ws + w.part_o);
@@ -113,12 +113,12 @@ int plan_attention(PagedAttn& p, bool& split, const S* cache, const void* q, int
   return ONE_OK;
 }
 
-size_t attention_bytes(int b, int hq, int hkv, int dh, int rows, int page_size, int max_pages, bool with_mass) {
+size_t attention_bytes(int b, int hq, int hkv, int dh, int rows, int page_size, int max_pages, bool with_mass, int per_sm) {
   if (b < 1 || hq < 1 || hkv < 1 || dh < 1 || page_size < 1 || max_pages < 1) return 0;
   const int64_t slots = (int64_t)max_pages * page_size;
   const int tiles = (hq / hkv + rows - 1) / rows;
   if (!with_mass && !paged_split((int64_t)b * hkv * tiles, slots)) return 0;
-  return PagedWs(b, hq, rows, pad_dh(dh), slots, with_mass).total + 256;
+  return PagedWs(b, hq, rows, pad_dh(dh), slots, with_mass, per_sm).total + 256;
 }
 
 template <typename E, bool RUN, PaMode MODE>

@@ -13,12 +13,14 @@
 //  - keys: sum q u starts from -z sum q (per query and group, computed once), so u needs no subtraction.
 //    That costs three bits of the fp32 sum at most (u reaches 2 z, c reaches z).
 //  - values: u - z by one packed addition (exact), since a sum over many slots of p z would drown o.
-//  - ldmatrix brings a 16-byte piece of eight rows to the lanes as the B operands need it: keys straight,
-//    values transposed, where a 16-bit element is four (two) codes of one slot.
+//  - the codes are the instructions' 16 rows: S^T = K Q^T has slots as rows, O^T = V^T P^T dims, and the
+//    queries are the 8 columns. ldmatrix brings 16-byte pieces of eight slots to the lanes as both need
+//    them: keys straight, values transposed, where a 16-bit element is four (two) codes of one slot.
+//    movmatrix turns the weights from rows to columns in between.
 // fp16 takes q scaled by a power of two to [2^14, 2^15) per row, and 2^(s - m) vs 2^15 / ref with ref a
 // power of two above all the value scales so far, which rises like the running maximum. A bf16 q is exact
-// in it down to 2^-38 of the row's largest; the weights are rounded to 11 bits (2^-11 each, against the
-// output's 2^-8). In fp32, q and the weights are two fp16 parts (22 bits), in rows r and r + 8.
+// in it down to 2^-34 of the row's largest; the weights are rounded to 11 bits (2^-11 each, against the
+// output's 2^-8). In fp32, q and the weights are two fp16 parts (22 bits), in neighbouring columns.
 #pragma once
 
 #include "paged_attn.cuh"
@@ -26,18 +28,18 @@
 
 namespace one {
 
-ONE_DEVINL void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, float c0,
-                              float c1) {
+ONE_DEVINL void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1,
+                              const float (&c)[4]) {
   asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %11, %11};"
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
-ONE_DEVINL void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+// Lane (r, c) holds elements 2 c, 2 c + 1 of row r of an 8 x 8 matrix; the same of the transposed one
+ONE_DEVINL uint32_t movmatrix_trans(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
 }
 template <bool TRANS>
 ONE_DEVINL void ldmatrix_x4(uint32_t (&w)[4], uint32_t at) {
@@ -84,38 +86,44 @@ ONE_DEVINL void cp_async_some(uint32_t s, const void* g, int bytes) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(s), "l"(g), "n"(N), "r"(bytes) : "memory");
 }
 
-// PQ_8, PQ_16: bf16, up to 8 or 16 query heads. PQ_PAIR: fp32, up to 8, in two parts.
-enum PqKind { PQ_8, PQ_16, PQ_PAIR };
+// PQ_8, PQ_16: bf16, up to 8 or 16 query heads. PQ_PAIR4, PQ_PAIR8: fp32 in two parts, up to 4 or 8.
+enum PqKind { PQ_8, PQ_16, PQ_PAIR4, PQ_PAIR8 };
+
+#ifndef PQ_UNITS
+#define PQ_UNITS 2
+#endif
+constexpr int kQuantUnits = PQ_UNITS;
 
 template <int DH_, int BITS_, PqKind KIND>
 struct PaQuant {
-  using T = std::conditional_t<KIND == PQ_PAIR, float, __nv_bfloat16>;
+  static constexpr bool PAIR = KIND == PQ_PAIR4 || KIND == PQ_PAIR8;
+  using T = std::conditional_t<PAIR, float, __nv_bfloat16>;
   using Cell = uint8_t;
   static constexpr bool kQuant = true;
-  static constexpr int DH = DH_, BITS = BITS_, ROWS = KIND == PQ_16 ? 16 : 8;
-  static constexpr bool SECOND = KIND != PQ_8;           // rows r + 8 are used
-  static constexpr int RW = KIND == PQ_16 ? 2 : 1;       // query rows of a lane
+  static constexpr int DH = DH_, BITS = BITS_, ROWS = KIND == PQ_16 ? 16 : KIND == PQ_PAIR4 ? 4 : 8;
+  static constexpr int NL = KIND == PQ_16 || KIND == PQ_PAIR8 ? 2 : 1;  // tiles of 8 columns
+  static constexpr int QL = PAIR ? 1 : 2, NQ = NL * QL;  // queries of a lane, per tile and in all
   static constexpr int G = DH / kQuantGroup;             // groups of a row
   static constexpr int RB = DH * BITS / 8, CH = RB / 16; // bytes and pieces of a row
   static constexpr int SR = 4 * G;                       // bytes of a slot's scales
   static constexpr int PG = CH / G;                      // pieces of a group: 1 or 2
-  static constexpr int NT = DH / 8;                      // value tiles
-  static constexpr int EP = BITS == 4 ? 4 : 2;           // codes in 16 bits
+  static constexpr int NT = DH / 16;                     // value tiles
   static constexpr float kZero = BITS == 4 ? 8.f : 128.f;
   static constexpr int kGroup = 16 * (2 * RB + SR);      // bytes of 16 slots
   static constexpr int kValues = 16 * RB, kScales = 32 * RB;
   static constexpr int kGroups = DH * BITS <= 128 ? 4 : DH * BITS <= 256 ? 2 : 1;  // 16-slot groups per warp and step
   static constexpr int TILE = 16 * kGroups * kPaWarps;
   static constexpr int kStages = 4, kStagesFew = kStages;
-  static constexpr int kExtra = 0;
-  ONE_DEVINL static float weight(float x) { return KIND == PQ_PAIR ? exp2f(x) : ex2_approx(x); }
+  static constexpr int kExtra = 0, kMaxPerSm = NL == 1 ? (DH <= 96 ? 4 : 3) : DH <= 64 ? 3 : 2;
+  static constexpr int kSegmentUnits = kQuantUnits;
+  ONE_DEVINL static float weight(float x) { return PAIR ? exp2f(x) : ex2_approx(x); }
 
-  uint32_t qa[G][2][SECOND ? 4 : 2];  // A operands of a group's two products: a0, a2, then a1, a3
-  float off[G][SECOND ? 2 : 1];       // -z sum q, rows r and r + 8
-  float fac[RW];                      // from sums to scores
-  float o[NT][4];
-  float m[RW], l[RW];
-  float ref, mult;                    // above all the value scales so far; 2^15 / ref
+  uint32_t qb[NL][G][2][2];  // B operands of a group's two products
+  float off[NL][G][4];       // -z sum q as their first sums
+  float fac[NQ];             // from sums to scores, positive
+  float o[NL][NT][4];
+  float m[NQ], l[NQ];
+  float ref, mult;           // above all the value scales so far; 2^15 / ref
 
   // Where piece ch of row `row` lies: eight rows' pieces ch are on different banks, and a 128-byte line of
   // memory stays one.
@@ -171,32 +179,31 @@ struct PaQuant {
   ONE_DEVINL void begin(const PagedAttn& p, uint8_t*, const T* q, int rows) {
     const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
 #pragma unroll
-    for (int w = 0; w < RW; ++w) {
-      // this lane's 8 dims of each group, in memory's order: 8 c .., or 4 c .. and 16 + 4 c ..
+    for (int n = 0; n < NL; ++n) {
+      // column r: query 8 n + r, or part r % 2 of query 4 n + r / 2. This lane's 8 dims of each group in memory's
+      // order: 8 c .., or 4 c .. and 16 + 4 c ..
+      const int row = PAIR ? 4 * n + (r >> 1) : 8 * n + r;
       float x[G][8], top = 0.f;
-      const bool in = r + 8 * w < rows;
-      const T* y = q + (int64_t)(r + 8 * w) * p.q_hs;
+      const T* y = q + (int64_t)row * p.q_hs;
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        const int d0 = g * 32 + (BITS == 4 ? 8 * c : 4 * c);
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
-          const int d = d0 + (BITS == 4 ? 4 : 16) * hh;
-          const bool there = in && d < p.c.Dh;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) x[g][4 * hh + i] = 0.f;
-          if (there) {
+          const int d = g * 32 + (BITS == 4 ? 8 * c + 4 * hh : 4 * c + 16 * hh);
+          float* z = x[g] + 4 * hh;
+          z[0] = z[1] = z[2] = z[3] = 0.f;
+          if (row < rows && d < p.c.Dh) {
             if (p.q_vec) {
-              if constexpr (KIND == PQ_PAIR) {
+              if constexpr (PAIR) {
                 const float4 u = *reinterpret_cast<const float4*>(y + d);
-                x[g][4 * hh] = u.x; x[g][4 * hh + 1] = u.y; x[g][4 * hh + 2] = u.z; x[g][4 * hh + 3] = u.w;
+                z[0] = u.x; z[1] = u.y; z[2] = u.z; z[3] = u.w;
               } else {
                 const uint2 u = *reinterpret_cast<const uint2*>(y + d);
-                x[g][4 * hh] = bf2_lo(u.x); x[g][4 * hh + 1] = bf2_hi(u.x); x[g][4 * hh + 2] = bf2_lo(u.y); x[g][4 * hh + 3] = bf2_hi(u.y);
+                z[0] = bf2_lo(u.x); z[1] = bf2_hi(u.x); z[2] = bf2_lo(u.y); z[3] = bf2_hi(u.y);
               }
             } else {
 #pragma unroll
-              for (int i = 0; i < 4; ++i) x[g][4 * hh + i] = ld<T>(y + d + i);
+              for (int i = 0; i < 4; ++i) z[i] = ld<T>(y + d + i);
             }
           }
         }
@@ -205,66 +212,64 @@ struct PaQuant {
       }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const int e = (int)(__float_as_uint(top) >> 23);                  // 0 .. 255
-      const float up = __uint_as_float((uint32_t)min(254, 268 - e) << 23);  // 2^14 over the power of two of top
-      // acc = sum q up u 2^-24; halves that read as u 2^-20 have q up 2^-4
-      fac[w] = p.scale_log2 * 1024.f * __uint_as_float((uint32_t)max(14, e) << 23);
+      const int e = (int)(__float_as_uint(top) >> 23);                      // 0 .. 255
+      // 2^14 over the power of two of top, with the scale's sign
+      const float up = copysignf(__uint_as_float((uint32_t)min(254, 268 - e) << 23), p.scale_log2);
+      // sums are q up u 2^-24; halves that read as u 2^-20 have q up 2^-4. A masked slot's -inf stays -inf
+      // under a scale of 0 (2^-126)
+      const float back = fmaxf(fabsf(p.scale_log2) * 1024.f * __uint_as_float((uint32_t)max(14, e) << 23), 1.17549435e-38f);
+      // lane (r, c) has columns 2 c and 2 c + 1 of the sums
+#pragma unroll
+      for (int h = 0; h < QL; ++h) fac[n * QL + h] = __shfl_sync(0xffffffffu, back, (2 * c + h) * 4);
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        float sum[2] = {0.f, 0.f};
+        float sum = 0.f;
 #pragma unroll
         for (int k = 0; k < 2; ++k)
 #pragma unroll
           for (int a = 0; a < 2; ++a) {
-            const float f = BITS == 4 && k ? up * 0.0625f : up, back = BITS == 4 && k ? 16.f : 1.f;
-            // dims of this register in memory's order
+            const float f = BITS == 4 && k ? up * 0.0625f : up;
             const int i0 = BITS == 4 ? k + 2 * a : 4 * k + a, i1 = BITS == 4 ? i0 + 4 : i0 + 2;
             const float y0 = x[g][i0] * f, y1 = x[g][i1] * f;
-            const uint32_t hi = pack_f16x2(y0, y1);
-            sum[0] += (f16_lo(hi) + f16_hi(hi)) * back;
-            if (KIND == PQ_16 && w == 1) {
-              qa[g][k][(SECOND ? 2 : 0) + a] = hi;
-            } else {
-              qa[g][k][a] = hi;
-            }
-            if constexpr (KIND == PQ_PAIR) {
-              const uint32_t lo = pack_f16x2(y0 - f16_lo(hi), y1 - f16_hi(hi));
-              sum[1] += (f16_lo(lo) + f16_hi(lo)) * back;
-              qa[g][k][2 + a] = lo;
-            }
+            uint32_t w = pack_f16x2(y0, y1);
+            if (PAIR && (r & 1)) w = pack_f16x2(y0 - f16_lo(w), y1 - f16_hi(w));
+            qb[n][g][k][a] = w;
+            sum += (f16_lo(w) + f16_hi(w)) * (BITS == 4 && k ? 16.f : 1.f);
           }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        sum *= -kZero * 5.9604644775390625e-8f;
 #pragma unroll
-        for (int j = 0; j < (KIND == PQ_PAIR ? 2 : 1); ++j) {
-          sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 1);
-          sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 2);
-          off[g][SECOND ? w + j : 0] = sum[j] * (-kZero * 5.9604644775390625e-8f);
-        }
+        for (int i = 0; i < 4; ++i) off[n][g][i] = __shfl_sync(0xffffffffu, sum, (2 * c + (i & 1)) * 4);
       }
-      m[w] = -INFINITY;
-      l[w] = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+      m[i] = -INFINITY;
+      l[i] = 0.f;
     }
     ref = 0.f;
     mult = 0.f;
 #pragma unroll
-    for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    for (int n = 0; n < NL; ++n)
+#pragma unroll
+      for (int i = 0; i < NT; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
   }
 
-  // A slot pair's scales: element i of slot h (K_0 .., V_0 ..)
+  // A slot's scales, K_0 .., V_0 ..
   struct Scales {
-    uint32_t w[2 * G];
-    ONE_DEVINL float operator()(int h, int i) const {
-      const uint32_t x = w[h * G + i / 2];
-      return i & 1 ? bf2_hi(x) : bf2_lo(x);
-    }
-    ONE_DEVINL void load(uint32_t at) {
-      if constexpr (G % 2 == 0) {
-#pragma unroll
-        for (int k = 0; k < 2 * G; k += 4)
-          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[k]), "=r"(w[k + 1]), "=r"(w[k + 2]), "=r"(w[k + 3]) : "r"(at + k * 4) : "memory");
+    uint32_t w[G];
+    ONE_DEVINL float operator[](int i) const { return i & 1 ? bf2_hi(w[i / 2]) : bf2_lo(w[i / 2]); }
+    ONE_DEVINL void load(const uint8_t* at) {
+      if constexpr (G == 4) {
+        const uint4 u = *reinterpret_cast<const uint4*>(at);
+        w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+      } else if constexpr (G == 2) {
+        const uint2 u = *reinterpret_cast<const uint2*>(at);
+        w[0] = u.x; w[1] = u.y;
       } else {
 #pragma unroll
-        for (int k = 0; k < 2 * G; k += 2)
-          asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[k]), "=r"(w[k + 1]) : "r"(at + k * 4) : "memory");
+        for (int k = 0; k < G; ++k) w[k] = reinterpret_cast<const uint32_t*>(at)[k];
       }
     }
   };
@@ -286,148 +291,156 @@ struct PaQuant {
     return (e ? w >> 8 : w) & 0x00ff00ffu;
   }
 
-  ONE_DEVINL void consume(const PagedAttn& p, const uint8_t* stage, const uint32_t (&live)[kGroups], float* scores, int rows) {
+  // kGroups x 16 slots, all of them copied; live: a bit per slot of each group, full: all are set. scores:
+  // row 0's scores of these slots, or null.
+  ONE_DEVINL void consume(const PagedAttn& p, const uint8_t* stage, const uint32_t (&live)[kGroups], bool full, float* scores, int rows) {
     const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
     const uint32_t base = smem_u32(stage);
-    float pr[kGroups][RW][4];
+    float pr[kGroups][NQ][2];  // slots r and r + 8
+    Scales sc[kGroups][2];
     float vmax = 0.f;
 #pragma unroll
     for (int i = 0; i < kGroups; ++i) {
-      float s[RW][4];
+      uint32_t kw[CH][2];
+      pieces<false>(kw, base + i * kGroup);
+      sc[i][0].load(stage + i * kGroup + kScales + r * SR);
+      sc[i][1].load(stage + i * kGroup + kScales + (r + 8) * SR);
 #pragma unroll
-      for (int w = 0; w < RW; ++w) s[w][0] = s[w][1] = s[w][2] = s[w][3] = 0.f;
-      if (live[i]) {
-        uint32_t kw[CH][2];
-        pieces<false>(kw, base + i * kGroup);
+      for (int g = 0; g < G; ++g) {
+        const uint32_t *w0 = kw[g * PG], *w1 = kw[g * PG + PG - 1];
+        // 4 bits: halves 0, 2 then 1, 3 of the words; 8 bits: bytes 0, 1 of the first piece, then of the second
+        constexpr int e1 = BITS == 4 ? 2 : 1, e2 = BITS == 4 ? 1 : 0, e3 = BITS == 4 ? 3 : 1;
+        const uint32_t x[2][4] = {{open(w0[0], 0), open(w0[1], 0), open(w0[0], e1), open(w0[1], e1)},
+                                  {open(w1[0], e2), open(w1[1], e2), open(w1[0], e3), open(w1[1], e3)}};
+        const float ks[2] = {sc[i][0][g], sc[i][1][g]};
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          Scales sc;
-          sc.load(base + i * kGroup + kScales + (8 * j + 2 * c) * SR);
+        for (int n = 0; n < NL; ++n) {
+          float a[4];
+          mma_f16_16816(a, x[0][0], x[0][1], x[0][2], x[0][3], qb[n][g][0][0], qb[n][g][0][1], off[n][g]);
+          mma_f16_16816(a, x[1][0], x[1][1], x[1][2], x[1][3], qb[n][g][1][0], qb[n][g][1][1], a);
 #pragma unroll
-          for (int g = 0; g < G; ++g) {
-            float a[4];
-            const uint32_t w0 = kw[g * PG][j], w1 = kw[g * PG + PG - 1][j];
-            // 4 bits: halves 0, 2 then 1, 3 of the word; 8 bits: bytes 0, 1 of the first word, then of the second
-            mma_f16_16816(a, qa[g][0][0], SECOND ? qa[g][0][SECOND ? 2 : 0] : 0, qa[g][0][1], SECOND ? qa[g][0][SECOND ? 3 : 0] : 0,
-                          open(w0, 0), open(w0, BITS == 4 ? 2 : 1), off[g][0], SECOND ? off[g][SECOND ? 1 : 0] : 0.f);
-            mma_f16_16816(a, qa[g][1][0], SECOND ? qa[g][1][SECOND ? 2 : 0] : 0, qa[g][1][1], SECOND ? qa[g][1][SECOND ? 3 : 0] : 0,
-                          open(w1, BITS == 4 ? 1 : 0), open(w1, BITS == 4 ? 3 : 1));
+          for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const float ks = sc(h, g);
-              if constexpr (KIND == PQ_PAIR) {
-                s[0][2 * j + h] += ks * (a[h] + a[2 + h]);
-              } else {
-#pragma unroll
-                for (int w = 0; w < RW; ++w) s[w][2 * j + h] += ks * a[2 * w + h];
-              }
-              vmax = fmaxf(vmax, sc(h, G + g));
+            for (int k = 0; k < QL; ++k) {
+              const float y = PAIR ? a[2 * h] + a[2 * h + 1] : a[2 * h + k];
+              float& s = pr[i][n * QL + k][h];
+              s = g ? s + ks[h] * y : ks[h] * y;
             }
+        }
+        vmax = fmax3(vmax, sc[i][0][G + g], sc[i][1][G + g]);
+      }
+    }
+    if (!full) {
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          if (!(live[i] >> (r + 8 * h) & 1)) {
+#pragma unroll
+            for (int t = 0; t < NQ; ++t) pr[i][t][h] = -INFINITY;
+          }
+    }
+    if (scores) {
+#pragma unroll
+      for (int t = 0; t < NQ; ++t) {
+        const int row = PAIR ? 4 * t + c : 8 * (t >> 1) + 2 * c + (t & 1);
+        if (row < rows) {
+          float* to = scores + row * p.score_ld + r;
+#pragma unroll
+          for (int i = 0; i < kGroups; ++i) {
+            to[16 * i] = pr[i][t][0] * fac[t];
+            to[16 * i + 8] = pr[i][t][1] * fac[t];
           }
         }
       }
-#pragma unroll
-      for (int w = 0; w < RW; ++w)
-#pragma unroll
-        for (int t = 0; t < 4; ++t) pr[i][w][t] = s[w][t] * fac[w];
-      if (live[i] != 0xffffu) {
-        const uint32_t mine = live[i] >> (2 * c);
-#pragma unroll
-        for (int w = 0; w < RW; ++w)
-#pragma unroll
-          for (int t = 0; t < 4; ++t)
-            if (!(mine >> (8 * (t >> 1) + (t & 1)) & 1)) pr[i][w][t] = -INFINITY;
-      }
-      if (scores) {
-#pragma unroll
-        for (int w = 0; w < RW; ++w)
-          if (r + 8 * w < rows) {
-            float* to = scores + (r + 8 * w) * p.score_ld + 16 * i + 2 * c;
-            *reinterpret_cast<float2*>(to) = make_float2(pr[i][w][0], pr[i][w][1]);
-            *reinterpret_cast<float2*>(to + 8) = make_float2(pr[i][w][2], pr[i][w][3]);
-          }
-      }
     }
-    float mx[RW];
+    float mx[NQ];
     bool rises = vmax > ref;
 #pragma unroll
-    for (int w = 0; w < RW; ++w) {
-      mx[w] = pr[0][w][0];
+    for (int t = 0; t < NQ; ++t) {
+      mx[t] = fmaxf(pr[0][t][0], pr[0][t][1]);
 #pragma unroll
-      for (int i = 0; i < kGroups; ++i) {
-        mx[w] = fmax3(mx[w], pr[i][w][0], pr[i][w][1]);
-        mx[w] = fmax3(mx[w], pr[i][w][2], pr[i][w][3]);
-      }
-      mx[w] = fmaxf(mx[w], __shfl_xor_sync(0xffffffffu, mx[w], 1));
-      mx[w] = fmaxf(mx[w], __shfl_xor_sync(0xffffffffu, mx[w], 2));
-      rises |= mx[w] > m[w];
+      for (int i = 1; i < kGroups; ++i) mx[t] = fmax3(mx[t], pr[i][t][0], pr[i][t][1]);
+      mx[t] *= fac[t];
+      rises |= mx[t] > m[t];
     }
+    // m stands in all the lanes of a column, so that it rises for none of them alone
     if (__any_sync(0xffffffffu, rises)) {
-      vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, 1));
-      vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, 2));
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) {
+        vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, d));
+#pragma unroll
+        for (int t = 0; t < NQ; ++t) mx[t] = fmaxf(mx[t], __shfl_xor_sync(0xffffffffu, mx[t], d));
+      }
       float f = 1.f;
-      if (vmax > ref) {  // the same in all lanes; 2^-100 < ref <= 2^127
+      if (vmax > ref) {  // 2^-100 < ref <= 2^127
         const uint32_t e = min(max(__float_as_uint(vmax) >> 23, 27u) + 1, 254u);
-        const float now = __uint_as_float(e << 23);
-        f = ref == 0.f ? 0.f : ref * __uint_as_float((254 - min(e, 253u)) << 23) * (e == 254u ? 0.5f : 1.f);
-        ref = now;
+        f = ref * __uint_as_float((254 - min(e, 253u)) << 23) * (e == 254u ? 0.5f : 1.f);
+        ref = __uint_as_float(e << 23);
         mult = __uint_as_float((269 - e) << 23);
       }
-      float a[2];
+      float a[NQ];
 #pragma unroll
-      for (int w = 0; w < RW; ++w) {
-        const float mn = fmaxf(m[w], mx[w]);
-        a[w] = weight(m[w] - (mn == -INFINITY ? 0.f : mn));
-        m[w] = mn;
-        l[w] *= a[w];
-        a[w] *= f;
+      for (int t = 0; t < NQ; ++t) {
+        const float mn = fmaxf(m[t], mx[t]);
+        a[t] = weight(m[t] - (mn == -INFINITY ? 0.f : mn));
+        m[t] = mn;
+        l[t] *= a[t];
+        a[t] *= f;
       }
-      if (RW == 1) a[1] = a[0];
 #pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        o[i][0] *= a[0]; o[i][1] *= a[0];
-        if (SECOND) { o[i][2] *= a[1]; o[i][3] *= a[1]; }
-      }
+      for (int n = 0; n < NL; ++n)
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) o[n][i][k] *= a[PAIR ? n : 2 * n + (k & 1)];
     }
-    float ms[RW];
+    float ms[NQ];
 #pragma unroll
-    for (int w = 0; w < RW; ++w) ms[w] = m[w] == -INFINITY ? 0.f : m[w];
+    for (int t = 0; t < NQ; ++t) ms[t] = m[t] == -INFINITY ? 0.f : m[t];
 #pragma unroll
     for (int i = 0; i < kGroups; ++i) {
-      if (!live[i]) continue;
 #pragma unroll
-      for (int w = 0; w < RW; ++w) {
-        float (&x)[4] = pr[i][w];
-#pragma unroll
-        for (int t = 0; t < 4; ++t) x[t] = weight(x[t] - ms[w]);
-        l[w] += (x[0] + x[1]) + (x[2] + x[3]);
-#pragma unroll
-        for (int t = 0; t < 4; ++t) x[t] *= mult;
+      for (int t = 0; t < NQ; ++t) {
+        float(&x)[2] = pr[i][t];
+        x[0] = weight(fmaf(x[0], fac[t], -ms[t]));
+        x[1] = weight(fmaf(x[1], fac[t], -ms[t]));
+        l[t] += x[0] + x[1];
+        x[0] *= mult;
+        x[1] *= mult;
       }
       uint32_t vw[CH][2];
       pieces<true>(vw, base + i * kGroup + kValues);
-      Scales sc[2];
-      sc[0].load(base + i * kGroup + kScales + 2 * c * SR);
-      sc[1].load(base + i * kGroup + kScales + (8 + 2 * c) * SR);
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        uint32_t hi[2], second[2] = {0, 0};
+        uint32_t b[NL][2];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float v0 = sc[j](0, G + g), v1 = sc[j](1, G + g);
-          const float y0 = pr[i][0][2 * j] * v0, y1 = pr[i][0][2 * j + 1] * v1;
-          hi[j] = pack_f16x2(y0, y1);
-          if constexpr (KIND == PQ_PAIR) second[j] = pack_f16x2(y0 - f16_lo(hi[j]), y1 - f16_hi(hi[j]));
-          if constexpr (KIND == PQ_16) second[j] = pack_f16x2(pr[i][RW - 1][2 * j] * v0, pr[i][RW - 1][2 * j + 1] * v1);
+        for (int h = 0; h < 2; ++h) {
+          const float v = sc[i][h][G + g];
+#pragma unroll
+          for (int n = 0; n < NL; ++n) {
+            uint32_t w;
+            if constexpr (PAIR) {
+              const float y = pr[i][n][h] * v;
+              const uint32_t hi = pack_f16x2(y, 0.f);
+              w = pack_f16x2(y, y - f16_lo(hi));
+            } else {
+              w = pack_f16x2(pr[i][2 * n][h] * v, pr[i][2 * n + 1][h] * v);
+            }
+            b[n][h] = movmatrix_trans(w);
+          }
         }
 #pragma unroll
-        for (int k = 0; k < PG; ++k)
+        for (int k = 0; k < 2; ++k) {
+          // rows r and r + 8: halves k and k + 2 (4 bits), bytes 0 and 1 of piece k (8 bits)
+          const uint32_t* w = vw[BITS == 4 ? g : 2 * g + k];
+          const int e = BITS == 4 ? k : 0, f = BITS == 4 ? k + 2 : 1;
+          const uint32_t z = BITS == 8 || k ? 0x80808080u : 0x80088008u;  // -z 2^-24 (bytes), -z 2^-20, -z 2^-24
+          const uint32_t x[4] = {f16x2_add(open(w[0], e), z), f16x2_add(open(w[0], f), z), f16x2_add(open(w[1], e), z),
+                                 f16x2_add(open(w[1], f), z)};
 #pragma unroll
-          for (int e = 0; e < EP; ++e) {
-            const uint32_t z = BITS == 8 || (e & 1) ? 0x80808080u : 0x80088008u;  // -z 2^-24 (bytes), -z 2^-20, -z 2^-24
-            mma_f16_16816(o[(g * PG + k) * EP + e], hi[0], second[0], hi[1], second[1],
-                          f16x2_add(open(vw[g * PG + k][0], e), z), f16x2_add(open(vw[g * PG + k][1], e), z));
-          }
+          for (int n = 0; n < NL; ++n) mma_f16_16816(o[n][2 * g + k], x[0], x[1], x[2], x[3], b[n][0], b[n][1], o[n][2 * g + k]);
+        }
       }
     }
   }
@@ -436,25 +449,24 @@ struct PaQuant {
   ONE_DEVINL void leave(float* ml, float* so, int rows) {
     const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
 #pragma unroll
-    for (int w = 0; w < RW; ++w) {
-      float t = l[w];
-      t += __shfl_xor_sync(0xffffffffu, t, 1);
-      t += __shfl_xor_sync(0xffffffffu, t, 2);
-      if (c == 0) {
-        ml[2 * (r + 8 * w)] = m[w];
-        ml[2 * (r + 8 * w) + 1] = t;
+    for (int t = 0; t < NQ; ++t) {
+      const int n = t / QL, h = t % QL, row = PAIR ? 4 * n + c : 8 * n + 2 * c + h;
+      float x = l[t];
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+      if (r == 0) {
+        ml[2 * row] = m[t];
+        ml[2 * row + 1] = x;
       }
-      if (r + 8 * w >= rows) continue;
+      if (row >= rows) continue;
 #pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        const int e = i % EP, d0 = i / EP * 8 * EP + e;  // column n is dim d0 + EP n
-        const float f = BITS == 4 && (e & 1) ? 32.f : 512.f;  // 2^24 or 2^20, over mult's 2^15
+      for (int i = 0; i < NT; ++i)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float x = KIND == PQ_PAIR ? o[i][h] + o[i][2 + h] : o[i][2 * w + h];
-          so[(r + 8 * w) * DH + d0 + EP * (2 * c + h)] = x * f * ref;
+        for (int k = 0; k < 2; ++k) {  // rows r and r + 8 of the tile
+          const int d = BITS == 4 ? i / 2 * 32 + 4 * r + i % 2 + 2 * k : i * 16 + 2 * r + k;
+          const float f = BITS == 4 && i % 2 ? 32.f : 512.f;  // 2^20 or 2^24, over mult's 2^15
+          so[row * DH + d] = (PAIR ? o[n][i][2 * k] + o[n][i][2 * k + 1] : o[n][i][2 * k + h]) * f * ref;
         }
-      }
     }
   }
 };

@@ -32,7 +32,7 @@ int check_cache(PagedCache& c, const one_paged_cache* x) {
 extern "C" size_t one_paged_attention_workspace_bytes(int32_t b, int32_t hq, int32_t hkv, int32_t dh, int32_t page_size,
                                                       int32_t max_pages, int32_t dtype, int32_t with_mass) {
   if (hq < 1 || hkv < 1) return 0;
-  return attention_bytes(b, hq, hkv, dh, paged_rows(dtype, hq / hkv), page_size, max_pages, with_mass != 0);
+  return attention_bytes(b, hq, hkv, dh, paged_rows(dtype, hq / hkv), page_size, max_pages, with_mass != 0, 3);
 }
 
 extern "C" int one_paged_attention(const one_paged_cache* cache, const void* q, int64_t q_batch_stride,
@@ -47,7 +47,7 @@ extern "C" int one_paged_attention(const one_paged_cache* cache, const void* q, 
   const size_t need = one_paged_attention_workspace_bytes(b, hq, hkv, dh, cache->page_size, cache->max_pages, dtype, cache->mass != nullptr);
   const int rows = paged_rows(dtype, hq / hkv);
   bool split;
-  rc = plan_attention(p, split, cache, q, q_batch_stride, q_head_stride, hq, rows, scale, out, workspace, workspace_bytes, need);
+  rc = plan_attention(p, split, cache, q, q_batch_stride, q_head_stride, hq, rows, 3, 0, scale, out, workspace, workspace_bytes, need);
   if (rc) return rc;
   cudaStream_t st = (cudaStream_t)stream;
   const int d = pad_dh(dh);

@@ -96,15 +96,15 @@ extern "C" int one_paged_quant_read(const one_paged_quant_cache* cache, const in
 namespace {
 
 // Query heads that one pass over a kv head's cache serves.
-int quant_rows(int dtype, int G) { return dtype != ONE_DTYPE_F32 && G > 8 ? 16 : 8; }
+int quant_rows(int dtype, int G) { return dtype == ONE_DTYPE_F32 ? (G > 4 ? 8 : 4) : G > 8 ? 16 : 8; }
 
 template <int BITS>
 int attend_bits(PagedAttn& p, bool split, int dtype, int rows, cudaStream_t st) {
   auto dims = [&](auto dh) -> int {
     constexpr int DH = decltype(dh)::value;
-    return dtype == ONE_DTYPE_F32 ? attend<PaQuant<DH, BITS, PQ_PAIR>>(p, split, st)
-           : rows == 16           ? attend<PaQuant<DH, BITS, PQ_16>>(p, split, st)
-                                  : attend<PaQuant<DH, BITS, PQ_8>>(p, split, st);
+    if (dtype == ONE_DTYPE_F32)
+      return rows == 4 ? attend<PaQuant<DH, BITS, PQ_PAIR4>>(p, split, st) : attend<PaQuant<DH, BITS, PQ_PAIR8>>(p, split, st);
+    return rows == 16 ? attend<PaQuant<DH, BITS, PQ_16>>(p, split, st) : attend<PaQuant<DH, BITS, PQ_8>>(p, split, st);
   };
   switch (pad_dh(p.c.Dh)) {
     case 32: return dims(Int<32>());
@@ -119,7 +119,7 @@ int attend_bits(PagedAttn& p, bool split, int dtype, int rows, cudaStream_t st) 
 extern "C" size_t one_paged_quant_attention_workspace_bytes(int32_t b, int32_t hq, int32_t hkv, int32_t dh, int32_t page_size,
                                                             int32_t max_pages, int32_t dtype, int32_t with_mass) {
   if (hq < 1 || hkv < 1) return 0;
-  return attention_bytes(b, hq, hkv, dh, quant_rows(dtype, hq / hkv), page_size, max_pages, with_mass != 0);
+  return attention_bytes(b, hq, hkv, dh, quant_rows(dtype, hq / hkv), page_size, max_pages, with_mass != 0, kPaPerSm);
 }
 
 extern "C" int one_paged_quant_attention(const one_paged_quant_cache* cache, const void* q, int64_t q_batch_stride,
@@ -138,9 +138,11 @@ extern "C" int one_paged_quant_attention(const one_paged_quant_cache* cache, con
   p.c = m.c; p.scales = (const uint8_t*)m.scales; p.s_stride = 2 * m.s_stride; p.row = m.row;
   const int64_t at = reinterpret_cast<uintptr_t>(m.c.k) | reinterpret_cast<uintptr_t>(m.c.v) | m.c.k_stride | m.c.v_stride;
   p.vec16 = ((at | m.row) & 15) == 0;
-  p.run = ((at | reinterpret_cast<uintptr_t>(m.scales) | p.s_stride) & 15) == 0;
+  // and places in a pool count in 32 bits of 16 bytes
+  p.run = ((at | reinterpret_cast<uintptr_t>(m.scales) | p.s_stride) & 15) == 0 &&
+          cache->num_pages * std::max({m.c.k_stride, m.c.v_stride, p.s_stride}) < 0xfffffff0ll * 16;
   bool split;
-  rc = plan_attention(p, split, cache, q, q_batch_stride, q_head_stride, hq, rows, scale, out, workspace, workspace_bytes, need);
+  rc = plan_attention(p, split, cache, q, q_batch_stride, q_head_stride, hq, rows, kPaPerSm, kQuantUnits, scale, out, workspace, workspace_bytes, need);
   if (rc) return rc;
   return cache->bits == 4 ? attend_bits<4>(p, split, dtype, rows, (cudaStream_t)stream)
                           : attend_bits<8>(p, split, dtype, rows, (cudaStream_t)stream);
