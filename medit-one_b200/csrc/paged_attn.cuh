@@ -690,6 +690,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, MODE>::kPerSm) paged_
   uint32_t dead = 0;                    // LOOK: a bit per group without a page of the tiles in the ring, the newest last
   static_assert(!LOOK || S::kStages * GR <= 32, "bits");
   int look = 0, looked = 0;
+  uint32_t gone = 0;                    // lanes whose group lacks its page
   uint32_t k_at = 0, v_at = 0, s_at = 0;  // of this lane's group, in 16 bytes
 #pragma unroll
   for (int k = 0; k < S::kStages; ++k)
@@ -743,28 +744,37 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, MODE>::kPerSm) paged_
       if (to_copy > 0) {
         if (looked == 1) {  // the page numbers have come
           looked = 2;
-          const bool good = (uint32_t)pg[0] < (uint32_t)c.num_pages;
-          if (!good && row[0] >= 0) set_err(c.err, ERR_BAD_ARG, SITE_QUANT_ATTN);
+          const bool good = (uint32_t)pg[0] < (uint32_t)c.num_pages, missing = !good && row[0] >= 0;
+          if (missing) set_err(c.err, ERR_BAD_ARG, SITE_QUANT_ATTN);
           const int64_t n = good ? pg[0] : 0, r = good ? row[0] : 0;
-          k_at = good ? (uint32_t)((n * ks + r * p.row) >> 4) : 0xffffffffu;
+          k_at = (uint32_t)((n * ks + r * p.row) >> 4);
           v_at = (uint32_t)((n * vs + r * p.row) >> 4);
           s_at = (uint32_t)((n * p.s_stride + r * E::SR) >> 4);
+          gone = __ballot_sync(0xffffffffu, missing);
         }
+        const uint32_t to = smem_u32(ring) + put;
+        const int from = (src.tile - look) * GR;
+        auto place = [&](int g, const uint8_t*& kp, const uint8_t*& vp, const uint8_t*& sp) {
+          kp = keys + (uint64_t)__shfl_sync(0xffffffffu, k_at, from + g) * 16;
+          vp = values + (uint64_t)__shfl_sync(0xffffffffu, v_at, from + g) * 16;
+          sp = scales + (uint64_t)__shfl_sync(0xffffffffu, s_at, from + g) * 16;
+        };
+        if (ahead >= 16 * GR && gone == 0) {
 #pragma unroll
-        for (int g = 0; g < GR; ++g) {
-          const int n = ahead - 16 * g;
-          const int from = (src.tile - look) * GR + g;
-          const uint32_t k16 = __shfl_sync(0xffffffffu, k_at, from), v16 = __shfl_sync(0xffffffffu, v_at, from);
-          const uint32_t s16 = __shfl_sync(0xffffffffu, s_at, from);
-          const uint32_t to = smem_u32(ring) + put + g * E::kGroup;
-          const uint8_t *kp = keys + (uint64_t)k16 * 16, *vp = values + (uint64_t)v16 * 16, *sp = scales + (uint64_t)s16 * 16;
-          if (n >= 16 && k16 != 0xffffffffu) {
-            E::template copy<true>(to, kp, vp, sp, 16);
-          } else if (n > 0 && k16 != 0xffffffffu) {
-            E::template copy<false>(to, kp, vp, sp, n);
-          } else {  // zeros: scales must be finite where the weights are 0
-            E::template copy<false>(to, keys, values, scales, 0);
-            dead |= 1u << g;
+          for (int g = 0; g < GR; ++g) {
+            const uint8_t *kp, *vp, *sp;
+            place(g, kp, vp, sp);
+            E::template copy<true>(to + g * E::kGroup, kp, vp, sp, 16);
+          }
+        } else {
+#pragma unroll 1
+          for (int g = 0; g < GR; ++g) {
+            const uint8_t *kp, *vp, *sp;
+            place(g, kp, vp, sp);
+            // zeros for the rest: scales must be finite where the weights are 0
+            const bool there = ahead > 16 * g && !(gone >> (from + g) & 1);
+            E::template copy<false>(to + g * E::kGroup, kp, vp, sp, there ? min(ahead - 16 * g, 16) : 0);
+            if (!there) dead |= 1u << g;
           }
         }
         if (--to_copy > 0) {
@@ -858,20 +868,22 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, MODE>::kPerSm) paged_
       if (!copied) copy();
       copied = false;
       cp_async_wait<S::kStages - 1>();
+      float* scores = p.scores ? p.scores + hq0 * p.score_ld + tile * TILE + warp * (16 * GR) : nullptr;
+      __syncwarp();
       if constexpr (LOOK) {
         const int n = cur.len - tile * TILE - warp * (16 * GR);
+        const uint32_t no = dead >> (S::kStages - 1) * GR;
+        if (n > 0 || scores)
+          eng.consume(p, smem_u32(ring) + get, n >= 16 * GR && (no & ((1u << GR) - 1)) == 0,
+                      [&](int g) { return no >> g & 1 ? 0 : n >= 16 * g + 16 ? 0xffffu : n > 16 * g ? (1u << (n - 16 * g)) - 1 : 0u; }, scores, rows);
+      } else {
+        uint32_t any = 0, all = 0xffffu;
 #pragma unroll
-        for (int g = 0; g < GR; ++g)
-          live[0][g] = dead >> ((S::kStages - 1) * GR + g) & 1 ? 0 : n - 16 * g >= 16 ? 0xffffu : n > 16 * g ? (1u << (n - 16 * g)) - 1 : 0;
-      }
-      uint32_t any = 0, all = 0xffffu;
-#pragma unroll
-      for (int g = 0; g < GR; ++g) any |= live[0][g], all &= live[0][g];
-      __syncwarp();
-      float* scores = p.scores ? p.scores + hq0 * p.score_ld + tile * TILE + warp * (16 * GR) : nullptr;
-      if (any || p.scores) {
-        if constexpr (E::kQuant) eng.consume(p, ring + get, live[0], all == 0xffffu, scores, rows);
-        else eng.consume(p, ring + get, live[0], scores, rows);
+        for (int g = 0; g < GR; ++g) any |= live[0][g], all &= live[0][g];
+        if (any || scores) {
+          if constexpr (E::kQuant) eng.consume(p, smem_u32(ring) + get, all == 0xffffu, [&](int g) { return live[0][g]; }, scores, rows);
+          else eng.consume(p, ring + get, live[0], scores, rows);
+        }
       }
       __syncwarp();
       get = get + S::kStage == S::kWarp ? 0 : get + S::kStage;

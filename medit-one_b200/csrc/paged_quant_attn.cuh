@@ -12,7 +12,9 @@
 //    or the output's scaling, takes up the difference.
 //  - keys: sum q u starts from -z sum q (per query and group, computed once), so u needs no subtraction.
 //    That costs three bits of the fp32 sum at most (u reaches 2 z, c reaches z).
-//  - values: u - z by one packed addition (exact), since a sum over many slots of p z would drown o.
+//  - values: u - z by one packed addition (exact), since a sum over many slots of p z would drown o. (-z sum p
+//    as one more tile per step of 64 slots, from which its sums start, saves the additions and no time: 38.8
+//    and 40.3 us at 64 sequences up to 4096 x 12 x 64.)
 //  - the codes are the instructions' 16 rows: S^T = K Q^T has slots as rows, O^T = V^T P^T dims, and the
 //    queries are the 8 columns. ldmatrix brings 16-byte pieces of eight slots to the lanes as both need
 //    them: keys straight, values transposed, where a 16-bit element is four (two) codes of one slot.
@@ -30,15 +32,14 @@ namespace one {
 
 ONE_DEVINL void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1,
                               const float (&c)[4]) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 // Lane (r, c) holds elements 2 c, 2 c + 1 of row r of an 8 x 8 matrix; the same of the transposed one
 ONE_DEVINL uint32_t movmatrix_trans(uint32_t a) {
   uint32_t d;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
 template <bool TRANS>
@@ -86,8 +87,9 @@ ONE_DEVINL void cp_async_some(uint32_t s, const void* g, int bytes) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(s), "l"(g), "n"(N), "r"(bytes) : "memory");
 }
 
-// PQ_8, PQ_16: bf16, up to 8 or 16 query heads. PQ_PAIR4, PQ_PAIR8: fp32 in two parts, up to 4 or 8.
-enum PqKind { PQ_8, PQ_16, PQ_PAIR4, PQ_PAIR8 };
+// PQ_4, PQ_8, PQ_16: bf16, up to so many query heads. PQ_PAIR4, PQ_PAIR8: fp32 in two parts, up to 4 or 8.
+// PQ_4 leaves the odd columns empty, so that a lane has the scores of one head rather than of two.
+enum PqKind { PQ_4, PQ_8, PQ_16, PQ_PAIR4, PQ_PAIR8 };
 
 #ifndef PQ_UNITS
 #define PQ_UNITS 2
@@ -100,9 +102,10 @@ struct PaQuant {
   using T = std::conditional_t<PAIR, float, __nv_bfloat16>;
   using Cell = uint8_t;
   static constexpr bool kQuant = true;
-  static constexpr int DH = DH_, BITS = BITS_, ROWS = KIND == PQ_16 ? 16 : KIND == PQ_PAIR4 ? 4 : 8;
+  static constexpr int DH = DH_, BITS = BITS_, ROWS = KIND == PQ_16 ? 16 : KIND == PQ_4 || KIND == PQ_PAIR4 ? 4 : 8;
   static constexpr int NL = KIND == PQ_16 || KIND == PQ_PAIR8 ? 2 : 1;  // tiles of 8 columns
-  static constexpr int QL = PAIR ? 1 : 2, NQ = NL * QL;  // queries of a lane, per tile and in all
+  static constexpr bool ODD = KIND == PQ_8 || KIND == PQ_16;  // odd columns are queries of their own
+  static constexpr int QL = ODD ? 2 : 1, NQ = NL * QL;   // queries of a lane, per tile and in all
   static constexpr int G = DH / kQuantGroup;             // groups of a row
   static constexpr int RB = DH * BITS / 8, CH = RB / 16; // bytes and pieces of a row
   static constexpr int SR = 4 * G;                       // bytes of a slot's scales
@@ -111,10 +114,10 @@ struct PaQuant {
   static constexpr float kZero = BITS == 4 ? 8.f : 128.f;
   static constexpr int kGroup = 16 * (2 * RB + SR);      // bytes of 16 slots
   static constexpr int kValues = 16 * RB, kScales = 32 * RB;
-  static constexpr int kGroups = DH * BITS <= 128 ? 4 : DH * BITS <= 256 ? 2 : 1;  // 16-slot groups per warp and step
+  static constexpr int kGroups = DH * BITS <= 256 && NL == 1 ? 4 : DH * BITS <= 256 ? 2 : 1;  // 16-slot groups per warp and step
   static constexpr int TILE = 16 * kGroups * kPaWarps;
-  static constexpr int kStages = 4, kStagesFew = kStages;
-  static constexpr int kExtra = 0, kMaxPerSm = NL == 1 ? (DH <= 96 ? 4 : 3) : DH <= 64 ? 3 : 2;
+  static constexpr int kStages = kGroups == 4 ? 2 : 4, kStagesFew = kStages;
+  static constexpr int kExtra = 0, kMaxPerSm = NL == 1 ? (DH <= 64 ? 4 : 3) : DH <= 64 ? 3 : 2;
   static constexpr int kSegmentUnits = kQuantUnits;
   ONE_DEVINL static float weight(float x) { return PAIR ? exp2f(x) : ex2_approx(x); }
 
@@ -124,6 +127,7 @@ struct PaQuant {
   float o[NL][NT][4];
   float m[NQ], l[NQ];
   float ref, mult;           // above all the value scales so far; 2^15 / ref
+  uint32_t mine;             // where this lane's row of the first pieces lies
 
   // Where piece ch of row `row` lies: eight rows' pieces ch are on different banks, and a 128-byte line of
   // memory stays one.
@@ -131,6 +135,8 @@ struct PaQuant {
     const int x = CH == 2 || CH == 6 ? row >> 2 & 1 : CH == 4 ? row >> 1 & 3 : CH == 8 ? row & 7 : 0;
     return row * RB + (ch ^ x) * 16;
   }
+  // at(row, 2 i + up) from at(row, up), for even i
+  ONE_DEVINL static uint32_t step(uint32_t first, int i) { return (CH & (CH - 1)) == 0 ? first ^ (16 * i) : first + 16 * i; }
   // The copies of 16 rows that follow one another in memory; k, v, s from this lane's 16 bytes on. live:
   // of so many rows, the rest as zeros.
   template <bool ALL>
@@ -178,11 +184,12 @@ struct PaQuant {
 
   ONE_DEVINL void begin(const PagedAttn& p, uint8_t*, const T* q, int rows) {
     const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+    mine = at(8 * (lane >> 3 & 1) + (lane & 7), CH == 1 ? 0 : lane >> 4);
 #pragma unroll
     for (int n = 0; n < NL; ++n) {
-      // column r: query 8 n + r, or part r % 2 of query 4 n + r / 2. This lane's 8 dims of each group in memory's
+      // column r: query 8 n + r, or part r % 2 of query 4 n + r / 2 (PQ_4: the second part is 0). This lane's 8 dims of each group in memory's
       // order: 8 c .., or 4 c .. and 16 + 4 c ..
-      const int row = PAIR ? 4 * n + (r >> 1) : 8 * n + r;
+      const int row = ODD ? 8 * n + r : 4 * n + (r >> 1);
       float x[G][8], top = 0.f;
       const T* y = q + (int64_t)row * p.q_hs;
 #pragma unroll
@@ -232,7 +239,7 @@ struct PaQuant {
             const int i0 = BITS == 4 ? k + 2 * a : 4 * k + a, i1 = BITS == 4 ? i0 + 4 : i0 + 2;
             const float y0 = x[g][i0] * f, y1 = x[g][i1] * f;
             uint32_t w = pack_f16x2(y0, y1);
-            if (PAIR && (r & 1)) w = pack_f16x2(y0 - f16_lo(w), y1 - f16_hi(w));
+            if (!ODD && (r & 1)) w = PAIR ? pack_f16x2(y0 - f16_lo(w), y1 - f16_hi(w)) : 0;
             qb[n][g][k][a] = w;
             sum += (f16_lo(w) + f16_hi(w)) * (BITS == 4 && k ? 16.f : 1.f);
           }
@@ -260,30 +267,32 @@ struct PaQuant {
   struct Scales {
     uint32_t w[G];
     ONE_DEVINL float operator[](int i) const { return i & 1 ? bf2_hi(w[i / 2]) : bf2_lo(w[i / 2]); }
-    ONE_DEVINL void load(const uint8_t* at) {
-      if constexpr (G == 4) {
-        const uint4 u = *reinterpret_cast<const uint4*>(at);
-        w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
-      } else if constexpr (G == 2) {
-        const uint2 u = *reinterpret_cast<const uint2*>(at);
-        w[0] = u.x; w[1] = u.y;
-      } else {
+    ONE_DEVINL void load(uint32_t at) {
+      if constexpr (G == 4)
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
+      else if constexpr (G == 2)
+        asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at) : "memory");
+      else {
 #pragma unroll
-        for (int k = 0; k < G; ++k) w[k] = reinterpret_cast<const uint32_t*>(at)[k];
+        for (int k = 0; k < G; ++k) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[k]) : "r"(at + 4 * k) : "memory");
       }
+    }
+    // the values' times a power of two (bf16x2)
+    ONE_DEVINL void times(uint32_t f) {
+#pragma unroll
+      for (int k = G / 2; k < G; ++k) w[k] = bf2_mul(w[k], f);
     }
   };
   // [piece][slots 0-7, 8-15] of a group's 16 rows
   template <bool TRANS>
-  ONE_DEVINL static void pieces(uint32_t (&w)[CH][2], uint32_t base) {
-    const int lane = threadIdx.x & 31, row = 8 * (lane >> 3 & 1) + (lane & 7), up = lane >> 4;
+  ONE_DEVINL void pieces(uint32_t (&w)[CH][2], uint32_t base) const {
 #pragma unroll
     for (int i = 0; i + 1 < CH; i += 2) {
       uint32_t x[4];
-      ldmatrix_x4<TRANS>(x, base + at(row, i + up));
+      ldmatrix_x4<TRANS>(x, base + step(mine, i));
       w[i][0] = x[0]; w[i][1] = x[1]; w[i + 1][0] = x[2]; w[i + 1][1] = x[3];
     }
-    if constexpr (CH % 2) ldmatrix_x2<TRANS>(w[CH - 1][0], w[CH - 1][1], base + at(row, CH - 1));
+    if constexpr (CH % 2) ldmatrix_x2<TRANS>(w[CH - 1][0], w[CH - 1][1], base + step(mine, CH - 1));
   }
   // Two codes of a word as fp16: those at half (4 bits) or byte (8 bits) e of each of its 16-bit elements
   ONE_DEVINL static uint32_t open(uint32_t w, int e) {
@@ -291,11 +300,12 @@ struct PaQuant {
     return (e ? w >> 8 : w) & 0x00ff00ffu;
   }
 
-  // kGroups x 16 slots, all of them copied; live: a bit per slot of each group, full: all are set. scores:
+  // kGroups x 16 slots, all of them copied; live(i): a bit per slot of group i, full: all are set. scores:
   // row 0's scores of these slots, or null.
-  ONE_DEVINL void consume(const PagedAttn& p, const uint8_t* stage, const uint32_t (&live)[kGroups], bool full, float* scores, int rows) {
+  template <typename F>
+  ONE_DEVINL void consume(const PagedAttn& p, uint32_t base, bool full, F&& live, float* scores, int rows) {
     const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-    const uint32_t base = smem_u32(stage);
+    const uint32_t scale_at = base + kScales + r * SR;
     float pr[kGroups][NQ][2];  // slots r and r + 8
     Scales sc[kGroups][2];
     float vmax = 0.f;
@@ -303,8 +313,8 @@ struct PaQuant {
     for (int i = 0; i < kGroups; ++i) {
       uint32_t kw[CH][2];
       pieces<false>(kw, base + i * kGroup);
-      sc[i][0].load(stage + i * kGroup + kScales + r * SR);
-      sc[i][1].load(stage + i * kGroup + kScales + (r + 8) * SR);
+      sc[i][0].load(scale_at + i * kGroup);
+      sc[i][1].load(scale_at + i * kGroup + 8 * SR);
 #pragma unroll
       for (int g = 0; g < G; ++g) {
         const uint32_t *w0 = kw[g * PG], *w1 = kw[g * PG + PG - 1];
@@ -332,18 +342,19 @@ struct PaQuant {
     }
     if (!full) {
 #pragma unroll
-      for (int i = 0; i < kGroups; ++i)
+      for (int i = 0; i < kGroups; ++i) {
+        const uint32_t bits = live(i) >> r;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-          if (!(live[i] >> (r + 8 * h) & 1)) {
 #pragma unroll
-            for (int t = 0; t < NQ; ++t) pr[i][t][h] = -INFINITY;
-          }
+          for (int t = 0; t < NQ; ++t)
+            if (!(bits >> (8 * h) & 1)) pr[i][t][h] = -INFINITY;
+      }
     }
     if (scores) {
 #pragma unroll
       for (int t = 0; t < NQ; ++t) {
-        const int row = PAIR ? 4 * t + c : 8 * (t >> 1) + 2 * c + (t & 1);
+        const int row = ODD ? 8 * (t >> 1) + 2 * c + (t & 1) : 4 * t + c;
         if (row < rows) {
           float* to = scores + row * p.score_ld + r;
 #pragma unroll
@@ -393,11 +404,12 @@ struct PaQuant {
 #pragma unroll
         for (int i = 0; i < NT; ++i)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) o[n][i][k] *= a[PAIR ? n : 2 * n + (k & 1)];
+          for (int k = 0; k < 4; ++k) o[n][i][k] *= a[ODD ? 2 * n + (k & 1) : n];
     }
     float ms[NQ];
 #pragma unroll
     for (int t = 0; t < NQ; ++t) ms[t] = m[t] == -INFINITY ? 0.f : m[t];
+    const uint32_t mult2 = pack_bf16x2(mult, mult);
 #pragma unroll
     for (int i = 0; i < kGroups; ++i) {
 #pragma unroll
@@ -406,38 +418,34 @@ struct PaQuant {
         x[0] = weight(fmaf(x[0], fac[t], -ms[t]));
         x[1] = weight(fmaf(x[1], fac[t], -ms[t]));
         l[t] += x[0] + x[1];
-        x[0] *= mult;
-        x[1] *= mult;
       }
+      sc[i][0].times(mult2);
+      sc[i][1].times(mult2);
       uint32_t vw[CH][2];
       pieces<true>(vw, base + i * kGroup + kValues);
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        uint32_t b[NL][2];
+        uint32_t b[NL][2];  // the weights, times the values' scales
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const float v = sc[i][h][G + g];
 #pragma unroll
           for (int n = 0; n < NL; ++n) {
+            const float y = pr[i][n * QL][h] * v;
             uint32_t w;
-            if constexpr (PAIR) {
-              const float y = pr[i][n][h] * v;
-              const uint32_t hi = pack_f16x2(y, 0.f);
-              w = pack_f16x2(y, y - f16_lo(hi));
-            } else {
-              w = pack_f16x2(pr[i][2 * n][h] * v, pr[i][2 * n + 1][h] * v);
-            }
+            if constexpr (PAIR) w = pack_f16x2(y, y - f16_lo(pack_f16x2(y, 0.f)));
+            else w = pack_f16x2(y, ODD ? pr[i][n * QL + QL - 1][h] * v : 0.f);
             b[n][h] = movmatrix_trans(w);
           }
         }
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          // rows r and r + 8: halves k and k + 2 (4 bits), bytes 0 and 1 of piece k (8 bits)
+          // rows r and r + 8: halves 2 k and 2 k + 1 (4 bits), bytes 0 and 1 of piece k (8 bits)
           const uint32_t* w = vw[BITS == 4 ? g : 2 * g + k];
-          const int e = BITS == 4 ? k : 0, f = BITS == 4 ? k + 2 : 1;
-          const uint32_t z = BITS == 8 || k ? 0x80808080u : 0x80088008u;  // -z 2^-24 (bytes), -z 2^-20, -z 2^-24
-          const uint32_t x[4] = {f16x2_add(open(w[0], e), z), f16x2_add(open(w[0], f), z), f16x2_add(open(w[1], e), z),
-                                 f16x2_add(open(w[1], f), z)};
+          const int e = BITS == 4 ? 2 * k : 0;
+          constexpr uint32_t z0 = BITS == 4 ? 0x80088008u : 0x80808080u, z1 = 0x80808080u;  // -z as they read
+          const uint32_t x[4] = {f16x2_add(open(w[0], e), z0), f16x2_add(open(w[0], e + 1), z1), f16x2_add(open(w[1], e), z0),
+                                 f16x2_add(open(w[1], e + 1), z1)};
 #pragma unroll
           for (int n = 0; n < NL; ++n) mma_f16_16816(o[n][2 * g + k], x[0], x[1], x[2], x[3], b[n][0], b[n][1], o[n][2 * g + k]);
         }
@@ -450,7 +458,7 @@ struct PaQuant {
     const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
 #pragma unroll
     for (int t = 0; t < NQ; ++t) {
-      const int n = t / QL, h = t % QL, row = PAIR ? 4 * n + c : 8 * n + 2 * c + h;
+      const int n = t / QL, h = t % QL, row = ODD ? 8 * n + 2 * c + h : 4 * n + c;
       float x = l[t];
 #pragma unroll
       for (int d = 4; d < 32; d <<= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
@@ -463,8 +471,8 @@ struct PaQuant {
       for (int i = 0; i < NT; ++i)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {  // rows r and r + 8 of the tile
-          const int d = BITS == 4 ? i / 2 * 32 + 4 * r + i % 2 + 2 * k : i * 16 + 2 * r + k;
-          const float f = BITS == 4 && i % 2 ? 32.f : 512.f;  // 2^20 or 2^24, over mult's 2^15
+          const int d = BITS == 4 ? i / 2 * 32 + 4 * r + i % 2 * 2 + k : i * 16 + 2 * r + k;
+          const float f = BITS == 4 && k ? 32.f : 512.f;  // 2^20 or 2^24, over mult's 2^15
           so[row * DH + d] = (PAIR ? o[n][i][2 * k] + o[n][i][2 * k + 1] : o[n][i][2 * k + h]) * f * ref;
         }
     }

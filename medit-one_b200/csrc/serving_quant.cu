@@ -96,7 +96,7 @@ extern "C" int one_paged_quant_read(const one_paged_quant_cache* cache, const in
 namespace {
 
 // Query heads that one pass over a kv head's cache serves.
-int quant_rows(int dtype, int G) { return dtype == ONE_DTYPE_F32 ? (G > 4 ? 8 : 4) : G > 8 ? 16 : 8; }
+int quant_rows(int dtype, int G) { return G <= 4 ? 4 : dtype == ONE_DTYPE_F32 || G <= 8 ? 8 : 16; }
 
 template <int BITS>
 int attend_bits(PagedAttn& p, bool split, int dtype, int rows, cudaStream_t st) {
@@ -104,7 +104,9 @@ int attend_bits(PagedAttn& p, bool split, int dtype, int rows, cudaStream_t st) 
     constexpr int DH = decltype(dh)::value;
     if (dtype == ONE_DTYPE_F32)
       return rows == 4 ? attend<PaQuant<DH, BITS, PQ_PAIR4>>(p, split, st) : attend<PaQuant<DH, BITS, PQ_PAIR8>>(p, split, st);
-    return rows == 16 ? attend<PaQuant<DH, BITS, PQ_16>>(p, split, st) : attend<PaQuant<DH, BITS, PQ_8>>(p, split, st);
+    return rows == 16  ? attend<PaQuant<DH, BITS, PQ_16>>(p, split, st)
+           : rows == 8 ? attend<PaQuant<DH, BITS, PQ_8>>(p, split, st)
+                       : attend<PaQuant<DH, BITS, PQ_4>>(p, split, st);
   };
   switch (pad_dh(p.c.Dh)) {
     case 32: return dims(Int<32>());
