@@ -237,6 +237,7 @@ struct PaBf16 {
   static constexpr int kStages = 2, kStagesFew = 3;    // where CTAs fill the SMs; where they are few
   static constexpr int kExtra = 0;                     // further shared bytes per warp
   static constexpr int kMaxPerSm = 3;                  // CTAs on an SM, at most
+  static constexpr int kQueries = 0;                   // bytes of a segment's queries in a stage
   static constexpr int kSegmentUnits = 0;              // tiles that a segment's begin and end take in a list
   ONE_DEVINL static float weight(float x) { return ex2_approx(x); }  // 2^x as consume computes it
   uint32_t qa[WIDE ? 2 : 1][KC][4];
@@ -458,7 +459,7 @@ struct PaF32 {
   static constexpr int kValues = 64 * DH;
   static constexpr int kStages = DH == 32 ? 4 : DH == 96 ? 2 : 3, kStagesFew = kStages;
   static constexpr int kExtra = ROWS * DH * 4 + 16 * ROWS * 4;  // q [ROWS][DH], weights [16][ROWS]
-  static constexpr int kMaxPerSm = 3, kSegmentUnits = 0;
+  static constexpr int kMaxPerSm = 3, kSegmentUnits = 0, kQueries = 0;
   ONE_DEVINL static float weight(float x) { return exp2f(x); }   // 2^x as consume computes it
   float o[ROWS][VC];
   float m, l;  // of head c
@@ -621,7 +622,8 @@ enum PaMode { PA_LIST, PA_SEGMENT, PA_DEEP };
 template <typename E, PaMode MODE>
 struct PaSmem {
   static constexpr bool SPLIT = MODE == PA_LIST;
-  static constexpr int kStage = E::kGroup * E::kGroups;                  // bytes per warp
+  static constexpr int kSlots = E::kGroup * E::kGroups;                  // bytes per warp, and a segment's queries behind them
+  static constexpr int kStage = kSlots + E::kQueries;
   static constexpr int kStages = MODE == PA_DEEP ? E::kStagesFew : E::kStages;
   static constexpr int kWarp = kStage * kStages;
   static constexpr int kML = kPaWarps * kWarp;                           // [2][warps][ROWS][2]
@@ -692,6 +694,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, MODE>::kPerSm) paged_
   int look = 0, looked = 0;
   uint32_t gone = 0;                    // lanes whose group lacks its page
   uint32_t k_at = 0, v_at = 0, s_at = 0;  // of this lane's group, in 16 bytes
+  bool fresh = true;                    // LOOK: the next tile is the first of its piece
 #pragma unroll
   for (int k = 0; k < S::kStages; ++k)
 #pragma unroll
@@ -753,6 +756,11 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, MODE>::kPerSm) paged_
           gone = __ballot_sync(0xffffffffu, missing);
         }
         const uint32_t to = smem_u32(ring) + put;
+        if (fresh && p.q_vec) {  // the queries come with it, so that no piece waits for them
+          const int g0 = src.gi * E::ROWS;
+          E::copy_q(to + S::kSlots, p, (const T*)p.q + src.b * p.q_bs + ((int64_t)src.kv * p.G + g0) * p.q_hs, min(E::ROWS, p.G - g0));
+        }
+        fresh = false;
         const int from = (src.tile - look) * GR;
         auto place = [&](int g, const uint8_t*& kp, const uint8_t*& vp, const uint8_t*& sp) {
           kp = keys + (uint64_t)__shfl_sync(0xffffffffu, k_at, from + g) * 16;
@@ -783,6 +791,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, MODE>::kPerSm) paged_
             to_copy -= MORE;
             segment();
             looked = 0;
+            fresh = true;
             ahead = src.len - src.tile * TILE - mine;
           }
           ask();
@@ -863,7 +872,19 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, MODE>::kPerSm) paged_
     const int64_t hq0 = ((int64_t)cur.b * c.Hkv + kv) * p.G + g0;  // output row of this query-head tile
     const int first = cur.tile, last = min(cur.tiles, cur.tile + left);
     if (SPLIT && (cur.b >= c.B || last <= first)) break;  // lengths that changed during the call
-    eng.begin(p, extra, (const T*)p.q + cur.b * p.q_bs + ((int64_t)kv * p.G + g0) * p.q_hs, rows);
+    const T* q = (const T*)p.q + cur.b * p.q_bs + ((int64_t)kv * p.G + g0) * p.q_hs;
+    if constexpr (LOOK) {
+      if (!copied) copy();
+      copied = true;
+      cp_async_wait<S::kStages - 1>();
+      __syncwarp();
+      if (p.q_vec) eng.begin(p, reinterpret_cast<const T*>(ring + get + S::kSlots), E::DH, true, rows);
+      else eng.begin(p, q, p.q_hs, false, rows);
+    } else if constexpr (E::kQuant) {
+      eng.begin(p, q, p.q_hs, p.q_vec, rows);
+    } else {
+      eng.begin(p, extra, q, rows);
+    }
     for (int tile = first; tile < last; ++tile) {
       if (!copied) copy();
       copied = false;

@@ -114,10 +114,11 @@ struct PaQuant {
   static constexpr float kZero = BITS == 4 ? 8.f : 128.f;
   static constexpr int kGroup = 16 * (2 * RB + SR);      // bytes of 16 slots
   static constexpr int kValues = 16 * RB, kScales = 32 * RB;
-  static constexpr int kGroups = DH * BITS <= 256 && NL == 1 ? 4 : DH * BITS <= 256 ? 2 : 1;  // 16-slot groups per warp and step
+  static constexpr int kGroups = NL == 1 ? (DH * BITS <= 256 || BITS == 4 ? 4 : 2) : DH * BITS <= 256 ? 2 : 1;  // 16-slot groups per warp and step
   static constexpr int TILE = 16 * kGroups * kPaWarps;
-  static constexpr int kStages = kGroups == 4 ? 2 : 4, kStagesFew = kStages;
-  static constexpr int kExtra = 0, kMaxPerSm = NL == 1 ? (DH <= 64 ? 4 : 3) : DH <= 64 ? 3 : 2;
+  static constexpr int kStages = NL == 1 ? 2 : 4, kStagesFew = kStages;
+  static constexpr int kQueries = ROWS * DH * (int)sizeof(T);  // bytes of a segment's queries
+  static constexpr int kExtra = 0, kMaxPerSm = NL == 1 ? (DH <= 64 ? 4 : DH * BITS <= 512 ? 2 : 3) : DH <= 64 ? 3 : 2;
   static constexpr int kSegmentUnits = kQuantUnits;
   ONE_DEVINL static float weight(float x) { return PAIR ? exp2f(x) : ex2_approx(x); }
 
@@ -182,7 +183,14 @@ struct PaQuant {
     }
   }
 
-  ONE_DEVINL void begin(const PagedAttn& p, uint8_t*, const T* q, int rows) {
+  // The queries of a segment, 16 bytes per copy, into [ROWS][DH]; only where q_vec and Dh is DH
+  ONE_DEVINL static void copy_q(uint32_t to, const PagedAttn& p, const T* q, int rows) {
+    constexpr int PER = DH * (int)sizeof(T) / 16;
+    for (int e = threadIdx.x & 31; e < rows * PER; e += 32)
+      cp_async_some<16>(to + e * 16, q + (e / PER) * p.q_hs + e % PER * (16 / (int)sizeof(T)), 16);
+  }
+  // q: rows `stride` apart, of whole vectors where vec
+  ONE_DEVINL void begin(const PagedAttn& p, const T* q, int64_t stride, bool vec, int rows) {
     const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
     mine = at(8 * (lane >> 3 & 1) + (lane & 7), CH == 1 ? 0 : lane >> 4);
 #pragma unroll
@@ -191,7 +199,7 @@ struct PaQuant {
       // order: 8 c .., or 4 c .. and 16 + 4 c ..
       const int row = ODD ? 8 * n + r : 4 * n + (r >> 1);
       float x[G][8], top = 0.f;
-      const T* y = q + (int64_t)row * p.q_hs;
+      const T* y = q + row * stride;
 #pragma unroll
       for (int g = 0; g < G; ++g) {
 #pragma unroll
@@ -200,7 +208,7 @@ struct PaQuant {
           float* z = x[g] + 4 * hh;
           z[0] = z[1] = z[2] = z[3] = 0.f;
           if (row < rows && d < p.c.Dh) {
-            if (p.q_vec) {
+            if (vec) {
               if constexpr (PAIR) {
                 const float4 u = *reinterpret_cast<const float4*>(y + d);
                 z[0] = u.x; z[1] = u.y; z[2] = u.z; z[3] = u.w;
