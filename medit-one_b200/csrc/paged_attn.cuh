@@ -31,7 +31,7 @@ namespace one {
 constexpr int kPaWarps = 4;
 constexpr size_t kSmPerSm = 228 * 1024;    // shared memory of an SM, 1 KB of it per CTA reserved
 constexpr int kMaxSms = 160;            // SMs that share a list, at most
-constexpr int kPaPerSm = 5;             // CTAs of these kernels on an SM, at most
+constexpr int kPaPerSm = 3;             // CTAs of these kernels on an SM, at most (a dense cache)
 
 struct PagedAttn {
   PagedCache c;
@@ -51,7 +51,7 @@ struct PagedAttn {
   float* scores;          // [B * Hq][score_ld], log2 domain
   int64_t score_ld;
   int2* parts;            // [B * Hkv * hv_per_kv]: first CTA of a segment; last << 1 | (its first part is slot 1)
-  int ranges;             // CTAs that share the list
+  int ranges;             // CTAs, or warps, that share the list
   int cluster;            // CTAs per segment, where there is no list
   // of a cache in 4 or 8 bits:
   const uint8_t* scales;
@@ -622,6 +622,7 @@ enum PaMode { PA_LIST, PA_SEGMENT, PA_DEEP };
 template <typename E, PaMode MODE>
 struct PaSmem {
   static constexpr bool SPLIT = MODE == PA_LIST;
+  static constexpr bool kLone = SPLIT && E::kQuant;  // warps have shares of a list each
   static constexpr int kSlots = E::kGroup * E::kGroups;                  // bytes per warp, and a segment's queries behind them
   static constexpr int kStage = kSlots + E::kQueries;
   static constexpr int kStages = MODE == PA_DEEP ? E::kStagesFew : E::kStages;
@@ -636,7 +637,7 @@ struct PaSmem {
   static_assert(kInStage || kWarp >= kSums, "ring");
   // of a cluster: this CTA's sums [ROWS][DH]; of a list: the warps' sums [1 or 2][warps][rows][DH] where they fit
   static constexpr int kLeast = kInStage ? 0 : kPaWarps * kSums, kMost = kLeast > 9216 ? kLeast : 9216;
-  static constexpr int kApart = 2 * kPaWarps * kSums < kMost ? 2 * kPaWarps * kSums : kMost;
+  static constexpr int kApart = kLone ? kPaWarps * kSums : 2 * kPaWarps * kSums < kMost ? 2 * kPaWarps * kSums : kMost;
   static constexpr int kTotal = kSum + (SPLIT ? kApart : E::ROWS * E::DH * 4);
   static constexpr int kPerSm = kSmPerSm / (kTotal + 1024) < E::kMaxPerSm ? kSmPerSm / (kTotal + 1024) : E::kMaxPerSm;
 };
@@ -653,7 +654,15 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, MODE>::kPerSm) paged_
   using T = typename E::T;
   using Cell = typename E::Cell;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  constexpr int TILE = E::TILE, GR = E::kGroups;
+  // Who takes a tile together: the CTA's warps, or (LONE) a warp by itself, with a share of the list of its own
+  constexpr bool LONE = S::kLone;
+  constexpr int TEAM = LONE ? 1 : kPaWarps, GR = E::kGroups, TILE = 16 * GR * TEAM;
+  const int team = LONE ? blockIdx.x * kPaWarps + warp : blockIdx.x, first_slot = LONE ? 0 : warp * (16 * GR);
+  const int team_tid = LONE ? lane : threadIdx.x;
+  auto team_sync = [] {
+    if (LONE) __syncwarp();
+    else __syncthreads();
+  };
   uint8_t* ring = smem + warp * S::kWarp;
   float* fin = reinterpret_cast<float*>(smem + S::kFin);
   uint8_t* extra = smem + S::kExtra + warp * E::kExtra;
@@ -667,7 +676,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, MODE>::kPerSm) paged_
   if (SPLIT) {
     const int total = pa_total<TILE, MORE>(p);
     share = max(1, (total + p.ranges - 1) / p.ranges);
-    const long long w0 = (long long)share * blockIdx.x;
+    const long long w0 = (long long)share * team;
     if (w0 >= total) return;
     left = min(share, total - (int)w0);
     left -= cur.seek(c, ng, (int)w0);
@@ -699,7 +708,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, MODE>::kPerSm) paged_
   for (int k = 0; k < S::kStages; ++k)
 #pragma unroll
     for (int g = 0; g < GR; ++g) live[k][g] = 0;
-  const int mine = warp * (16 * GR) + (RUN ? 0 : lane & 15);
+  const int mine = first_slot + (RUN ? 0 : lane & 15);
   const int* table;          // of the segment being copied:
   const Cell *keys, *values; // its block table, and its head in page 0 (RUN: this lane's first piece)
   const uint8_t* scales = nullptr;
@@ -717,7 +726,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, MODE>::kPerSm) paged_
       if (src.tile - look < 32 / GR && looked != 0) return;
       look = src.tile;
       looked = 1;
-      const int t = (look + lane / GR) * TILE + warp * (16 * GR) + lane % GR * 16;
+      const int t = (look + lane / GR) * TILE + first_slot + lane % GR * 16;
       pg[0] = -1;
       row[0] = -1;
       if (t < src.len) {
@@ -768,12 +777,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, MODE>::kPerSm) paged_
           sp = scales + (uint64_t)__shfl_sync(0xffffffffu, s_at, from + g) * 16;
         };
         if (ahead >= 16 * GR && gone == 0) {
-#pragma unroll
-          for (int g = 0; g < GR; ++g) {
-            const uint8_t *kp, *vp, *sp;
-            place(g, kp, vp, sp);
-            E::template copy<true>(to + g * E::kGroup, kp, vp, sp, 16);
-          }
+          E::copy_step(to, keys, values, scales, k_at, v_at, s_at, from);
         } else {
 #pragma unroll 1
           for (int g = 0; g < GR; ++g) {
@@ -864,8 +868,8 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, MODE>::kPerSm) paged_
   E eng;
   bool begun_inside = false, copied = false;  // the piece does not start this CTA's share; its first tile is on its way
   const int most = min(E::ROWS, p.G);
-  const bool apart = SPLIT && kPaWarps * most * E::DH * 4 <= S::kApart;
-  const bool twice = SPLIT && 2 * kPaWarps * most * E::DH * 4 <= S::kApart;
+  const bool apart = SPLIT && (LONE || kPaWarps * most * E::DH * 4 <= S::kApart);
+  const bool twice = SPLIT && !LONE && 2 * kPaWarps * most * E::DH * 4 <= S::kApart;
   int parity = 0;
   do {
     const int kv = cur.kv, g0 = cur.gi * E::ROWS, rows = min(E::ROWS, p.G - g0);
@@ -889,10 +893,10 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, MODE>::kPerSm) paged_
       if (!copied) copy();
       copied = false;
       cp_async_wait<S::kStages - 1>();
-      float* scores = p.scores ? p.scores + hq0 * p.score_ld + tile * TILE + warp * (16 * GR) : nullptr;
+      float* scores = p.scores ? p.scores + hq0 * p.score_ld + tile * TILE + first_slot : nullptr;
       __syncwarp();
       if constexpr (LOOK) {
-        const int n = cur.len - tile * TILE - warp * (16 * GR);
+        const int n = cur.len - tile * TILE - first_slot;
         const uint32_t no = dead >> (S::kStages - 1) * GR;
         if (n > 0 || scores)
           eng.consume(p, smem_u32(ring) + get, n >= 16 * GR && (no & ((1u << GR) - 1)) == 0,
@@ -915,28 +919,29 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, MODE>::kPerSm) paged_
     }
     float* so = reinterpret_cast<float*>(smem + (apart ? S::kSum : S::kInStage ? put : 0));
     const int so_warp = apart ? most * E::DH : S::kWarp / 4;
-    if (apart) so += parity * kPaWarps * so_warp;
-    float* ml = reinterpret_cast<float*>(smem + S::kML) + parity * kPaWarps * E::ROWS * 2;
-    eng.leave(ml + warp * E::ROWS * 2, so + warp * so_warp, rows);
-    __syncthreads();
+    if (apart) so += (LONE ? warp : parity * kPaWarps) * so_warp;
+    float* ml = reinterpret_cast<float*>(smem + S::kML) + (LONE ? warp : parity * kPaWarps) * E::ROWS * 2;
+    if (LONE) eng.leave(ml, so, rows);
+    else eng.leave(ml + warp * E::ROWS * 2, so + warp * so_warp, rows);
+    team_sync();
     const bool whole = first == 0 && last == cur.tiles;
-    if (SPLIT && first == 0 && threadIdx.x == 0) {  // which CTAs hold this segment: tiles from `left` on go to later ones
+    if (SPLIT && first == 0 && team_tid == 0) {  // which teams hold this segment: tiles from `left` on go to later ones
       const int more = (cur.tiles - left + share - 1) / share;
       p.parts[(cur.b * c.Hkv + cur.kv) * ng + cur.gi] =
-          make_int2((int)blockIdx.x, ((int)blockIdx.x + max(0, more)) << 1 | (int)begun_inside);
+          make_int2(team, (team + max(0, more)) << 1 | (int)begun_inside);
     }
-    const int64_t part = 2ll * blockIdx.x + begun_inside;
+    const int64_t part = 2ll * team + begun_inside;
     float* sum = reinterpret_cast<float*>(smem + S::kSum);
-    for (int i = threadIdx.x; i < rows * (E::DH / 4); i += blockDim.x) {
+    for (int i = team_tid; i < rows * (E::DH / 4); i += TEAM * 32) {
       const int g = i / (E::DH / 4), d = i % (E::DH / 4) * 4;
       float M = -INFINITY, L = 0.f;
 #pragma unroll
-      for (int k = 0; k < kPaWarps; ++k) M = fmaxf(M, ml[(k * E::ROWS + g) * 2]);
+      for (int k = 0; k < TEAM; ++k) M = fmaxf(M, ml[(k * E::ROWS + g) * 2]);
       const float Ms = M == -INFINITY ? 0.f : M;
       float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int k = 0; k < kPaWarps; ++k) {
-        const float f = exp2f(ml[(k * E::ROWS + g) * 2] - Ms);
+      for (int k = 0; k < TEAM; ++k) {
+        const float f = TEAM == 1 ? 1.f : exp2f(ml[(k * E::ROWS + g) * 2] - Ms);
         L += f * ml[(k * E::ROWS + g) * 2 + 1];
         const float4 x = *reinterpret_cast<const float4*>(so + k * so_warp + g * E::DH + d);
         a.x += f * x.x; a.y += f * x.y; a.z += f * x.z; a.w += f * x.w;
@@ -967,7 +972,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, MODE>::kPerSm) paged_
       }
     }
     if (twice) parity ^= 1;
-    else __syncthreads();
+    else team_sync();
     const float* joint = fin;  // m, 1 / l of the whole segment
     if (!SPLIT && p.cluster > 1) {
       cluster_sync();
@@ -1052,7 +1057,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
   using T = typename E::T;
   constexpr int ROWS = E::ROWS, DH = E::DH;
   __shared__ float4 red[kJoinThreads];
-  __shared__ float weight[kMaxSms * E::kMaxPerSm];  // 2^(m - M) of each part
+  __shared__ float weight[kMaxSms * E::kMaxPerSm * (E::kQuant ? kPaWarps : 1)];  // 2^(m - M) of each part
   __shared__ float fin[2][128];                 // M and 1 / l of a kv head's query heads
   const PagedCache& c = p.c;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;

@@ -84,7 +84,7 @@ struct PagedWs {
 int pad_dh(int dh) { return dh <= 32 ? 32 : dh <= 64 ? 64 : dh <= 96 ? 96 : 128; }
 
 // What the attention over a cache of either kind, in p.c, asks of its arguments, and its plan; `rows` query
-// heads per pass, at most per_sm CTAs on an SM, `units` as E::kSegmentUnits. need: workspace bytes.
+// heads per pass, at most per_sm shares of a list per SM, `units` as E::kSegmentUnits. need: workspace bytes.
 template <typename S>
 int plan_attention(PagedAttn& p, bool& split, const S* cache, const void* q, int64_t q_bs, int64_t q_hs, int hq, int rows, int per_sm, int units,
                    float scale, void* out, void* workspace, size_t workspace_bytes, size_t need) {
@@ -128,9 +128,10 @@ int attend(PagedAttn& p, int cluster, cudaStream_t st) {
   int rc = allow_smem(paged_attn_kernel<E, RUN, MODE>, PaSmem<E, MODE>::kTotal, done);
   if (rc) return rc;
   const int64_t heads = (int64_t)p.c.B * p.c.Hkv, slots = (int64_t)p.c.max_pages * p.c.page_size;
-  p.ranges = std::min(num_sms(), kMaxSms) * PaSmem<E, MODE>::kPerSm;
+  const int ctas = std::min(num_sms(), kMaxSms) * PaSmem<E, MODE>::kPerSm;
+  p.ranges = ctas * (PaSmem<E, MODE>::kLone ? kPaWarps : 1);
   p.cluster = SPLIT ? 1 : cluster;
-  rc = launched(launch_cluster(p.cluster, paged_attn_kernel<E, RUN, MODE>, dim3((unsigned)(SPLIT ? p.ranges : heads * p.hv_per_kv * cluster)),
+  rc = launched(launch_cluster(p.cluster, paged_attn_kernel<E, RUN, MODE>, dim3((unsigned)(SPLIT ? ctas : heads * p.hv_per_kv * cluster)),
                                dim3(kPaWarps * 32), PaSmem<E, MODE>::kTotal, st, p),
                 "paged attention");
   if (rc || !SPLIT) return rc;

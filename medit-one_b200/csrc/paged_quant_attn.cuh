@@ -92,7 +92,7 @@ ONE_DEVINL void cp_async_some(uint32_t s, const void* g, int bytes) {
 enum PqKind { PQ_4, PQ_8, PQ_16, PQ_PAIR4, PQ_PAIR8 };
 
 #ifndef PQ_UNITS
-#define PQ_UNITS 2
+#define PQ_UNITS 3
 #endif
 constexpr int kQuantUnits = PQ_UNITS;
 
@@ -114,11 +114,14 @@ struct PaQuant {
   static constexpr float kZero = BITS == 4 ? 8.f : 128.f;
   static constexpr int kGroup = 16 * (2 * RB + SR);      // bytes of 16 slots
   static constexpr int kValues = 16 * RB, kScales = 32 * RB;
-  static constexpr int kGroups = NL == 1 ? (DH * BITS <= 256 || BITS == 4 ? 4 : 2) : DH * BITS <= 256 ? 2 : 1;  // 16-slot groups per warp and step
+  // 16-slot groups per warp and step, CTAs on an SM at most: long steps for independent work between the
+  // instructions of a warp, as far as registers go. Us at 1, 2, 4 groups: 64 x 4096 ragged x 12 x 64, 4 bits 53, 42,
+  // 38; 8 x 32768 x 8 x 4 x 128 52, 46, 42; in 8 bits 58, 56, 62; of 16 queries 127, 70, 87.
+  static constexpr int kGroups = RB <= 64 && (NL == 1 || DH <= 64) ? 4 : 2;
   static constexpr int TILE = 16 * kGroups * kPaWarps;
-  static constexpr int kStages = NL == 1 ? 2 : 4, kStagesFew = kStages;
+  static constexpr int kStages = 2, kStagesFew = kStages;
   static constexpr int kQueries = ROWS * DH * (int)sizeof(T);  // bytes of a segment's queries
-  static constexpr int kExtra = 0, kMaxPerSm = NL == 1 ? (DH <= 64 ? 4 : DH * BITS <= 512 ? 2 : 3) : DH <= 64 ? 3 : 2;
+  static constexpr int kExtra = 0, kMaxPerSm = DH <= 32 ? (NL == 1 ? 4 : 3) : DH <= 64 && NL == 1 ? 3 : 2;
   static constexpr int kSegmentUnits = kQuantUnits;
   ONE_DEVINL static float weight(float x) { return PAIR ? exp2f(x) : ex2_approx(x); }
 
@@ -138,8 +141,8 @@ struct PaQuant {
   }
   // at(row, 2 i + up) from at(row, up), for even i
   ONE_DEVINL static uint32_t step(uint32_t first, int i) { return (CH & (CH - 1)) == 0 ? first ^ (16 * i) : first + 16 * i; }
-  // The copies of 16 rows that follow one another in memory; k, v, s from this lane's 16 bytes on. live:
-  // of so many rows, the rest as zeros.
+  // The copies of 16 rows that follow one another in memory; k, v, s from this lane's 16 bytes on. ALL: but
+  // for the scales. live: of so many rows, the rest as zeros.
   template <bool ALL>
   ONE_DEVINL static void copy(uint32_t to, const uint8_t* k, const uint8_t* v, const uint8_t* s, int live) {
     const int lane = threadIdx.x & 31;
@@ -152,7 +155,41 @@ struct PaQuant {
         cp_async_some<16>(x + kValues, v + n * 512, ALL || row < live ? 16 : 0);
       }
     }
-    if (lane < 4 * G) cp_async_some<16>(to + kScales + lane * 16, s, ALL ? 16 : min(16, max(0, live * SR - lane * 16)));
+    if (!ALL && lane < 4 * G) cp_async_some<16>(to + kScales + lane * 16, s, min(16, max(0, live * SR - lane * 16)));
+  }
+  // The same of kGroups whole groups; lane from + g holds the places of group g in the pools, in 16 bytes
+  ONE_DEVINL static void copy_step(uint32_t to, const uint8_t* k, const uint8_t* v, const uint8_t* s, uint32_t k_at, uint32_t v_at,
+                                   uint32_t s_at, int from) {
+    const int lane = threadIdx.x & 31;
+    if constexpr (16 * CH % 32 == 0) {
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) {
+        const uint8_t* kp = k + (uint64_t)__shfl_sync(0xffffffffu, k_at, from + g) * 16;
+        const uint8_t* vp = v + (uint64_t)__shfl_sync(0xffffffffu, v_at, from + g) * 16;
+#pragma unroll
+        for (int n = 0; n < CH / 2; ++n) {
+          const int e = n * 32 + lane;
+          const uint32_t x = to + g * kGroup + at(e / CH, e % CH);
+          cp_async_some<16>(x, kp + n * 512, 16);
+          cp_async_some<16>(x + kValues, vp + n * 512, 16);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) {
+        const uint8_t* kp = k + (uint64_t)__shfl_sync(0xffffffffu, k_at, from + g) * 16;
+        const uint8_t* vp = v + (uint64_t)__shfl_sync(0xffffffffu, v_at, from + g) * 16;
+        copy<true>(to + g * kGroup, kp, vp, nullptr, 16);
+      }
+    }
+    // scales: 4 G pieces per group, of all groups together
+#pragma unroll
+    for (int n = 0; n < (kGroups * 4 * G + 31) / 32; ++n) {
+      const int e = n * 32 + lane, g = min(e / (4 * G), kGroups - 1), piece = e - g * (4 * G);
+      // s is this lane's 16 bytes on; the piece's instead
+      const uint8_t* sp = s + (uint64_t)__shfl_sync(0xffffffffu, s_at, from + g) * 16 + (piece - lane) * 16;
+      if (kGroups * 4 * G % 32 == 0 || e < kGroups * 4 * G) cp_async_some<16>(to + g * kGroup + kScales + piece * 16, sp, 16);
+    }
   }
   // Rows anywhere: lane t (16 + t) holds slot t's page and row in the head, or -1; pieces of 16 bytes or of 8.
   ONE_DEVINL static void copy_any(uint32_t to, const PagedAttn& p, const uint8_t* k, const uint8_t* v, const uint8_t* s, int page,
@@ -271,10 +308,16 @@ struct PaQuant {
       for (int i = 0; i < NT; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
   }
 
-  // A slot's scales, K_0 .., V_0 ..
+  // A slot's scales, K_0 .., V_0 .., two of bf16 to a word. Products in bf16 with powers of two are exact, and
+  // one with (0, f) leaves the upper value alone in its word: as an fp32.
+  static constexpr int kFirstV = G / 2;  // word of V_0
   struct Scales {
     uint32_t w[G];
-    ONE_DEVINL float operator[](int i) const { return i & 1 ? bf2_hi(w[i / 2]) : bf2_lo(w[i / 2]); }
+    // element i times the power of two f
+    ONE_DEVINL float get(int i, uint32_t f) const {
+      const uint32_t x = w[i / 2];
+      return i & 1 ? __uint_as_float(bf2_mul(x, f & 0xffff0000u)) : bf2_lo(x);
+    }
     ONE_DEVINL void load(uint32_t at) {
       if constexpr (G == 4)
         asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
@@ -284,11 +327,6 @@ struct PaQuant {
 #pragma unroll
         for (int k = 0; k < G; ++k) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[k]) : "r"(at + 4 * k) : "memory");
       }
-    }
-    // the values' times a power of two (bf16x2)
-    ONE_DEVINL void times(uint32_t f) {
-#pragma unroll
-      for (int k = G / 2; k < G; ++k) w[k] = bf2_mul(w[k], f);
     }
   };
   // [piece][slots 0-7, 8-15] of a group's 16 rows
@@ -316,7 +354,8 @@ struct PaQuant {
     const uint32_t scale_at = base + kScales + r * SR;
     float pr[kGroups][NQ][2];  // slots r and r + 8
     Scales sc[kGroups][2];
-    float vmax = 0.f;
+    uint32_t top[G - kFirstV] = {};  // largest value scales, halves apart (as whole numbers: NaN is above all, and makes
+                                     // its own group's sums NaN only)
 #pragma unroll
     for (int i = 0; i < kGroups; ++i) {
       uint32_t kw[CH][2];
@@ -330,7 +369,7 @@ struct PaQuant {
         constexpr int e1 = BITS == 4 ? 2 : 1, e2 = BITS == 4 ? 1 : 0, e3 = BITS == 4 ? 3 : 1;
         const uint32_t x[2][4] = {{open(w0[0], 0), open(w0[1], 0), open(w0[0], e1), open(w0[1], e1)},
                                   {open(w1[0], e2), open(w1[1], e2), open(w1[0], e3), open(w1[1], e3)}};
-        const float ks[2] = {sc[i][0][g], sc[i][1][g]};
+        const float ks[2] = {sc[i][0].get(g, 0x3f803f80u), sc[i][1].get(g, 0x3f803f80u)};
 #pragma unroll
         for (int n = 0; n < NL; ++n) {
           float a[4];
@@ -345,8 +384,15 @@ struct PaQuant {
               s = g ? s + ks[h] * y : ks[h] * y;
             }
         }
-        vmax = fmax3(vmax, sc[i][0][G + g], sc[i][1][G + g]);
       }
+#pragma unroll
+      for (int k = kFirstV; k < G; ++k) top[k - kFirstV] = __vmaxu2(top[k - kFirstV], __vmaxu2(sc[i][0].w[k], sc[i][1].w[k]));
+    }
+    float vmax = 0.f;
+#pragma unroll
+    for (int k = kFirstV; k < G; ++k) {
+      if (k > kFirstV || G % 2 == 0) vmax = fmaxf(vmax, bf2_lo(top[k - kFirstV]));
+      vmax = fmaxf(vmax, bf2_hi(top[k - kFirstV]));
     }
     if (!full) {
 #pragma unroll
@@ -427,8 +473,6 @@ struct PaQuant {
         x[1] = weight(fmaf(x[1], fac[t], -ms[t]));
         l[t] += x[0] + x[1];
       }
-      sc[i][0].times(mult2);
-      sc[i][1].times(mult2);
       uint32_t vw[CH][2];
       pieces<true>(vw, base + i * kGroup + kValues);
 #pragma unroll
@@ -436,7 +480,7 @@ struct PaQuant {
         uint32_t b[NL][2];  // the weights, times the values' scales
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float v = sc[i][h][G + g];
+          const float v = (G + g) % 2 ? sc[i][h].get(G + g, mult2) : bf2_lo(bf2_mul(sc[i][h].w[(G + g) / 2], mult2));
 #pragma unroll
           for (int n = 0; n < NL; ++n) {
             const float y = pr[i][n * QL][h] * v;

@@ -121,7 +121,7 @@ int attend_bits(PagedAttn& p, bool split, int dtype, int rows, cudaStream_t st) 
 extern "C" size_t one_paged_quant_attention_workspace_bytes(int32_t b, int32_t hq, int32_t hkv, int32_t dh, int32_t page_size,
                                                             int32_t max_pages, int32_t dtype, int32_t with_mass) {
   if (hq < 1 || hkv < 1) return 0;
-  return attention_bytes(b, hq, hkv, dh, quant_rows(dtype, hq / hkv), page_size, max_pages, with_mass != 0, kPaPerSm);
+  return attention_bytes(b, hq, hkv, dh, quant_rows(dtype, hq / hkv), page_size, max_pages, with_mass != 0, 4 * kPaWarps);
 }
 
 extern "C" int one_paged_quant_attention(const one_paged_quant_cache* cache, const void* q, int64_t q_batch_stride,
@@ -144,7 +144,7 @@ extern "C" int one_paged_quant_attention(const one_paged_quant_cache* cache, con
   p.run = ((at | reinterpret_cast<uintptr_t>(m.scales) | p.s_stride) & 15) == 0 &&
           cache->num_pages * std::max({m.c.k_stride, m.c.v_stride, p.s_stride}) < 0xfffffff0ll * 16;
   bool split;
-  rc = plan_attention(p, split, cache, q, q_batch_stride, q_head_stride, hq, rows, kPaPerSm, kQuantUnits, scale, out, workspace, workspace_bytes, need);
+  rc = plan_attention(p, split, cache, q, q_batch_stride, q_head_stride, hq, rows, 4 * kPaWarps, kQuantUnits, scale, out, workspace, workspace_bytes, need);
   if (rc) return rc;
   return cache->bits == 4 ? attend_bits<4>(p, split, dtype, rows, (cudaStream_t)stream)
                           : attend_bits<8>(p, split, dtype, rows, (cudaStream_t)stream);
