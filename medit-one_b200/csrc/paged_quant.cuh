@@ -56,6 +56,169 @@ struct QuantAppendParams {
   int row, groups;
 };
 
+// 8 values as codes, 4 (8) bits each, the first lowest. The quotient by the reciprocal and one residual
+// (Markstein, IBM J. Res. Dev. 34(1), 1990) is the rounded one: inv is the rounded reciprocal. Adding
+// 1.5 * 2^23 rounds it to a whole number, halves to even, in the low bits of the sum.
+template <int BITS>
+ONE_DEVINL void quant_codes(const float2 (&x)[4], float scale, float inv, uint32_t (&out)[BITS / 4]) {
+  const float2 by = make_float2(inv, inv), minus = make_float2(-scale, -scale);
+  const float magic = 12582912.f + QuantCode<BITS>::kZero;
+  uint32_t u[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float2 t = mul2(x[i], by);
+    t = fma2(fma2(t, minus, x[i]), by, t);
+    t = add2(t, make_float2(magic, magic));
+    u[2 * i] = __float_as_uint(t.x);
+    u[2 * i + 1] = __float_as_uint(t.y);
+  }
+  auto bytes = [](uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+  };
+  constexpr uint32_t kNone = BITS == 4 ? 0x88888888u : 0x80808080u;
+  if constexpr (BITS == 4) {
+    out[0] = bytes(u[0] + 16 * u[1], u[2] + 16 * u[3], u[4] + 16 * u[5], u[6] + 16 * u[7]);
+    if (inv == 0.f) out[0] = kNone;
+  } else {
+    out[0] = bytes(u[0], u[1], u[2], u[3]);
+    out[1] = bytes(u[4], u[5], u[6], u[7]);
+    if (inv == 0.f) out[0] = out[1] = kNone;
+  }
+}
+
+// 8 values of T, 16-byte aligned
+template <typename T> struct Eight;
+template <> struct Eight<__nv_bfloat16> {
+  uint4 u;
+  ONE_DEVINL void load(const __nv_bfloat16* p) { u = *reinterpret_cast<const uint4*>(p); }
+  ONE_DEVINL void ldg(const __nv_bfloat16* p) { u = __ldg(reinterpret_cast<const uint4*>(p)); }
+  ONE_DEVINL void store(__nv_bfloat16* p) const { *reinterpret_cast<uint4*>(p) = u; }
+  ONE_DEVINL void open(float2 (&v)[4]) const { Piece<__nv_bfloat16>::open(u, v); }
+  ONE_DEVINL void close(const float2 (&v)[4]) { u = Piece<__nv_bfloat16>::close(v); }
+  ONE_DEVINL Eight from_lane(int lane) const {
+    return {make_uint4(__shfl_sync(0xffffffffu, u.x, lane), __shfl_sync(0xffffffffu, u.y, lane), __shfl_sync(0xffffffffu, u.z, lane),
+                       __shfl_sync(0xffffffffu, u.w, lane))};
+  }
+};
+template <> struct Eight<float> {
+  float4 a, b;
+  ONE_DEVINL void load(const float* p) { a = *reinterpret_cast<const float4*>(p); b = *reinterpret_cast<const float4*>(p + 4); }
+  ONE_DEVINL void ldg(const float* p) { a = __ldg(reinterpret_cast<const float4*>(p)); b = __ldg(reinterpret_cast<const float4*>(p + 4)); }
+  ONE_DEVINL void store(float* p) const { *reinterpret_cast<float4*>(p) = a; *reinterpret_cast<float4*>(p + 4) = b; }
+  ONE_DEVINL void open(float2 (&v)[4]) const {
+    v[0] = make_float2(a.x, a.y); v[1] = make_float2(a.z, a.w); v[2] = make_float2(b.x, b.y); v[3] = make_float2(b.z, b.w);
+  }
+  ONE_DEVINL void close(const float2 (&v)[4]) {
+    a = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+    b = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
+  }
+  ONE_DEVINL Eight from_lane(int lane) const {
+    auto s = [&](float x) { return __shfl_sync(0xffffffffu, x, lane); };
+    return {make_float4(s(a.x), s(a.y), s(a.z), s(a.w)), make_float4(s(b.x), s(b.y), s(b.z), s(b.w))};
+  }
+};
+
+// New tokens into the pages, rotated and quantised: a copy of 2 or 4 bytes per value in and a half or one
+// out, with some eight instructions per value in between; bound by HBM (prompts) or by the chain lengths ->
+// page -> store (single tokens).
+//
+// A lane has 8 dims of kQuantRows heads of a token's keys, queries or values, which share cos and sin; a
+// row's lanes lie side by side in a warp, as many rows of lanes as fit. The half that the rotation needs
+// and the largest value of a group come from the row's other lanes. All loads are asked for before the
+// first is used. Rows must be whole 16-byte pieces; quant_append_any_kernel takes the rest. Sequence
+// blockIdx.y.
+template <typename T>
+constexpr int kQuantRows = sizeof(T) == 2 ? 4 : 2;
+
+template <typename T, typename C, int BITS>
+__global__ void __launch_bounds__(256, 4) quant_append_kernel(const __grid_constant__ QuantAppendParams p) {
+  constexpr int ROWS = kQuantRows<T>;
+  pdl_wait();
+  const PagedAppendParams& a = p.a;
+  const PagedCache& c = a.c;
+  const int lane = threadIdx.x & 31, pieces = c.Dh / 8, per = 32 / pieces, sub = lane / pieces, piece = lane - sub * pieces, b = blockIdx.y;
+  const int hq = a.q ? a.Hq : 0, kvg = (c.Hkv + ROWS - 1) / ROWS, qg = (hq + ROWS - 1) / ROWS, items = 2 * kvg + qg;
+  const uint32_t item = ((blockIdx.x * blockDim.x + threadIdx.x) >> 5) * per + sub;
+  int t = (int)(item / items);
+  const int g = (int)(item - (uint32_t)t * items);
+  const bool there = sub < per && t < a.N;
+  if (!there) t = 0;
+  const int kind = g < kvg ? 0 : g < kvg + qg ? 1 : 2;  // keys, queries, values
+  const int r0 = (kind == 0 ? g : kind == 1 ? g - kvg : g - kvg - qg) * ROWS, rows = there ? min(ROWS, (kind == 1 ? hq : c.Hkv) - r0) : 0;
+  const int64_t* s = kind == 0 ? a.ks : kind == 1 ? a.qs : a.vs;
+  const T* from = (const T*)(kind == 0 ? a.k : kind == 1 ? a.q : a.v) + b * s[0] + r0 * s[1] + t * s[2] + piece * 8;
+  const bool turn = kind < 2 && a.cosv;
+  Eight<T> x[ROWS];
+#pragma unroll
+  for (int k = 0; k < ROWS; ++k) {
+    if (k < rows) x[k].load(from + k * s[1]);
+    else x[k] = Eight<T>{};
+  }
+  Eight<C> cs{}, sn{};
+  if (turn) {
+    const int64_t at = b * a.cos_bs + (int64_t)t * c.Dh + piece * 8;
+    cs.ldg((const C*)a.cosv + at);
+    sn.ldg((const C*)a.sinv + at);
+  }
+  int64_t slot;
+  int page = 0, row = 0;
+  const bool stored = kind != 1 && there && append_place(a, b, t, slot, page, row, SITE_QUANT_APPEND);
+  const int base = sub * pieces, half = pieces / 2, other = base + (piece < half ? piece + half : piece - half);
+  float2 co[4], si[4];
+  cs.open(co);
+  sn.open(si);
+  if (piece < half) {
+#pragma unroll
+    for (int d = 0; d < 4; ++d) si[d] = make_float2(-si[d].x, -si[d].y);
+  }
+  const int64_t head = (int64_t)r0 * c.page_size + row;  // row of the first head in the page
+  uint8_t* codes = (uint8_t*)(kind ? c.v : c.k) + page * (kind ? c.v_stride : c.k_stride) + head * p.row + piece * BITS;
+  __nv_bfloat16* scales = (__nv_bfloat16*)p.scales + page * p.s_stride + (head * 2 + (kind != 0)) * p.groups + piece / 4;
+  if (stored && kind == 0 && a.mass)
+    for (int k = piece; k < rows; k += pieces) a.mass[((int64_t)b * c.Hkv + r0 + k) * a.mass_width + slot] = 0.f;
+#pragma unroll
+  for (int k = 0; k < ROWS; ++k) {
+    float2 v[4];
+    x[k].open(v);
+    if (a.cosv) {  // all lanes, for the exchange; values stay as they are
+      float2 w[4];
+      x[k].from_lane(other).open(w);
+      if (turn) {
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          if constexpr (sizeof(T) == 2 && sizeof(C) == 2)
+            v[d] = fma2(v[d], co[d], mul2(w[d], si[d]));  // products of bf16 values are exact
+          else
+            v[d] = make_float2(quant_rotate(T(), C(), v[d].x, w[d].x, co[d].x, si[d].x),
+                               quant_rotate(T(), C(), v[d].y, w[d].y, co[d].y, si[d].y));
+        }
+      }
+    }
+    uint32_t largest = 0;
+#pragma unroll
+    for (int d = 0; d < 4; ++d)
+      largest = max(largest, max(__float_as_uint(v[d].x) & 0x7fffffffu, __float_as_uint(v[d].y) & 0x7fffffffu));
+    largest = max(largest, __shfl_sync(0xffffffffu, largest, base + (piece ^ 1)));
+    largest = max(largest, __shfl_sync(0xffffffffu, largest, base + ((piece ^ 2) < pieces ? piece ^ 2 : piece)));
+    if (k >= rows) continue;
+    if (kind == 1) {
+      Eight<T> y;
+      y.close(v);
+      y.store((T*)a.q_out + (((int64_t)b * hq + r0 + k) * a.N + t) * c.Dh + piece * 8);
+      continue;
+    }
+    if (!stored) continue;
+    float scale, inv;
+    quant_scale<BITS>(largest, scale, inv);
+    uint32_t out[BITS / 4];
+    quant_codes<BITS>(v, scale, inv, out);
+    uint8_t* to = codes + (int64_t)k * c.page_size * p.row;
+    if constexpr (BITS == 4) *reinterpret_cast<uint32_t*>(to) = out[0];
+    else *reinterpret_cast<uint2*>(to) = make_uint2(out[0], out[1]);
+    if (piece % 4 == 0) scales[(int64_t)k * c.page_size * 2 * p.groups] = __float2bfloat16_rn(scale);
+  }
+}
+
 // New tokens, one warp per row of q, k or v, any alignment; a lane holds dim 32 g + lane of group g.
 template <typename T, typename C, int BITS>
 __global__ void __launch_bounds__(256) quant_append_any_kernel(const __grid_constant__ QuantAppendParams p) {
@@ -114,16 +277,51 @@ struct QuantReadParams {
   int N;
 };
 
-// Slots starts[b] .. starts[b] + N - 1 of every sequence, those not below lengths[b] as zeros; a thread
-// has 8 dims of a slot's key and value.
+// 8 codes of 4 or 8 bits times their scale. bf16 from 4 bits: 128 + u is a bf16 with u in its last bits, and
+// its difference to 136 and the product are one rounding each, the first exact.
+template <int BITS>
+ONE_DEVINL void quant_open(const uint32_t (&w)[BITS / 4], __nv_bfloat16 scale, Eight<__nv_bfloat16>& out) {
+  const uint32_t s = __bfloat16_as_ushort(scale) * 0x10001u;
+  if constexpr (BITS == 4) {
+    uint32_t x[4];  // dims j and j + 4
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = bf2_mul(bf2_add((w[0] >> 4 * j & 0x000f000fu) | 0x43004300u, 0xc308c308u), s);
+    out.u = make_uint4(__byte_perm(x[0], x[1], 0x5410), __byte_perm(x[2], x[3], 0x5410), __byte_perm(x[0], x[1], 0x7632),
+                       __byte_perm(x[2], x[3], 0x7632));
+  } else {
+    const float f = __bfloat162float(scale);
+    float2 v[4];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      (&v[j / 2].x)[j & 1] = (__uint_as_float(__byte_perm(w[j / 4], 0x4b000000u, 0x7540 + j % 4)) - 8388736.f) * f;
+    out.close(v);
+  }
+}
+template <int BITS>
+ONE_DEVINL void quant_open(const uint32_t (&w)[BITS / 4], __nv_bfloat16 scale, Eight<float>& out) {
+  const float f = __bfloat162float(scale);
+  float2 v[4];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint32_t u = BITS == 4 ? (w[0] >> 4 * j & 15u) | 0x4b000000u : __byte_perm(w[j / 4 % (BITS / 4)], 0x4b000000u, 0x7540 + j % 4);
+    (&v[j / 2].x)[j & 1] = (__uint_as_float(u) - (8388608.f + QuantCode<BITS>::kZero)) * f;
+  }
+  out.close(v);
+}
+
+// Slots starts[b] .. starts[b] + N - 1 of every sequence, those not below lengths[b] as zeros. A lane has 8
+// dims of a slot's keys and values of kReadHeads heads, which share the page; its loads are in flight
+// together. A copy that grows fourfold: bound by HBM, that is by what it writes.
+constexpr int kReadHeads = 4;
+
 template <typename T, int BITS>
 __global__ void __launch_bounds__(256) quant_read_kernel(const __grid_constant__ QuantReadParams p) {
   pdl_wait();
   const PagedCache& c = p.m.c;
-  const int pieces = c.Dh / 8, b = blockIdx.y;
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, row = i / pieces;
-  if (row >= (int64_t)c.Hkv * p.N) return;
-  const int piece = (int)(i - row * pieces), h = (int)(row / p.N), t = (int)(row - (int64_t)h * p.N);
+  const int pieces = c.Dh / 8, b = blockIdx.y, hg = blockIdx.z * kReadHeads;
+  const uint32_t i = blockIdx.x * blockDim.x + threadIdx.x;
+  const int t = (int)(i / pieces), piece = (int)(i - (uint32_t)t * pieces), heads = min(kReadHeads, c.Hkv - hg);
+  if (t >= p.N) return;
   const int len = paged_length(c, b, SITE_QUANT_READ), first = p.starts ? p.starts[b] : 0;
   const int64_t slot = (int64_t)first + t;
   int page = -1, at = 0;
@@ -133,24 +331,38 @@ __global__ void __launch_bounds__(256) quant_read_kernel(const __grid_constant__
     page = paged_page(c, c.table, b * c.table_stride, index, SITE_QUANT_READ);
     at = (int)slot - index * c.page_size;
   }
-  T* to[2] = {(T*)p.k, (T*)p.v};
-  const int64_t out = (((int64_t)b * c.Hkv + h) * p.N + t) * c.Dh + piece * 8;
-  for (int w = 0; w < 2; ++w) {
-    float x[8];
-    if (page >= 0) {
-      const int64_t r = (int64_t)h * c.page_size + at;
-      const uint8_t* codes = (const uint8_t*)(w ? c.v : c.k) + page * (w ? c.v_stride : c.k_stride) + r * p.m.row + piece * BITS;
-      const float s = __bfloat162float(((const __nv_bfloat16*)p.m.scales)[page * p.m.s_stride + (r * 2 + w) * p.m.groups + piece / 4]);
+  uint32_t w[2][kReadHeads][BITS / 4] = {};
+  __nv_bfloat16 s[2][kReadHeads];
 #pragma unroll
-      for (int d = 0; d < 8; ++d) {
-        const int u = BITS == 4 ? codes[d >> 1] >> (d & 1) * 4 & 15 : codes[d];
-        x[d] = s * (float)(u - QuantCode<BITS>::kZero);
+  for (int h = 0; h < kReadHeads; ++h) {
+    s[0][h] = s[1][h] = __float2bfloat16_rn(0.f);
+    if (page >= 0 && h < heads) {
+      const int64_t r = (int64_t)(hg + h) * c.page_size + at;
+      const uint8_t *k = (const uint8_t*)c.k + page * c.k_stride + r * p.m.row + piece * BITS;
+      const uint8_t *v = (const uint8_t*)c.v + page * c.v_stride + r * p.m.row + piece * BITS;
+      const __nv_bfloat16* sc = (const __nv_bfloat16*)p.m.scales + page * p.m.s_stride + r * 2 * p.m.groups + piece / 4;
+      if constexpr (BITS == 4) {
+        w[0][h][0] = *reinterpret_cast<const uint32_t*>(k);
+        w[1][h][0] = *reinterpret_cast<const uint32_t*>(v);
+      } else {
+        const uint2 x = *reinterpret_cast<const uint2*>(k), y = *reinterpret_cast<const uint2*>(v);
+        w[0][h][0] = x.x; w[0][h][1] = x.y; w[1][h][0] = y.x; w[1][h][1] = y.y;
       }
-    } else {
-#pragma unroll
-      for (int d = 0; d < 8; ++d) x[d] = 0.f;
+      s[0][h] = sc[0];
+      s[1][h] = sc[p.m.groups];
     }
-    store8(to[w] + out, x);
+  }
+  const int64_t out = (((int64_t)b * c.Hkv + hg) * p.N + t) * c.Dh + piece * 8, step = (int64_t)p.N * c.Dh;
+#pragma unroll
+  for (int h = 0; h < kReadHeads; ++h) {
+    if (h >= heads) break;
+    Eight<T> x;
+    quant_open<BITS>(w[0][h], s[0][h], x);
+    if (page < 0) x = Eight<T>{};
+    x.store((T*)p.k + out + h * step);
+    quant_open<BITS>(w[1][h], s[1][h], x);
+    if (page < 0) x = Eight<T>{};
+    x.store((T*)p.v + out + h * step);
   }
 }
 

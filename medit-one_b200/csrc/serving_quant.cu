@@ -55,14 +55,25 @@ extern "C" int one_paged_quant_append(const one_paged_quant_cache* cache, const 
   }
   p.a.cosv = x.cos; p.a.sinv = x.sin; p.a.cos_bs = x.cos_batch == 1 ? 0 : (int64_t)x.n * cache->dh; p.a.counts = x.counts;
   p.a.mass = cache->mass; p.a.mass_width = cache->mass_width; p.a.q_out = x.q_out; p.a.N = x.n; p.a.Hq = x.hq;
-  const int64_t threads = x.n * (2 * (int64_t)cache->hkv + (x.q ? x.hq : 0)) * 32;
-  if (threads > 0x7fffffff) return fail(ONE_ERR_UNSUPPORTED, "paged append: too many rows");
-  const dim3 grid((unsigned)((threads + 255) / 256), cache->b);
+  // whole 16-byte pieces of rows; anything else goes element by element
+  const int64_t unit = 16 / elem_bytes(dtype);
+  auto aligned = [&](const void* at, const int64_t* s) {
+    return (reinterpret_cast<uintptr_t>(at) & 15) == 0 && s[0] % unit == 0 && s[1] % unit == 0 && s[2] % unit == 0;
+  };
+  const bool vec = aligned(x.k, x.k_strides) && aligned(x.v, x.v_strides) && (!x.q || aligned(x.q, x.q_strides)) &&
+                   ((reinterpret_cast<uintptr_t>(x.q_out) | reinterpret_cast<uintptr_t>(x.cos) | reinterpret_cast<uintptr_t>(x.sin)) & 15) == 0;
+  const int64_t hq = x.q ? x.hq : 0, per = 32 / (cache->dh / 8), rows = dtype == ONE_DTYPE_F32 ? kQuantRows<float> : kQuantRows<__nv_bfloat16>;
+  auto groups = [&](int64_t heads) { return (heads + rows - 1) / rows; };
+  const int64_t warps = vec ? (x.n * (2 * groups(cache->hkv) + groups(hq)) + per - 1) / per : x.n * (2 * (int64_t)cache->hkv + hq);
+  if (x.n * (2 * (int64_t)cache->hkv + hq) > 0x7fffffff / 32) return fail(ONE_ERR_UNSUPPORTED, "paged append: too many rows");
+  const dim3 grid((unsigned)((warps + 7) / 8), cache->b);
+  cudaStream_t st = (cudaStream_t)stream;
   auto append = [&](auto t, auto c) {
     using T = decltype(t);
     using C = decltype(c);
-    return cache->bits == 4 ? launch(quant_append_any_kernel<T, C, 4>, grid, dim3(256), 0, (cudaStream_t)stream, p)
-                            : launch(quant_append_any_kernel<T, C, 8>, grid, dim3(256), 0, (cudaStream_t)stream, p);
+    if (cache->bits == 4)
+      return vec ? launch(quant_append_kernel<T, C, 4>, grid, dim3(256), 0, st, p) : launch(quant_append_any_kernel<T, C, 4>, grid, dim3(256), 0, st, p);
+    return vec ? launch(quant_append_kernel<T, C, 8>, grid, dim3(256), 0, st, p) : launch(quant_append_any_kernel<T, C, 8>, grid, dim3(256), 0, st, p);
   };
   return launched(dtype == ONE_DTYPE_F32   ? append(float(0), float(0))
                   : x.cos && x.tables_fp32 ? append(__nv_bfloat16(), float(0))
@@ -81,9 +92,9 @@ extern "C" int one_paged_quant_read(const one_paged_quant_cache* cache, const in
   if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15)
     return fail(ONE_ERR_INVALID, "paged read: k and v must start on 16-byte boundaries");
   p.starts = starts; p.k = k; p.v = v; p.N = n;
-  const int64_t threads = (int64_t)cache->hkv * n * (cache->dh / 8);
+  const int64_t threads = (int64_t)n * (cache->dh / 8), heads = (cache->hkv + kReadHeads - 1) / kReadHeads;
   if (threads > 0x7fffffff) return fail(ONE_ERR_UNSUPPORTED, "paged read: too many rows");
-  const dim3 grid((unsigned)((threads + 255) / 256), cache->b);
+  const dim3 grid((unsigned)((threads + 255) / 256), cache->b, (unsigned)heads);
   cudaStream_t st = (cudaStream_t)stream;
   auto read = [&](auto t) {
     using T = decltype(t);
