@@ -6,9 +6,11 @@
 //
 // A row of Dh values is cut into groups of 32 (the last may be shorter) of scale * code:
 //   scale = bf16(max |x| / m), m = 7 or 127       code = rint(x / scale)
-// where x is the value in fp32. Codes do not depend on how the quotient is computed as long as it is
-// rounded correctly: scale has 8 significant bits and x 24, so that x / scale, when it is no multiple
-// of 1/2, is at least an ulp away from one. The same holds for max |x| / m and the bf16 rounding.
+// where x is the value in fp32. Codes do not depend on how the quotient is computed as long as its error
+// stays well below 2^-24: scale has at most 8 significant bits and x 24, so that (n + 1/2) scale is an fp32, x
+// differs from it by an ulp or not at all, and x / scale from n + 1/2 by more than half an ulp (by 1 / 1.992
+// of one; the rounding of a quotient off by 2^-40 is therefore the exact one's). The same holds for max |x| /
+// m and the halfway points of bf16.
 // Symmetric codes, so that a product with a code needs no second sum for an offset of its own; 32
 // values to a scale, so that a large channel spoils few others, for half a bit per value.
 #pragma once
@@ -33,13 +35,23 @@ struct QuantCode {
   static constexpr int kZero = BITS == 4 ? 8 : 128;
 };
 
-// The scale (as a float that bf16 holds), its reciprocal and whether codes count, from the bits of max |x|.
+// The scale (as a float that bf16 holds) and about its reciprocal, 0 where codes do not count, from max |x|. The
+// quotient is one by a rounded reciprocal with one residual (Markstein, IBM J. Res. Dev. 34(1), 1990).
 template <int BITS>
-ONE_DEVINL void quant_scale(uint32_t largest, float& scale, float& inv) {
-  const float s = __bfloat162float(__float2bfloat16_rn(__fdiv_rn(__uint_as_float(largest), QuantCode<BITS>::kTop)));
-  const bool finite = largest < 0x7f800000u, there = finite && s >= kQuantLeast;
+ONE_DEVINL void quant_scale(float largest, float& scale, float& inv) {
+  constexpr float m = QuantCode<BITS>::kTop, by = 1.f / m;
+  const float q = largest * by;
+  const float s = __bfloat162float(__float2bfloat16_rn(fmaf(fmaf(-q, m, largest), by, q)));
+  const bool finite = largest < INFINITY, there = finite && s >= kQuantLeast;
   scale = there ? s : finite ? 0.f : __uint_as_float(0x7fc00000u);
-  inv = there ? __frcp_rn(s) : 0.f;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));  // 2^-125 at least
+  if (!there) inv = 0.f;
+}
+// max |.| of three, NaN if one is
+ONE_DEVINL float max_abs(float a, float b, float c) {
+  float d;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 
 // x cos + y sin in fp32 with one rounding: products of bf16 values are exact in fp32, those of fp32 in fp64.
@@ -54,11 +66,11 @@ struct QuantAppendParams {
   void* scales;
   int64_t s_stride;
   int row, groups;
+  int per, lane_m;  // rows of lanes per warp; lane / (Dh / 8) = lane * lane_m >> 10
 };
 
-// 8 values as codes, 4 (8) bits each, the first lowest. The quotient by the reciprocal and one residual
-// (Markstein, IBM J. Res. Dev. 34(1), 1990) is the rounded one: inv is the rounded reciprocal. Adding
-// 1.5 * 2^23 rounds it to a whole number, halves to even, in the low bits of the sum.
+// 8 values as codes, 4 (8) bits each, the first lowest. The quotient is x inv with one residual; adding 1.5 *
+// 2^23 rounds it to a whole number, halves to even, in the low bits of the sum.
 template <int BITS>
 ONE_DEVINL void quant_codes(const float2 (&x)[4], float scale, float inv, uint32_t (&out)[BITS / 4]) {
   const float2 by = make_float2(inv, inv), minus = make_float2(-scale, -scale);
@@ -123,10 +135,10 @@ template <> struct Eight<float> {
 // page -> store (single tokens).
 //
 // A lane has 8 dims of kQuantRows heads of a token's keys, queries or values, which share cos and sin; a
-// row's lanes lie side by side in a warp, as many rows of lanes as fit. The half that the rotation needs
-// and the largest value of a group come from the row's other lanes. All loads are asked for before the
-// first is used. Rows must be whole 16-byte pieces; quant_append_any_kernel takes the rest. Sequence
-// blockIdx.y.
+// row's lanes lie side by side in a warp, as many tokens as fit. CTAs of one kind and group of heads each
+// (blockIdx.z), so that warps do not diverge. The half that the rotation needs and the largest value of a
+// group come from the row's other lanes. All loads are asked for before the first is used. Rows must be
+// whole 16-byte pieces; quant_append_any_kernel takes the rest. Sequence blockIdx.y.
 template <typename T>
 constexpr int kQuantRows = sizeof(T) == 2 ? 4 : 2;
 
@@ -136,34 +148,32 @@ __global__ void __launch_bounds__(256, 4) quant_append_kernel(const __grid_const
   pdl_wait();
   const PagedAppendParams& a = p.a;
   const PagedCache& c = a.c;
-  const int lane = threadIdx.x & 31, pieces = c.Dh / 8, per = 32 / pieces, sub = lane / pieces, piece = lane - sub * pieces, b = blockIdx.y;
-  const int hq = a.q ? a.Hq : 0, kvg = (c.Hkv + ROWS - 1) / ROWS, qg = (hq + ROWS - 1) / ROWS, items = 2 * kvg + qg;
-  const uint32_t item = ((blockIdx.x * blockDim.x + threadIdx.x) >> 5) * per + sub;
-  int t = (int)(item / items);
-  const int g = (int)(item - (uint32_t)t * items);
-  const bool there = sub < per && t < a.N;
+  const int lane = threadIdx.x & 31, pieces = c.Dh / 8, b = blockIdx.y;
+  const int sub = lane * p.lane_m >> 10, piece = lane - sub * pieces;  // lane / pieces
+  int t = (blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) * p.per + sub;
+  const int kvg = (c.Hkv + ROWS - 1) / ROWS, z = blockIdx.z;
+  const int kind = z < kvg ? 0 : z < 2 * kvg ? 2 : 1;  // keys, values, queries
+  const int r0 = (z - (kind == 0 ? 0 : kind == 2 ? kvg : 2 * kvg)) * ROWS;
+  const bool there = sub < p.per && t < a.N && (kind == 1 || !a.counts || t < a.counts[b]);
+  if (!__any_sync(0xffffffffu, there)) return;
   if (!there) t = 0;
-  const int kind = g < kvg ? 0 : g < kvg + qg ? 1 : 2;  // keys, queries, values
-  const int r0 = (kind == 0 ? g : kind == 1 ? g - kvg : g - kvg - qg) * ROWS, rows = there ? min(ROWS, (kind == 1 ? hq : c.Hkv) - r0) : 0;
+  const int rows = there ? min(ROWS, (kind == 1 ? a.Hq : c.Hkv) - r0) : 0;
   const int64_t* s = kind == 0 ? a.ks : kind == 1 ? a.qs : a.vs;
   const T* from = (const T*)(kind == 0 ? a.k : kind == 1 ? a.q : a.v) + b * s[0] + r0 * s[1] + t * s[2] + piece * 8;
-  const bool turn = kind < 2 && a.cosv;
   Eight<T> x[ROWS];
 #pragma unroll
   for (int k = 0; k < ROWS; ++k) {
     if (k < rows) x[k].load(from + k * s[1]);
     else x[k] = Eight<T>{};
   }
+  const bool turn = kind != 2 && a.cosv;
   Eight<C> cs{}, sn{};
   if (turn) {
     const int64_t at = b * a.cos_bs + (int64_t)t * c.Dh + piece * 8;
     cs.ldg((const C*)a.cosv + at);
     sn.ldg((const C*)a.sinv + at);
   }
-  int64_t slot;
-  int page = 0, row = 0;
-  const bool stored = kind != 1 && there && append_place(a, b, t, slot, page, row, SITE_QUANT_APPEND);
-  const int base = sub * pieces, half = pieces / 2, other = base + (piece < half ? piece + half : piece - half);
+  const int base = lane - piece, half = pieces / 2, other = base + (piece < half ? piece + half : piece - half);
   float2 co[4], si[4];
   cs.open(co);
   sn.open(si);
@@ -171,51 +181,58 @@ __global__ void __launch_bounds__(256, 4) quant_append_kernel(const __grid_const
 #pragma unroll
     for (int d = 0; d < 4; ++d) si[d] = make_float2(-si[d].x, -si[d].y);
   }
+  auto rotate = [&](const Eight<T>& in, float2 (&v)[4]) {
+    in.open(v);
+    if (!turn) return;
+    float2 w[4];
+    in.from_lane(other).open(w);
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+      if constexpr (sizeof(T) == 2 && sizeof(C) == 2)
+        v[d] = fma2(v[d], co[d], mul2(w[d], si[d]));  // products of bf16 values are exact
+      else
+        v[d] = make_float2(quant_rotate(T(), C(), v[d].x, w[d].x, co[d].x, si[d].x),
+                           quant_rotate(T(), C(), v[d].y, w[d].y, co[d].y, si[d].y));
+    }
+  };
+  if (kind == 1) {
+    T* to = (T*)a.q_out + (((int64_t)b * a.Hq + r0) * a.N + t) * c.Dh + piece * 8;
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+      float2 v[4];
+      rotate(x[k], v);
+      Eight<T> y;
+      y.close(v);
+      if (k < rows) y.store(to + k * ((int64_t)a.N * c.Dh));
+    }
+    return;
+  }
+  int64_t slot;
+  int page = 0, row = 0;
+  const bool stored = there && append_place(a, b, t, slot, page, row, SITE_QUANT_APPEND);
   const int64_t head = (int64_t)r0 * c.page_size + row;  // row of the first head in the page
   uint8_t* codes = (uint8_t*)(kind ? c.v : c.k) + page * (kind ? c.v_stride : c.k_stride) + head * p.row + piece * BITS;
   __nv_bfloat16* scales = (__nv_bfloat16*)p.scales + page * p.s_stride + (head * 2 + (kind != 0)) * p.groups + piece / 4;
+  const int64_t code_step = (int64_t)c.page_size * p.row, scale_step = (int64_t)c.page_size * 2 * p.groups;
   if (stored && kind == 0 && a.mass)
     for (int k = piece; k < rows; k += pieces) a.mass[((int64_t)b * c.Hkv + r0 + k) * a.mass_width + slot] = 0.f;
+  const int next = base + (piece ^ 1), over = base + ((piece ^ 2) < pieces ? piece ^ 2 : piece);  // of the same group
 #pragma unroll
   for (int k = 0; k < ROWS; ++k) {
     float2 v[4];
-    x[k].open(v);
-    if (a.cosv) {  // all lanes, for the exchange; values stay as they are
-      float2 w[4];
-      x[k].from_lane(other).open(w);
-      if (turn) {
-#pragma unroll
-        for (int d = 0; d < 4; ++d) {
-          if constexpr (sizeof(T) == 2 && sizeof(C) == 2)
-            v[d] = fma2(v[d], co[d], mul2(w[d], si[d]));  // products of bf16 values are exact
-          else
-            v[d] = make_float2(quant_rotate(T(), C(), v[d].x, w[d].x, co[d].x, si[d].x),
-                               quant_rotate(T(), C(), v[d].y, w[d].y, co[d].y, si[d].y));
-        }
-      }
-    }
-    uint32_t largest = 0;
-#pragma unroll
-    for (int d = 0; d < 4; ++d)
-      largest = max(largest, max(__float_as_uint(v[d].x) & 0x7fffffffu, __float_as_uint(v[d].y) & 0x7fffffffu));
-    largest = max(largest, __shfl_sync(0xffffffffu, largest, base + (piece ^ 1)));
-    largest = max(largest, __shfl_sync(0xffffffffu, largest, base + ((piece ^ 2) < pieces ? piece ^ 2 : piece)));
-    if (k >= rows) continue;
-    if (kind == 1) {
-      Eight<T> y;
-      y.close(v);
-      y.store((T*)a.q_out + (((int64_t)b * hq + r0 + k) * a.N + t) * c.Dh + piece * 8);
-      continue;
-    }
-    if (!stored) continue;
+    rotate(x[k], v);
+    float largest = max_abs(v[0].x, v[0].y, v[1].x);
+    largest = max_abs(max_abs(largest, v[1].y, v[2].x), max_abs(v[2].y, v[3].x, v[3].y), 0.f);
+    largest = max_abs(largest, __shfl_sync(0xffffffffu, largest, next), 0.f);
+    largest = max_abs(largest, __shfl_sync(0xffffffffu, largest, over), 0.f);
     float scale, inv;
     quant_scale<BITS>(largest, scale, inv);
     uint32_t out[BITS / 4];
     quant_codes<BITS>(v, scale, inv, out);
-    uint8_t* to = codes + (int64_t)k * c.page_size * p.row;
-    if constexpr (BITS == 4) *reinterpret_cast<uint32_t*>(to) = out[0];
-    else *reinterpret_cast<uint2*>(to) = make_uint2(out[0], out[1]);
-    if (piece % 4 == 0) scales[(int64_t)k * c.page_size * 2 * p.groups] = __float2bfloat16_rn(scale);
+    if (!stored || k >= rows) continue;
+    if constexpr (BITS == 4) *reinterpret_cast<uint32_t*>(codes + k * code_step) = out[0];
+    else *reinterpret_cast<uint2*>(codes + k * code_step) = make_uint2(out[0], out[1]);
+    if (piece % 4 == 0) scales[k * scale_step] = __float2bfloat16_rn(scale);
   }
 }
 
@@ -257,7 +274,7 @@ __global__ void __launch_bounds__(256) quant_append_any_kernel(const __grid_cons
     }
     if (is_q) continue;
     float scale, inv;
-    quant_scale<BITS>(__reduce_max_sync(0xffffffffu, __float_as_uint(r) & 0x7fffffffu), scale, inv);
+    quant_scale<BITS>(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(r) & 0x7fffffffu)), scale, inv);
     const int code = inv == 0.f ? 0 : __float2int_rn(__fdiv_rn(r, scale));
     const uint32_t u = (uint32_t)(code + QuantCode<BITS>::kZero);
     if (BITS == 4) {

@@ -64,16 +64,20 @@ extern "C" int one_paged_quant_append(const one_paged_quant_cache* cache, const 
                    ((reinterpret_cast<uintptr_t>(x.q_out) | reinterpret_cast<uintptr_t>(x.cos) | reinterpret_cast<uintptr_t>(x.sin)) & 15) == 0;
   const int64_t hq = x.q ? x.hq : 0, per = 32 / (cache->dh / 8), rows = dtype == ONE_DTYPE_F32 ? kQuantRows<float> : kQuantRows<__nv_bfloat16>;
   auto groups = [&](int64_t heads) { return (heads + rows - 1) / rows; };
-  const int64_t warps = vec ? (x.n * (2 * groups(cache->hkv) + groups(hq)) + per - 1) / per : x.n * (2 * (int64_t)cache->hkv + hq);
-  if (x.n * (2 * (int64_t)cache->hkv + hq) > 0x7fffffff / 32) return fail(ONE_ERR_UNSUPPORTED, "paged append: too many rows");
-  const dim3 grid((unsigned)((warps + 7) / 8), cache->b);
+  const int64_t all = x.n * (2 * (int64_t)cache->hkv + hq), kinds = 2 * groups(cache->hkv) + groups(hq);
+  if (all > 0x7fffffff / 32 || kinds > 65535) return fail(ONE_ERR_UNSUPPORTED, "paged append: too many rows");
+  p.per = (int)per;
+  p.lane_m = (1024 + cache->dh / 8 - 1) / (cache->dh / 8);
+  const int64_t warps = (x.n + per - 1) / per, block = std::min<int64_t>(8, warps);  // of a kind and group of heads
+  const dim3 grid = vec ? dim3((unsigned)((warps + block - 1) / block), cache->b, (unsigned)kinds) : dim3((unsigned)((all + 7) / 8), cache->b);
+  const dim3 threads((unsigned)(vec ? 32 * block : 256));
   cudaStream_t st = (cudaStream_t)stream;
   auto append = [&](auto t, auto c) {
     using T = decltype(t);
     using C = decltype(c);
     if (cache->bits == 4)
-      return vec ? launch(quant_append_kernel<T, C, 4>, grid, dim3(256), 0, st, p) : launch(quant_append_any_kernel<T, C, 4>, grid, dim3(256), 0, st, p);
-    return vec ? launch(quant_append_kernel<T, C, 8>, grid, dim3(256), 0, st, p) : launch(quant_append_any_kernel<T, C, 8>, grid, dim3(256), 0, st, p);
+      return vec ? launch(quant_append_kernel<T, C, 4>, grid, threads, 0, st, p) : launch(quant_append_any_kernel<T, C, 4>, grid, threads, 0, st, p);
+    return vec ? launch(quant_append_kernel<T, C, 8>, grid, threads, 0, st, p) : launch(quant_append_any_kernel<T, C, 8>, grid, threads, 0, st, p);
   };
   return launched(dtype == ONE_DTYPE_F32   ? append(float(0), float(0))
                   : x.cos && x.tables_fp32 ? append(__nv_bfloat16(), float(0))
