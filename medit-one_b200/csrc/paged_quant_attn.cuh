@@ -7,14 +7,17 @@
 // The scales of a group of 32 dims factor out of its products, so the matrix instructions take the codes
 // themselves. HBM bounds the long cases in principle (72 bytes per slot and kv head of 64 dims at 4 bits);
 // per byte read there are four times the products of a bf16 cache, so what counts is instructions per code:
-//  - a code lies in the low bits of an fp16 whose exponent is 0 (or 1), and that fp16 is u 2^-24, exactly:
-//    one AND opens two codes, and no conversion follows. Halves of bytes at bits 4-7 read as u 2^-20; q,
-//    or the output's scaling, takes up the difference.
-//  - keys: sum q u starts from -z sum q (per query and group, computed once), so u needs no subtraction.
-//    That costs three bits of the fp32 sum at most (u reaches 2 z, c reaches z).
+//  - a code lies in the low bits of an fp16 whose exponent is 0, and that fp16 is u 2^-24, exactly: one AND
+//    opens two codes, and no conversion follows. Halves of bytes at bits 4-7 read as u 2^-20; q, or the
+//    output's scaling, takes up the difference. An instruction aligns its terms by their exponents, which for
+//    such small numbers is up to 2^10 above them: a term of code 1 is good to 2^-14, of larger ones better, far
+//    below bf16's 2^-8. In fp32 the bits of 1024 are put above the code (fp32 outputs of 8 x 3001 slots are
+//    off by 7e-6 of their size without, by 3e-7 with them; bf16 would pay 36.1 -> 38.7 us at 64 x 4096 ragged).
+//  - keys: sum q u starts from -z sum q (per query and group, computed once), so u needs no subtraction; in
+//    fp32 it has one, exact in fp16.
 //  - values: u - z by one packed addition (exact), since a sum over many slots of p z would drown o. (-z sum p
 //    as one more tile per step of 64 slots, from which its sums start, saves the additions and no time: 38.8
-//    and 40.3 us at 64 sequences up to 4096 x 12 x 64.)
+//    and 40.3 us.)
 //  - the codes are the instructions' 16 rows: S^T = K Q^T has slots as rows, O^T = V^T P^T dims, and the
 //    queries are the 8 columns. ldmatrix brings 16-byte pieces of eight slots to the lanes as both need
 //    them: keys straight, values transposed, where a 16-bit element is four (two) codes of one slot.
@@ -91,10 +94,10 @@ ONE_DEVINL void cp_async_some(uint32_t s, const void* g, int bytes) {
 // PQ_4 leaves the odd columns empty, so that a lane has the scores of one head rather than of two.
 enum PqKind { PQ_4, PQ_8, PQ_16, PQ_PAIR4, PQ_PAIR8 };
 
-#ifndef PQ_UNITS
-#define PQ_UNITS 3
-#endif
-constexpr int kQuantUnits = PQ_UNITS;
+// Tiles of a list that a segment's begin and end count as. Us at 0, 1, 2, 4 of them with 128 slots to a tile: 64 x
+// 4096 ragged x 12 x 64 61.8, 49.9, 47.4, 50.1; as it is now, with 64 slots, at 2, 3, 5, 8: 36.6, 36.4, 38.0, 39.3,
+// 64 x 1024 17.8, 18.4, 19.1, 20.9.
+constexpr int kQuantUnits = 2;
 
 template <int DH_, int BITS_, PqKind KIND>
 struct PaQuant {
@@ -126,7 +129,7 @@ struct PaQuant {
   ONE_DEVINL static float weight(float x) { return PAIR ? exp2f(x) : ex2_approx(x); }
 
   uint32_t qb[NL][G][2][2];  // B operands of a group's two products
-  float off[NL][G][4];       // -z sum q as their first sums
+  float off[NL][G][4];       // -z sum q as their first sums (PAIR: 0)
   float fac[NQ];             // from sums to scores, positive
   float o[NL][NT][4];
   float m[NQ], l[NQ];
@@ -267,9 +270,9 @@ struct PaQuant {
       const int e = (int)(__float_as_uint(top) >> 23);                      // 0 .. 255
       // 2^14 over the power of two of top, with the scale's sign
       const float up = copysignf(__uint_as_float((uint32_t)min(254, 268 - e) << 23), p.scale_log2);
-      // sums are q up u 2^-24; halves that read as u 2^-20 have q up 2^-4. A masked slot's -inf stays -inf
-      // under a scale of 0 (2^-126)
-      const float back = fmaxf(fabsf(p.scale_log2) * 1024.f * __uint_as_float((uint32_t)max(14, e) << 23), 1.17549435e-38f);
+      // sums are q up u 2^-24 (PAIR: q up c); halves that read as 16 times as much have q up 2^-4. A masked slot's
+      // -inf stays -inf under a scale of 0 (2^-126)
+      const float back = fmaxf(fabsf(p.scale_log2) * (PAIR ? 0x1p-14f : 0x1p10f) * __uint_as_float((uint32_t)max(14, e) << 23), 0x1p-126f);
       // lane (r, c) has columns 2 c and 2 c + 1 of the sums
 #pragma unroll
       for (int h = 0; h < QL; ++h) fac[n * QL + h] = __shfl_sync(0xffffffffu, back, (2 * c + h) * 4);
@@ -290,9 +293,9 @@ struct PaQuant {
           }
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        sum *= -kZero * 5.9604644775390625e-8f;
+        sum *= -kZero * 0x1p-24f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) off[n][g][i] = __shfl_sync(0xffffffffu, sum, (2 * c + (i & 1)) * 4);
+        for (int i = 0; i < 4; ++i) off[n][g][i] = PAIR ? 0.f : __shfl_sync(0xffffffffu, sum, (2 * c + (i & 1)) * 4);
       }
     }
 #pragma unroll
@@ -340,11 +343,19 @@ struct PaQuant {
     }
     if constexpr (CH % 2) ldmatrix_x2<TRANS>(w[CH - 1][0], w[CH - 1][1], base + step(mine, CH - 1));
   }
-  // Two codes of a word as fp16: those at half (4 bits) or byte (8 bits) e of each of its 16-bit elements
+  // Two stored codes of a word: those at half (4 bits) or byte (8 bits) e of each of its 16-bit elements. As fp16
+  // they are u 2^-24, or u 2^-20 (4 bits, e odd)
   ONE_DEVINL static uint32_t open(uint32_t w, int e) {
     if (BITS == 4) return (e & 2 ? w >> 8 : w) & (e & 1 ? 0x00f000f0u : 0x000f000fu);
     return (e ? w >> 8 : w) & 0x00ff00ffu;
   }
+  // The codes, or 16 times them (4 bits, e odd), 2^-24 times as large unless PAIR
+  ONE_DEVINL static uint32_t open_code(uint32_t w, int e) {
+    const bool high = BITS == 8 || (e & 1);
+    if (PAIR) return f16x2_add(open(w, e) | 0x64006400u, high ? 0xe480e480u : 0xe408e408u);  // -(1024 + z), 16 z
+    return f16x2_add(open(w, e), high ? 0x80808080u : 0x80088008u);
+  }
+  ONE_DEVINL static uint32_t open_key(uint32_t w, int e) { return PAIR ? open_code(w, e) : open(w, e); }
 
   // kGroups x 16 slots, all of them copied; live(i): a bit per slot of group i, full: all are set. scores:
   // row 0's scores of these slots, or null.
@@ -367,8 +378,8 @@ struct PaQuant {
         const uint32_t *w0 = kw[g * PG], *w1 = kw[g * PG + PG - 1];
         // 4 bits: halves 0, 2 then 1, 3 of the words; 8 bits: bytes 0, 1 of the first piece, then of the second
         constexpr int e1 = BITS == 4 ? 2 : 1, e2 = BITS == 4 ? 1 : 0, e3 = BITS == 4 ? 3 : 1;
-        const uint32_t x[2][4] = {{open(w0[0], 0), open(w0[1], 0), open(w0[0], e1), open(w0[1], e1)},
-                                  {open(w1[0], e2), open(w1[1], e2), open(w1[0], e3), open(w1[1], e3)}};
+        const uint32_t x[2][4] = {{open_key(w0[0], 0), open_key(w0[1], 0), open_key(w0[0], e1), open_key(w0[1], e1)},
+                                  {open_key(w1[0], e2), open_key(w1[1], e2), open_key(w1[0], e3), open_key(w1[1], e3)}};
         const float ks[2] = {sc[i][0].get(g, 0x3f803f80u), sc[i][1].get(g, 0x3f803f80u)};
 #pragma unroll
         for (int n = 0; n < NL; ++n) {
@@ -495,9 +506,7 @@ struct PaQuant {
           // rows r and r + 8: halves 2 k and 2 k + 1 (4 bits), bytes 0 and 1 of piece k (8 bits)
           const uint32_t* w = vw[BITS == 4 ? g : 2 * g + k];
           const int e = BITS == 4 ? 2 * k : 0;
-          constexpr uint32_t z0 = BITS == 4 ? 0x80088008u : 0x80808080u, z1 = 0x80808080u;  // -z as they read
-          const uint32_t x[4] = {f16x2_add(open(w[0], e), z0), f16x2_add(open(w[0], e + 1), z1), f16x2_add(open(w[1], e), z0),
-                                 f16x2_add(open(w[1], e + 1), z1)};
+          const uint32_t x[4] = {open_code(w[0], e), open_code(w[0], e + 1), open_code(w[1], e), open_code(w[1], e + 1)};
 #pragma unroll
           for (int n = 0; n < NL; ++n) mma_f16_16816(o[n][2 * g + k], x[0], x[1], x[2], x[3], b[n][0], b[n][1], o[n][2 * g + k]);
         }
@@ -524,7 +533,7 @@ struct PaQuant {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {  // rows r and r + 8 of the tile
           const int d = BITS == 4 ? i / 2 * 32 + 4 * r + i % 2 * 2 + k : i * 16 + 2 * r + k;
-          const float f = BITS == 4 && k ? 32.f : 512.f;  // 2^20 or 2^24, over mult's 2^15
+          const float f = (BITS == 4 && k ? 0x1p-4f : 1.f) * (PAIR ? 0x1p-15f : 0x1p9f);  // 1, 2^24 over mult's 2^15
           so[row * DH + d] = (PAIR ? o[n][i][2 * k] + o[n][i][2 * k + 1] : o[n][i][2 * k + h]) * f * ref;
         }
     }
