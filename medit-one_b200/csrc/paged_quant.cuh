@@ -134,6 +134,9 @@ template <> struct Eight<float> {
 // out, with some eight instructions per value in between; bound by HBM (prompts) or by the chain lengths ->
 // page -> store (single tokens).
 //
+// 8 prompts of up to 4096 tokens, 12 heads x 64, bf16 to 4 bits: 46 us, 60 % of the copy rate; with four heads per lane
+// and four CTAs per SM (that and the read: 66 us; three CTAs 74, two 86; two heads 74 to 78).
+//
 // A lane has 8 dims of kQuantRows heads of a token's keys, queries or values, which share cos and sin; a
 // row's lanes lie side by side in a warp, as many tokens as fit. CTAs of one kind and group of heads each
 // (blockIdx.z), so that warps do not diverge. The half that the rotation needs and the largest value of a
@@ -328,7 +331,8 @@ ONE_DEVINL void quant_open(const uint32_t (&w)[BITS / 4], __nv_bfloat16 scale, E
 
 // Slots starts[b] .. starts[b] + N - 1 of every sequence, those not below lengths[b] as zeros. A lane has 8
 // dims of a slot's keys and values of kReadHeads heads, which share the page; its loads are in flight
-// together. A copy that grows fourfold: bound by HBM, that is by what it writes.
+// together. A copy that grows fourfold: bound by HBM, that is by what it writes: 16 x up to 4096 slots, 12
+// heads x 64, 4 bits to bf16: 40 us, 89 % of the copy rate.
 constexpr int kReadHeads = 4;
 
 template <typename T, int BITS>

@@ -22,6 +22,8 @@
 //    queries are the 8 columns. ldmatrix brings 16-byte pieces of eight slots to the lanes as both need
 //    them: keys straight, values transposed, where a 16-bit element is four (two) codes of one slot.
 //    movmatrix turns the weights from rows to columns in between.
+// Measured: 64 ragged sequences up to 4096 slots, 12 heads x 64, 4 bits: 36 us, 49 % of the measured copy rate (dense
+// bf16: 73); 8 up to 32768, 8 heads x 128 of 4 queries: 42 us, 59 %; one of 1048576, 12 x 64: 178 us, 78 %.
 // fp16 takes q scaled by a power of two to [2^14, 2^15) per row, and 2^(s - m) vs 2^15 / ref with ref a
 // power of two above all the value scales so far, which rises like the running maximum. A bf16 q is exact
 // in it down to 2^-34 of the row's largest; the weights are rounded to 11 bits (2^-11 each, against the
