@@ -84,15 +84,15 @@ struct PagedWs {
 int pad_dh(int dh) { return dh <= 32 ? 32 : dh <= 64 ? 64 : dh <= 96 ? 96 : 128; }
 
 // What the attention over a cache of either kind, in p.c, asks of its arguments, and its plan; `rows` query
-// heads per pass, at most per_sm shares of a list per SM, `units` as E::kSegmentUnits. need: workspace bytes.
+// heads per pass, at most per_sm shares of a list per SM, `units` as E::kSegmentUnits, tiles of least_tile slots or more. need: workspace bytes.
 template <typename S>
-int plan_attention(PagedAttn& p, bool& split, const S* cache, const void* q, int64_t q_bs, int64_t q_hs, int hq, int rows, int per_sm, int units,
+int plan_attention(PagedAttn& p, bool& split, const S* cache, const void* q, int64_t q_bs, int64_t q_hs, int hq, int rows, int per_sm, int units, int least_tile,
                    float scale, void* out, void* workspace, size_t workspace_bytes, size_t need) {
   const int b = cache->b, hkv = cache->hkv, dh = cache->dh, page_size = cache->page_size;
   float* mass = cache->mass;
   const int64_t slots = (int64_t)cache->max_pages * page_size;
   // tiles and a segment's further units, and the list's length rounded up to equal shares, in 31 bits
-  if ((int64_t)b * hq > 0x3fffffff || (int64_t)b * hq * (slots / 64 + 1 + units) > 0x7fffffff - kMaxSms * per_sm)
+  if ((int64_t)b * hq > 0x3fffffff || (int64_t)b * hq * (slots / least_tile + 1 + units) > 0x7fffffff - kMaxSms * per_sm)
     return fail(ONE_ERR_UNSUPPORTED, "paged attention: too many rows");
   if (need && (!workspace || workspace_bytes < need)) return fail(ONE_ERR_INVALID, "workspace too small");
   p.q = q; p.q_bs = q_bs; p.q_hs = q_hs; p.G = hq / hkv;

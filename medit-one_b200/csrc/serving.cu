@@ -47,7 +47,7 @@ extern "C" int one_paged_attention(const one_paged_cache* cache, const void* q, 
   const size_t need = one_paged_attention_workspace_bytes(b, hq, hkv, dh, cache->page_size, cache->max_pages, dtype, cache->mass != nullptr);
   const int rows = paged_rows(dtype, hq / hkv);
   bool split;
-  rc = plan_attention(p, split, cache, q, q_batch_stride, q_head_stride, hq, rows, 3, 0, scale, out, workspace, workspace_bytes, need);
+  rc = plan_attention(p, split, cache, q, q_batch_stride, q_head_stride, hq, rows, 3, 0, 64, scale, out, workspace, workspace_bytes, need);
   if (rc) return rc;
   cudaStream_t st = (cudaStream_t)stream;
   const int d = pad_dh(dh);

@@ -159,7 +159,7 @@ extern "C" int one_paged_quant_attention(const one_paged_quant_cache* cache, con
   p.run = ((at | reinterpret_cast<uintptr_t>(m.scales) | p.s_stride) & 15) == 0 &&
           cache->num_pages * std::max({m.c.k_stride, m.c.v_stride, p.s_stride}) < 0xfffffff0ll * 16;
   bool split;
-  rc = plan_attention(p, split, cache, q, q_batch_stride, q_head_stride, hq, rows, 4 * kPaWarps, kQuantUnits, scale, out, workspace, workspace_bytes, need);
+  rc = plan_attention(p, split, cache, q, q_batch_stride, q_head_stride, hq, rows, 4 * kPaWarps, kQuantUnits, 32, scale, out, workspace, workspace_bytes, need);
   if (rc) return rc;
   return cache->bits == 4 ? attend_bits<4>(p, split, dtype, rows, (cudaStream_t)stream)
                           : attend_bits<8>(p, split, dtype, rows, (cudaStream_t)stream);

@@ -152,6 +152,14 @@ def test_c_entry_points_check_the_rest():
     assert L.one_paged_quant_attention_workspace_bytes(0, 4, 2, 64, 16, 4, 0, 1) == 0
 
 
+def test_lists_past_31_bits_are_refused():
+    """A list counts tiles of 32 slots, for every head of every sequence."""
+    f = C.LIB.one_paged_quant_attention
+    for dh in (32, 64, 128):
+        c = pack(b=4096, hkv=64, dh=dh, ps=16, mp=1 << 14, ts=1 << 14, ks=1 << 20, vs=1 << 20, ss=1 << 20)
+        assert f(c, 64, 4096, 64, 64, 1.0, 0, 64, None, 0, None) == C.ONE_ERR_UNSUPPORTED
+
+
 def test_quantising_on_the_cpu():
     """The tests' own formulas: values come back within half a step, ties go to the even code."""
     x = torch.randn(50, 80, generator=torch.Generator().manual_seed(3)) * 3
