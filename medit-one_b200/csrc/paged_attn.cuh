@@ -736,16 +736,16 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, MODE>::kPerSm) paged_
       }
       return;
     } else {
-    const int t0 = src.len - ahead;
+      const int t0 = src.len - ahead;
 #pragma unroll
-    for (int g = 0; g < GR; ++g) {
-      pg[g] = -1;
-      if (ahead > 16 * g) {
-        const int t = t0 + 16 * g, index = (int)(((uint64_t)(uint32_t)t * p.div_m) >> p.div_s);
-        row[g] = (t - index * c.page_size) * (E::kQuant ? 1 : c.Dh);
-        pg[g] = table[index];
+      for (int g = 0; g < GR; ++g) {
+        pg[g] = -1;
+        if (ahead > 16 * g) {
+          const int t = t0 + 16 * g, index = (int)(((uint64_t)(uint32_t)t * p.div_m) >> p.div_s);
+          row[g] = (t - index * c.page_size) * (E::kQuant ? 1 : c.Dh);
+          pg[g] = table[index];
+        }
       }
-    }
     }
   };
   const int ks = (int)c.k_stride, vs = (int)c.v_stride;
@@ -806,53 +806,53 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, MODE>::kPerSm) paged_
       return;
     } else {
 #pragma unroll
-    for (int k = 0; k + 1 < S::kStages; ++k)
+      for (int k = 0; k + 1 < S::kStages; ++k)
 #pragma unroll
-      for (int g = 0; g < GR; ++g) live[k][g] = live[k + 1][g];
-    if (to_copy > 0) {
+        for (int g = 0; g < GR; ++g) live[k][g] = live[k + 1][g];
+      if (to_copy > 0) {
 #pragma unroll
-      for (int g = 0; g < GR; ++g) {
-        uint8_t* to = ring + put + g * E::kGroup;
-        uint32_t& alive = live[S::kStages - 1][g];
-        const bool good = (uint32_t)pg[g] < (uint32_t)c.num_pages;
-        if (!good && ahead > 16 * g) set_err(c.err, ERR_BAD_ARG, SITE_PAGED_ATTN);
-        if constexpr (E::kQuant) {
-          alive = __ballot_sync(0xffffffffu, good) & 0xffffu;
-          E::copy_any(smem_u32(to), p, keys, values, scales, good ? pg[g] : -1, row[g]);
-        } else if (RUN) {
-          alive = 0;
-          if (good) {
-            const uint8_t* kp = (const uint8_t*)(keys + ((int64_t)pg[g] * ks + row[g]));
-            const uint8_t* vp = (const uint8_t*)(values + ((int64_t)pg[g] * vs + row[g]));
-            if (ahead >= 16 * g + 16) {
-              alive = 0xffffu;
-              E::Keys::full(smem_u32(to), kp);
-              E::Values::full(smem_u32(to) + E::kValues, vp);
-            } else {
-              const int n = ahead - 16 * g;
-              alive = (1u << n) - 1;
-              E::Keys::some(to, kp, n);
-              E::Values::some(to + E::kValues, vp, n);
+        for (int g = 0; g < GR; ++g) {
+          uint8_t* to = ring + put + g * E::kGroup;
+          uint32_t& alive = live[S::kStages - 1][g];
+          const bool good = (uint32_t)pg[g] < (uint32_t)c.num_pages;
+          if (!good && ahead > 16 * g) set_err(c.err, ERR_BAD_ARG, SITE_PAGED_ATTN);
+          if constexpr (E::kQuant) {
+            alive = __ballot_sync(0xffffffffu, good) & 0xffffu;
+            E::copy_any(smem_u32(to), p, keys, values, scales, good ? pg[g] : -1, row[g]);
+          } else if (RUN) {
+            alive = 0;
+            if (good) {
+              const uint8_t* kp = (const uint8_t*)(keys + ((int64_t)pg[g] * ks + row[g]));
+              const uint8_t* vp = (const uint8_t*)(values + ((int64_t)pg[g] * vs + row[g]));
+              if (ahead >= 16 * g + 16) {
+                alive = 0xffffu;
+                E::Keys::full(smem_u32(to), kp);
+                E::Values::full(smem_u32(to) + E::kValues, vp);
+              } else {
+                const int n = ahead - 16 * g;
+                alive = (1u << n) - 1;
+                E::Keys::some(to, kp, n);
+                E::Values::some(to + E::kValues, vp, n);
+              }
             }
+          } else {
+            const int64_t off = !good ? -1 : lane < 16 ? (int64_t)pg[g] * ks + row[g] : (int64_t)pg[g] * vs + row[g];
+            alive = __ballot_sync(0xffffffffu, good) & 0xffffu;
+            if (alive) E::issue_any(to, keys, values, off, c.Dh);
           }
-        } else {
-          const int64_t off = !good ? -1 : lane < 16 ? (int64_t)pg[g] * ks + row[g] : (int64_t)pg[g] * vs + row[g];
-          alive = __ballot_sync(0xffffffffu, good) & 0xffffu;
-          if (alive) E::issue_any(to, keys, values, off, c.Dh);
+        }
+        if (--to_copy > 0) {
+          ahead -= TILE;
+          if (src.next(c, ng)) {
+            to_copy -= MORE;
+            segment();
+            ahead = src.len - src.tile * TILE - mine;
+          }
+          ask();
         }
       }
-      if (--to_copy > 0) {
-        ahead -= TILE;
-        if (src.next(c, ng)) {
-          to_copy -= MORE;
-          segment();
-          ahead = src.len - src.tile * TILE - mine;
-        }
-        ask();
-      }
-    }
-    cp_async_commit();
-    put = put + S::kStage == S::kWarp ? 0 : put + S::kStage;
+      cp_async_commit();
+      put = put + S::kStage == S::kWarp ? 0 : put + S::kStage;
     }
   };
   segment();
