@@ -313,16 +313,15 @@ struct PaQuant {
       for (int i = 0; i < NT; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
   }
 
-  // A slot's scales, K_0 .., V_0 .., two of bf16 to a word. Products in bf16 with powers of two are exact, and
-  // one with (0, f) leaves the upper value alone in its word: as an fp32.
+  // A slot's scales, K_0 .., V_0 .., two of bf16 to a word. Products in bf16 with powers of two are exact; the upper
+  // value is an fp32 once the lower one's bits are cleared (not by a product with 0, which leaves a NaN one).
   static constexpr int kFirstV = G / 2;  // word of V_0
   struct Scales {
     uint32_t w[G];
-    // element i times the power of two f
-    ONE_DEVINL float get(int i, uint32_t f) const {
-      const uint32_t x = w[i / 2];
-      return i & 1 ? __uint_as_float(bf2_mul(x, f & 0xffff0000u)) : bf2_lo(x);
-    }
+    ONE_DEVINL static float half(uint32_t x, int i) { return i & 1 ? bf2_hi(x) : bf2_lo(x); }
+    ONE_DEVINL float get(int i) const { return half(w[i / 2], i); }
+    // element i times the powers of two in f
+    ONE_DEVINL float get(int i, uint32_t f) const { return half(bf2_mul(w[i / 2], f), i); }
     ONE_DEVINL void load(uint32_t at) {
       if constexpr (G == 4)
         asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
@@ -382,7 +381,7 @@ struct PaQuant {
         constexpr int e1 = BITS == 4 ? 2 : 1, e2 = BITS == 4 ? 1 : 0, e3 = BITS == 4 ? 3 : 1;
         const uint32_t x[2][4] = {{open_key(w0[0], 0), open_key(w0[1], 0), open_key(w0[0], e1), open_key(w0[1], e1)},
                                   {open_key(w1[0], e2), open_key(w1[1], e2), open_key(w1[0], e3), open_key(w1[1], e3)}};
-        const float ks[2] = {sc[i][0].get(g, 0x3f803f80u), sc[i][1].get(g, 0x3f803f80u)};
+        const float ks[2] = {sc[i][0].get(g), sc[i][1].get(g)};
 #pragma unroll
         for (int n = 0; n < NL; ++n) {
           float a[4];
@@ -493,7 +492,7 @@ struct PaQuant {
         uint32_t b[NL][2];  // the weights, times the values' scales
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float v = (G + g) % 2 ? sc[i][h].get(G + g, mult2) : bf2_lo(bf2_mul(sc[i][h].w[(G + g) / 2], mult2));
+          const float v = sc[i][h].get(G + g, mult2);
 #pragma unroll
           for (int n = 0; n < NL; ++n) {
             const float y = pr[i][n * QL][h] * v;
