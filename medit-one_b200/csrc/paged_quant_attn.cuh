@@ -7,27 +7,27 @@
 // The scales of a group of 32 dims factor out of its products, so the matrix instructions take the codes
 // themselves. HBM bounds the long cases in principle (72 bytes per slot and kv head of 64 dims at 4 bits);
 // per byte read there are four times the products of a bf16 cache, so what counts is instructions per code:
-//  - a code lies in the low bits of an fp16 whose exponent is 0, and that fp16 is u 2^-24, exactly: one AND
-//    opens two codes, and no conversion follows. Halves of bytes at bits 4-7 read as u 2^-20; q, or the
-//    output's scaling, takes up the difference. An instruction aligns its terms by their exponents, which for
-//    such small numbers is up to 2^10 above them: a term of code 1 is good to 2^-14, of larger ones better, far
-//    below bf16's 2^-8. In fp32 the bits of 1024 are put above the code (fp32 outputs of 8 x 3001 slots are
-//    off by 7e-6 of their size without, by 3e-7 with them; bf16 would pay 36.1 -> 38.7 us at 64 x 4096 ragged).
-//  - keys: sum q u starts from -z sum q (per query and group, computed once), so u needs no subtraction; in
-//    fp32 it has one, exact in fp16.
-//  - values: u - z by one packed addition (exact), since a sum over many slots of p z would drown o. (-z sum p
-//    as one more tile per step of 64 slots, from which its sums start, saves the additions and no time: 38.8
-//    and 40.3 us.)
+//  - keys, in fp16: a code lies in the low bits of an fp16 whose exponent is 0, and that fp16 is u 2^-24,
+//    exactly: one AND opens two codes, and no conversion follows. Halves of bytes at bits 4-7 read as u 2^-20;
+//    q takes up the difference. An instruction aligns its terms by their exponents, which for such small
+//    numbers is up to 2^10 above them: a term of code 1 is good to 2^-14, of larger ones better, far below
+//    bf16's 2^-8. In fp32 the bits of 1024 are put above the code.
+//  - sum q u starts from -z sum q (per query and group, computed once), so u needs no subtraction; in fp32 it
+//    has one, exact in fp16.
+//  - values, in bf16: the bits of 128 or 16 above the code and one packed addition of -(128 + z) or -(16 + z),
+//    both exact (a sum over many slots of p z would drown o).
+//  - weights times their scales, in bf16 parts, which together have 16 bits (fp32: all 24): a part has its own
+//    exponent, so that each output is as good as its own terms, whatever the scales of other slots and
+//    groups are. (fp16 with an exponent in common, of the largest scale so far, lost values 2^-28 of it, and took 36 us where this
+//    takes 41.)
 //  - the codes are the instructions' 16 rows: S^T = K Q^T has slots as rows, O^T = V^T P^T dims, and the
 //    queries are the 8 columns. ldmatrix brings 16-byte pieces of eight slots to the lanes as both need
 //    them: keys straight, values transposed, where a 16-bit element is four (two) codes of one slot.
 //    movmatrix turns the weights from rows to columns in between.
-// Measured: 64 ragged sequences up to 4096 slots, 12 heads x 64, 4 bits: 36 us, 49 % of the measured copy rate (dense
-// bf16: 73); 8 up to 32768, 8 heads x 128 of 4 queries: 42 us, 59 %; one of 1048576, 12 x 64: 178 us, 78 %.
-// fp16 takes q scaled by a power of two to [2^14, 2^15) per row, and 2^(s - m) vs 2^15 / ref with ref a
-// power of two above all the value scales so far, which rises like the running maximum. A bf16 q is exact
-// in it down to 2^-34 of the row's largest; the weights are rounded to 11 bits (2^-11 each, against the
-// output's 2^-8). In fp32, q and the weights are two fp16 parts (22 bits), in neighbouring columns.
+// Measured: 64 ragged sequences up to 4096 slots, 12 heads x 64, 4 bits: 41 us, 44 % of the measured copy rate (dense
+// bf16: 73); 8 up to 32768, 8 heads x 128 of 4 queries: 48 us, 52 %; one of 1048576, 12 x 64: 214 us, 65 %.
+// fp16 takes q scaled by a power of two to [2^14, 2^15) per row. A bf16 q is exact in it down to 2^-34 of
+// the row's largest; in fp32, q is two fp16 parts (22 bits), in neighbouring columns.
 #pragma once
 
 #include "paged_attn.cuh"
@@ -35,6 +35,11 @@
 
 namespace one {
 
+ONE_DEVINL void mma_bf16_acc(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
 ONE_DEVINL void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1,
                               const float (&c)[4]) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
@@ -93,7 +98,8 @@ ONE_DEVINL void cp_async_some(uint32_t s, const void* g, int bytes) {
 }
 
 // PQ_4, PQ_8, PQ_16: bf16, up to so many query heads. PQ_PAIR4, PQ_PAIR8: fp32 in two parts, up to 4 or 8.
-// PQ_4 leaves the odd columns empty, so that a lane has the scores of one head rather than of two.
+// PQ_4 and the pairs have a query's parts in the columns 2 c and 2 c + 1, so that a lane has the scores of one
+// head rather than of two (PQ_4: q has one part, its weights two).
 enum PqKind { PQ_4, PQ_8, PQ_16, PQ_PAIR4, PQ_PAIR8 };
 
 // Tiles of a list that a segment's begin and end count as. Us at 0, 1, 2, 4 of them with 128 slots to a tile: 64 x
@@ -110,6 +116,7 @@ struct PaQuant {
   static constexpr int DH = DH_, BITS = BITS_, ROWS = KIND == PQ_16 ? 16 : KIND == PQ_4 || KIND == PQ_PAIR4 ? 4 : 8;
   static constexpr int NL = KIND == PQ_16 || KIND == PQ_PAIR8 ? 2 : 1;  // tiles of 8 columns
   static constexpr bool ODD = KIND == PQ_8 || KIND == PQ_16;  // odd columns are queries of their own
+  static constexpr int NP = KIND == PQ_4 ? 1 : 2;        // instructions that a weight's parts take: 2, or 3 of fp32
   static constexpr int QL = ODD ? 2 : 1, NQ = NL * QL;   // queries of a lane, per tile and in all
   static constexpr int G = DH / kQuantGroup;             // groups of a row
   static constexpr int RB = DH * BITS / 8, CH = RB / 16; // bytes and pieces of a row
@@ -135,7 +142,6 @@ struct PaQuant {
   float fac[NQ];             // from sums to scores, positive
   float o[NL][NT][4];
   float m[NQ], l[NQ];
-  float ref, mult;           // above all the value scales so far; 2^15 / ref
   uint32_t mine;             // where this lane's row of the first pieces lies
 
   // Where piece ch of row `row` lies: eight rows' pieces ch are on different banks, and a 128-byte line of
@@ -305,23 +311,17 @@ struct PaQuant {
       m[i] = -INFINITY;
       l[i] = 0.f;
     }
-    ref = 0.f;
-    mult = 0.f;
 #pragma unroll
     for (int n = 0; n < NL; ++n)
 #pragma unroll
       for (int i = 0; i < NT; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
   }
 
-  // A slot's scales, K_0 .., V_0 .., two of bf16 to a word. Products in bf16 with powers of two are exact; the upper
-  // value is an fp32 once the lower one's bits are cleared (not by a product with 0, which leaves a NaN one).
-  static constexpr int kFirstV = G / 2;  // word of V_0
+  // A slot's scales, K_0 .., V_0 .., two of bf16 to a word. The upper one is an fp32 once the lower one's bits are
+  // cleared (not by a product with 0, which leaves a NaN one).
   struct Scales {
     uint32_t w[G];
-    ONE_DEVINL static float half(uint32_t x, int i) { return i & 1 ? bf2_hi(x) : bf2_lo(x); }
-    ONE_DEVINL float get(int i) const { return half(w[i / 2], i); }
-    // element i times the powers of two in f
-    ONE_DEVINL float get(int i, uint32_t f) const { return half(bf2_mul(w[i / 2], f), i); }
+    ONE_DEVINL float get(int i) const { return i & 1 ? bf2_hi(w[i / 2]) : bf2_lo(w[i / 2]); }
     ONE_DEVINL void load(uint32_t at) {
       if constexpr (G == 4)
         asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
@@ -350,13 +350,34 @@ struct PaQuant {
     if (BITS == 4) return (e & 2 ? w >> 8 : w) & (e & 1 ? 0x00f000f0u : 0x000f000fu);
     return (e ? w >> 8 : w) & 0x00ff00ffu;
   }
-  // The codes, or 16 times them (4 bits, e odd), 2^-24 times as large unless PAIR
-  ONE_DEVINL static uint32_t open_code(uint32_t w, int e) {
-    const bool high = BITS == 8 || (e & 1);
-    if (PAIR) return f16x2_add(open(w, e) | 0x64006400u, high ? 0xe480e480u : 0xe408e408u);  // -(1024 + z), 16 z
-    return f16x2_add(open(w, e), high ? 0x80808080u : 0x80088008u);
+  ONE_DEVINL static uint32_t open_key(uint32_t w, int e) {
+    if (!PAIR) return open(w, e);
+    return f16x2_add(open(w, e) | 0x64006400u, BITS == 8 || (e & 1) ? 0xe480e480u : 0xe408e408u);  // -(1024 + z), 16 z
   }
-  ONE_DEVINL static uint32_t open_key(uint32_t w, int e) { return PAIR ? open_code(w, e) : open(w, e); }
+  // The same two codes, without their offset, in bf16
+  ONE_DEVINL static uint32_t open_value(uint32_t w, int e) {
+    if (BITS == 4) {
+      if (e & 1) return bf2_add(((e & 2 ? w >> 9 : w >> 1) & 0x00780078u) | 0x41804180u, 0xc1c0c1c0u);  // 16 + u - 24
+      return bf2_add(((e & 2 ? w >> 8 : w) & 0x000f000fu) | 0x43004300u, 0xc308c308u);                  // 128 + u - 136
+    }
+    const uint32_t x = e ? w >> 8 : w;  // of the 8 bits 7 fit: 128 + u % 128 - (u < 128 ? 256 : 128)
+    return bf2_add((x & 0x007f007fu) | 0x43004300u, (x & 0x00800080u) ^ 0xc380c380u);
+  }
+  // Weights as bf16 parts whose sum is the weight to 16 bits (PAIR: all 24), as B operands before their turn:
+  // the two columns of y0 and y1, or of the parts of y0
+  ONE_DEVINL static void parts(float y0, float y1, uint32_t (&w)[NP]) {
+    const uint32_t u0 = __float_as_uint(y0), u1 = __float_as_uint(y1);
+    const float r0 = y0 - bf2_hi(u0), r1 = y1 - bf2_hi(u1);  // exact
+    if constexpr (ODD) {
+      w[0] = __byte_perm(u0, u1, 0x7632);
+      w[1] = pack_bf16x2(r0, r1);
+    } else if constexpr (PAIR) {
+      w[0] = __byte_perm(u0, __float_as_uint(r0), 0x7632);
+      w[1] = __float_as_uint(r0 - bf2_hi(__float_as_uint(r0))) >> 16;
+    } else {
+      w[0] = pack_bf16x2(bf2_hi(u0), r0);
+    }
+  }
 
   // kGroups x 16 slots, all of them copied; live(i): a bit per slot of group i, full: all are set. scores:
   // row 0's scores of these slots, or null.
@@ -366,8 +387,6 @@ struct PaQuant {
     const uint32_t scale_at = base + kScales + r * SR;
     float pr[kGroups][NQ][2];  // slots r and r + 8
     Scales sc[kGroups][2];
-    uint32_t top[G - kFirstV] = {};  // largest value scales, halves apart (as whole numbers: NaN is above all, and makes
-                                     // its own group's sums NaN only)
 #pragma unroll
     for (int i = 0; i < kGroups; ++i) {
       uint32_t kw[CH][2];
@@ -397,14 +416,6 @@ struct PaQuant {
             }
         }
       }
-#pragma unroll
-      for (int k = kFirstV; k < G; ++k) top[k - kFirstV] = __vmaxu2(top[k - kFirstV], __vmaxu2(sc[i][0].w[k], sc[i][1].w[k]));
-    }
-    float vmax = 0.f;
-#pragma unroll
-    for (int k = kFirstV; k < G; ++k) {
-      if (k > kFirstV || G % 2 == 0) vmax = fmaxf(vmax, bf2_lo(top[k - kFirstV]));
-      vmax = fmaxf(vmax, bf2_hi(top[k - kFirstV]));
     }
     if (!full) {
 #pragma unroll
@@ -432,7 +443,7 @@ struct PaQuant {
       }
     }
     float mx[NQ];
-    bool rises = vmax > ref;
+    bool rises = false;
 #pragma unroll
     for (int t = 0; t < NQ; ++t) {
       mx[t] = fmaxf(pr[0][t][0], pr[0][t][1]);
@@ -444,18 +455,9 @@ struct PaQuant {
     // m stands in all the lanes of a column, so that it rises for none of them alone
     if (__any_sync(0xffffffffu, rises)) {
 #pragma unroll
-      for (int d = 4; d < 32; d <<= 1) {
-        vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, d));
+      for (int d = 4; d < 32; d <<= 1)
 #pragma unroll
         for (int t = 0; t < NQ; ++t) mx[t] = fmaxf(mx[t], __shfl_xor_sync(0xffffffffu, mx[t], d));
-      }
-      float f = 1.f;
-      if (vmax > ref) {  // 2^-100 < ref <= 2^127
-        const uint32_t e = min(max(__float_as_uint(vmax) >> 23, 27u) + 1, 254u);
-        f = ref * __uint_as_float((254 - min(e, 253u)) << 23) * (e == 254u ? 0.5f : 1.f);
-        ref = __uint_as_float(e << 23);
-        mult = __uint_as_float((269 - e) << 23);
-      }
       float a[NQ];
 #pragma unroll
       for (int t = 0; t < NQ; ++t) {
@@ -463,7 +465,6 @@ struct PaQuant {
         a[t] = weight(m[t] - (mn == -INFINITY ? 0.f : mn));
         m[t] = mn;
         l[t] *= a[t];
-        a[t] *= f;
       }
 #pragma unroll
       for (int n = 0; n < NL; ++n)
@@ -475,7 +476,6 @@ struct PaQuant {
     float ms[NQ];
 #pragma unroll
     for (int t = 0; t < NQ; ++t) ms[t] = m[t] == -INFINITY ? 0.f : m[t];
-    const uint32_t mult2 = pack_bf16x2(mult, mult);
 #pragma unroll
     for (int i = 0; i < kGroups; ++i) {
 #pragma unroll
@@ -489,17 +489,16 @@ struct PaQuant {
       pieces<true>(vw, base + i * kGroup + kValues);
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        uint32_t b[NL][2];  // the weights, times the values' scales
+        uint32_t b[NL][NP][2];  // the weights, times the values' scales
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float v = sc[i][h].get(G + g, mult2);
+          const float v = sc[i][h].get(G + g);
 #pragma unroll
           for (int n = 0; n < NL; ++n) {
-            const float y = pr[i][n * QL][h] * v;
-            uint32_t w;
-            if constexpr (PAIR) w = pack_f16x2(y, y - f16_lo(pack_f16x2(y, 0.f)));
-            else w = pack_f16x2(y, ODD ? pr[i][n * QL + QL - 1][h] * v : 0.f);
-            b[n][h] = movmatrix_trans(w);
+            uint32_t w[NP];
+            parts(pr[i][n * QL][h] * v, pr[i][n * QL + QL - 1][h] * v, w);
+#pragma unroll
+            for (int k = 0; k < NP; ++k) b[n][k][h] = movmatrix_trans(w[k]);
           }
         }
 #pragma unroll
@@ -507,9 +506,11 @@ struct PaQuant {
           // rows r and r + 8: halves 2 k and 2 k + 1 (4 bits), bytes 0 and 1 of piece k (8 bits)
           const uint32_t* w = vw[BITS == 4 ? g : 2 * g + k];
           const int e = BITS == 4 ? 2 * k : 0;
-          const uint32_t x[4] = {open_code(w[0], e), open_code(w[0], e + 1), open_code(w[1], e), open_code(w[1], e + 1)};
+          const uint32_t x[4] = {open_value(w[0], e), open_value(w[0], e + 1), open_value(w[1], e), open_value(w[1], e + 1)};
 #pragma unroll
-          for (int n = 0; n < NL; ++n) mma_f16_16816(o[n][2 * g + k], x[0], x[1], x[2], x[3], b[n][0], b[n][1], o[n][2 * g + k]);
+          for (int n = 0; n < NL; ++n)
+#pragma unroll
+            for (int part = 0; part < NP; ++part) mma_bf16_acc(o[n][2 * g + k], x, b[n][part]);
         }
       }
     }
@@ -534,8 +535,7 @@ struct PaQuant {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {  // rows r and r + 8 of the tile
           const int d = BITS == 4 ? i / 2 * 32 + 4 * r + i % 2 * 2 + k : i * 16 + 2 * r + k;
-          const float f = (BITS == 4 && k ? 0x1p-4f : 1.f) * (PAIR ? 0x1p-15f : 0x1p9f);  // 1, 2^24 over mult's 2^15
-          so[row * DH + d] = (PAIR ? o[n][i][2 * k] + o[n][i][2 * k + 1] : o[n][i][2 * k + h]) * f * ref;
+          so[row * DH + d] = ODD ? o[n][i][2 * k + h] : o[n][i][2 * k] + o[n][i][2 * k + 1];
         }
     }
   }

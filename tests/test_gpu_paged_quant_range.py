@@ -3,12 +3,14 @@ formula, by the sizes of its own terms."""
 import pytest
 import torch
 
+import quant_range_util as R
 import quant_util as Q
 
 pytestmark = pytest.mark.gpu
 BF, F32 = torch.bfloat16, torch.float32
 INF, NAN = float("inf"), float("nan")
 KINDS = [(BF, 1), (BF, 4), (BF, 6), (BF, 12), (F32, 2), (F32, 7)]  # dtype and queries per kv head: every kind of kernel
+SHAPES = [([513], 64, 16), ([300], 128, 16), ([200], 96, 5), ([9000, 700], 64, 16), ([5000], 48, 7)]  # whole groups, rows looked up; clusters, lists
 
 
 @pytest.fixture(autouse=True)
@@ -56,3 +58,77 @@ def test_groups_beside_one_that_is_not_finite(bits, dt, g, dh, page):
         e = Q.weight_error(40, dh, smax, dt)
         d, tol = (out.double() - ref).abs(), e * mag + torch.finfo(dt).eps / 2 * ref.abs() * (1 + e)
         assert bool((d <= tol)[..., ~nan].all()), float((d / tol)[..., ~nan].max())
+
+
+def zero_code(bits):
+    return 0x88 if bits == 4 else 128
+
+
+def least_code(bits):
+    return 0x11 if bits == 4 else 1
+
+
+def check(q, cache, bits, scale, mass=False, floor=0.0):
+    ref, tol, w, wt = R.attention(q, cache, bits, scale)
+    m0 = m = None
+    if mass:
+        m0 = torch.rand(q.shape[0], cache[0].shape[1], cache[3].shape[1] * cache[0].shape[2], generator=torch.Generator().manual_seed(1))
+        m = m0.cuda()
+    out = ops().turbo_paged_quant_attention(q.cuda(), *(x.cuda() for x in cache), scale_factor=scale, mass=m)
+    R.check_out(out, ref, tol, floor)
+    if mass:
+        R.check_mass(m, m0, w, wt, q.shape[1] // cache[0].shape[1])
+    return out
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dt,g", KINDS)
+@pytest.mark.parametrize("lengths,dh,page", SHAPES)
+def test_a_huge_value_that_nobody_attends_to(bits, dt, g, lengths, dh, page):
+    """One slot of values 2^40 times the others', and a score some 50 below them: it adds 2^-30 of the output."""
+    for at in (0, lengths[0] // 2, lengths[0] - 1):
+        cache, q, _ = make(lengths, 2, g, dh, page, bits, dt, 11 + at, positive=True)
+        pg, row = place(cache, 0, at)
+        cache[0][pg, :, row] = least_code(bits)
+        cache[2][pg, :, row, 0] = 50.0 / (Q.top(bits) * float(q.float().sum(-1).mean()) * dh ** -0.5)
+        cache[2][pg, :, row, 1] *= 2.0 ** 40
+        check(q, cache, bits, dh ** -0.5, mass=at == 0)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dt,g", KINDS)
+@pytest.mark.parametrize("lengths,dh,page", SHAPES)
+@pytest.mark.parametrize("far", [30, 60])
+def test_groups_of_values_far_apart(bits, dt, g, lengths, dh, page, far):
+    """One group of 32 dims of every value is 2^far times the others: each dim by its own terms."""
+    cache, q, _ = make(lengths, 2, g, dh, page, bits, dt, 21 + far)
+    for group in (0, Q.groups(dh) - 1):
+        c = list(cache)
+        c[2] = cache[2].clone()
+        c[2][..., 1, group] *= 2.0 ** far
+        check(q, c, bits, dh ** -0.5)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dt,g", KINDS)
+@pytest.mark.parametrize("dh,page", [(64, 16), (128, 16), (80, 8)])
+def test_dims_that_a_huge_value_leaves_alone(bits, dt, g, dh, page):
+    """A slot like any other, of values 2^50 times the others', whose code is 0 in some dims."""
+    cache, q, _ = make([400, 90], 2, g, dh, page, bits, dt, 31)
+    for b, at in ((0, 0), (0, 200), (1, 89)):
+        pg, row = place(cache, b, at)
+        cache[1][pg, :, row, ::3] = zero_code(bits)
+        cache[2][pg, :, row, 1] *= 2.0 ** 50
+    check(q, cache, bits, dh ** -0.5)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dt,g", KINDS)
+@pytest.mark.parametrize("size", [-100, -60, 90])
+def test_values_of_the_smallest_and_of_large_scales(bits, dt, g, size):
+    """Scales from 2^-100 on; products of the smallest ones and of small weights end at 2^-133 (bf16's last
+    step) in their last part, of at most 128 times 400."""
+    cache, q, _ = make([400, 33], 2, g, 64, 16, bits, dt, 41)
+    used = torch.isfinite(cache[2][..., 1, :].float())
+    cache[2][..., 1, :] = torch.where(used, torch.exp2(torch.full(used.shape, float(size))).bfloat16(), cache[2][..., 1, :])
+    check(q, cache, bits, 0.125, floor=2.0 ** -133 * 128 * 400)
