@@ -9,25 +9,26 @@
 // per byte read there are four times the products of a bf16 cache, so what counts is instructions per code:
 //  - keys, in fp16: a code lies in the low bits of an fp16 whose exponent is 0, and that fp16 is u 2^-24,
 //    exactly: one AND opens two codes, and no conversion follows. Halves of bytes at bits 4-7 read as u 2^-20;
-//    q takes up the difference. An instruction aligns its terms by their exponents, which for such small
-//    numbers is up to 2^10 above them: a term of code 1 is good to 2^-14, of larger ones better, far below
-//    bf16's 2^-8. In fp32 the bits of 1024 are put above the code.
-//  - sum q u starts from -z sum q (per query and group, computed once), so u needs no subtraction; in fp32 it
-//    has one, exact in fp16.
+//    q takes up the difference. sum q u starts from -z sum q (per query and group, computed once), so u needs
+//    no subtraction. An instruction aligns its terms by their exponents, which for such small numbers is up to
+//    2^10 above them; products of a bf16 q and a code have 16 bits at most and lose little by that (weights of
+//    scores whose terms sum to 2000 are off by 1e-5 either way). In fp32 the bits of 1024 are put above
+//    the code and taken off with its offset, exactly; so they are for 9 to 16 queries, whose first sums would
+//    take registers that spill (8 x 32768 slots, 8 heads x 128 of 16 queries: 96 us, so 93; of 8: 59, so 67).
+//  - q scaled by a power of two per row and group, its largest to [2^14, 2^15): a bf16 q is exact in it down to
+//    2^-27 of its group's largest; in fp32, q is two fp16 parts (22 bits), in neighbouring columns.
 //  - values, in bf16: the bits of 128 or 16 above the code and one packed addition of -(128 + z) or -(16 + z),
 //    both exact (a sum over many slots of p z would drown o).
 //  - weights times their scales, in bf16 parts, which together have 16 bits (fp32: all 24): a part has its own
 //    exponent, so that each output is as good as its own terms, whatever the scales of other slots and
-//    groups are. (fp16 with an exponent in common, of the largest scale so far, lost values 2^-28 of it, and took 36 us where this
-//    takes 41.)
+//    groups are. (fp16 with an exponent in common, of the largest scale so far, lost values 2^-28 of it,
+//    and took 36 us where this takes 41.)
 //  - the codes are the instructions' 16 rows: S^T = K Q^T has slots as rows, O^T = V^T P^T dims, and the
 //    queries are the 8 columns. ldmatrix brings 16-byte pieces of eight slots to the lanes as both need
 //    them: keys straight, values transposed, where a 16-bit element is four (two) codes of one slot.
 //    movmatrix turns the weights from rows to columns in between.
-// Measured: 64 ragged sequences up to 4096 slots, 12 heads x 64, 4 bits: 41 us, 44 % of the measured copy rate (dense
-// bf16: 73); 8 up to 32768, 8 heads x 128 of 4 queries: 48 us, 52 %; one of 1048576, 12 x 64: 214 us, 65 %.
-// fp16 takes q scaled by a power of two to [2^14, 2^15) per row. A bf16 q is exact in it down to 2^-34 of
-// the row's largest; in fp32, q is two fp16 parts (22 bits), in neighbouring columns.
+// Measured: 64 ragged sequences up to 4096 slots, 12 heads x 64, 4 bits: 41 us, 43 % of the measured copy rate (dense
+// bf16: 73); 8 up to 32768, 8 heads x 128 of 4 queries: 49 us, 51 %; one of 1048576, 12 x 64: 217 us, 64 %.
 #pragma once
 
 #include "paged_attn.cuh"
@@ -117,6 +118,7 @@ struct PaQuant {
   static constexpr int NL = KIND == PQ_16 || KIND == PQ_PAIR8 ? 2 : 1;  // tiles of 8 columns
   static constexpr bool ODD = KIND == PQ_8 || KIND == PQ_16;  // odd columns are queries of their own
   static constexpr int NP = KIND == PQ_4 ? 1 : 2;        // instructions that a weight's parts take: 2, or 3 of fp32
+  static constexpr bool OPEN = PAIR || KIND == PQ_16;    // keys without their offset
   static constexpr int QL = ODD ? 2 : 1, NQ = NL * QL;   // queries of a lane, per tile and in all
   static constexpr int G = DH / kQuantGroup;             // groups of a row
   static constexpr int RB = DH * BITS / 8, CH = RB / 16; // bytes and pieces of a row
@@ -138,8 +140,8 @@ struct PaQuant {
   ONE_DEVINL static float weight(float x) { return PAIR ? exp2f(x) : ex2_approx(x); }
 
   uint32_t qb[NL][G][2][2];  // B operands of a group's two products
-  float off[NL][G][4];       // -z sum q as their first sums (PAIR: 0)
-  float fac[NQ];             // from sums to scores, positive
+  float off[NL][G][4];       // -z sum q as their first sums (OPEN: 0)
+  float fac[NQ][G];          // from a group's sums to scores, positive
   float o[NL][NT][4];
   float m[NQ], l[NQ];
   uint32_t mine;             // where this lane's row of the first pieces lies
@@ -243,10 +245,10 @@ struct PaQuant {
     mine = at(8 * (lane >> 3 & 1) + (lane & 7), CH == 1 ? 0 : lane >> 4);
 #pragma unroll
     for (int n = 0; n < NL; ++n) {
-      // column r: query 8 n + r, or part r % 2 of query 4 n + r / 2 (PQ_4: the second part is 0). This lane's 8 dims of each group in memory's
-      // order: 8 c .., or 4 c .. and 16 + 4 c ..
+      // column r: query 8 n + r, or part r % 2 of query 4 n + r / 2 (PQ_4: the second part is 0). This lane's 8
+      // dims of each group in memory's order: 8 c .., or 4 c .. and 16 + 4 c ..
       const int row = ODD ? 8 * n + r : 4 * n + (r >> 1);
-      float x[G][8], top = 0.f;
+      float x[G][8];
       const T* y = q + row * stride;
 #pragma unroll
       for (int g = 0; g < G; ++g) {
@@ -270,23 +272,19 @@ struct PaQuant {
             }
           }
         }
+        float top = 0.f, sum = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[g][i]));
-      }
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const int e = (int)(__float_as_uint(top) >> 23);                      // 0 .. 255
-      // 2^14 over the power of two of top, with the scale's sign
-      const float up = copysignf(__uint_as_float((uint32_t)min(254, 268 - e) << 23), p.scale_log2);
-      // sums are q up u 2^-24 (PAIR: q up c); halves that read as 16 times as much have q up 2^-4. A masked slot's
-      // -inf stays -inf under a scale of 0 (2^-126)
-      const float back = fmaxf(fabsf(p.scale_log2) * (PAIR ? 0x1p-14f : 0x1p10f) * __uint_as_float((uint32_t)max(14, e) << 23), 0x1p-126f);
-      // lane (r, c) has columns 2 c and 2 c + 1 of the sums
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int e = (int)(__float_as_uint(top) >> 23);                      // 0 .. 255
+        // 2^14 over the power of two of top, with the scale's sign
+        const float up = copysignf(__uint_as_float((uint32_t)min(254, 268 - e) << 23), p.scale_log2);
+        // the sums are of q up u 2^-24 (OPEN: q up c); halves that read as 16 times as much have q up 2^-4
+        const float back = fabsf(p.scale_log2) * __uint_as_float((uint32_t)max(14, e) << 23) * (OPEN ? 0x1p-14f : 0x1p10f);
+        // lane (r, c) has columns 2 c and 2 c + 1 of the sums
 #pragma unroll
-      for (int h = 0; h < QL; ++h) fac[n * QL + h] = __shfl_sync(0xffffffffu, back, (2 * c + h) * 4);
-#pragma unroll
-      for (int g = 0; g < G; ++g) {
-        float sum = 0.f;
+        for (int h = 0; h < QL; ++h) fac[n * QL + h][g] = __shfl_sync(0xffffffffu, back, (2 * c + h) * 4);
 #pragma unroll
         for (int k = 0; k < 2; ++k)
 #pragma unroll
@@ -303,7 +301,7 @@ struct PaQuant {
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
         sum *= -kZero * 0x1p-24f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) off[n][g][i] = PAIR ? 0.f : __shfl_sync(0xffffffffu, sum, (2 * c + (i & 1)) * 4);
+        for (int i = 0; i < 4; ++i) off[n][g][i] = OPEN ? 0.f : __shfl_sync(0xffffffffu, sum, (2 * c + (i & 1)) * 4);
       }
     }
 #pragma unroll
@@ -351,7 +349,7 @@ struct PaQuant {
     return (e ? w >> 8 : w) & 0x00ff00ffu;
   }
   ONE_DEVINL static uint32_t open_key(uint32_t w, int e) {
-    if (!PAIR) return open(w, e);
+    if (!OPEN) return open(w, e);
     return f16x2_add(open(w, e) | 0x64006400u, BITS == 8 || (e & 1) ? 0xe480e480u : 0xe408e408u);  // -(1024 + z), 16 z
   }
   // The same two codes, without their offset, in bf16
@@ -411,8 +409,9 @@ struct PaQuant {
 #pragma unroll
             for (int k = 0; k < QL; ++k) {
               const float y = PAIR ? a[2 * h] + a[2 * h + 1] : a[2 * h + k];
+              const float f = ks[h] * fac[n * QL + k][g];
               float& s = pr[i][n * QL + k][h];
-              s = g ? s + ks[h] * y : ks[h] * y;
+              s = g ? s + f * y : f * y;
             }
         }
       }
@@ -436,8 +435,8 @@ struct PaQuant {
           float* to = scores + row * p.score_ld + r;
 #pragma unroll
           for (int i = 0; i < kGroups; ++i) {
-            to[16 * i] = pr[i][t][0] * fac[t];
-            to[16 * i + 8] = pr[i][t][1] * fac[t];
+            to[16 * i] = pr[i][t][0];
+            to[16 * i + 8] = pr[i][t][1];
           }
         }
       }
@@ -449,7 +448,6 @@ struct PaQuant {
       mx[t] = fmaxf(pr[0][t][0], pr[0][t][1]);
 #pragma unroll
       for (int i = 1; i < kGroups; ++i) mx[t] = fmax3(mx[t], pr[i][t][0], pr[i][t][1]);
-      mx[t] *= fac[t];
       rises |= mx[t] > m[t];
     }
     // m stands in all the lanes of a column, so that it rises for none of them alone
@@ -481,8 +479,8 @@ struct PaQuant {
 #pragma unroll
       for (int t = 0; t < NQ; ++t) {
         float(&x)[2] = pr[i][t];
-        x[0] = weight(fmaf(x[0], fac[t], -ms[t]));
-        x[1] = weight(fmaf(x[1], fac[t], -ms[t]));
+        x[0] = weight(x[0] - ms[t]);
+        x[1] = weight(x[1] - ms[t]);
         l[t] += x[0] + x[1];
       }
       uint32_t vw[CH][2];

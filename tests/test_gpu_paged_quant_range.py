@@ -132,3 +132,67 @@ def test_values_of_the_smallest_and_of_large_scales(bits, dt, g, size):
     used = torch.isfinite(cache[2][..., 1, :].float())
     cache[2][..., 1, :] = torch.where(used, torch.exp2(torch.full(used.shape, float(size))).bfloat16(), cache[2][..., 1, :])
     check(q, cache, bits, 0.125, floor=2.0 ** -133 * 128 * 400)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dt,g", KINDS)
+@pytest.mark.parametrize("dh,page", [(64, 16), (128, 16), (80, 8)])
+def test_scores_whose_terms_are_large(bits, dt, g, dh, page):
+    """Small codes, sums of terms of some 2000 in all, which cancel to scores near 0: the weights show each
+    score's error."""
+    gen = torch.Generator().manual_seed(51)
+    n, groups, top = 200, Q.groups(dh), Q.top(bits)
+    q = torch.randn(1, g, 1, dh, generator=gen).to(dt)
+    codes = torch.randint(-1, 2, (1 << 17, dh), generator=gen)
+    ks = (torch.rand(1 << 17, groups, generator=gen) + 0.5).bfloat16()
+    k = codes.double() * ks.double().repeat_interleave(32, -1)[:, :dh]
+    lead = q[0, 0, 0].double()
+    scale = 2000.0 / float((k.abs() @ lead.abs()).mean())
+    pick = torch.argsort((k @ lead).abs())[:n]  # of the first query; the others' are what they are
+    pick = pick[torch.randperm(n, generator=gen)]
+    u = (codes[pick] + top + 1).to(torch.uint8)
+    u = u[:, 0::2] + 16 * u[:, 1::2] if bits == 4 else u
+    cache, _, _ = make([n], 1, 1, dh, page, bits, dt, 52)
+    for t in range(n):
+        pg, row = place(cache, 0, t)
+        cache[0][pg, 0, row] = u[t]
+        cache[2][pg, 0, row, 0] = ks[pick[t]]
+    check(q, cache, bits, scale, mass=True)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dt,g", KINDS)
+@pytest.mark.parametrize("dh,page", [(64, 16), (128, 16), (80, 8)])
+@pytest.mark.parametrize("far", [-45, 45])
+def test_groups_of_queries_and_keys_far_apart(bits, dt, g, dh, page, far):
+    """A group of the query's dims 2^far times the others, and its keys 2^-far times: ordinary scores."""
+    cache, q, _ = make([300, 40], 2, g, dh, page, bits, dt, 61)
+    q = q.float()
+    q[..., :32] *= 2.0 ** far
+    cache[2][..., 0, 0] *= 2.0 ** -far
+    check(q.to(dt), cache, bits, dh ** -0.5, mass=True)
+
+
+def test_scale_of_zero_and_queries_of_every_size():
+    cache, q, _ = make([200, 30], 2, 3, 64, 16, 4, F32, 91)
+    for dt in (BF, F32):
+        for size, scale in ((1.0, 0.0), (2.0 ** 120, 2.0 ** -122), (2.0 ** -120, 2.0 ** 118), (1.0, -0.3), (2.0 ** -60, 0.125)):
+            check((q * size).to(dt), cache, 4, scale, mass=True)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dt,g", KINDS)
+@pytest.mark.parametrize("lengths,dh,page", SHAPES)
+@pytest.mark.parametrize("what", [-INF, INF, NAN])
+def test_queries_that_are_not_finite_are_nan_alone(bits, dt, g, lengths, dh, page, what):
+    T = ops()
+    cache, q, _ = make(lengths, 2, g, dh, page, bits, dt, 71)
+    dev = [x.cuda() for x in cache]
+    clean = T.turbo_paged_quant_attention(q.cuda(), *dev)
+    for head, d in ((0, 0), (2 * g - 1, dh - 1), (g, dh // 2)):
+        x = q.clone()
+        x[0, head, 0, d] = what
+        out = T.turbo_paged_quant_attention(x.cuda(), *dev)
+        assert bool(out[0, head].isnan().all())
+        out[0, head] = clean[0, head]
+        assert torch.equal(out, clean)
