@@ -60,22 +60,23 @@ struct PagedAttn {
   int run, vec16;         // groups of 16 slots may be copied as they lie; rows are whole 16-byte pieces
 };
 
-template <int TILE>
+// SITE: what a bad length or page is recorded as, here and below
+template <int TILE, int SITE>
 ONE_DEVINL int pa_tiles(const PagedCache& c, int b) {
-  return (paged_length(c, b, SITE_PAGED_ATTN) + TILE - 1) / TILE;
+  return (paged_length(c, b, SITE) + TILE - 1) / TILE;
 }
 
 // Units of the list (the host keeps them, rounded up to shares, below 2^31): a segment's tiles, and MORE for
 // a segment's begin and end. Every warp computes them for itself.
-template <int TILE, int MORE>
+template <int TILE, int MORE, int SITE>
 ONE_DEVINL int pa_units(const PagedCache& c, int b) {
-  const int n = pa_tiles<TILE>(c, b);
+  const int n = pa_tiles<TILE, SITE>(c, b);
   return MORE && n ? n + MORE : n;
 }
-template <int TILE, int MORE>
+template <int TILE, int MORE, int SITE>
 ONE_DEVINL int pa_total(const PagedAttn& p) {
   int n = 0;
-  for (int b = threadIdx.x & 31; b < p.c.B; b += 32) n += pa_units<TILE, MORE>(p.c, b);
+  for (int b = threadIdx.x & 31; b < p.c.B; b += 32) n += pa_units<TILE, MORE, SITE>(p.c, b);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
   return n * p.c.Hkv * p.hv_per_kv;
@@ -83,18 +84,18 @@ ONE_DEVINL int pa_total(const PagedAttn& p) {
 
 // A place in the list: tile `tile` of query-head tile gi of kv head kv of sequence b; the heads' tiles
 // of a sequence follow one another, ng query-head tiles per kv head.
-template <int TILE, int MORE = 0>
+template <int TILE, int MORE, int SITE>
 struct PaCursor {
   int b, kv, gi, tile, tiles, len;
   ONE_DEVINL void load(const PagedCache& c) {
-    len = b < c.B ? paged_length(c, b, SITE_PAGED_ATTN) : 0;
+    len = b < c.B ? paged_length(c, b, SITE) : 0;
     tiles = (len + TILE - 1) / TILE;
   }
   // To unit w; returns how many of the segment's first MORE units are left.
   ONE_DEVINL int seek(const PagedCache& c, int ng, int w) {
     const int HV = c.Hkv * ng, lane = threadIdx.x & 31;
     for (int base = 0; base < c.B; base += 32) {
-      const int n = base + lane < c.B ? pa_units<TILE, MORE>(c, base + lane) : 0;
+      const int n = base + lane < c.B ? pa_units<TILE, MORE, SITE>(c, base + lane) : 0;
       int incl = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -227,6 +228,7 @@ struct PaBf16 {
   using T = __nv_bfloat16;
   using Cell = T;                                      // of the cache
   static constexpr bool kQuant = false;
+  static constexpr int kSite = SITE_PAGED_ATTN;
   static constexpr int DH = DH_, ROWS = WIDE ? 16 : 8;
   static constexpr int KC = DH / 32;                   // 16-byte chunks of a key row per lane
   static constexpr int VC = DH / 64, VH = DH % 64 / 32;  // 16-byte and 8-byte pieces of a value row per lane
@@ -452,6 +454,7 @@ struct PaF32 {
   using T = float;
   using Cell = T;
   static constexpr bool kQuant = false;
+  static constexpr int kSite = SITE_PAGED_ATTN;
   static constexpr int DH = DH_, ROWS = ROWS_;
   static constexpr int KC = DH / 16, VC = DH / 32, CH = DH / 4;
   static constexpr int kGroups = 1, TILE = 16 * kPaWarps;
@@ -671,10 +674,10 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, MODE>::kPerSm) paged_
   pdl_wait();
   pdl_launch_dependents();
   constexpr int MORE = SPLIT ? E::kSegmentUnits : 0;
-  PaCursor<TILE, MORE> cur;
+  PaCursor<TILE, MORE, E::kSite> cur;
   int left, share = 0;  // units to do; a full share
   if (SPLIT) {
-    const int total = pa_total<TILE, MORE>(p);
+    const int total = pa_total<TILE, MORE, E::kSite>(p);
     share = max(1, (total + p.ranges - 1) / p.ranges);
     const long long w0 = (long long)share * team;
     if (w0 >= total) return;
@@ -695,7 +698,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, MODE>::kPerSm) paged_
   //      groups are a quarter as long: lane i has those of the i-th group from tile `look` of the segment on,
   //      so that one look serves 32 groups.
   constexpr bool LOOK = RUN && E::kQuant;
-  PaCursor<TILE, MORE> src = cur;
+  PaCursor<TILE, MORE, E::kSite> src = cur;
   int to_copy = left, pg[GR], row[GR];  // page and first element (kQuant: row) in its head of each group
   uint32_t live[S::kStages][GR];        // slots in use of the tiles in the ring, the oldest first (not LOOK)
   uint32_t dead = 0;                    // LOOK: a bit per group without a page of the tiles in the ring, the newest last
@@ -757,7 +760,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, MODE>::kPerSm) paged_
         if (looked == 1) {  // the page numbers have come
           looked = 2;
           const bool good = (uint32_t)pg[0] < (uint32_t)c.num_pages, missing = !good && row[0] >= 0;
-          if (missing) set_err(c.err, ERR_BAD_ARG, SITE_QUANT_ATTN);
+          if (missing) set_err(c.err, ERR_BAD_ARG, E::kSite);
           const int64_t n = good ? pg[0] : 0, r = good ? row[0] : 0;
           k_at = (uint32_t)((n * ks + r * p.row) >> 4);
           v_at = (uint32_t)((n * vs + r * p.row) >> 4);
@@ -815,7 +818,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaSmem<E, MODE>::kPerSm) paged_
           uint8_t* to = ring + put + g * E::kGroup;
           uint32_t& alive = live[S::kStages - 1][g];
           const bool good = (uint32_t)pg[g] < (uint32_t)c.num_pages;
-          if (!good && ahead > 16 * g) set_err(c.err, ERR_BAD_ARG, SITE_PAGED_ATTN);
+          if (!good && ahead > 16 * g) set_err(c.err, ERR_BAD_ARG, E::kSite);
           if constexpr (E::kQuant) {
             alive = __ballot_sync(0xffffffffu, good) & 0xffffu;
             E::copy_any(smem_u32(to), p, keys, values, scales, good ? pg[g] : -1, row[g]);
@@ -1086,7 +1089,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
     const int b = blockIdx.x / hq, j = blockIdx.x % hq, kv = j / p.G, g = j % p.G, row = g % ROWS;
     const int2 seg = p.parts[(b * c.Hkv + kv) * ng + g / ROWS];
     T* out = (T*)p.out + (int64_t)blockIdx.x * c.Dh;
-    if (paged_length(c, b, SITE_PAGED_ATTN) == 0) {  // no CTA holds it
+    if (paged_length(c, b, E::kSite) == 0) {  // no CTA holds it
       for (int d = tid; d < c.Dh; d += kJoinThreads) st<T>(out + d, 0.f);
       return;
     }
@@ -1131,7 +1134,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
   }
   // ---- mass: four slots per thread; rows of scores are padded, so that they may be read past the length
   const int at = blockIdx.x - c.B * hq, bh = at / mass_blocks, t = at % mass_blocks * kJoinSlots + tid * 4, b = bh / c.Hkv;
-  const int len = paged_length(c, b, SITE_PAGED_ATTN);
+  const int len = paged_length(c, b, E::kSite);
   if (at % mass_blocks * kJoinSlots >= len) return;
   const int64_t row0 = (int64_t)bh * p.G;
   float add[4] = {0.f, 0.f, 0.f, 0.f};

@@ -189,7 +189,7 @@ int evict(PagedEvictParams& p, const S* cache, int pieces, const int32_t* dst_ta
     constexpr int KPT = decltype(keys)::value;
     return one_launch ? launch(paged_evict_kernel<KPT, true, U>, dim3((unsigned)(heads * parts)), dim3(kEvictThreads), 0, st, p,
                                (int)parts, pieces)
-                      : launch(paged_evict_kernel<KPT, false>, dim3((unsigned)heads), dim3(kEvictThreads), 0, st, p, 1, pieces);
+                      : launch(paged_evict_kernel<KPT, false, U>, dim3((unsigned)heads), dim3(kEvictThreads), 0, st, p, 1, pieces);
   };
   const int rc = launched(slots <= 1024    ? select(Int<2>())
                           : slots <= 2048  ? select(Int<4>())

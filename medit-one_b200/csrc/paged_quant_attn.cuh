@@ -114,6 +114,7 @@ struct PaQuant {
   using T = std::conditional_t<PAIR, float, __nv_bfloat16>;
   using Cell = uint8_t;
   static constexpr bool kQuant = true;
+  static constexpr int kSite = SITE_QUANT_ATTN;
   static constexpr int DH = DH_, BITS = BITS_, ROWS = KIND == PQ_16 ? 16 : KIND == PQ_4 || KIND == PQ_PAIR4 ? 4 : 8;
   static constexpr int NL = KIND == PQ_16 || KIND == PQ_PAIR8 ? 2 : 1;  // tiles of 8 columns
   static constexpr bool ODD = KIND == PQ_8 || KIND == PQ_16;  // odd columns are queries of their own
