@@ -14,7 +14,8 @@
 //    2^10 above them; products of a bf16 q and a code have 16 bits at most and lose little by that (weights of
 //    scores whose terms sum to 2000 are off by 1e-5 either way). In fp32 the bits of 1024 are put above
 //    the code and taken off with its offset, exactly; so they are for 9 to 16 queries, whose first sums would
-//    take registers that spill (8 x 32768 slots, 8 heads x 128 of 16 queries: 96 us, so 93; of 8: 59, so 67).
+//    take registers that spill (8 x 32768 slots, 8 heads x 128 of 16 queries: 96 us, so 93; of 8: 59, so 67;
+//    86 and 55 now).
 //  - q scaled by a power of two per row and group, its largest to [2^14, 2^15): a bf16 q is exact in it down to
 //    2^-27 of its group's largest; in fp32, q is two fp16 parts (22 bits), in neighbouring columns.
 //  - values, in bf16: the bits of 128 or 16 above the code and one packed addition of -(128 + z) or -(16 + z),
@@ -22,13 +23,13 @@
 //  - weights times their scales, in bf16 parts, which together have 16 bits (fp32: all 24): a part has its own
 //    exponent, so that each output is as good as its own terms, whatever the scales of other slots and
 //    groups are. (fp16 with an exponent in common, of the largest scale so far, lost values 2^-28 of it,
-//    and took 36 us where this takes 41.)
+//    and took 36 us where this takes 39.)
 //  - the codes are the instructions' 16 rows: S^T = K Q^T has slots as rows, O^T = V^T P^T dims, and the
 //    queries are the 8 columns. ldmatrix brings 16-byte pieces of eight slots to the lanes as both need
 //    them: keys straight, values transposed, where a 16-bit element is four (two) codes of one slot.
 //    movmatrix turns the weights from rows to columns in between.
-// Measured: 64 ragged sequences up to 4096 slots, 12 heads x 64, 4 bits: 41 us, 43 % of the measured copy rate (dense
-// bf16: 73); 8 up to 32768, 8 heads x 128 of 4 queries: 49 us, 51 %; one of 1048576, 12 x 64: 217 us, 64 %.
+// Measured: 64 ragged sequences up to 4096 slots, 12 heads x 64, 4 bits: 39 us, 46 % of the measured copy rate (dense
+// bf16: 73); 8 up to 32768, 8 heads x 128 of 4 queries: 44 us, 56 %; one of 1048576, 12 x 64: 201 us, 69 %.
 #pragma once
 
 #include "paged_attn.cuh"
@@ -89,6 +90,13 @@ ONE_DEVINL uint32_t f16x2_add(uint32_t a, uint32_t b) {
   asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
+// (a & mask) | bits in one instruction (two, where the compiler was left to it: 64 x 4096 ragged 41.5 us, 38.9 so; fp32
+// 50.3, 44.4)
+ONE_DEVINL uint32_t and_or(uint32_t a, uint32_t mask, uint32_t bits) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(d) : "r"(a), "r"(mask), "r"(bits));
+  return d;
+}
 // The first `bytes` of 16, 8 or 4 bytes, the rest as zeros
 template <int N>
 ONE_DEVINL void cp_async_some(uint32_t s, const void* g, int bytes) {
@@ -103,9 +111,9 @@ ONE_DEVINL void cp_async_some(uint32_t s, const void* g, int bytes) {
 // head rather than of two (PQ_4: q has one part, its weights two).
 enum PqKind { PQ_4, PQ_8, PQ_16, PQ_PAIR4, PQ_PAIR8 };
 
-// Tiles of a list that a segment's begin and end count as. Us at 0, 1, 2, 4 of them with 128 slots to a tile: 64 x
-// 4096 ragged x 12 x 64 61.8, 49.9, 47.4, 50.1; as it is now, with 64 slots, at 2, 3, 5, 8: 36.6, 36.4, 38.0, 39.3,
-// 64 x 1024 17.8, 18.4, 19.1, 20.9.
+// Tiles of a list that a segment's begin and end count as. Us at 0, 2, 3, 5 of them: 64 x 4096 ragged x 12 x 64 55.0,
+// 41.6, 41.5, 43.5; in 8 bits 69, 50.0, 51.6, 53.5; 64 x 1024 21.8, 19.1, 20.2, 20.9 (before codes opened with one
+// instruction less each, as below).
 constexpr int kQuantUnits = 2;
 
 template <int DH_, int BITS_, PqKind KIND>
@@ -130,8 +138,8 @@ struct PaQuant {
   static constexpr int kGroup = 16 * (2 * RB + SR);      // bytes of 16 slots
   static constexpr int kValues = 16 * RB, kScales = 32 * RB;
   // 16-slot groups per warp and step, CTAs on an SM at most: long steps for independent work between the
-  // instructions of a warp, as far as registers go. Us at 1, 2, 4 groups: 64 x 4096 ragged x 12 x 64, 4 bits 53, 42,
-  // 38; 8 x 32768 x 8 x 4 x 128 52, 46, 42; in 8 bits 58, 56, 62; of 16 queries 127, 70, 87.
+  // instructions of a warp, as far as registers go. Us at 1, 2, 4 groups: 64 x 4096 ragged x 12 x 64, 4 bits 56, 45,
+  // 42; in 8 bits 63, 53, 50; 8 x 32768 x 8 x 4 x 128 65, 51, 49; of 16 queries 105, 93, 174.
   static constexpr int kGroups = RB <= 64 && (NL == 1 || DH <= 64) ? 4 : 2;
   static constexpr int TILE = 16 * kGroups * kPaWarps;
   static constexpr int kStages = 2, kStagesFew = kStages;
@@ -343,24 +351,22 @@ struct PaQuant {
     }
     if constexpr (CH % 2) ldmatrix_x2<TRANS>(w[CH - 1][0], w[CH - 1][1], base + step(mine, CH - 1));
   }
-  // Two stored codes of a word: those at half (4 bits) or byte (8 bits) e of each of its 16-bit elements. As fp16
-  // they are u 2^-24, or u 2^-20 (4 bits, e odd)
-  ONE_DEVINL static uint32_t open(uint32_t w, int e) {
-    if (BITS == 4) return (e & 2 ? w >> 8 : w) & (e & 1 ? 0x00f000f0u : 0x000f000fu);
-    return (e ? w >> 8 : w) & 0x00ff00ffu;
-  }
+  // Two codes of a word, those at half (4 bits) or byte (8 bits) e of each of its 16-bit elements, in fp16: as stored,
+  // u 2^-24 or u 2^-20 (4 bits, e odd); OPEN: without their offset, as they are or 16 times as much
   ONE_DEVINL static uint32_t open_key(uint32_t w, int e) {
-    if (!OPEN) return open(w, e);
-    return f16x2_add(open(w, e) | 0x64006400u, BITS == 8 || (e & 1) ? 0xe480e480u : 0xe408e408u);  // -(1024 + z), 16 z
+    const bool high = BITS == 4 && (e & 1);
+    const uint32_t x = e & (BITS == 4 ? 2 : 1) ? w >> 8 : w, mask = BITS == 8 ? 0x00ff00ffu : high ? 0x00f000f0u : 0x000f000fu;
+    if (!OPEN) return x & mask;
+    return f16x2_add(and_or(x, mask, 0x64006400u), BITS == 8 || high ? 0xe480e480u : 0xe408e408u);  // -(1024 + z), 16 z
   }
   // The same two codes, without their offset, in bf16
   ONE_DEVINL static uint32_t open_value(uint32_t w, int e) {
     if (BITS == 4) {
-      if (e & 1) return bf2_add(((e & 2 ? w >> 9 : w >> 1) & 0x00780078u) | 0x41804180u, 0xc1c0c1c0u);  // 16 + u - 24
-      return bf2_add(((e & 2 ? w >> 8 : w) & 0x000f000fu) | 0x43004300u, 0xc308c308u);                  // 128 + u - 136
+      if (e & 1) return bf2_add(and_or(e & 2 ? w >> 9 : w >> 1, 0x00780078u, 0x41804180u), 0xc1c0c1c0u);  // 16 + u - 24
+      return bf2_add(and_or(e & 2 ? w >> 8 : w, 0x000f000fu, 0x43004300u), 0xc308c308u);             // 128 + u - 136
     }
     const uint32_t x = e ? w >> 8 : w;  // of the 8 bits 7 fit: 128 + u % 128 - (u < 128 ? 256 : 128)
-    return bf2_add((x & 0x007f007fu) | 0x43004300u, (x & 0x00800080u) ^ 0xc380c380u);
+    return bf2_add(and_or(x, 0x007f007fu, 0x43004300u), (x & 0x00800080u) ^ 0xc380c380u);
   }
   // Weights as bf16 parts whose sum is the weight to 16 bits (PAIR: all 24), as B operands before their turn:
   // the two columns of y0 and y1, or of the parts of y0
