@@ -314,7 +314,7 @@ int one_paged_evict(const one_paged_cache* cache, const int32_t* dst_table, int6
 /* The same operators over a paged cache held in 4 or 8 bits. A row of dh values is cut into groups of
  * 32 (the last may be shorter), each standing for scale * code: scale = bf16(max |x| / m), m = 7 (4
  * bits) or 127 (8 bits), code = x / scale to the nearest whole number, halves to the even one, x the
- * value in fp32 (a rotated key: rounded to it once). Scales below 2^-100 are held as 0, with codes of
+ * value in fp32 (a rotated key: that of 64 bits, rounded). Scales below 2^-100 are held as 0, with codes of
  * 0; a group with an infinity or NaN has the scale NaN, and codes of 0: it reads as NaN.
  *
  * k_pages, v_pages hold num_pages pages uint8 [hkv][page_size][dh * bits / 8]: a byte is code + 128 (8

@@ -54,7 +54,8 @@ ONE_DEVINL float max_abs(float a, float b, float c) {
   return d;
 }
 
-// x cos + y sin in fp32 with one rounding: products of bf16 values are exact in fp32, those of fp32 in fp64.
+// x cos + y sin, rounded to fp32: products of bf16 values are exact in fp32, so that there is one rounding; those of
+// fp32 in fp64, whose sum is rounded to fp64 first.
 ONE_DEVINL float quant_rotate(__nv_bfloat16, __nv_bfloat16, float x, float y, float cs, float sn) { return fmaf(x, cs, y * sn); }
 template <typename T, typename C>
 ONE_DEVINL float quant_rotate(T, C, float x, float y, float cs, float sn) {
