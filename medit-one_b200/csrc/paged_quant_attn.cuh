@@ -7,17 +7,14 @@
 // The scales of a group of 32 dims factor out of its products, so the matrix instructions take the codes
 // themselves. HBM bounds the long cases in principle (72 bytes per slot and kv head of 64 dims at 4 bits);
 // per byte read there are four times the products of a bf16 cache, so what counts is instructions per code:
-//  - keys, in fp16: a code lies in the low bits of an fp16 whose exponent is 0, and that fp16 is u 2^-24,
-//    exactly: one AND opens two codes, and no conversion follows. Halves of bytes at bits 4-7 read as u 2^-20;
-//    q takes up the difference. sum q u starts from -z sum q (per query and group, computed once), so u needs
-//    no subtraction. An instruction aligns its terms by their exponents, which for such small numbers is up to
-//    2^10 above them; products of a bf16 q and a code have 16 bits at most and lose little by that (weights of
-//    scores whose terms sum to 2000 are off by 1e-5 either way). In fp32 the bits of 1024 are put above
-//    the code and taken off with its offset, exactly; so they are for 9 to 16 queries, whose first sums would
-//    take registers that spill (8 x 32768 slots, 8 heads x 128 of 16 queries: 96 us, so 93; of 8: 59, so 67;
-//    86 and 55 now).
+//  - keys, in fp16: the bits of 1024 above the code (16 times it, of halves of bytes at bits 4-7) and one packed
+//    addition or fma, which takes 1024 and z off (and 16 out), exactly. (A code as it lies is an fp16 u 2^-24 whose
+//    exponent is 0: one AND opens two, and the offset goes off their sum. But an instruction aligns its terms by
+//    their operands' exponents, up to 2^10 above such numbers, and where large dims of q meet codes of 0 their
+//    offsets cancel: the scores of dims 2^8 below those were off by ten times an fp32 sum's bound, of dims 2^16
+//    below by thousands of times, at 38.8 us instead of 39.0 and 44.3 instead of 45.8 in the cases below.)
 //  - q scaled by a power of two per row and group, its largest to [2^14, 2^15): a bf16 q is exact in it down to
-//    2^-27 of its group's largest; in fp32, q is two fp16 parts (22 bits), in neighbouring columns.
+//    2^-31 of its group's largest; in fp32, q is two fp16 parts (22 bits), in neighbouring columns.
 //  - values, in bf16: the bits of 128 or 16 above the code and one packed addition of -(128 + z) or -(16 + z),
 //    both exact (a sum over many slots of p z would drown o).
 //  - weights times their scales, in bf16 parts, which together have 16 bits (fp32: all 24): a part has its own
@@ -29,7 +26,7 @@
 //    them: keys straight, values transposed, where a 16-bit element is four (two) codes of one slot.
 //    movmatrix turns the weights from rows to columns in between.
 // Measured: 64 ragged sequences up to 4096 slots, 12 heads x 64, 4 bits: 39 us, 46 % of the measured copy rate (dense
-// bf16: 73); 8 up to 32768, 8 heads x 128 of 4 queries: 44 us, 56 %; one of 1048576, 12 x 64: 201 us, 69 %.
+// bf16: 73); 8 up to 32768, 8 heads x 128 of 4 queries: 46 us, 54 %; one of 1048576, 12 x 64: 202 us, 69 %.
 #pragma once
 
 #include "paged_attn.cuh"
@@ -42,11 +39,10 @@ ONE_DEVINL void mma_bf16_acc(float (&d)[4], const uint32_t (&a)[4], const uint32
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
-ONE_DEVINL void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1,
-                              const float (&c)[4]) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
-      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+ONE_DEVINL void mma_f16_acc(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
 // Lane (r, c) holds elements 2 c, 2 c + 1 of row r of an 8 x 8 matrix; the same of the transposed one
 ONE_DEVINL uint32_t movmatrix_trans(uint32_t a) {
@@ -90,6 +86,11 @@ ONE_DEVINL uint32_t f16x2_add(uint32_t a, uint32_t b) {
   asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
+ONE_DEVINL uint32_t f16x2_fma(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
 // (a & mask) | bits in one instruction (two, where the compiler was left to it: 64 x 4096 ragged 41.5 us, 38.9 so; fp32
 // 50.3, 44.4)
 ONE_DEVINL uint32_t and_or(uint32_t a, uint32_t mask, uint32_t bits) {
@@ -127,14 +128,12 @@ struct PaQuant {
   static constexpr int NL = KIND == PQ_16 || KIND == PQ_PAIR8 ? 2 : 1;  // tiles of 8 columns
   static constexpr bool ODD = KIND == PQ_8 || KIND == PQ_16;  // odd columns are queries of their own
   static constexpr int NP = KIND == PQ_4 ? 1 : 2;        // instructions that a weight's parts take: 2, or 3 of fp32
-  static constexpr bool OPEN = PAIR || KIND == PQ_16;    // keys without their offset
   static constexpr int QL = ODD ? 2 : 1, NQ = NL * QL;   // queries of a lane, per tile and in all
   static constexpr int G = DH / kQuantGroup;             // groups of a row
   static constexpr int RB = DH * BITS / 8, CH = RB / 16; // bytes and pieces of a row
   static constexpr int SR = 4 * G;                       // bytes of a slot's scales
   static constexpr int PG = CH / G;                      // pieces of a group: 1 or 2
   static constexpr int NT = DH / 16;                     // value tiles
-  static constexpr float kZero = BITS == 4 ? 8.f : 128.f;
   static constexpr int kGroup = 16 * (2 * RB + SR);      // bytes of 16 slots
   static constexpr int kValues = 16 * RB, kScales = 32 * RB;
   // 16-slot groups per warp and step, CTAs on an SM at most: long steps for independent work between the
@@ -149,7 +148,6 @@ struct PaQuant {
   ONE_DEVINL static float weight(float x) { return PAIR ? exp2f(x) : ex2_approx(x); }
 
   uint32_t qb[NL][G][2][2];  // B operands of a group's two products
-  float off[NL][G][4];       // -z sum q as their first sums (OPEN: 0)
   float fac[NQ][G];          // from a group's sums to scores, positive
   float o[NL][NT][4];
   float m[NQ], l[NQ];
@@ -281,7 +279,7 @@ struct PaQuant {
             }
           }
         }
-        float top = 0.f, sum = 0.f;
+        float top = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[g][i]));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -289,8 +287,7 @@ struct PaQuant {
         const int e = (int)(__float_as_uint(top) >> 23);                      // 0 .. 255
         // 2^14 over the power of two of top, with the scale's sign
         const float up = copysignf(__uint_as_float((uint32_t)min(254, 268 - e) << 23), p.scale_log2);
-        // the sums are of q up u 2^-24 (OPEN: q up c); halves that read as 16 times as much have q up 2^-4
-        const float back = fabsf(p.scale_log2) * __uint_as_float((uint32_t)max(14, e) << 23) * (OPEN ? 0x1p-14f : 0x1p10f);
+        const float back = fabsf(p.scale_log2) * __uint_as_float((uint32_t)max(14, e) << 23) * 0x1p-14f;
         // lane (r, c) has columns 2 c and 2 c + 1 of the sums
 #pragma unroll
         for (int h = 0; h < QL; ++h) fac[n * QL + h][g] = __shfl_sync(0xffffffffu, back, (2 * c + h) * 4);
@@ -298,19 +295,12 @@ struct PaQuant {
         for (int k = 0; k < 2; ++k)
 #pragma unroll
           for (int a = 0; a < 2; ++a) {
-            const float f = BITS == 4 && k ? up * 0.0625f : up;
             const int i0 = BITS == 4 ? k + 2 * a : 4 * k + a, i1 = BITS == 4 ? i0 + 4 : i0 + 2;
-            const float y0 = x[g][i0] * f, y1 = x[g][i1] * f;
+            const float y0 = x[g][i0] * up, y1 = x[g][i1] * up;
             uint32_t w = pack_f16x2(y0, y1);
             if (!ODD && (r & 1)) w = PAIR ? pack_f16x2(y0 - f16_lo(w), y1 - f16_hi(w)) : 0;
             qb[n][g][k][a] = w;
-            sum += (f16_lo(w) + f16_hi(w)) * (BITS == 4 && k ? 16.f : 1.f);
           }
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        sum *= -kZero * 0x1p-24f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) off[n][g][i] = OPEN ? 0.f : __shfl_sync(0xffffffffu, sum, (2 * c + (i & 1)) * 4);
       }
     }
 #pragma unroll
@@ -351,15 +341,14 @@ struct PaQuant {
     }
     if constexpr (CH % 2) ldmatrix_x2<TRANS>(w[CH - 1][0], w[CH - 1][1], base + step(mine, CH - 1));
   }
-  // Two codes of a word, those at half (4 bits) or byte (8 bits) e of each of its 16-bit elements, in fp16: as stored,
-  // u 2^-24 or u 2^-20 (4 bits, e odd); OPEN: without their offset, as they are or 16 times as much
+  // Two codes of a word, those at half (4 bits) or byte (8 bits) e of each of its 16-bit elements, in fp16
   ONE_DEVINL static uint32_t open_key(uint32_t w, int e) {
-    const bool high = BITS == 4 && (e & 1);
-    const uint32_t x = e & (BITS == 4 ? 2 : 1) ? w >> 8 : w, mask = BITS == 8 ? 0x00ff00ffu : high ? 0x00f000f0u : 0x000f000fu;
-    if (!OPEN) return x & mask;
-    return f16x2_add(and_or(x, mask, 0x64006400u), BITS == 8 || high ? 0xe480e480u : 0xe408e408u);  // -(1024 + z), 16 z
+    if (BITS == 8) return f16x2_add(and_or(e ? w >> 8 : w, 0x00ff00ffu, 0x64006400u), 0xe480e480u);        // 1024 + u - 1152
+    const uint32_t x = e & 2 ? w >> 8 : w;
+    if (e & 1) return f16x2_fma(and_or(x, 0x00f000f0u, 0x64006400u), 0x2c002c00u, 0xd480d480u);  // (1024 + 16 u) / 16 - 72
+    return f16x2_add(and_or(x, 0x000f000fu, 0x64006400u), 0xe408e408u);                          // 1024 + u - 1032
   }
-  // The same two codes, without their offset, in bf16
+  // The same in bf16
   ONE_DEVINL static uint32_t open_value(uint32_t w, int e) {
     if (BITS == 4) {
       if (e & 1) return bf2_add(and_or(e & 2 ? w >> 9 : w >> 1, 0x00780078u, 0x41804180u), 0xc1c0c1c0u);  // 16 + u - 24
@@ -408,9 +397,9 @@ struct PaQuant {
         const float ks[2] = {sc[i][0].get(g), sc[i][1].get(g)};
 #pragma unroll
         for (int n = 0; n < NL; ++n) {
-          float a[4];
-          mma_f16_16816(a, x[0][0], x[0][1], x[0][2], x[0][3], qb[n][g][0][0], qb[n][g][0][1], off[n][g]);
-          mma_f16_16816(a, x[1][0], x[1][1], x[1][2], x[1][3], qb[n][g][1][0], qb[n][g][1][1], a);
+          float a[4] = {0.f, 0.f, 0.f, 0.f};
+          mma_f16_acc(a, x[0], qb[n][g][0]);
+          mma_f16_acc(a, x[1], qb[n][g][1]);
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll

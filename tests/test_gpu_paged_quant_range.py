@@ -196,3 +196,20 @@ def test_queries_that_are_not_finite_are_nan_alone(bits, dt, g, lengths, dh, pag
         assert bool(out[0, head].isnan().all())
         out[0, head] = clean[0, head]
         assert torch.equal(out, clean)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dt,g", KINDS)
+@pytest.mark.parametrize("lengths,dh,page", SHAPES)
+@pytest.mark.parametrize("far", [8, 16])
+def test_large_dims_of_queries_that_keys_leave_alone(bits, dt, g, lengths, dh, page, far):
+    """Two dims of the query 2^far times the others, where all keys have the code 0: they add nothing."""
+    cache, q, _ = make(lengths, 2, g, dh, page, bits, dt, 101)
+    q = q.float()
+    for d in (0, dh - 1):
+        q[..., d] *= 2.0 ** far
+        if bits == 8:
+            cache[0][..., d] = zero_code(bits)
+        else:
+            cache[0][..., d // 2] = cache[0][..., d // 2] & (0x0f if d % 2 else 0xf0) | (0x80 if d % 2 else 0x08)
+    check(q.to(dt), cache, bits, 3 * dh ** -0.5, mass=True)
