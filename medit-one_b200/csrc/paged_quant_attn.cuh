@@ -298,7 +298,10 @@ struct PaQuant {
             const int i0 = BITS == 4 ? k + 2 * a : 4 * k + a, i1 = BITS == 4 ? i0 + 4 : i0 + 2;
             const float y0 = x[g][i0] * up, y1 = x[g][i1] * up;
             uint32_t w = pack_f16x2(y0, y1);
-            if (!ODD && (r & 1)) w = PAIR ? pack_f16x2(y0 - f16_lo(w), y1 - f16_hi(w)) : 0;
+            if (!ODD && (r & 1)) {  // what the first part leaves: nothing of an infinity
+              const float h0 = f16_lo(w), h1 = f16_hi(w);
+              w = PAIR ? pack_f16x2(y0 == h0 ? 0.f : y0 - h0, y1 == h1 ? 0.f : y1 - h1) : 0;
+            }
             qb[n][g][k][a] = w;
           }
       }

@@ -519,7 +519,7 @@ def turbo_paged_quant_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages:
                                 block_table: torch.Tensor, lengths: torch.Tensor, scale_factor: Optional[float] = None,
                                 mass: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """turbo_paged_attention over the values that a cache in 4 or 8 bits stands for; q and the result
-    in bf16 or fp32. A query with an infinity gives NaN."""
+    in bf16 or fp32."""
     return _attend(*_paged_quant(k_pages, v_pages, scales, block_table, lengths, mass, q.shape[-1]), q, scale_factor, mass, out,
                    quant=_code(q.dtype))
 

@@ -213,3 +213,33 @@ def test_large_dims_of_queries_that_keys_leave_alone(bits, dt, g, lengths, dh, p
         else:
             cache[0][..., d // 2] = cache[0][..., d // 2] & (0x0f if d % 2 else 0xf0) | (0x80 if d % 2 else 0x08)
     check(q.to(dt), cache, bits, 3 * dh ** -0.5, mass=True)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dt,g", KINDS)
+@pytest.mark.parametrize("lengths,dh,page", SHAPES)
+def test_rows_whose_scores_are_all_minus_infinity(bits, dt, g, lengths, dh, page):
+    """A query of -inf in a dim where every key is positive: nothing is attended to, as by the dense operator:
+    zeros and no masses, and the other queries as ever."""
+    T = ops()
+    cache, q, _ = make(lengths, 2, g, dh, page, bits, dt, 71)
+    if bits == 4:  # codes of 3 in dims 0, 2, ..
+        cache[0] = cache[0] & 0xf0 | 0x0b
+    else:  # codes of 1 and more
+        cache[0] |= 0x81
+    dev = [x.cuda() for x in cache]
+    clean = T.turbo_paged_quant_attention(q.cuda(), *dev)
+    kd, vd = T.turbo_paged_quant_read(*dev, max(lengths), dh, dtype=dt)  # a dense cache of one page per sequence
+    table = torch.arange(len(lengths), dtype=torch.int32, device="cuda")[:, None]
+    for none in ([0], [2 * g - 1], list(range(2 * g))):
+        x = q.clone()
+        x[0, none, 0, 0] = -INF
+        m = torch.zeros(len(lengths), 2, cache[3].shape[1] * page, device="cuda")
+        out = T.turbo_paged_quant_attention(x.cuda(), *dev, mass=m)
+        assert bool((out[0, none] == 0).all())
+        assert bool((T.turbo_paged_attention(x.cuda(), kd, vd, table, dev[4])[0, none] == 0).all())
+        left = [h for h in range(2 * g) if h not in none]
+        assert torch.equal(out[0, left], clean[0, left]) and torch.equal(out[1:], clean[1:])
+        # a live query's weights sum to 1, each of n within a few roundings of it
+        total = torch.tensor([sum(h // g == kv and h not in none for h in range(2 * g)) for kv in range(2)], dtype=torch.float32)
+        assert torch.allclose(m[0].sum(-1).cpu(), total, rtol=0, atol=g * max(lengths) * 2.0 ** -22)
