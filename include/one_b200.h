@@ -347,7 +347,7 @@ int one_paged_quant_read(const one_paged_quant_cache* cache, const int32_t* star
                          void* stream);
 
 /* Attention of one new token per sequence, q and out in dtype: as one_paged_attention over the values that
- * the cache stands for. */
+ * the cache stands for. Dims of a query are held down to 2^-31 of the largest one in their group of 32. */
 size_t one_paged_quant_attention_workspace_bytes(int32_t b, int32_t hq, int32_t hkv, int32_t dh, int32_t page_size,
                                                  int32_t max_pages, int32_t dtype, int32_t with_mass);
 int one_paged_quant_attention(const one_paged_quant_cache* cache, const void* q, int64_t q_batch_stride,

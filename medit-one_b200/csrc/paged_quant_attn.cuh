@@ -14,7 +14,9 @@
 //    offsets cancel: the scores of dims 2^8 below those were off by ten times an fp32 sum's bound, of dims 2^16
 //    below by thousands of times, at 38.8 us instead of 39.0 and 44.3 instead of 45.8 in the cases below.)
 //  - q scaled by a power of two per row and group, its largest to [2^14, 2^15): a bf16 q is exact in it down to
-//    2^-31 of its group's largest; in fp32, q is two fp16 parts (22 bits), in neighbouring columns.
+//    2^-31 of its group's largest; in fp32, q is two fp16 parts (22 bits), in neighbouring columns, the second with
+//    2^11 more: 18 bits are left at 2^-30. (Keys in bf16, as the values are, would take any q as it is: 40.4 us
+//    instead of 39.1 at 64 x 4096 ragged, in 8 bits, which bf16 opens in two steps, 54 instead of 48.)
 //  - values, in bf16: the bits of 128 or 16 above the code and one packed addition of -(128 + z) or -(16 + z),
 //    both exact (a sum over many slots of p z would drown o).
 //  - weights times their scales, in bf16 parts, which together have 16 bits (fp32: all 24): a part has its own
@@ -298,9 +300,9 @@ struct PaQuant {
             const int i0 = BITS == 4 ? k + 2 * a : 4 * k + a, i1 = BITS == 4 ? i0 + 4 : i0 + 2;
             const float y0 = x[g][i0] * up, y1 = x[g][i1] * up;
             uint32_t w = pack_f16x2(y0, y1);
-            if (!ODD && (r & 1)) {  // what the first part leaves: nothing of an infinity
+            if (!ODD && (r & 1)) {  // 2^11 times what the first part leaves: nothing of an infinity
               const float h0 = f16_lo(w), h1 = f16_hi(w);
-              w = PAIR ? pack_f16x2(y0 == h0 ? 0.f : y0 - h0, y1 == h1 ? 0.f : y1 - h1) : 0;
+              w = PAIR ? pack_f16x2(y0 == h0 ? 0.f : (y0 - h0) * 2048.f, y1 == h1 ? 0.f : (y1 - h1) * 2048.f) : 0;
             }
             qb[n][g][k][a] = w;
           }
@@ -407,7 +409,7 @@ struct PaQuant {
           for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int k = 0; k < QL; ++k) {
-              const float y = PAIR ? a[2 * h] + a[2 * h + 1] : a[2 * h + k];
+              const float y = PAIR ? a[2 * h] + a[2 * h + 1] * 0x1p-11f : a[2 * h + k];
               const float f = ks[h] * fac[n * QL + k][g];
               float& s = pr[i][n * QL + k][h];
               s = g ? s + f * y : f * y;

@@ -201,7 +201,7 @@ def test_queries_that_are_not_finite_are_nan_alone(bits, dt, g, lengths, dh, pag
 @pytest.mark.parametrize("bits", [4, 8])
 @pytest.mark.parametrize("dt,g", KINDS)
 @pytest.mark.parametrize("lengths,dh,page", SHAPES)
-@pytest.mark.parametrize("far", [8, 16])
+@pytest.mark.parametrize("far", [8, 16, 20])
 def test_large_dims_of_queries_that_keys_leave_alone(bits, dt, g, lengths, dh, page, far):
     """Two dims of the query 2^far times the others, where all keys have the code 0: they add nothing."""
     cache, q, _ = make(lengths, 2, g, dh, page, bits, dt, 101)
@@ -243,3 +243,11 @@ def test_rows_whose_scores_are_all_minus_infinity(bits, dt, g, lengths, dh, page
         # a live query's weights sum to 1, each of n within a few roundings of it
         total = torch.tensor([sum(h // g == kv and h not in none for h in range(2 * g)) for kv in range(2)], dtype=torch.float32)
         assert torch.allclose(m[0].sum(-1).cpu(), total, rtol=0, atol=g * max(lengths) * 2.0 ** -22)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("g", [2, 7])
+@pytest.mark.parametrize("lengths,dh,page", SHAPES)
+def test_larger_dims_of_fp32_queries_that_keys_leave_alone(bits, g, lengths, dh, page):
+    """fp32 holds dims 2^28 below their group's largest as well as a sum's own rounding."""
+    test_large_dims_of_queries_that_keys_leave_alone(bits, F32, g, lengths, dh, page, 28)
